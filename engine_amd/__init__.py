@@ -14,8 +14,9 @@ from .kquant import (  # noqa: F401
     AmdKernelError, AmdQuantizedKernelError, AmdModelKernelError, AmdWeightError,
     validate_quantized_geometry,
 )
-from .gguf import GgufError, GgufFile, TensorInfo, load_qwen3_decode, qwen3_config_from_gguf  # noqa: F401
-from .qwen3 import AmdKvCache, AmdQwen3Config, AmdQwen3Decode, QWEN3_8B, attention_decode, attention_prefill  # noqa: F401
+from .gguf import GgufError, GgufFile, TensorInfo, load_qwen3_decode, qwen3_config_from_gguf, rope_from_gguf  # noqa: F401
+from .qwen3 import KV_F16, KV_I8, AmdKvCache, AmdQwen3Config, AmdQwen3Decode, QWEN3_8B, attention_decode, attention_prefill  # noqa: F401
+from .rope import AmdRope, AmdRopeSpec, rope_frequencies  # noqa: F401
 from .serving import AmdBackend, AmdDispatcher, AmdServingDispatcher, BackendError, plan_memory  # noqa: F401
 
 __all__ = [
@@ -23,8 +24,9 @@ __all__ = [
     "AmdQ4KGemv", "AmdQ5KGemv", "AmdQ6KGemv", "QwenGemvKernel", "AmdQwenOps", "AmdQ4KEmbedding",
     "AmdKQuantEmbedding", "AmdKernelError",
     "AmdQuantizedKernelError", "AmdModelKernelError", "AmdWeightError", "validate_quantized_geometry",
-    "AmdKvCache", "AmdQwen3Config", "AmdQwen3Decode", "QWEN3_8B", "attention_decode",
+    "AmdKvCache", "AmdQwen3Config", "AmdQwen3Decode", "QWEN3_8B", "attention_decode", "attention_prefill",
+    "KV_F16", "KV_I8", "AmdRope", "AmdRopeSpec", "rope_frequencies",
     "AmdQ8_1Quantizer", "AmdQ4KQ8_1Gemv", "AmdQ5KQ8_1Gemv", "AmdQ6KQ8_1Gemv",
-    "GgufError", "GgufFile", "TensorInfo", "load_qwen3_decode", "qwen3_config_from_gguf",
+    "GgufError", "GgufFile", "TensorInfo", "load_qwen3_decode", "qwen3_config_from_gguf", "rope_from_gguf",
     "AmdBackend", "AmdDispatcher", "AmdServingDispatcher", "BackendError", "plan_memory",
 ]

@@ -85,6 +85,27 @@ class MemoryPlan(ctypes.Structure):
                 ("reserved_sequence_bytes", ctypes.c_uint64)]
 
 
+class RopeSpec(ctypes.Structure):
+    """ribn_amd_rope_spec."""
+    _fields_ = [("layout", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("rotary_dim", ctypes.c_uint32),
+                ("scaling", ctypes.c_uint32), ("base", ctypes.c_float), ("factor", ctypes.c_float),
+                ("original_context", ctypes.c_uint32), ("beta_fast", ctypes.c_float), ("beta_slow", ctypes.c_float),
+                ("attention_factor", ctypes.c_float), ("freq_factors", ctypes.POINTER(ctypes.c_float))]
+
+
+class RopeRows(ctypes.Structure):
+    """ribn_amd_rope_rows."""
+    _fields_ = [("input", ctypes.c_void_p), ("input_len", ctypes.c_size_t), ("input_token_stride", ctypes.c_size_t),
+                ("input_head_stride", ctypes.c_size_t), ("output", ctypes.c_void_p), ("output_len", ctypes.c_size_t),
+                ("output_token_stride", ctypes.c_size_t), ("output_head_stride", ctypes.c_size_t),
+                ("heads", ctypes.c_size_t)]
+
+
+class KvOptions(ctypes.Structure):
+    """ribn_amd_kv_options."""
+    _fields_ = [("format", ctypes.c_uint32), ("rope", ctypes.POINTER(RopeSpec))]
+
+
 READ_FN = ctypes.CFUNCTYPE(ctypes.c_int64, ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint8), ctypes.c_size_t)
 
 _vp = ctypes.c_void_p
@@ -163,6 +184,17 @@ SIGNATURES = {
     "ribn_amd_gguf_tensor_data_range": (_i32, [_vp, ctypes.c_char_p, ctypes.POINTER(_u64), ctypes.POINTER(_u64)]),
     "ribn_amd_gguf_stage": (_i32, [_vp, _vp, ctypes.POINTER(ctypes.c_char_p), _sz, _u64, _pvp]),
     "ribn_amd_kv_cache_create": (_i32, [_vp, ctypes.POINTER(Qwen3Config), _u32, _pvp]),
+    "ribn_amd_rope_frequencies": (_i32, [ctypes.POINTER(RopeSpec), ctypes.POINTER(ctypes.c_double), _sz,
+                                         ctypes.POINTER(ctypes.c_double)]),
+    "ribn_amd_rope_create": (_i32, [_vp, ctypes.POINTER(RopeSpec), _pvp]),
+    "ribn_amd_rope_destroy": (None, [_vp]),
+    "ribn_amd_rope_execute": (_i32, [_vp, _vp, _sz, ctypes.POINTER(RopeRows), _sz, _u32]),
+    "ribn_amd_kv_cache_create_with": (_i32, [_vp, ctypes.POINTER(Qwen3Config), _u32, ctypes.POINTER(KvOptions), _pvp]),
+    "ribn_amd_kv_cache_format": (_u32, [_vp]),
+    "ribn_amd_kv_bytes": (_u64, [ctypes.POINTER(Qwen3Config), _u32, _u32]),
+    "ribn_amd_kv_cache_tail": (_i32, [_vp, _u32, _pvp, _pvp, ctypes.POINTER(_sz)]),
+    "ribn_amd_kv_cache_write": (_i32, [_vp, _vp, _u32, _u32, _sz, _vp, _vp, _sz, _u32]),
+    "ribn_amd_kv_cache_read": (_i32, [_vp, _vp, _u32, _u32, _sz, _vp, _vp, _sz, _u32]),
     "ribn_amd_kv_cache_destroy": (None, [_vp]),
     "ribn_amd_kv_cache_capacity": (_u32, [_vp]),
     "ribn_amd_kv_cache_layer": (_i32, [_vp, _u32, _pvp, _pvp]),
@@ -193,6 +225,7 @@ SIGNATURES = {
     "ribn_amd_serving_destroy": (None, [_vp]),
     "ribn_amd_serving_set_prefill_chunk": (_i32, [_vp, _u32]),
     "ribn_amd_serving_set_prompt_prefill": (_i32, [_vp, _u32]),
+    "ribn_amd_serving_set_kv_options": (_i32, [_vp, ctypes.POINTER(KvOptions)]),
     "ribn_amd_serving_set_grouped_decode": (_i32, [_vp, _i32]),
     "ribn_amd_serving_dispatch_batch": (_i32, [_vp, ctypes.POINTER(ServingRow), _sz, ctypes.POINTER(ServingOutcome)]),
     "ribn_amd_serving_submit_batch": (_i32, [_vp, _u64, ctypes.POINTER(ServingRow), _sz]),

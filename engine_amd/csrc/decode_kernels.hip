@@ -37,6 +37,8 @@
 // model_ops.rs:201-258) with the same ordering key, tie rule and NaN rule.
 #include "decode_launch.hpp"
 #include "kquant_device.hpp"
+#include "kv8_device.hpp"
+#include "rope_device.hpp"
 
 #include <float.h>
 
@@ -114,6 +116,17 @@ __device__ __forceinline__ Rot rope_rot(float pos, float freq) {
     return r;
 }
 
+// The same rotation as its cache forms it: by its table (64-bit angles), or from the base.
+template <bool TABLE>
+__device__ __forceinline__ Rot cache_rot(const double* table, int pair, int pos, float freq) {
+    if constexpr (TABLE) {
+        const Rot64 r = table_rot(table, kHeadDim / 2, pair, pos);
+        return Rot{(float)r.s, (float)r.c};
+    } else {
+        return rope_rot((float)pos, freq);
+    }
+}
+
 // One 128-wide head held by a wave as lane l: x0 = dim l, x1 = dim l + 64.
 // RMSNorm with the shared per-head weight (x * inv * w, model_ops.rs:660-685),
 // then the rotation of the pair (l, l + 64) by the lane's angle.
@@ -126,7 +139,7 @@ __device__ __forceinline__ void norm_rope(float& x0, float& x1, float w0, float 
     x1 = y0 * r.s + y1 * r.c;
 }
 
-template <int QPK>
+template <int QPK, bool TABLE>
 __global__ __launch_bounds__(kThreads) void attn_decode_kernel(AttnArgs a) {
     constexpr int kHeadsPerWave = (QPK + kWaves - 1) / kWaves;
     __shared__ float qs[QPK][kHeadDim];
@@ -163,7 +176,7 @@ __global__ __launch_bounds__(kThreads) void attn_decode_kernel(AttnArgs a) {
     }
     const float qw0 = a.q_norm[lane];
     const float qw1 = a.q_norm[lane + 64];
-    const float freq = rope_freq(a.rope_base, lane);
+    const float freq = TABLE ? 0.f : rope_freq(a.rope_base, lane);
     float nx0 = 0.f, nx1 = 0.f, kw0 = 0.f, kw1 = 0.f;
     if (wave < 2) {
         const float* src = (wave == 0 ? a.k : a.v) + ((size_t)m * a.kv_heads + kvh) * kHeadDim;
@@ -209,7 +222,7 @@ __global__ __launch_bounds__(kThreads) void attn_decode_kernel(AttnArgs a) {
 
     // ---- query heads (and the new K/V): norm + rope into LDS
     const bool new_wave = has_new && wave < 2;  // wave 0: K, wave 1: V
-    const Rot rot = rope_rot((float)pos, freq);
+    const Rot rot = cache_rot<TABLE>(mb.rope, lane, pos, freq);
 #pragma unroll
     for (int i = 0; i < kHeadsPerWave; ++i) {
         const int h = wave + kWaves * i;
@@ -374,6 +387,7 @@ __global__ __launch_bounds__(kThreads) void attn_decode_kernel(AttnArgs a) {
 // The fused kernel's new-token path on its own: wave 0 normalises and ropes
 // the member's raw K of one KV head, wave 1 takes V, both stored as f16 at
 // the member's position. Grid (KV head, member).
+template <bool TABLE>
 __global__ __launch_bounds__(128) void kv_append_kernel(AttnArgs a) {
     const int kvh = blockIdx.x;
     const int m = blockIdx.y;
@@ -385,7 +399,8 @@ __global__ __launch_bounds__(128) void kv_append_kernel(AttnArgs a) {
     float x1 = src[lane + 64];
     const int pos = a.positions[m];
     if (wave == 0) {
-        norm_rope(x0, x1, a.k_norm[lane], a.k_norm[lane + 64], a.eps, rope_rot((float)pos, rope_freq(a.rope_base, lane)));
+        norm_rope(x0, x1, a.k_norm[lane], a.k_norm[lane + 64], a.eps,
+                  cache_rot<TABLE>(mb.rope, lane, pos, TABLE ? 0.f : rope_freq(a.rope_base, lane)));
     }
     if (pos < 0 || pos >= mb.capacity) return;
     const size_t head_elems = (size_t)mb.capacity * kHeadDim;
@@ -585,6 +600,7 @@ __global__ __launch_bounds__(64) void argmax_final_kernel(const uint2* part, int
 // kv_append_seq_kernel: the K/V of a prompt chunk's tokens, as kv_append_kernel
 // computes them for one token (K RMSNorm + rope, f16 round to nearest even),
 // at positions p0 + t. Grid (KV head, token).
+template <bool TABLE>
 __global__ __launch_bounds__(128) void kv_append_seq_kernel(PrefillAttnArgs a) {
     const int kvh = blockIdx.x;
     const int t = blockIdx.y;
@@ -595,7 +611,8 @@ __global__ __launch_bounds__(128) void kv_append_seq_kernel(PrefillAttnArgs a) {
     float x1 = src[lane + 64];
     const int pos = a.p0 + t;
     if (wave == 0) {
-        norm_rope(x0, x1, a.k_norm[lane], a.k_norm[lane + 64], a.eps, rope_rot((float)pos, rope_freq(a.rope_base, lane)));
+        norm_rope(x0, x1, a.k_norm[lane], a.k_norm[lane + 64], a.eps,
+                  cache_rot<TABLE>(a.mem.rope, lane, pos, TABLE ? 0.f : rope_freq(a.rope_base, lane)));
     }
     const size_t head_elems = (size_t)a.mem.capacity * kHeadDim;
     uint16_t* dst = (wave == 0 ? a.mem.keys : a.mem.values) + (size_t)a.layer * a.mem.layer_elems +
@@ -673,8 +690,67 @@ __device__ __forceinline__ float4 nonfinite_values(uint2 w) {
                        by & 0x8000u ? half_bits_to_float(w.y & 0xffffu) : 0.f, by >> 31 ? half_bits_to_float(w.y >> 16) : 0.f);
 }
 
-template <int QPK>
+// A block pair (64 keys) of an 8-bit cache as the prompt kernels stage it: 512
+// 16-byte pieces of keys and as many of values, in the order of their codes
+// (kv8.hpp), dequantised exactly into the f16 the LDS tiles hold. The block
+// that is not whole (keys from the sequence's last multiple of 32 on) comes from the tail, with
+// the same lanes and no prefetch: it is one half pair of a launch. Blocks past it read
+// as zeros.
+struct PrefillI8 {
+    __amdgpu_buffer_rsrc_t cr, sr;
+    const _Float16* tail_k;
+    const _Float16* tail_v;
+    int whole;     // whole blocks
+    int tail_blk;  // the block in the tail, or one no launch reaches
+
+    __device__ __forceinline__ PrefillI8(const PrefillAttnArgs& a, int kvh) {
+        const Kv8Head h = kv8_head(a.mem, a.layer, kvh);
+        const int end = a.p0 + a.tokens;
+        cr = make_rsrc(h.codes, (uint32_t)kv8_tail_offset(a.mem.capacity));
+        sr = make_rsrc(h.scales, (uint32_t)(kv8_blocks(a.mem.capacity) * sizeof(float2)));
+        tail_k = h.tail_k;
+        tail_v = h.tail_v;
+        whole = end / kKv8Block;
+        tail_blk = end % kKv8Block != 0 ? whole : -1;
+    }
+    __device__ __forceinline__ int block_of(int kb, int idx) const { return 2 * kb + (idx >> 8); }
+    __device__ __forceinline__ uint4 codes(int kb, int idx, int part) const {
+        const int b = block_of(kb, idx);
+        return load_b128(cr, b < whole ? (uint32_t)b * kKv8BlockBytes + (uint32_t)part + 16u * (uint32_t)(idx & 255) : kOOR);
+    }
+    __device__ __forceinline__ float scale(int kb, int idx, int part) const {
+        const int b = block_of(kb, idx);
+        return __builtin_bit_cast(float, load_b32(sr, b < whole ? 8u * (uint32_t)b + (uint32_t)part : kOOR));
+    }
+    // keys: the piece's key within the pair, and its first 8-dim slot
+    __device__ __forceinline__ int key_of(int idx) const { return 32 * (idx >> 8) + kv8_key_row((idx >> 7) & 1, idx & 15); }
+    __device__ __forceinline__ int piece_of(int idx) const { return 8 * ((idx >> 6) & 1) + 2 * ((idx >> 4) & 3); }
+    // values: the piece's first dim (of two) and first key (of eight) within the pair
+    __device__ __forceinline__ int dim_of(int idx) const { return 32 * ((idx >> 6) & 3) + 2 * (idx & 15); }
+    __device__ __forceinline__ int keys_of(int idx) const { return 32 * (idx >> 8) + 8 * ((idx >> 4) & 3); }
+    __device__ __forceinline__ void keys(int kb, int idx, uint4 w, float scale, kv8_half8 (&x)[2]) const {
+        x[0] = kv8_values(w.x, w.y, (_Float16)scale);
+        x[1] = kv8_values(w.z, w.w, (_Float16)scale);
+        if (block_of(kb, idx) == tail_blk) {
+            const kv8_half8* p = reinterpret_cast<const kv8_half8*>(tail_k + (key_of(idx) & 31) * kHeadDim) + piece_of(idx);
+            x[0] = p[0];
+            x[1] = p[1];
+        }
+    }
+    __device__ __forceinline__ void values(int kb, int idx, uint4 w, float scale, kv8_half8 (&x)[2]) const {
+        x[0] = kv8_values(w.x, w.y, (_Float16)scale);
+        x[1] = kv8_values(w.z, w.w, (_Float16)scale);
+        if (block_of(kb, idx) == tail_blk) {
+            const _Float16* p = tail_v + dim_of(idx) * kKv8Block + (keys_of(idx) & 31);
+            x[0] = *reinterpret_cast<const kv8_half8*>(p);
+            x[1] = *reinterpret_cast<const kv8_half8*>(p + kKv8Block);
+        }
+    }
+};
+
+template <int QPK, int CACHE>
 __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(PrefillAttnArgs a) {
+    constexpr bool TABLE = CACHE != kCacheF16;
     constexpr int W = QPK < 4 ? 4 : QPK;  // waves
     constexpr int NT = 64 * W;
     constexpr int TT = W / QPK;           // token tiles per workgroup
@@ -710,7 +786,20 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
     const int va = tid & 15;        // V unit: keys 4va .. 4va + 3
     const int vc = (tid >> 4) & 15; // dims 8vc .. 8vc + 7
     uint4 kp[KP], vp[4];
+    const PrefillI8 c8(a, kvh);
+    constexpr int P8 = 512 / NT;  // 16-byte pieces of an 8-bit block pair's keys (values) per thread
+    float kscale[P8], vscale[P8];
     auto issue = [&](int kb) {
+        if constexpr (CACHE == kCacheI8) {
+#pragma unroll
+            for (int r = 0; r < P8; ++r) {
+                kp[r] = c8.codes(kb, tid + NT * r, 0);
+                vp[r] = c8.codes(kb, tid + NT * r, kKv8PartBytes);
+                kscale[r] = c8.scale(kb, tid + NT * r, 0);
+                vscale[r] = c8.scale(kb, tid + NT * r, 4);
+            }
+            return;
+        }
 #pragma unroll
         for (int r = 0; r < KP; ++r) {
             const int idx = tid + NT * r;
@@ -725,6 +814,26 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
     const int wg_first = a.p0 + (int)blockIdx.x * TT * kPrefillTileTokens;  // a token's first position
     if (tid == 0) v_dropped = 0;
     auto stage = [&](int buf, int kb) {
+        if constexpr (CACHE == kCacheI8) {
+#pragma unroll
+            for (int r = 0; r < P8; ++r) {
+                const int idx = tid + NT * r;
+                kv8_half8 x[2];
+                c8.keys(kb, idx, kp[r], kscale[r], x);
+                const int key = c8.key_of(idx), piece = c8.piece_of(idx);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) *reinterpret_cast<kv8_half8*>(&ks[buf][key][8 * ((piece + i) ^ (key & 15))]) = x[i];
+                c8.values(kb, idx, vp[r], vscale[r], x);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint4 w = __builtin_bit_cast(uint4, x[i]);
+                    uint2* row = reinterpret_cast<uint2*>(&vt[buf][c8.dim_of(idx) + i][c8.keys_of(idx)]);
+                    row[0] = make_uint2(w.x, w.y);
+                    row[1] = make_uint2(w.z, w.w);
+                }
+            }
+            return;
+        }
         if (kb * kPfKeys + kPfKeys - 1 > wg_first && drop_nonfinite(vp)) v_dropped = 1;
 #pragma unroll
         for (int r = 0; r < KP; ++r) {
@@ -762,8 +871,8 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
         for (int r = 0; r < TT * kPrefillTileTokens * 64 / NT; ++r) {
             const int e = tid + NT * r;
             const int row = e >> 6, d = e & 63;
-            const Rot rr = rope_rot((float)(a.p0 + (int)blockIdx.x * TT * kPrefillTileTokens + row),
-                                    rope_freq(a.rope_base, d));
+            const Rot rr = cache_rot<TABLE>(a.mem.rope, d, a.p0 + (int)blockIdx.x * TT * kPrefillTileTokens + row,
+                                            TABLE ? 0.f : rope_freq(a.rope_base, d));
             rot_tab[row * kRotRow + d] = make_float2(rr.c, rr.s);
         }
     }
@@ -808,7 +917,7 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
                 r.c = cs.x;
                 r.s = cs.y;
             } else {
-                r = rope_rot((float)pos, rope_freq(a.rope_base, d));
+                r = cache_rot<TABLE>(a.mem.rope, d, pos, TABLE ? 0.f : rope_freq(a.rope_base, d));
             }
             const float q0 = y0 * r.c - y1 * r.s;
             const float q1 = y0 * r.s + y1 * r.c;
@@ -932,7 +1041,7 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
     }
 
     // ---- non-finite values, to the tokens that attend them
-    if (__builtin_expect(__builtin_amdgcn_readfirstlane(v_dropped) != 0, 0)) {
+    if (CACHE != kCacheI8 && __builtin_expect(__builtin_amdgcn_readfirstlane(v_dropped) != 0, 0)) {
 #pragma unroll 1
         for (int key = (wg_first + 1) / kPfKeys * kPfKeys; key <= last; ++key) {
             // (the largest offset added to kOOR stays past any cache too)
@@ -1012,8 +1121,9 @@ __device__ __forceinline__ float pair_combine(float v, OP op) {
     return op(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
 }
 
-template <int QPK>
+template <int QPK, int CACHE>
 __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnArgs a, int tiles) {
+    constexpr bool TABLE = CACHE != kCacheF16;
     constexpr int KS = QPK < 8 ? 2 : 1;   // key halves
     constexpr int W = 8 / KS;             // waves per key half
     constexpr int NT = 64 * W;
@@ -1062,14 +1172,37 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
     const bool v_unit = tid < 256;
     const int va = tid & 15;        // V unit: keys 4va .. 4va + 3
     const int vc = (tid >> 4) & 15; // dims 8vc .. 8vc + 7
+    const PrefillI8 c8(a, kvh);
+    constexpr int P8 = 512 / NT;  // 16-byte pieces of an 8-bit block pair's keys (values) per thread
+    float kscale[P8], vscale[P8];
     auto issue_k = [&](int kb, uint4 (&kp)[KP]) {
+        if constexpr (CACHE == kCacheI8) {
+#pragma unroll
+            for (int r = 0; r < P8; ++r) {
+                kp[r] = c8.codes(kb, tid + NT * r, 0);
+                kscale[r] = c8.scale(kb, tid + NT * r, 0);
+            }
+            return;
+        }
 #pragma unroll
         for (int r = 0; r < KP; ++r) {
             const int idx = tid + NT * r;
             kp[r] = load_b128(kr, ((uint32_t)(kb * kPfKeys + (idx >> 4)) * kHeadDim + 8u * (uint32_t)(idx & 15)) * 2u);
         }
     };
-    auto stage_k = [&](int buf, const uint4 (&kp)[KP]) {
+    auto stage_k = [&](int buf, int kb, const uint4 (&kp)[KP]) {
+        if constexpr (CACHE == kCacheI8) {
+#pragma unroll
+            for (int r = 0; r < P8; ++r) {
+                const int idx = tid + NT * r;
+                kv8_half8 x[2];
+                c8.keys(kb, idx, kp[r], kscale[r], x);
+                const int key = c8.key_of(idx), piece = c8.piece_of(idx);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) *reinterpret_cast<kv8_half8*>(&bufs[buf][half].k[key][8 * ((piece + i) ^ (key & 15))]) = x[i];
+            }
+            return;
+        }
 #pragma unroll
         for (int r = 0; r < KP; ++r) {
             const int idx = tid + NT * r;
@@ -1077,6 +1210,14 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
         }
     };
     auto issue_v = [&](int kb, uint4 (&vp)[4]) {
+        if constexpr (CACHE == kCacheI8) {
+#pragma unroll
+            for (int r = 0; r < P8; ++r) {
+                vp[r] = c8.codes(kb, tid + NT * r, kKv8PartBytes);
+                vscale[r] = c8.scale(kb, tid + NT * r, 4);
+            }
+            return;
+        }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const uint32_t off = ((uint32_t)(kb * kPfKeys + 4 * va + r) * kHeadDim + 8u * (uint32_t)vc) * 2u;
@@ -1086,6 +1227,23 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
     const int wg_first = a.p0 + tile * TT * TOK;  // a token's first position
     if (threadIdx.x == 0) v_dropped = 0;
     auto stage_v = [&](int buf, int kb, uint4 (&vp)[4]) {
+        if constexpr (CACHE == kCacheI8) {
+#pragma unroll
+            for (int r = 0; r < P8; ++r) {
+                const int idx = tid + NT * r;
+                kv8_half8 x[2];
+                c8.values(kb, idx, vp[r], vscale[r], x);
+                const int k0 = c8.keys_of(idx);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint4 w = __builtin_bit_cast(uint4, x[i]);
+                    _Float16* row = bufs[buf][half].v[c8.dim_of(idx) + i];
+                    *reinterpret_cast<uint2*>(row + vt_pos(k0)) = make_uint2(w.x, w.y);
+                    *reinterpret_cast<uint2*>(row + vt_pos(k0 + 4)) = make_uint2(w.z, w.w);
+                }
+            }
+            return;
+        }
         if (v_unit) {
             if (kb * kPfKeys + kPfKeys - 1 > wg_first && drop_nonfinite(vp)) v_dropped = 1;
             // row j of the unit: dim 8vc + j of keys 4va .. 4va + 3
@@ -1133,10 +1291,10 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
     // of pair (d, d + 64) at position p0 + first token + row, the rope_rot /
     // rope_freq values of the decode kernel
     float2* const rot_tab = reinterpret_cast<float2*>(lds + kQBytes);
-    const float freq = rope_freq(a.rope_base, lane);
+    const float freq = TABLE ? 0.f : rope_freq(a.rope_base, lane);
 #pragma unroll 1
     for (int r = (int)threadIdx.x >> 6; r < TT * TOK; r += 8) {
-        const Rot rr = rope_rot((float)(a.p0 + tile * TT * TOK + r), freq);
+        const Rot rr = cache_rot<TABLE>(a.mem.rope, lane, a.p0 + tile * TT * TOK + r, freq);
         rot_tab[r * kRotRow + lane] = make_float2(rr.c, rr.s);
     }
     __syncthreads();
@@ -1213,7 +1371,7 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
     // key half `half` takes blocks half, half + KS, ...; a block past the last
     // is wholly masked (its loads read zeros)
     const int rounds = (last / kPfKeys + KS) / KS;
-    stage_k(0, kp0);
+    stage_k(0, half, kp0);
     stage_v(0, half, vp0);
     __syncthreads();
     for (int round = 0; round < rounds; ++round) {
@@ -1253,7 +1411,7 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
         // into the other buffer: every wave finished reading it before the
         // previous barrier
         if (round + 1 < rounds) {
-            stage_k(buf ^ 1, kp);
+            stage_k(buf ^ 1, kb + KS, kp);
             issue_v(kb + KS, vp);
         }
         // keys past a token's position are masked; a block wholly at or below
@@ -1364,7 +1522,7 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
     }
 
     // ---- non-finite values, to the tokens that attend them
-    if (__builtin_expect(__builtin_amdgcn_readfirstlane(v_dropped) != 0, 0)) {
+    if (CACHE != kCacheI8 && __builtin_expect(__builtin_amdgcn_readfirstlane(v_dropped) != 0, 0)) {
 #pragma unroll 1
         for (int key = (wg_first + 1) / kPfKeys * kPfKeys; key <= last; ++key) {
             // (the largest offset added to kOOR stays past any cache too)
@@ -1403,7 +1561,21 @@ int attn_grid_chunks(int max_capacity, int members) {
     return std::max(1, std::min(kAttnChunks, (max_capacity + min_chunk - 1) / min_chunk));
 }
 
-hipError_t launch_attention(const AttnArgs& args, int members, hipStream_t stream) {
+namespace {
+template <bool TABLE>
+hipError_t launch_decode_heads(const AttnArgs& b, dim3 grid, hipStream_t stream) {
+    switch (b.q_heads / b.kv_heads) {
+    case 1: hipLaunchKernelGGL((attn_decode_kernel<1, TABLE>), grid, dim3(kThreads), 0, stream, b); break;
+    case 2: hipLaunchKernelGGL((attn_decode_kernel<2, TABLE>), grid, dim3(kThreads), 0, stream, b); break;
+    case 4: hipLaunchKernelGGL((attn_decode_kernel<4, TABLE>), grid, dim3(kThreads), 0, stream, b); break;
+    case 8: hipLaunchKernelGGL((attn_decode_kernel<8, TABLE>), grid, dim3(kThreads), 0, stream, b); break;
+    default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
+}  // namespace
+
+hipError_t launch_attention(const AttnArgs& args, int members, hipStream_t stream, bool rope_table) {
     if (members < 1 || members > kAttnMaxMembers || args.kv_heads < 1 || args.q_heads % args.kv_heads != 0 ||
         args.chunks < 1 || args.chunks > kAttnChunks || args.mem == nullptr) {
         return hipErrorInvalidValue;
@@ -1416,14 +1588,7 @@ hipError_t launch_attention(const AttnArgs& args, int members, hipStream_t strea
     AttnArgs b = args;
     b.min_chunk = attn_min_chunk(members);
     const dim3 grid((unsigned)b.chunks, (unsigned)b.kv_heads, (unsigned)members);
-    switch (b.q_heads / b.kv_heads) {
-    case 1: hipLaunchKernelGGL(attn_decode_kernel<1>, grid, dim3(kThreads), 0, stream, b); break;
-    case 2: hipLaunchKernelGGL(attn_decode_kernel<2>, grid, dim3(kThreads), 0, stream, b); break;
-    case 4: hipLaunchKernelGGL(attn_decode_kernel<4>, grid, dim3(kThreads), 0, stream, b); break;
-    case 8: hipLaunchKernelGGL(attn_decode_kernel<8>, grid, dim3(kThreads), 0, stream, b); break;
-    default: return hipErrorInvalidValue;
-    }
-    hipError_t e = hipGetLastError();
+    hipError_t e = rope_table ? launch_decode_heads<true>(b, grid, stream) : launch_decode_heads<false>(b, grid, stream);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(attn_combine_kernel, dim3((unsigned)b.q_heads, (unsigned)members), dim3(kHeadDim), 0, stream,
                        b);
@@ -1446,12 +1611,13 @@ hipError_t launch_swiglu(const float* gate, const float* up, float* out, size_t 
     return hipGetLastError();
 }
 
-hipError_t launch_kv_append(const AttnArgs& args, int members, hipStream_t stream) {
+hipError_t launch_kv_append(const AttnArgs& args, int members, hipStream_t stream, bool rope_table) {
     if (members < 1 || members > kAttnMaxMembers || args.kv_heads < 1 || args.mem == nullptr) {
         return hipErrorInvalidValue;
     }
-    hipLaunchKernelGGL(kv_append_kernel, dim3((unsigned)args.kv_heads, (unsigned)members), dim3(128), 0, stream,
-                       args);
+    const dim3 grid((unsigned)args.kv_heads, (unsigned)members);
+    if (rope_table) hipLaunchKernelGGL(kv_append_kernel<true>, grid, dim3(128), 0, stream, args);
+    else hipLaunchKernelGGL(kv_append_kernel<false>, grid, dim3(128), 0, stream, args);
     return hipGetLastError();
 }
 
@@ -1470,33 +1636,51 @@ bool wide_prefill(const PrefillAttnArgs& a, int tiles, int cu_count) {
     return 16 * tiles * a.kv_heads >= (qpk == 1 ? 4 : qpk == 8 ? 16 : 11) * cu_count;
 }
 
-template <int QPK>
+template <int QPK, int CACHE>
 hipError_t launch_prefill_heads(const PrefillAttnArgs& a, int cu_count, hipStream_t stream) {
     constexpr int TT = QPK < 4 ? 4 / QPK : 1;  // token tiles per workgroup
     const int wide = (a.tokens + kPrefillWideTokens * TT - 1) / (kPrefillWideTokens * TT);
     if (wide_prefill(a, wide, cu_count)) {
-        hipLaunchKernelGGL(attn_prefill_wide_kernel<QPK>, dim3((unsigned)wide * (unsigned)a.kv_heads), dim3(512), 0, stream, a, wide);
+        hipLaunchKernelGGL((attn_prefill_wide_kernel<QPK, CACHE>), dim3((unsigned)wide * (unsigned)a.kv_heads), dim3(512), 0, stream, a, wide);
     } else {
         const int tiles = (a.tokens + kPrefillTileTokens * TT - 1) / (kPrefillTileTokens * TT);
-        hipLaunchKernelGGL(attn_prefill_kernel<QPK>, dim3((unsigned)tiles, (unsigned)a.kv_heads), dim3(QPK < 8 ? 256 : 512), 0, stream, a);
+        hipLaunchKernelGGL((attn_prefill_kernel<QPK, CACHE>), dim3((unsigned)tiles, (unsigned)a.kv_heads), dim3(QPK < 8 ? 256 : 512), 0, stream, a);
     }
     return hipGetLastError();
 }
+
+template <int CACHE>
+hipError_t launch_prefill_cache(const PrefillAttnArgs& a, int cu_count, hipStream_t stream) {
+    switch (a.q_heads / a.kv_heads) {
+    case 1: return launch_prefill_heads<1, CACHE>(a, cu_count, stream);
+    case 2: return launch_prefill_heads<2, CACHE>(a, cu_count, stream);
+    case 4: return launch_prefill_heads<4, CACHE>(a, cu_count, stream);
+    case 8: return launch_prefill_heads<8, CACHE>(a, cu_count, stream);
+    default: return hipErrorInvalidValue;
+    }
+}
 }  // namespace
 
-hipError_t launch_prefill_attention(const PrefillAttnArgs& a, int cu_count, hipStream_t stream) {
+hipError_t launch_prefill_attention(const PrefillAttnArgs& a, int cu_count, hipStream_t stream, int cache) {
     if (a.tokens < 1 || a.kv_heads < 1 || a.q_heads % a.kv_heads != 0 || a.p0 < 0 ||
-        (long long)a.p0 + a.tokens > a.mem.capacity || a.mem.keys == nullptr || a.mem.values == nullptr) {
+        (long long)a.p0 + a.tokens > a.mem.capacity || a.mem.keys == nullptr ||
+        (cache == kCacheI8 ? a.mem.rope == nullptr : a.mem.values == nullptr)) {
         return hipErrorInvalidValue;
     }
-    hipLaunchKernelGGL(kv_append_seq_kernel, dim3((unsigned)a.kv_heads, (unsigned)a.tokens), dim3(128), 0, stream, a);
-    hipError_t e = hipGetLastError();
+    const dim3 grid((unsigned)a.kv_heads, (unsigned)a.tokens);
+    hipError_t e = hipSuccess;
+    if (cache == kCacheI8) {
+        e = launch_kv8_append_seq(a, stream);
+    } else {
+        if (cache == kCacheF16Table) hipLaunchKernelGGL(kv_append_seq_kernel<true>, grid, dim3(128), 0, stream, a);
+        else hipLaunchKernelGGL(kv_append_seq_kernel<false>, grid, dim3(128), 0, stream, a);
+        e = hipGetLastError();
+    }
     if (e != hipSuccess || a.out == nullptr) return e;
-    switch (a.q_heads / a.kv_heads) {
-    case 1: return launch_prefill_heads<1>(a, cu_count, stream);
-    case 2: return launch_prefill_heads<2>(a, cu_count, stream);
-    case 4: return launch_prefill_heads<4>(a, cu_count, stream);
-    case 8: return launch_prefill_heads<8>(a, cu_count, stream);
+    switch (cache) {
+    case kCacheF16: return launch_prefill_cache<kCacheF16>(a, cu_count, stream);
+    case kCacheF16Table: return launch_prefill_cache<kCacheF16Table>(a, cu_count, stream);
+    case kCacheI8: return launch_prefill_cache<kCacheI8>(a, cu_count, stream);
     default: return hipErrorInvalidValue;
     }
 }

@@ -26,13 +26,19 @@ constexpr int kPartStride = kHeadDim + 4;
 // One member's cache, as a device-resident descriptor: the attention kernel
 // reads it from memory, so a captured step serves any set of caches.
 struct AttnMember {
-    uint16_t* keys;       // f16 [layers][kv_heads][capacity][128]
-    uint16_t* values;     // f16 [layers][kv_heads][capacity][128]
+    uint16_t* keys;       // f16 [layers][kv_heads][capacity][128]; an 8-bit cache: its regions [layers][kv_heads] (kv8.hpp)
+    uint16_t* values;     // f16 [layers][kv_heads][capacity][128]; an 8-bit cache: unused
     float* partials;      // [q_heads][kAttnChunks][kPartStride], this member's own
-    uint64_t layer_elems; // kv_heads * capacity * 128: one layer's elements
+    uint64_t layer_elems; // kv_heads * capacity * 128: one layer's elements; an 8-bit cache: one layer's bytes
+    const double* rope;   // the cache's rotary table (rope_device.hpp), null: f32 angles from the launch's rope base
     int capacity;         // cache tokens per (layer, KV head)
     int pad;
 };
+
+// What the caches of a launch hold (all of one kind).
+constexpr int kCacheF16 = 0;       // f16, f32 angles
+constexpr int kCacheF16Table = 1;  // f16, angles from the caches' rotary tables
+constexpr int kCacheI8 = 2;        // 8 bits (kv8.hpp), angles from the tables
 
 struct AttnArgs {
     const AttnMember* mem;     // device [members] descriptors
@@ -66,16 +72,17 @@ int attn_grid_chunks(int max_capacity, int members);
 
 // Two launches: the chunked attention writing partials, then their merge into
 // `out`. members <= kAttnMaxMembers; q_heads / kv_heads in {1, 2, 4, 8}.
+// With `rope_table`, q and k are rotated by the caches' tables (every cache has one).
 // Without `appended`, the workgroup whose chunk holds a member's position
 // normalises, ropes and appends that member's new K/V (members must then
 // hold distinct caches); with it the caches already hold them.
-hipError_t launch_attention(const AttnArgs& args, int members, hipStream_t stream);
+hipError_t launch_attention(const AttnArgs& args, int members, hipStream_t stream, bool rope_table = false);
 
 // The K/V append of `members` new tokens, ahead of an `appended` attention
 // launch: per (member, KV head) the K RMSNorm + rope and the f16 store of K
 // and V at positions[m], computed as the fused attention kernel does. Members
 // may share a cache (consecutive positions of one sequence).
-hipError_t launch_kv_append(const AttnArgs& args, int members, hipStream_t stream);
+hipError_t launch_kv_append(const AttnArgs& args, int members, hipStream_t stream, bool rope_table = false);
 
 // out[i] = silu(gate[i]) * up[i] over n values (model_ops.rs:316-328, the
 // same operations as the GEMVs' SwiGLU prologue and pair epilogue); out may
@@ -130,7 +137,7 @@ constexpr int kPrefillWideTokens = 32;
 // The chunk's K (RMSNorm + rope) and V stored as f16 at their positions, then
 // (when `out` is set) causal attention of every token over positions
 // 0 .. its own on the matrix cores. q_heads / kv_heads in {1, 2, 4, 8}.
-hipError_t launch_prefill_attention(const PrefillAttnArgs& args, int cu_count, hipStream_t stream);
+hipError_t launch_prefill_attention(const PrefillAttnArgs& args, int cu_count, hipStream_t stream, int cache = kCacheF16);
 
 // Slice results a two-stage greedy selection keeps per member.
 constexpr int kArgmaxSlices = 64;

@@ -1,0 +1,663 @@
+// Kernels of the 8-bit KV cache for gfx950 (kv8.hpp has the layout and the
+// arithmetic of a code): the append of new tokens, decode attention over the
+// cache, and rows moved in and out of it.
+#include "kv8.hpp"
+
+#include <float.h>
+
+#include <algorithm>
+
+#include "kquant_device.hpp"
+#include "kv8_device.hpp"
+#include "rope_device.hpp"
+
+namespace ribn_amd {
+
+namespace {
+
+constexpr uint32_t kOOR = 0xffffff00u;  // buffer offset past any region: loads return 0
+constexpr int kRowHalfs = kHeadDim + 8;  // LDS row of a staged token (272 B: 16-byte reads of 8 rows fall in distinct banks)
+
+// ------------------------------------------------------------------- append
+//
+// One workgroup a (KV head, block of 32 positions). The block's new rows are
+// staged in LDS as f16; a block that is whole after the append has its earlier
+// rows added (from the tail, or from the codes of a block taken back into), its
+// two scales found and its codes written, 16 of keys and 16 of values a
+// thread. Workgroup 0, which reads the tail as it was, also writes what the
+// tail holds after the call (the last block's rows) and `end`: no other one touches
+// them. Traffic is the rows in (f32) and a byte a value out.
+
+struct Rows {
+    const void* k;    // the head's first row
+    const void* v;
+    size_t stride;    // values between tokens
+};
+
+// How rows arrive: raw projections (keys to be normalised and rotated), or as they are.
+constexpr int kRowsRaw = 0, kRowsF32 = 1, kRowsF16 = 2;
+
+struct Stage {
+    _Float16 k[kKv8Block][kRowHalfs];
+    _Float16 v[kKv8Block][kRowHalfs];
+    float amax[2][4];
+};
+
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+}
+
+template <int ROWS>
+__device__ __forceinline__ void stage_rows(Stage& st, const Rows& in, int first, int count, int row0, const float* k_norm,
+                                           double eps, const double* rope, int position) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    double w0 = 1.0, w1 = 1.0, turns = 0.0, gain = 1.0;
+    if constexpr (ROWS == kRowsRaw) {
+        w0 = k_norm[lane];
+        w1 = k_norm[lane + 64];
+        turns = rope[lane];
+        gain = rope[64];
+    }
+    for (int i = wave; i < count; i += 4) {
+        const size_t at = (size_t)(first + i) * in.stride;
+        float k0, k1, v0, v1;
+        if constexpr (ROWS == kRowsF16) {
+            const _Float16* k = static_cast<const _Float16*>(in.k) + at;
+            const _Float16* v = static_cast<const _Float16*>(in.v) + at;
+            k0 = k[lane]; k1 = k[lane + 64];
+            v0 = v[lane]; v1 = v[lane + 64];
+        } else {
+            const float* k = static_cast<const float*>(in.k) + at;
+            const float* v = static_cast<const float*>(in.v) + at;
+            k0 = k[lane]; k1 = k[lane + 64];
+            v0 = v[lane]; v1 = v[lane + 64];
+        }
+        if constexpr (ROWS == kRowsRaw) {
+            // 64 bits up to the one rounding to f32: where a key falls between two
+            // codes then does not depend on the order of a sum
+            const double x0 = k0, x1 = k1;
+            const double ssq = wave_sum64(__builtin_fma(x0, x0, x1 * x1));
+            const double inv = 1.0 / sqrt(ssq / (double)kHeadDim + eps);
+            const Rot64 r = turn_sincos((double)(position + i) * turns);
+            const double y0 = x0 * inv * w0 * gain, y1 = x1 * inv * w1 * gain;
+            k0 = (float)__builtin_fma(y0, r.c, -y1 * r.s);
+            k1 = (float)__builtin_fma(y0, r.s, y1 * r.c);
+        }
+        st.k[row0 + i][lane] = kv8_half(k0);
+        st.k[row0 + i][lane + 64] = kv8_half(k1);
+        st.v[row0 + i][lane] = kv8_half(v0);
+        st.v[row0 + i][lane + 64] = kv8_half(v1);
+    }
+}
+
+// Rows 0 .. count - 1 of block b as the cache has them, from its tail or its codes.
+__device__ __forceinline__ void stage_held(Stage& st, const Kv8Head& h, int b, int count, bool tail) {
+    const int tid = threadIdx.x;
+    if (tail) {
+        for (int i = tid; i < count * kHeadDim; i += 256) {
+            st.k[i >> 7][i & 127] = h.tail_k[i];
+            st.v[i >> 7][i & 127] = h.tail_v[(i & 127) * kKv8Block + (i >> 7)];
+        }
+        return;
+    }
+    const uint8_t* codes = h.codes + (size_t)b * kKv8BlockBytes;
+    const float2 sc = h.scales[b];
+    const int lane = tid & 63, g = lane >> 4, m = lane & 15;
+    const int row = kv8_key_row(tid >> 7, m);
+    for (int j = 0; j < 16; ++j) {
+        const int dim = 64 * ((tid >> 6) & 1) + 16 * g + j;
+        if (row < count) st.k[row][dim] = (_Float16)((float)((int)codes[tid * 16 + j] - 128) * sc.x);
+        const int key = 8 * g + (j & 7), vd = 32 * (tid >> 6) + 2 * m + (j >> 3);
+        if (key < count) st.v[key][vd] = (_Float16)((float)((int)codes[kKv8PartBytes + tid * 16 + j] - 128) * sc.y);
+    }
+}
+
+// The staged block's 32 rows into codes and scales.
+__device__ __forceinline__ void quantise(Stage& st, const Kv8Head& h, int b) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
+    // this thread's 16 keys (one row) and 16 values (8 rows of two dims)
+    float kx[16], vx[16];
+    const kv8_half8* kr = reinterpret_cast<const kv8_half8*>(&st.k[kv8_key_row(wave >> 1, m)][64 * (wave & 1) + 16 * g]);
+    const kv8_half8 k0 = kr[0], k1 = kr[1];
+    float ka = 0.f, va = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        kx[j] = (float)k0[j];
+        kx[8 + j] = (float)k1[j];
+        const kv8_half2 v = *reinterpret_cast<const kv8_half2*>(&st.v[8 * g + j][32 * wave + 2 * m]);
+        vx[j] = (float)v[0];
+        vx[8 + j] = (float)v[1];
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        ka = fmaxf(ka, fabsf(kx[j]));
+        va = fmaxf(va, fabsf(vx[j]));
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        ka = fmaxf(ka, __shfl_xor(ka, off, 64));
+        va = fmaxf(va, __shfl_xor(va, off, 64));
+    }
+    if (lane == 0) {
+        st.amax[0][wave] = ka;
+        st.amax[1][wave] = va;
+    }
+    __syncthreads();
+    const int ek = kv8_exponent(fmaxf(fmaxf(st.amax[0][0], st.amax[0][1]), fmaxf(st.amax[0][2], st.amax[0][3])));
+    const int ev = kv8_exponent(fmaxf(fmaxf(st.amax[1][0], st.amax[1][1]), fmaxf(st.amax[1][2], st.amax[1][3])));
+    const float ik = kv8_power(-ek), iv = kv8_power(-ev);
+    uint32_t kw[4], vw[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        kw[w] = vw[w] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            kw[w] |= kv8_code(kx[4 * w + j], ik) << (8 * j);
+            vw[w] |= kv8_code(vx[4 * w + j], iv) << (8 * j);
+        }
+    }
+    uint8_t* codes = h.codes + (size_t)b * kKv8BlockBytes + tid * 16;
+    *reinterpret_cast<uint4*>(codes) = make_uint4(kw[0], kw[1], kw[2], kw[3]);
+    *reinterpret_cast<uint4*>(codes + kKv8PartBytes) = make_uint4(vw[0], vw[1], vw[2], vw[3]);
+    if (tid == 0) h.scales[b] = make_float2(kv8_power(ek), kv8_power(ev));
+}
+
+__device__ __forceinline__ void store_tail(const Stage& st, const Kv8Head& h, int row0, int rows) {
+    for (int i = threadIdx.x; i < (rows - row0) * kHeadDim; i += 256) {
+        const int r = row0 + (i >> 7), d = i & 127;
+        h.tail_k[r * kHeadDim + d] = st.k[r][d];
+        h.tail_v[d * kKv8Block + r] = st.v[r][d];
+    }
+}
+
+// Block p0 / 32 + j of an append of `tokens` rows at p0 (0 <= p0, p0 + tokens <= capacity).
+template <int ROWS>
+__device__ __forceinline__ void append_block(Stage& st, const Kv8Head& h, const Rows& in, int p0, int tokens, int j,
+                                             const float* k_norm, double eps, const double* rope) {
+    const int end = p0 + tokens;
+    const int b = p0 / kKv8Block + j;
+    const int last = (end - 1) / kKv8Block;
+    const int first = j == 0 ? p0 : b * kKv8Block;             // this block's new positions
+    const int fill = min(end - b * kKv8Block, kKv8Block);      // rows it holds afterwards
+    const bool whole = fill == kKv8Block;
+    if (j != 0 && !whole) return;  // the last block, which workgroup 0 puts into the tail
+    const int row0 = first - b * kKv8Block;
+    stage_rows<ROWS>(st, in, first - p0, fill - row0, row0, k_norm, eps, rope, first);
+    int kept = row0;  // rows of the tail that stay as they are
+    if (row0 != 0) {
+        const int old = *h.end;
+        const bool held = old > 0 && (old - 1) / kKv8Block == b;
+        if (whole || !held) stage_held(st, h, b, row0, held);
+        if (!held) kept = 0;
+    }
+    __syncthreads();
+    if (whole) quantise(st, h, b);
+    if (j != 0) return;
+    if (b == last) {
+        store_tail(st, h, kept, fill);
+    } else {
+        __syncthreads();  // the staged rows are read
+        const int f = last * kKv8Block, n = end - f;
+        stage_rows<ROWS>(st, in, f - p0, n, 0, k_norm, eps, rope, f);
+        __syncthreads();
+        store_tail(st, h, 0, n);
+    }
+    if (threadIdx.x == 0) *h.end = end;
+}
+
+// Grid (KV head, member), or (KV head, block) of the one cache the members share.
+__global__ __launch_bounds__(256) void kv8_append_kernel(AttnArgs a, int members) {
+    __shared__ Stage st;
+    const int kvh = blockIdx.x;
+    const int m = members == 0 ? (int)blockIdx.y : 0;
+    const AttnMember mb = a.mem[m];
+    const int pos = a.positions[m];
+    const int tokens = members == 0 ? 1 : members;
+    if (pos < 0 || pos > mb.capacity - tokens) return;
+    const int j = members == 0 ? 0 : (int)blockIdx.y;
+    if (pos / kKv8Block + j > (pos + tokens - 1) / kKv8Block) return;
+    const size_t at = ((size_t)m * a.kv_heads + kvh) * kHeadDim;
+    const Rows in{a.k + at, a.v + at, (size_t)a.kv_heads * kHeadDim};
+    append_block<kRowsRaw>(st, kv8_head(mb, a.layer, kvh), in, pos, tokens, j, a.k_norm, a.eps, mb.rope);
+}
+
+__global__ __launch_bounds__(256) void kv8_append_seq_kernel(PrefillAttnArgs a) {
+    __shared__ Stage st;
+    const int kvh = blockIdx.x;
+    const size_t at = (size_t)kvh * kHeadDim;
+    const Rows in{a.k + at, a.v + at, (size_t)a.kv_heads * kHeadDim};
+    append_block<kRowsRaw>(st, kv8_head(a.mem, a.layer, kvh), in, a.p0, a.tokens, blockIdx.y, a.k_norm, a.eps, a.mem.rope);
+}
+
+template <int ROWS>
+__global__ __launch_bounds__(256) void kv8_write_kernel(KvMoveArgs a) {
+    __shared__ Stage st;
+    const int kvh = blockIdx.x;
+    const size_t at = (size_t)kvh * kHeadDim * (ROWS == kRowsF16 ? 2 : 4);
+    const Rows in{static_cast<const char*>(a.keys) + at, static_cast<const char*>(a.values) + at, (size_t)a.kv_heads * kHeadDim};
+    append_block<ROWS>(st, kv8_head(a.mem, a.layer, kvh), in, a.p0, a.tokens, blockIdx.y, nullptr, 0.0, nullptr);
+}
+
+// Rows out of an 8-bit cache, grid (KV head, block): the values its codes stand
+// for, the tail's f16 values of the block that is not whole, zeros past `end`.
+template <typename T>
+__global__ __launch_bounds__(256) void kv8_read_kernel(KvMoveArgs a) {
+    __shared__ Stage st;
+    const int kvh = blockIdx.x;
+    const int b = a.p0 / kKv8Block + (int)blockIdx.y;
+    const Kv8Head h = kv8_head(a.mem, a.layer, kvh);
+    const int end = *h.end;
+    const int rows = max(0, min(end - b * kKv8Block, kKv8Block));
+    stage_held(st, h, b, rows, rows < kKv8Block);
+    __syncthreads();
+    const int lo = max(a.p0, b * kKv8Block), hi = min(a.p0 + a.tokens, (b + 1) * kKv8Block);
+    const int lane = threadIdx.x & 127;
+    for (int p = lo + ((int)threadIdx.x >> 7); p < hi; p += 2) {
+        const int r = p - b * kKv8Block;
+        const size_t at = ((size_t)(p - a.p0) * a.kv_heads + kvh) * kHeadDim + lane;
+        static_cast<T*>(a.keys)[at] = r < rows ? (T)st.k[r][lane] : (T)0.f;
+        static_cast<T*>(a.values)[at] = r < rows ? (T)st.v[r][lane] : (T)0.f;
+    }
+}
+
+// An f16 cache's rows ([kv_head][token][128]), in and out. Grid (KV head, tokens in turn).
+template <typename T>
+__global__ __launch_bounds__(128) void kv16_write_kernel(KvMoveArgs a) {
+    const int kvh = blockIdx.x, d = threadIdx.x;
+    for (int t = blockIdx.y; t < a.tokens; t += gridDim.y) {
+        const size_t to = (size_t)a.layer * a.mem.layer_elems + ((size_t)kvh * a.mem.capacity + (size_t)(a.p0 + t)) * kHeadDim + d;
+        const size_t at = ((size_t)t * a.kv_heads + kvh) * kHeadDim + d;
+        reinterpret_cast<_Float16*>(a.mem.keys)[to] = (_Float16)static_cast<const T*>(a.keys)[at];
+        reinterpret_cast<_Float16*>(a.mem.values)[to] = (_Float16)static_cast<const T*>(a.values)[at];
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(128) void kv16_read_kernel(KvMoveArgs a) {
+    const int kvh = blockIdx.x, d = threadIdx.x;
+    for (int t = blockIdx.y; t < a.tokens; t += gridDim.y) {
+        const size_t from = (size_t)a.layer * a.mem.layer_elems + ((size_t)kvh * a.mem.capacity + (size_t)(a.p0 + t)) * kHeadDim + d;
+        const size_t at = ((size_t)t * a.kv_heads + kvh) * kHeadDim + d;
+        static_cast<T*>(a.keys)[at] = (T)reinterpret_cast<const _Float16*>(a.mem.keys)[from];
+        static_cast<T*>(a.values)[at] = (T)reinterpret_cast<const _Float16*>(a.mem.values)[from];
+    }
+}
+
+struct CacheInit {
+    double table[kHeadDim / 2 + 1];
+    double* table_dst;
+    char* regions;
+    size_t stride;  // bytes a region
+    size_t codes;   // its code bytes, left as they are
+};
+
+__global__ __launch_bounds__(256) void cache_init_kernel(CacheInit a) {
+    const int tid = threadIdx.x;
+    if (blockIdx.x == 0 && tid <= kHeadDim / 2) a.table_dst[tid] = a.table[tid];
+    if (a.regions == nullptr) return;
+    uint4* p = reinterpret_cast<uint4*>(a.regions + (size_t)blockIdx.x * a.stride + a.codes);
+    for (size_t i = tid; i < (a.stride - a.codes) / sizeof(uint4); i += 256) p[i] = make_uint4(0, 0, 0, 0);
+}
+
+// ---------------------------------------------------------- decode attention
+//
+// kv8_attn_kernel: one layer's attention of decode members over what their
+// caches hold (the append is a launch of its own before it), on the f16 matrix
+// cores: the cache's values are f16 exactly, and 128 query heads' worth of
+// products a byte would leave the VALU behind the memory.
+//
+// Split as attn_decode_kernel's: grid (chunk, KV head, member), a chunk one
+// contiguous run of whole blocks; its waves take the blocks in turn. A block is
+// 8 KB of codes, eight 16-byte loads a lane, each of them contiguous over
+// the wave (the codes lie in that order), kRing blocks in flight a wave.
+//
+// S^T = K Q^T (v_mfma_f32_16x16x32_f16: M = 16 keys, N = 16 columns, K = 32
+// dims): the columns are the QPK query heads of the KV head twice, the upper
+// f16 piece of each in columns 0..7 and the lower one in 8..15, so one product
+// carries 22 bits of q and the two halves of a score are one row rotation apart.
+// Row 4g + i of tile t is key 8g + 4t + i: lane group g ends up with eight
+// consecutive keys, which is the B operand's share of O^T += V^T P^T (M = 16
+// dims, K = 32 keys), the probabilities again in two pieces by column half.
+// Codes enter the scores as whole numbers, the block's key scale being applied to
+// the f32 score; values are scaled as f16 (both exact). The running maximum is
+// the column's and moves only when a score passes it by 2^kLazy (attn_prefill_kernel
+// does the same); denominators are f32 sums of f32 probabilities.
+constexpr float kLazy = 15.0f;
+constexpr int kRing = 2;
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+
+constexpr int kMinChunk = 128;  // a block a wave
+constexpr int kMinChunkWide = 256;
+constexpr int kBitLaneMembers = 8;
+int kv8_min_chunk(int members) { return members > kBitLaneMembers ? kMinChunkWide : kMinChunk; }
+
+__device__ __forceinline__ int kv8_chunk_tokens(int tokens, int chunks, int min_chunk) {
+    const int len = max((tokens + chunks - 1) / chunks, min_chunk);
+    return (len + kKv8Block - 1) / kKv8Block * kKv8Block;
+}
+
+// The value of lane ^ 8.
+__device__ __forceinline__ float other_half(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x128, 0xf, 0xf, false));
+}
+
+typedef float kv8_float4 __attribute__((ext_vector_type(4)));
+
+template <int QPK>
+__global__ __launch_bounds__(kThreads) void kv8_attn_kernel(AttnArgs a) {
+    __shared__ __attribute__((aligned(16))) _Float16 qs[2][QPK][kRowHalfs];
+    __shared__ float qfac[QPK];
+    __shared__ float2 st_ml[kWaves][QPK];
+    __shared__ float st_o[kWaves][QPK][kHeadDim];
+
+    const int chunk = blockIdx.x;
+    const int kvh = blockIdx.y;
+    const int m = blockIdx.z;
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4;
+    const int n = lane & 15;
+    const AttnMember mb = a.mem[m];
+    const int pos = a.positions[m];
+    const Kv8Head head = kv8_head(mb, a.layer, kvh);
+    const int end = *head.end;
+    // (an append past the capacity was dropped: nothing past `end` is read)
+    const int tokens = min(pos + 1, end);
+    const int len = kv8_chunk_tokens(tokens, a.chunks, a.min_chunk);
+    const int t0 = chunk * len;
+    if (t0 >= tokens) return;
+    const int t1 = min(t0 + len, tokens);
+
+    // ---- blocks of this wave: b0 + wave, + kWaves, ... below `coded`; the block
+    // that is not whole, if the chunk reaches it, is the last wave's first
+    const int b0 = t0 / kKv8Block;
+    const int coded = min((t1 + kKv8Block - 1) / kKv8Block, end / kKv8Block);
+    const bool tail = t1 > coded * kKv8Block && wave == kWaves - 1;
+    const __amdgpu_buffer_rsrc_t cr = make_rsrc(head.codes, (uint32_t)kv8_tail_offset(mb.capacity));
+    const __amdgpu_buffer_rsrc_t sr = make_rsrc(head.scales, (uint32_t)(kv8_blocks(mb.capacity) * sizeof(float2)));
+    uint4 kq[kRing][4], vq[kRing][4];
+    float2 sc[kRing];
+    auto issue = [&](int r, int b) {
+        const uint32_t at = b < coded ? (uint32_t)b * kKv8BlockBytes + 16u * (uint32_t)lane : kOOR;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kq[r][i] = load_b128(cr, at + 1024u * i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vq[r][i] = load_b128(cr, at + kKv8PartBytes + 1024u * i);
+        sc[r] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(sr, (int)(b < coded ? 8u * (uint32_t)b : kOOR), 0, 0));
+    };
+#pragma unroll
+    for (int r = 0; r < kRing; ++r) issue(r, b0 + wave + kWaves * r);
+    kv8_half8 tk[8], tv[8];
+    if (tail) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {  // keys (t, s), values (u, i)
+            tk[i] = *reinterpret_cast<const kv8_half8*>(head.tail_k + kv8_key_row(i >> 2, n) * kHeadDim + 64 * ((i >> 1) & 1) + 16 * g + 8 * (i & 1));
+            tv[i] = *reinterpret_cast<const kv8_half8*>(head.tail_v + (32 * (i >> 1) + 2 * n + (i & 1)) * kKv8Block + 8 * g);
+        }
+    }
+
+    // ---- query heads: norm and rope, scaled by a power of two to just below 2
+    // (whatever the norm's weights are, the pieces are in f16's range), in pieces
+    const Rot64 rot = table_rot(mb.rope, 64, lane, pos);
+    const float rc = (float)rot.c, rs = (float)rot.s;
+    const float* qm = a.q + ((size_t)m * a.q_heads + (size_t)kvh * QPK) * kHeadDim;
+    for (int h = wave; h < QPK; h += kWaves) {
+        const float x0 = qm[h * kHeadDim + lane], x1 = qm[h * kHeadDim + 64 + lane];
+        const float ssq = wave_sum(x0 * x0 + x1 * x1);
+        const float inv = 1.0f / sqrtf(ssq / (float)kHeadDim + a.eps);
+        const float y0 = x0 * inv * a.q_norm[lane], y1 = x1 * inv * a.q_norm[lane + 64];
+        const float q0 = y0 * rc - y1 * rs, q1 = y0 * rs + y1 * rc;
+        float top = fmaxf(fabsf(q0), fabsf(q1));
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+        const int e = max(-100, min(100, (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127));
+        const float p0 = q0 * kv8_power(-e), p1 = q1 * kv8_power(-e);
+        qs[0][h][lane] = (_Float16)p0;
+        qs[0][h][lane + 64] = (_Float16)p1;
+        qs[1][h][lane] = (_Float16)(p0 - (float)(_Float16)p0);
+        qs[1][h][lane + 64] = (_Float16)(p1 - (float)(_Float16)p1);
+        if (lane == 0) qfac[h] = a.scale * kv8_power(e);
+    }
+    __syncthreads();
+    const int hn = n & 7;
+    kv8_half8 qb[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        qb[s] = kv8_half8{};
+        if (hn < QPK) qb[s] = *reinterpret_cast<const kv8_half8*>(&qs[n >> 3][hn][64 * (s >> 1) + 16 * g + 8 * (s & 1)]);
+    }
+    const float fac = hn < QPK ? qfac[hn] : 0.f;
+
+    float mrun = -FLT_MAX, lrun = 0.f;
+    kv8_float4 o[8];
+#pragma unroll
+    for (int d = 0; d < 8; ++d) o[d] = kv8_float4{0.f, 0.f, 0.f, 0.f};
+
+    // Scores of a block's two key tiles to probabilities in pieces (s in f32, `scaled` by the key scale).
+    auto soften = [&](kv8_float4 (&s)[2], float scaled, int b, kv8_half8& pb) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = (s[j >> 2][j & 3] + other_half(s[j >> 2][j & 3])) * scaled;
+        if (b * kKv8Block + kKv8Block > tokens) {  // keys past the member's position
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (b * kKv8Block + 8 * g + j >= tokens) x[j] = -INFINITY;
+        }
+        float top = x[0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
+        if (__any(top > mrun + kLazy)) {
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float mn = top > mrun + kLazy ? top : mrun;
+            const float corr = __builtin_amdgcn_exp2f(mrun - mn);
+            mrun = mn;
+            lrun *= corr;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) o[d] *= corr;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(x[j] - mrun), p1 = __builtin_amdgcn_exp2f(x[j + 1] - mrun);
+            lrun += p0;
+            lrun += p1;
+            const auto hi = __builtin_amdgcn_cvt_pkrtz(p0, p1);
+            const auto lo = __builtin_amdgcn_cvt_pkrtz(p0 - (float)hi[0], p1 - (float)hi[1]);
+            const uint32_t hw = __builtin_bit_cast(uint32_t, hi), lw = __builtin_bit_cast(uint32_t, lo);
+            const kv8_half2 p = __builtin_bit_cast(kv8_half2, n < 8 ? hw : lw);
+            pb[j] = p[0];
+            pb[j + 1] = p[1];
+        }
+    };
+
+    if (tail) {
+        kv8_float4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(tk[4 * t + i], qb[i], s[t], 0, 0, 0);
+        kv8_half8 pb;
+        soften(s, fac, end / kKv8Block, pb);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(tv[d], pb, o[d], 0, 0, 0);
+    }
+    for (int b = b0 + wave; b < coded; b += kWaves * kRing) {
+#pragma unroll
+        for (int r = 0; r < kRing; ++r) {
+            const int bb = b + kWaves * r;
+            if (bb < coded) {
+                kv8_float4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const uint4 w = kq[r][2 * t + (i >> 1)];
+                        const kv8_half8 k = (i & 1) ? kv8_whole(w.z, w.w) : kv8_whole(w.x, w.y);
+                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qb[i], s[t], 0, 0, 0);
+                    }
+                }
+                const _Float16 vs = (_Float16)sc[r].y;
+                kv8_half8 pb;
+                soften(s, fac * sc[r].x, bb, pb);
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {
+                    const uint4 w = vq[r][d >> 1];
+                    const kv8_half8 v = (d & 1) ? kv8_values(w.z, w.w, vs) : kv8_values(w.x, w.y, vs);
+                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pb, o[d], 0, 0, 0);
+                }
+            }
+            issue(r, bb + kWaves * kRing);
+        }
+    }
+
+    // ---- the waves' states meet in LDS: the chunk's partial in attn_decode_kernel's layout
+    lrun += __shfl_xor(lrun, 16, 64);
+    lrun += __shfl_xor(lrun, 32, 64);
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float v = o[d][i] + other_half(o[d][i]);
+            if (n < QPK) st_o[wave][n][32 * (d >> 1) + 2 * (4 * g + i) + (d & 1)] = v;
+        }
+    }
+    if (g == 0 && n < QPK) st_ml[wave][n] = make_float2(mrun, lrun);
+    __syncthreads();
+    float* const own = a.partials != nullptr ? a.partials + (size_t)m * a.partial_floats : mb.partials;
+    for (int i = tid; i < QPK * kHeadDim; i += kThreads) {
+        const int h = i >> 7, d = i & 127;
+        float mx = -FLT_MAX;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, st_ml[w][h].x);
+        float l = 0.f, acc = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(st_ml[w][h].x - mx);
+            l = __builtin_fmaf(st_ml[w][h].y, f, l);
+            acc = __builtin_fmaf(st_o[w][h][d], f, acc);
+        }
+        float* part = own + ((size_t)(kvh * QPK + h) * kAttnChunks + chunk) * kPartStride;
+        part[d] = acc;
+        if (d == 0) {
+            part[kHeadDim] = mx;
+            part[kHeadDim + 1] = l;
+        }
+    }
+}
+
+// The chunks' partials of a (query head, member) merged in chunk order. A
+// member without tokens (a negative position) gets zeros.
+__global__ __launch_bounds__(kHeadDim) void kv8_combine_kernel(AttnArgs a) {
+    const int qh = blockIdx.x;
+    const int m = blockIdx.y;
+    const int d = threadIdx.x;
+    const AttnMember mb = a.mem[m];
+    const int end = *kv8_head(mb, a.layer, qh / (a.q_heads / a.kv_heads)).end;
+    const int tokens = min(a.positions[m] + 1, end);
+    const int len = kv8_chunk_tokens(tokens, a.chunks, a.min_chunk);
+    const int chunks = tokens > 0 ? (tokens + len - 1) / len : 0;
+    const float* part = (a.partials != nullptr ? a.partials + (size_t)m * a.partial_floats : mb.partials) +
+                        (size_t)qh * kAttnChunks * kPartStride;
+    float mx = -FLT_MAX;
+    for (int c = 0; c < chunks; ++c) mx = fmaxf(mx, part[c * kPartStride + kHeadDim]);
+    float l = 0.f, acc = 0.f;
+    for (int c = 0; c < chunks; ++c) {
+        const float f = __builtin_amdgcn_exp2f(part[c * kPartStride + kHeadDim] - mx);
+        l = __builtin_fmaf(part[c * kPartStride + kHeadDim + 1], f, l);
+        acc = __builtin_fmaf(part[c * kPartStride + d], f, acc);
+    }
+    a.out[((size_t)m * a.q_heads + qh) * kHeadDim + d] = chunks > 0 ? acc / l : 0.f;
+}
+
+}  // namespace
+
+int kv8_grid_chunks(int max_capacity, int members) {
+    const int min_chunk = kv8_min_chunk(members);
+    return std::max(1, std::min(kAttnChunks, (max_capacity + min_chunk - 1) / min_chunk));
+}
+
+hipError_t launch_cache_init(void* regions, size_t count, int capacity, const double* table, double* table_dst,
+                             hipStream_t stream) {
+    CacheInit a;
+    std::copy(table, table + kHeadDim / 2 + 1, a.table);
+    a.table_dst = table_dst;
+    a.regions = static_cast<char*>(regions);
+    a.stride = kv8_head_bytes(capacity);
+    a.codes = kv8_tail_offset(capacity);
+    hipLaunchKernelGGL(cache_init_kernel, dim3(regions != nullptr ? (unsigned)count : 1u), dim3(256), 0, stream, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv8_append(const AttnArgs& a, int members, hipStream_t stream) {
+    if (members < 1 || members > kAttnMaxMembers || a.kv_heads < 1 || a.mem == nullptr) return hipErrorInvalidValue;
+    // consecutive positions touch at most one block more than they fill
+    const int blocks = (members + kKv8Block - 2) / kKv8Block + 1;
+    hipLaunchKernelGGL(kv8_append_kernel, dim3((unsigned)a.kv_heads, (unsigned)(a.appended ? blocks : members)), dim3(256), 0,
+                       stream, a, a.appended ? members : 0);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv8_append_seq(const PrefillAttnArgs& a, hipStream_t stream) {
+    if (a.tokens < 1 || a.kv_heads < 1 || a.p0 < 0 || (long long)a.p0 + a.tokens > a.mem.capacity) return hipErrorInvalidValue;
+    const int blocks = (a.p0 + a.tokens - 1) / kKv8Block - a.p0 / kKv8Block + 1;
+    hipLaunchKernelGGL(kv8_append_seq_kernel, dim3((unsigned)a.kv_heads, (unsigned)blocks), dim3(256), 0, stream, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv8_attention(const AttnArgs& args, int members, hipStream_t stream) {
+    if (members < 1 || members > kAttnMaxMembers || args.kv_heads < 1 || args.q_heads % args.kv_heads != 0 ||
+        args.chunks < 1 || args.chunks > kAttnChunks || args.mem == nullptr) {
+        return hipErrorInvalidValue;
+    }
+    AttnArgs b = args;
+    b.min_chunk = kv8_min_chunk(members);
+    const dim3 grid((unsigned)b.chunks, (unsigned)b.kv_heads, (unsigned)members);
+    switch (b.q_heads / b.kv_heads) {
+    case 1: hipLaunchKernelGGL(kv8_attn_kernel<1>, grid, dim3(kThreads), 0, stream, b); break;
+    case 2: hipLaunchKernelGGL(kv8_attn_kernel<2>, grid, dim3(kThreads), 0, stream, b); break;
+    case 4: hipLaunchKernelGGL(kv8_attn_kernel<4>, grid, dim3(kThreads), 0, stream, b); break;
+    case 8: hipLaunchKernelGGL(kv8_attn_kernel<8>, grid, dim3(kThreads), 0, stream, b); break;
+    default: return hipErrorInvalidValue;
+    }
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kv8_combine_kernel, dim3((unsigned)b.q_heads, (unsigned)members), dim3(kHeadDim), 0, stream, b);
+    return hipGetLastError();
+}
+
+namespace {
+bool move_fits(const KvMoveArgs& a) {
+    return a.tokens >= 1 && a.kv_heads >= 1 && a.p0 >= 0 && (long long)a.p0 + a.tokens <= a.mem.capacity && a.mem.keys != nullptr;
+}
+dim3 move_grid(const KvMoveArgs& a, bool kv8) {
+    const int blocks = (a.p0 + a.tokens - 1) / kKv8Block - a.p0 / kKv8Block + 1;
+    return dim3((unsigned)a.kv_heads, (unsigned)(kv8 ? blocks : std::min(a.tokens, 32768)));
+}
+}  // namespace
+
+hipError_t launch_kv_write(const KvMoveArgs& a, bool half, bool kv8, hipStream_t stream) {
+    if (!move_fits(a)) return hipErrorInvalidValue;
+    const dim3 grid = move_grid(a, kv8);
+    if (kv8 && half) hipLaunchKernelGGL(kv8_write_kernel<kRowsF16>, grid, dim3(256), 0, stream, a);
+    else if (kv8) hipLaunchKernelGGL(kv8_write_kernel<kRowsF32>, grid, dim3(256), 0, stream, a);
+    else if (half) hipLaunchKernelGGL(kv16_write_kernel<_Float16>, grid, dim3(128), 0, stream, a);
+    else hipLaunchKernelGGL(kv16_write_kernel<float>, grid, dim3(128), 0, stream, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_read(const KvMoveArgs& a, bool half, bool kv8, hipStream_t stream) {
+    if (!move_fits(a)) return hipErrorInvalidValue;
+    const dim3 grid = move_grid(a, kv8);
+    if (kv8 && half) hipLaunchKernelGGL(kv8_read_kernel<_Float16>, grid, dim3(256), 0, stream, a);
+    else if (kv8) hipLaunchKernelGGL(kv8_read_kernel<float>, grid, dim3(256), 0, stream, a);
+    else if (half) hipLaunchKernelGGL(kv16_read_kernel<_Float16>, grid, dim3(128), 0, stream, a);
+    else hipLaunchKernelGGL(kv16_read_kernel<float>, grid, dim3(128), 0, stream, a);
+    return hipGetLastError();
+}
+
+}  // namespace ribn_amd

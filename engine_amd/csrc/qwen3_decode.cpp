@@ -40,7 +40,9 @@
 #include "abi_internal.hpp"
 #include "decode_launch.hpp"
 #include "kquant_launch.hpp"
+#include "kv8.hpp"
 #include "qwen3_internal.hpp"
+#include "rope.hpp"
 
 using namespace ribn_amd_abi;
 
@@ -50,10 +52,12 @@ struct ribn_amd_kv_cache {
     uint64_t id;  // distinguishes caches in captured-graph keys
     ribn_amd_qwen3_config cfg;
     uint32_t capacity;
-    size_t layer_elems;  // kv_heads * capacity * head_dim
-    void* block;         // one allocation: keys, values, partials
-    uint16_t* keys;      // [layers][kv_heads][capacity][head_dim]
-    uint16_t* values;
+    int kind;            // ribn_amd::kCache*: format, and whether it has a rotary table
+    size_t layer_elems;  // f16: kv_heads * capacity * head_dim; 8 bits: a layer's bytes
+    void* block;         // one allocation: keys, values, partials, rotary table
+    uint16_t* keys;      // f16 [layers][kv_heads][capacity][head_dim]; 8 bits: regions [layers][kv_heads] (kv8.hpp)
+    uint16_t* values;    // f16
+    const double* rope;  // rotary table, or null
     float* partials;     // attention partials of the standalone attention call
 };
 
@@ -73,9 +77,10 @@ struct GraphKey {
     bool advance;
     bool appended;
     int chunks;
+    int cache;  // ribn_amd::kCache*
     bool operator==(const GraphKey& o) const {
         return members == o.members && head == o.head && advance == o.advance && appended == o.appended &&
-               chunks == o.chunks;
+               chunks == o.chunks && cache == o.cache;
     }
 };
 
@@ -129,6 +134,27 @@ bool same_geometry(const ribn_amd_qwen3_config& a, const ribn_amd_qwen3_config& 
     return a.layers == b.layers && a.q_heads == b.q_heads && a.kv_heads == b.kv_heads && a.head_dim == b.head_dim;
 }
 
+// A cache of a call: one kind for all of them (`first`'s), and a rotary table
+// made for the call's rope base.
+ribn_amd_status check_kind(const ribn_amd_kv_cache* cache, const ribn_amd_kv_cache* first, const ribn_amd_qwen3_config& cfg,
+                           size_t member) {
+    if (cache->kind != first->kind) {
+        return fail(RIBN_AMD_INVALID_PLAN, (uint64_t)first->kind, (uint64_t)cache->kind,
+                    "member %zu's cache has another format than member 0's, or only one of them a rope of its own", member);
+    }
+    if (cache->rope != nullptr && cache->cfg.rope_base != cfg.rope_base) {
+        return fail(RIBN_AMD_INVALID_PLAN, 0, 0, "member %zu's cache was made for rope base %g, not %g", member,
+                    (double)cache->cfg.rope_base, (double)cfg.rope_base);
+    }
+    return RIBN_AMD_OK;
+}
+
+// Attention grid of a launch over caches of one kind.
+int grid_chunks(int kind, int max_capacity, int members) {
+    return kind == ribn_amd::kCacheI8 ? ribn_amd::kv8_grid_chunks(max_capacity, members)
+                                      : ribn_amd::attn_grid_chunks(max_capacity, members);
+}
+
 }  // namespace
 
 struct ribn_amd_qwen3_decode {
@@ -158,6 +184,7 @@ struct ribn_amd_qwen3_decode {
     float* partials;      // [members][attention partials]
     uint64_t* argmax_part;  // [members][kArgmaxSlices] slice results of the greedy selection
     int chunks;           // attention grid of the next step (from its caches' capacities)
+    int cache;            // their kind
     hipStream_t capture;  // private stream for graph capture
     bool graphs;
     uint32_t gemv_mode;   // RIBN_AMD_GEMV_WARP (f32 activations) or RIBN_AMD_GEMV_FIXED16
@@ -259,7 +286,7 @@ hipError_t wave_shared(const ribn_amd_qwen3_decode* d, const ribn_amd_quantized_
 // With `partials` set, member m's attention partials live at partials +
 // m * attn_partials_floats (the decoder's own buffer, whose address the merge
 // launch then takes from its arguments); else in the descriptors.
-hipError_t attention(const ribn_amd_qwen3_config& cfg, const ribn_amd::AttnMember* mem, int chunks, bool appended,
+hipError_t attention(const ribn_amd_qwen3_config& cfg, const ribn_amd::AttnMember* mem, int kind, int chunks, bool appended,
                      int members, uint32_t layer, const float* q, const float* k, const float* v, const float* q_norm,
                      const float* k_norm, const int32_t* positions, float* out, float* partials, hipStream_t stream) {
     const size_t part = ribn_amd::attn_partials_floats((int)cfg.q_heads);
@@ -287,9 +314,15 @@ hipError_t attention(const ribn_amd_qwen3_config& cfg, const ribn_amd::AttnMembe
         a.rope_base = cfg.rope_base;
         // softmax weights are exp2 of scores in log2 units: e^x = 2^(x log2 e)
         a.scale = 1.4426950408889634f / sqrtf((float)cfg.head_dim);
+        const bool table = kind == ribn_amd::kCacheF16Table;
         hipError_t e = hipSuccess;
-        if (appended) e = ribn_amd::launch_kv_append(a, mc, stream);
-        if (e == hipSuccess) e = ribn_amd::launch_attention(a, mc, stream);
+        if (kind == ribn_amd::kCacheI8) {
+            e = ribn_amd::launch_kv8_append(a, mc, stream);
+            if (e == hipSuccess) e = ribn_amd::launch_kv8_attention(a, mc, stream);
+        } else {
+            if (appended) e = ribn_amd::launch_kv_append(a, mc, stream, table);
+            if (e == hipSuccess) e = ribn_amd::launch_attention(a, mc, stream, table);
+        }
         if (e != hipSuccess) return e;
     }
     // appended members in position order: a member reads only earlier
@@ -317,7 +350,7 @@ hipError_t enqueue_step(ribn_amd_qwen3_decode* d, const GraphKey& key, hipStream
         float* qkv_out[3] = {d->q, d->k, d->v};
         e = wave_shared(d, qkv, qkv_out, 3, d->hidden, L.attn_norm, members, stream, &pending);
         if (e != hipSuccess) return e;
-        e = attention(c, d->members_dev, key.chunks, key.appended, members, l, d->q, d->k, d->v, L.attn_q_norm,
+        e = attention(c, d->members_dev, key.cache, key.chunks, key.appended, members, l, d->q, d->k, d->v, L.attn_q_norm,
                       L.attn_k_norm, d->positions, d->attn, d->partials, stream);
         if (e != hipSuccess) return e;
         e = wave(d, &L.attn_output, 1, d->attn, nullptr, nullptr, &d->hidden, members, true, stream, false, nullptr,
@@ -372,7 +405,7 @@ void destroy_graphs(ribn_amd_qwen3_decode* d) {
 // are off.
 ribn_amd_status run_step(ribn_amd_qwen3_decode* d, int members, bool head, bool advance, bool appended = false) {
     hipStream_t stream = d->ctx->stream;
-    const GraphKey key{members, head, advance, appended, d->chunks};
+    const GraphKey key{members, head, advance, appended, d->chunks, d->cache};
     if (!d->graphs) {
         hipError_t e = enqueue_step(d, key, stream);
         return e == hipSuccess ? ok() : driver(e, "launch decode step");
@@ -458,6 +491,8 @@ ribn_amd_status check_members(const ribn_amd_qwen3_decode* d, ribn_amd_kv_cache*
         if (!same_geometry(c->cfg, d->cfg)) {
             return fail(RIBN_AMD_INVALID_PLAN, 0, 0, "member %zu's cache has another layer or head geometry", m);
         }
+        const ribn_amd_status kind = check_kind(c, caches[0], d->cfg, m);
+        if (kind != RIBN_AMD_OK) return kind;
         for (size_t o = 0; o < m && !shared; ++o) {
             if (caches[o] == c) return fail(RIBN_AMD_INVALID_PLAN, o, m, "members %zu and %zu share a cache", o, m);
         }
@@ -480,6 +515,7 @@ ribn_amd::AttnMember descriptor(const ribn_amd_kv_cache* c, float* partials) {
     m.values = c->values;
     m.partials = partials;
     m.layer_elems = c->layer_elems;
+    m.rope = c->rope;
     m.capacity = (int)c->capacity;
     return m;
 }
@@ -507,7 +543,8 @@ ribn_amd_status upload_step(ribn_amd_qwen3_decode* d, ribn_amd_kv_cache* const* 
         hipError_t e = ribn_amd::launch_step_inputs(in, d->ctx->stream);
         if (e != hipSuccess) return driver(e, "upload step inputs");
     }
-    d->chunks = ribn_amd::attn_grid_chunks(max_capacity, (int)members);
+    d->cache = caches[0]->kind;
+    d->chunks = grid_chunks(d->cache, max_capacity, (int)members);
     return ok();
 }
 
@@ -609,7 +646,7 @@ hipError_t enqueue_prompt_chunk(ribn_amd_qwen3_decode* d, ribn_amd_kv_cache* cac
         a.eps = c.epsilon;
         a.rope_base = c.rope_base;
         a.scale = 1.4426950408889634f / sqrtf((float)c.head_dim);
-        e = ribn_amd::launch_prefill_attention(a, d->ctx->cu_count, stream);
+        e = ribn_amd::launch_prefill_attention(a, d->ctx->cu_count, stream, cache->kind);
         if (e != hipSuccess || last) break;
         e = ribn_amd::launch_act_f16(false, d->p_attn, nullptr, 0.f, tokens, qdim, d->p_gemm, stream);
         if (e == hipSuccess) e = prompt_gemm(d, L.attn_output, d->p_y, tokens, stream);
@@ -698,6 +735,19 @@ ribn_amd_status copy_selected_async(ribn_amd_qwen3_decode* d, size_t member, uin
     return e == hipSuccess ? ok() : driver(e, "copy selected token into pinned memory");
 }
 
+ribn_amd_status check_kv_options(const ribn_amd_kv_options* o) {
+    if (o == nullptr) return RIBN_AMD_OK;
+    if (o->format > RIBN_AMD_KV_I8) return fail(RIBN_AMD_INVALID_ARGUMENT, RIBN_AMD_KV_I8, o->format, "unknown cache format %u", o->format);
+    if (o->rope == nullptr) return RIBN_AMD_OK;
+    const ribn_amd_status st = check_rope_spec(o->rope);
+    if (st != RIBN_AMD_OK) return st;
+    if (o->rope->layout != RIBN_AMD_ROPE_HALF || o->rope->rotary_dim != o->rope->head_dim || o->rope->head_dim != (uint32_t)ribn_amd::kHeadDim) {
+        return fail(RIBN_AMD_INVALID_PLAN, ribn_amd::kHeadDim, o->rope->rotary_dim,
+                    "a cache's rope has the half layout over whole heads of %d", ribn_amd::kHeadDim);
+    }
+    return RIBN_AMD_OK;
+}
+
 ribn_amd_context* context(const ribn_amd_qwen3_decode* d) { return d->ctx; }
 uint32_t max_members(const ribn_amd_qwen3_decode* d) { return d->max_members; }
 const ribn_amd_qwen3_config& config(const ribn_amd_qwen3_decode* d) { return d->cfg; }
@@ -708,36 +758,69 @@ extern "C" {
 
 ribn_amd_status ribn_amd_kv_cache_create(ribn_amd_context* ctx, const ribn_amd_qwen3_config* config,
                                          uint32_t capacity, ribn_amd_kv_cache** out) {
+    return ribn_amd_kv_cache_create_with(ctx, config, capacity, nullptr, out);
+}
+
+ribn_amd_status ribn_amd_kv_cache_create_with(ribn_amd_context* ctx, const ribn_amd_qwen3_config* config,
+                                              uint32_t capacity, const ribn_amd_kv_options* options,
+                                              ribn_amd_kv_cache** out) {
     if (!ctx || !out) return fail(RIBN_AMD_INVALID_ARGUMENT, 0, 0, "null argument");
     ribn_amd_status st = check_config(config);
+    if (st == RIBN_AMD_OK) st = ribn_amd_decode::check_kv_options(options);
     if (st != RIBN_AMD_OK) return st;
     if (capacity == 0 || capacity > (1u << 20)) {
         return fail(RIBN_AMD_INVALID_PLAN, 1u << 20, capacity, "KV capacity must be 1..%u tokens", 1u << 20);
     }
-    const size_t layer_elems = (size_t)config->kv_heads * capacity * config->head_dim;
-    const size_t cache_bytes = align_up(layer_elems * config->layers * sizeof(uint16_t));
+    const bool i8 = options != nullptr && options->format == RIBN_AMD_KV_I8;
+    const ribn_amd_rope_spec* rope = options != nullptr ? options->rope : nullptr;
+    const bool table = i8 || rope != nullptr;
+    const size_t layer_elems = i8 ? config->kv_heads * ribn_amd::kv8_head_bytes((int)capacity)
+                                  : (size_t)config->kv_heads * capacity * config->head_dim;
+    const size_t cache_bytes = i8 ? layer_elems * config->layers : align_up(layer_elems * config->layers * sizeof(uint16_t));
+    const size_t held_bytes = i8 ? cache_bytes : 2 * cache_bytes;
     const size_t part_bytes = align_up(ribn_amd::attn_partials_floats((int)config->q_heads) * sizeof(float));
+    double turns[ribn_amd::kRopeTableMax];
+    size_t table_bytes = 0;
+    if (table) {
+        ribn_amd_rope_spec plain{};
+        plain.layout = RIBN_AMD_ROPE_HALF;
+        plain.head_dim = plain.rotary_dim = config->head_dim;
+        plain.base = config->rope_base;
+        if (rope == nullptr) {
+            st = check_rope_spec(&plain);
+            if (st != RIBN_AMD_OK) return st;
+            rope = &plain;
+        }
+        table_bytes = (size_t)rope_table(*rope, turns) * sizeof(double);
+    }
     DeviceGuard guard(ctx->device);
     void* block = nullptr;
-    hipError_t e = hipMalloc(&block, 2 * cache_bytes + part_bytes);
+    hipError_t e = hipMalloc(&block, held_bytes + part_bytes + table_bytes);
     if (e != hipSuccess) return driver(e, "hipMalloc KV cache");
     char* p = static_cast<char*>(block);
-    auto* c = new (std::nothrow) ribn_amd_kv_cache{};
+    if (table) {
+        // stream-ordered, from kernel arguments: a cache is made while earlier work runs
+        e = ribn_amd::launch_cache_init(i8 ? p : nullptr, (size_t)config->layers * config->kv_heads, (int)capacity, turns,
+                                        reinterpret_cast<double*>(p + held_bytes + part_bytes), ctx->stream);
+    }
+    auto* c = e == hipSuccess ? new (std::nothrow) ribn_amd_kv_cache{} : nullptr;
     if (!c) {
         hipFree(block);
-        return fail(RIBN_AMD_DRIVER, 0, 0, "host allocation failed");
+        return e != hipSuccess ? driver(e, "set up KV cache") : fail(RIBN_AMD_DRIVER, 0, 0, "host allocation failed");
     }
     c->ctx = ctx;
     c->device = ctx->device;
     c->id = g_cache_ids.fetch_add(1);
     c->cfg = *config;
     c->capacity = capacity;
+    c->kind = i8 ? ribn_amd::kCacheI8 : table ? ribn_amd::kCacheF16Table : ribn_amd::kCacheF16;
     c->layer_elems = layer_elems;
     c->block = block;
     c->keys = reinterpret_cast<uint16_t*>(p);
-    c->values = reinterpret_cast<uint16_t*>(p + cache_bytes);
-    c->partials = reinterpret_cast<float*>(p + 2 * cache_bytes);
-    // nothing is cleared: a position is written before it is read, and every
+    c->values = i8 ? nullptr : reinterpret_cast<uint16_t*>(p + cache_bytes);
+    c->partials = reinterpret_cast<float*>(p + held_bytes);
+    c->rope = table ? reinterpret_cast<const double*>(p + held_bytes + part_bytes) : nullptr;
+    // nothing else is cleared: a position is written before it is read, and every
     // partial is written before the merge reads it
     context_retain(ctx);  // released by ribn_amd_kv_cache_destroy, like every other handle's
     *out = c;
@@ -757,11 +840,98 @@ void ribn_amd_kv_cache_destroy(ribn_amd_kv_cache* cache) {
 
 uint32_t ribn_amd_kv_cache_capacity(const ribn_amd_kv_cache* cache) { return cache ? cache->capacity : 0; }
 
-ribn_amd_status ribn_amd_kv_cache_layer(ribn_amd_kv_cache* cache, uint32_t layer, uint16_t** keys, uint16_t** values) {
-    if (!cache || !keys || !values) return fail(RIBN_AMD_INVALID_ARGUMENT, 0, 0, "null argument");
+uint32_t ribn_amd_kv_cache_format(const ribn_amd_kv_cache* cache) {
+    return cache && cache->kind == ribn_amd::kCacheI8 ? RIBN_AMD_KV_I8 : RIBN_AMD_KV_F16;
+}
+
+uint64_t ribn_amd_kv_bytes(const ribn_amd_qwen3_config* c, uint32_t tokens, uint32_t format) {
+    if (!c || format > RIBN_AMD_KV_I8) return 0;
+    if (format == RIBN_AMD_KV_F16) return ribn_amd_qwen3_kv_bytes(c, tokens);
+    if (tokens > (1u << 20)) return 0;
+    return (uint64_t)c->layers * c->kv_heads * ribn_amd::kv8_head_bytes((int)tokens);
+}
+
+static ribn_amd_status check_layer(const ribn_amd_kv_cache* cache, uint32_t layer) {
     if (layer >= cache->cfg.layers) {
         return fail(RIBN_AMD_INVALID_PLAN, cache->cfg.layers, layer, "layer %u of a %u-layer cache", layer,
                     cache->cfg.layers);
+    }
+    return RIBN_AMD_OK;
+}
+
+ribn_amd_status ribn_amd_kv_cache_tail(ribn_amd_kv_cache* cache, uint32_t layer, uint16_t** keys, uint16_t** values,
+                                       size_t* head_stride) {
+    if (!cache || !keys || !values || !head_stride) return fail(RIBN_AMD_INVALID_ARGUMENT, 0, 0, "null argument");
+    const ribn_amd_status st = check_layer(cache, layer);
+    if (st != RIBN_AMD_OK) return st;
+    if (cache->kind != ribn_amd::kCacheI8) return fail(RIBN_AMD_UNSUPPORTED, RIBN_AMD_KV_I8, RIBN_AMD_KV_F16, "an f16 cache has no tail block");
+    char* region = reinterpret_cast<char*>(cache->keys) + (size_t)layer * cache->layer_elems;
+    *keys = reinterpret_cast<uint16_t*>(region + ribn_amd::kv8_tail_offset((int)cache->capacity));
+    *values = *keys + ribn_amd::kKv8TailElems;
+    *head_stride = ribn_amd::kv8_head_bytes((int)cache->capacity) / sizeof(uint16_t);
+    return ok();
+}
+
+static ribn_amd_status move_rows(ribn_amd_context* ctx, ribn_amd_kv_cache* cache, uint32_t layer, uint32_t position,
+                                 size_t tokens, void* keys, void* values, size_t len, uint32_t dtype, bool write) {
+    if (!ctx || !cache) return fail(RIBN_AMD_INVALID_ARGUMENT, 0, 0, "null argument");
+    ribn_amd_status st = check_layer(cache, layer);
+    if (st != RIBN_AMD_OK) return st;
+    if (dtype != RIBN_AMD_F32 && dtype != RIBN_AMD_F16) {
+        return fail(RIBN_AMD_INVALID_ARGUMENT, RIBN_AMD_F16, dtype, "cache rows are f32 or f16, not element type %u", dtype);
+    }
+    const uintptr_t size = dtype == RIBN_AMD_F16 ? 2 : 4;
+    st = check_device_ptr(ctx, keys, "keys", size);
+    if (st == RIBN_AMD_OK) st = check_device_ptr(ctx, values, "values", size);
+    if (st != RIBN_AMD_OK) return st;
+    if (cache->device != ctx->device) {
+        return fail(RIBN_AMD_CONTEXT_MISMATCH, (uint64_t)ctx->device, (uint64_t)cache->device,
+                    "the cache lives on device %d", cache->device);
+    }
+    if (tokens == 0) return fail(RIBN_AMD_INPUT_LENGTH, 1, 0, "at least one token is moved");
+    if (tokens > cache->capacity || (uint64_t)position + tokens > cache->capacity) {
+        return fail(RIBN_AMD_POSITION_OVERFLOW, cache->capacity, (uint64_t)position + tokens - 1,
+                    "token position %llu exceeds KV capacity %u", (unsigned long long)position + tokens - 1,
+                    cache->capacity);
+    }
+    const size_t want = tokens * cache->cfg.kv_heads * cache->cfg.head_dim;
+    if (len != want) {
+        return fail(write ? RIBN_AMD_INPUT_LENGTH : RIBN_AMD_OUTPUT_LENGTH, want, len,
+                    "keys and values have %zu values each, expected %zu", len, want);
+    }
+    DeviceGuard guard(ctx->device);
+    ribn_amd::KvMoveArgs a{};
+    a.mem = descriptor(cache, nullptr);
+    a.layer = (int)layer;
+    a.kv_heads = (int)cache->cfg.kv_heads;
+    a.p0 = (int)position;
+    a.tokens = (int)tokens;
+    a.keys = keys;
+    a.values = values;
+    const bool half = dtype == RIBN_AMD_F16, kv8 = cache->kind == ribn_amd::kCacheI8;
+    const hipError_t e = write ? ribn_amd::launch_kv_write(a, half, kv8, ctx->stream)
+                               : ribn_amd::launch_kv_read(a, half, kv8, ctx->stream);
+    return e == hipSuccess ? ok() : driver(e, write ? "cache write launch" : "cache read launch");
+}
+
+ribn_amd_status ribn_amd_kv_cache_write(ribn_amd_context* ctx, ribn_amd_kv_cache* cache, uint32_t layer,
+                                        uint32_t position, size_t tokens, const void* keys, const void* values,
+                                        size_t len, uint32_t dtype) {
+    return move_rows(ctx, cache, layer, position, tokens, const_cast<void*>(keys), const_cast<void*>(values), len, dtype, true);
+}
+
+ribn_amd_status ribn_amd_kv_cache_read(ribn_amd_context* ctx, ribn_amd_kv_cache* cache, uint32_t layer,
+                                       uint32_t position, size_t tokens, void* keys, void* values, size_t len,
+                                       uint32_t dtype) {
+    return move_rows(ctx, cache, layer, position, tokens, keys, values, len, dtype, false);
+}
+
+ribn_amd_status ribn_amd_kv_cache_layer(ribn_amd_kv_cache* cache, uint32_t layer, uint16_t** keys, uint16_t** values) {
+    if (!cache || !keys || !values) return fail(RIBN_AMD_INVALID_ARGUMENT, 0, 0, "null argument");
+    const ribn_amd_status st = check_layer(cache, layer);
+    if (st != RIBN_AMD_OK) return st;
+    if (cache->kind == ribn_amd::kCacheI8) {
+        return fail(RIBN_AMD_UNSUPPORTED, RIBN_AMD_KV_F16, RIBN_AMD_KV_I8, "an 8-bit cache has no f16 view (ribn_amd_kv_cache_read)");
     }
     *keys = cache->keys + (size_t)layer * cache->layer_elems;
     *values = cache->values + (size_t)layer * cache->layer_elems;
@@ -788,6 +958,8 @@ ribn_amd_status ribn_amd_attention_prefill(ribn_amd_context* ctx, const ribn_amd
     if (!same_geometry(cache->cfg, *config) || layer >= cache->cfg.layers) {
         return fail(RIBN_AMD_INVALID_PLAN, cache->cfg.layers, layer, "the cache does not hold layer %u", layer);
     }
+    st = check_kind(cache, cache, *config, 0);
+    if (st != RIBN_AMD_OK) return st;
     if (tokens == 0) return fail(RIBN_AMD_INPUT_LENGTH, 1, 0, "a prompt chunk needs at least one token");
     if ((uint64_t)position + tokens > cache->capacity) {
         return fail(RIBN_AMD_POSITION_OVERFLOW, cache->capacity, (uint64_t)position + tokens - 1,
@@ -816,7 +988,7 @@ ribn_amd_status ribn_amd_attention_prefill(ribn_amd_context* ctx, const ribn_amd
     a.eps = config->epsilon;
     a.rope_base = config->rope_base;
     a.scale = 1.4426950408889634f / sqrtf((float)config->head_dim);
-    hipError_t e = ribn_amd::launch_prefill_attention(a, ctx->cu_count, ctx->stream);
+    hipError_t e = ribn_amd::launch_prefill_attention(a, ctx->cu_count, ctx->stream, cache->kind);
     return e == hipSuccess ? ok() : driver(e, "prompt attention launch");
 }
 
@@ -849,6 +1021,8 @@ ribn_amd_status ribn_amd_attention_decode(ribn_amd_context* ctx, const ribn_amd_
             return fail(RIBN_AMD_INVALID_PLAN, c->cfg.layers, layer, "member %zu's cache does not hold layer %u", m,
                         layer);
         }
+        st = check_kind(c, caches[0], *config, m);
+        if (st != RIBN_AMD_OK) return st;
         for (size_t o = 0; o < m; ++o) {
             if (caches[o] == c) return fail(RIBN_AMD_INVALID_PLAN, o, m, "members %zu and %zu share a cache", o, m);
         }
@@ -876,8 +1050,9 @@ ribn_amd_status ribn_amd_attention_decode(ribn_amd_context* ctx, const ribn_amd_
     }
     // Positions are device values: the kernel checks them against each cache
     // and drops an append past its capacity.
-    const int chunks = ribn_amd::attn_grid_chunks(max_capacity, (int)members);
-    hipError_t e = attention(*config, mem, chunks, false, (int)members, layer, q, k, v, q_norm, k_norm, positions,
+    const int kind = caches[0]->kind;
+    const int chunks = grid_chunks(kind, max_capacity, (int)members);
+    hipError_t e = attention(*config, mem, kind, chunks, false, (int)members, layer, q, k, v, q_norm, k_norm, positions,
                              output, nullptr, ctx->stream);
     return e == hipSuccess ? ok() : driver(e, "launch attention");
 }
@@ -1127,6 +1302,8 @@ ribn_amd_status ribn_amd_qwen3_prefill_prompt(ribn_amd_qwen3_decode* d, ribn_amd
     if (!same_geometry(cache->cfg, d->cfg)) {
         return fail(RIBN_AMD_INVALID_PLAN, 0, 0, "the cache has another layer or head geometry");
     }
+    st = check_kind(cache, cache, d->cfg, 0);
+    if (st != RIBN_AMD_OK) return st;
     if ((uint64_t)position + count > cache->capacity) {
         return fail(RIBN_AMD_POSITION_OVERFLOW, cache->capacity, (uint64_t)position + count - 1,
                     "token position %llu exceeds KV capacity %u", (unsigned long long)position + count - 1,

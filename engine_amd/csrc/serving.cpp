@@ -46,6 +46,7 @@
 #include <vector>
 
 #include "abi_internal.hpp"
+#include "decode_launch.hpp"
 #include "qwen3_internal.hpp"
 #include "serving_submissions.hpp"
 
@@ -149,6 +150,12 @@ struct ribn_amd_serving {
     std::vector<uint64_t> deferred;  // released while a pending submission used them
     std::unordered_map<uint64_t, PhysicalState> states;
     std::unordered_map<uint32_t, std::vector<ribn_amd_kv_cache*>> spare;  // capacity -> caches for reuse
+    // What states' caches are made with (ribn_amd_serving_set_kv_options); the
+    // rope spec and its factors are copies.
+    uint32_t kv_format;
+    bool kv_roped;
+    ribn_amd_rope_spec kv_rope;
+    float kv_factors[ribn_amd::kHeadDim / 2];
     std::vector<hipEvent_t> events;  // completion events for reuse
 };
 
@@ -263,7 +270,7 @@ ribn_amd_status materialize(ribn_amd_serving* s, const ribn_amd_serving_row& row
             return fail(RIBN_AMD_EXECUTION_FAILED, 1, 0, "the Qwen3 decoder needs full-attention KV state (request %llu)",
                         (unsigned long long)row.request);
         }
-        const uint64_t bytes = ribn_amd_qwen3_kv_bytes(&s->cfg, row.kv_tokens);
+        const uint64_t bytes = ribn_amd_kv_bytes(&s->cfg, row.kv_tokens, s->kv_format);
         ribn_amd_kv_cache* cache = nullptr;
         auto pool = s->spare.find(row.kv_tokens);
         if (pool != s->spare.end() && !pool->second.empty()) {
@@ -277,7 +284,7 @@ ribn_amd_status materialize(ribn_amd_serving* s, const ribn_amd_serving_row& row
                     while (!kv.second.empty() && s->kv_in_use + s->kv_reusable + bytes > s->kv_budget) {
                         ribn_amd_kv_cache_destroy(kv.second.back());
                         kv.second.pop_back();
-                        s->kv_reusable -= ribn_amd_qwen3_kv_bytes(&s->cfg, kv.first);
+                        s->kv_reusable -= ribn_amd_kv_bytes(&s->cfg, kv.first, s->kv_format);
                     }
                 }
             }
@@ -287,7 +294,8 @@ ribn_amd_status materialize(ribn_amd_serving* s, const ribn_amd_serving_row& row
                             row.kv_tokens, (unsigned long long)bytes,
                             (unsigned long long)(s->kv_budget - s->kv_in_use), (unsigned long long)s->kv_budget);
             }
-            ribn_amd_status st = ribn_amd_kv_cache_create(s->ctx, &s->cfg, row.kv_tokens, &cache);
+            const ribn_amd_kv_options options{s->kv_format, s->kv_roped ? &s->kv_rope : nullptr};
+            ribn_amd_status st = ribn_amd_kv_cache_create_with(s->ctx, &s->cfg, row.kv_tokens, &options, &cache);
             if (st != RIBN_AMD_OK) return st;
         }
         PhysicalState phys;
@@ -634,6 +642,33 @@ ribn_amd_status ribn_amd_serving_set_prefill_chunk(ribn_amd_serving* s, uint32_t
 ribn_amd_status ribn_amd_serving_set_grouped_decode(ribn_amd_serving* s, int32_t enabled) {
     if (!s) return fail(RIBN_AMD_INVALID_ARGUMENT, 0, 0, "null dispatcher");
     s->grouped = enabled != 0;
+    return ok();
+}
+
+ribn_amd_status ribn_amd_serving_set_kv_options(ribn_amd_serving* s, const ribn_amd_kv_options* options) {
+    if (!s) return fail(RIBN_AMD_INVALID_ARGUMENT, 0, 0, "null dispatcher");
+    ribn_amd_status st = check_health(s);
+    if (st == RIBN_AMD_OK) st = ribn_amd_decode::check_kv_options(options);
+    if (st != RIBN_AMD_OK) return st;
+    if (!s->states.empty()) {
+        return fail(RIBN_AMD_EXECUTION_FAILED, 0, s->states.size(), "%zu states are materialized with the caches' present format",
+                    s->states.size());
+    }
+    DeviceGuard guard(s->ctx->device);
+    for (auto& kv : s->spare) {
+        for (ribn_amd_kv_cache* c : kv.second) ribn_amd_kv_cache_destroy(c);
+    }
+    s->spare.clear();
+    s->kv_reusable = 0;
+    s->kv_format = options != nullptr ? options->format : RIBN_AMD_KV_F16;
+    s->kv_roped = options != nullptr && options->rope != nullptr;
+    if (s->kv_roped) {
+        s->kv_rope = *options->rope;
+        if (s->kv_rope.freq_factors != nullptr) {
+            std::copy(s->kv_rope.freq_factors, s->kv_rope.freq_factors + ribn_amd::kHeadDim / 2, s->kv_factors);
+            s->kv_rope.freq_factors = s->kv_factors;
+        }
+    }
     return ok();
 }
 

@@ -195,9 +195,28 @@ def _optional_f32(file: GgufFile, key: str, default: float) -> float:
     return default if v is None else float(v)
 
 
+def rope_from_gguf(file: GgufFile, head_dim: int, base: float):
+    """The scaled rope a file's "qwen3.rope.scaling.*" metadata asks for, None if
+    it asks for none. Types other than linear and yarn are refused: run without
+    their scaling such a model answers wrongly."""
+    from .rope import AmdRopeSpec
+
+    kind = file.metadata("qwen3.rope.scaling.type")
+    if kind is None or kind == "none":
+        return None
+    if kind not in ("linear", "yarn"):
+        raise GgufError(36, 0, 0, f"UnsupportedRopeScaling: {kind}")
+    factor = file.metadata("qwen3.rope.scaling.factor")
+    if factor is None:
+        raise GgufError(35, 0, 0, "MissingMetadata: qwen3.rope.scaling.factor")
+    original = _required_u32(file, "qwen3.rope.scaling.original_context_length") if kind == "yarn" else 0
+    return AmdRopeSpec(head_dim=head_dim, base=base, scaling=kind, factor=float(factor), original_context=original)
+
+
 def qwen3_config_from_gguf(file: GgufFile):
     """Qwen3 dense geometry from "qwen3.*" metadata (the reference's
-    config_from_gguf reads "qwen35.*" for its hybrid model the same way)."""
+    config_from_gguf reads "qwen35.*" for its hybrid model the same way),
+    scaled rope included (rope_from_gguf)."""
     from .qwen3 import AmdQwen3Config
 
     arch = file.metadata("general.architecture")
@@ -212,11 +231,13 @@ def qwen3_config_from_gguf(file: GgufFile):
     embd = file.tensor("token_embd.weight")
     if embd is None:
         raise GgufError(18, 0, 0, "MissingTensor: token_embd.weight")
+    base = _optional_f32(file, "qwen3.rope.freq_base", 1.0e6)
     return AmdQwen3Config(layers=_required_u32(file, "qwen3.block_count"), hidden=hidden, q_heads=heads,
                           kv_heads=_required_u32(file, "qwen3.attention.head_count_kv"), head_dim=head_dim,
                           ffn=_required_u32(file, "qwen3.feed_forward_length"), vocab=int(embd.dimensions[1]),
-                          rope_base=_optional_f32(file, "qwen3.rope.freq_base", 1.0e6),
-                          epsilon=_optional_f32(file, "qwen3.attention.layer_norm_rms_epsilon", 1.0e-6))
+                          rope_base=base,
+                          epsilon=_optional_f32(file, "qwen3.attention.layer_norm_rms_epsilon", 1.0e-6),
+                          rope=rope_from_gguf(file, head_dim, base))
 
 
 LAYER_TENSORS = {"attn_q": "attn_q.weight", "attn_k": "attn_k.weight", "attn_v": "attn_v.weight",

@@ -15,11 +15,17 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
+from typing import Optional
 
 import numpy as np
 
 from . import _lib
 from .kquant import RANK_CACHE, RANK_DECODER, AmdModelKernelError, _check, _live, _own, _ptr
+from .rope import AmdRopeSpec
+
+# What a KV cache holds a value in: f16, or 8 bits with a power-of-two scale for
+# each block of 32 tokens and KV head.
+KV_F16, KV_I8 = 0, 1
 
 
 @dataclass(frozen=True)
@@ -33,6 +39,8 @@ class AmdQwen3Config:
     vocab: int = 151936
     rope_base: float = 1.0e6
     epsilon: float = 1.0e-6
+    # Rope of the caches made for this model, None: half layout, unscaled, rope_base.
+    rope: Optional[AmdRopeSpec] = None
 
     def to_c(self) -> _lib.Qwen3Config:
         return _lib.Qwen3Config(self.layers, self.hidden, self.q_heads, self.kv_heads, self.head_dim, self.ffn,
@@ -42,17 +50,64 @@ class AmdQwen3Config:
 QWEN3_8B = AmdQwen3Config()
 
 
-class AmdKvCache:
-    """One sequence's f16 KV cache for every layer ([layer][kv_head][token][head_dim])."""
+def kv_options(config: AmdQwen3Config, format: int = KV_F16, rope: Optional[AmdRopeSpec] = None):
+    """ribn_amd_kv_options for a model's caches: `rope`, or else the config's."""
+    options = _lib.KvOptions(format, None)
+    spec = rope if rope is not None else config.rope
+    if spec is not None:
+        options.rope = ctypes.pointer(spec.to_c())
+    return options
 
-    def __init__(self, ctx, config: AmdQwen3Config, capacity: int):
+
+class AmdKvCache:
+    """One sequence's KV cache for every layer: f16 ([layer][kv_head][token][head_dim])
+    or, with KV_I8, 8 bits (ribn_amd_kv_cache_create_with). `rope`, or the config's, is how
+    its keys (and the queries that read them) are rotated."""
+
+    def __init__(self, ctx, config: AmdQwen3Config, capacity: int, format: int = KV_F16,
+                 rope: Optional[AmdRopeSpec] = None):
         self.ctx = ctx
         self.config = config
         self._cfg = config.to_c()
         self.handle = ctypes.c_void_p()
-        _check(ctx._lib.ribn_amd_kv_cache_create(ctx.handle, ctypes.byref(self._cfg), capacity,
-                                                 ctypes.byref(self.handle)), AmdModelKernelError)
+        options = kv_options(config, format, rope)
+        _check(ctx._lib.ribn_amd_kv_cache_create_with(ctx.handle, ctypes.byref(self._cfg), capacity, ctypes.byref(options),
+                                                      ctypes.byref(self.handle)), AmdModelKernelError)
         _own(self, RANK_CACHE)
+
+    def format(self) -> int:
+        return int(self.ctx._lib.ribn_amd_kv_cache_format(self.handle))
+
+    def tail(self, layer: int):
+        """Of a KV_I8 cache: device addresses of the f16 block its sequence stands
+        in, keys [kv_heads][32][128] and values [kv_heads][128][32], and the
+        elements between KV heads."""
+        k, v, stride = ctypes.c_void_p(), ctypes.c_void_p(), ctypes.c_size_t()
+        _check(self.ctx._lib.ribn_amd_kv_cache_tail(self.handle, layer, ctypes.byref(k), ctypes.byref(v),
+                                                    ctypes.byref(stride)), AmdModelKernelError)
+        return k.value, v.value, int(stride.value)
+
+    def write(self, layer: int, keys, values, position: int):
+        """Puts rows [tokens][kv_heads][128] (f16 or f32; keys normalised and rotated
+        already) into the cache at position, position + 1, ..."""
+        self._move(self.ctx._lib.ribn_amd_kv_cache_write, layer, position, keys, values)
+
+    def read(self, layer: int, position: int, keys, values):
+        """Fills keys and values [tokens][kv_heads][128] (f16 or f32) with what the cache holds there."""
+        self._move(self.ctx._lib.ribn_amd_kv_cache_read, layer, position, keys, values)
+
+    def _move(self, call, layer, position, keys, values):
+        import torch
+        dtype = {torch.float32: 0, torch.float16: 2}.get(keys.dtype)
+        if dtype is None or values.dtype != keys.dtype:
+            raise TypeError(f"cache rows are float32 or float16, got {keys.dtype} and {values.dtype}")
+        if keys.shape != values.shape or not keys.is_contiguous() or not values.is_contiguous():
+            raise ValueError("keys and values must be contiguous and of one shape")
+        row = self.config.kv_heads * self.config.head_dim
+        if keys.numel() % row:
+            raise ValueError(f"cache rows have {row} values, got {keys.numel()}")
+        _check(call(self.ctx.handle, self.handle, layer, position, keys.numel() // row, _ptr(keys), _ptr(values),
+                    keys.numel(), dtype), AmdModelKernelError)
 
     def capacity(self) -> int:
         return int(self.ctx._lib.ribn_amd_kv_cache_capacity(self.handle))

@@ -1,0 +1,121 @@
+"""Rotary positions over the C ABI.
+
+  AmdRopeSpec  which dims turn together, their frequencies and how these are
+               stretched for contexts past the trained length
+  AmdRope      the operator on query and key rows; with the half layout, unscaled,
+               CudaQwen35Ops::rope_neox (model_ops.rs:2012-2070)
+
+A KV cache takes a spec too (AmdKvCache): its keys are cached rotated.
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+from typing import Optional, Sequence
+
+from . import _lib
+from .kquant import RANK_RESOURCE, AmdModelKernelError, _check, _live, _own, _ptr
+
+_LAYOUTS = {"half": 0, "interleaved": 1}
+_SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
+
+
+@dataclass(frozen=True)
+class AmdRopeSpec:
+    """ribn_amd_rope_spec. `rotary_dim` None: the whole head. `attention_factor` 0:
+    the scaling's own (YaRN 0.1 ln(factor) + 1). `freq_factors`: one divisor per pair."""
+    head_dim: int = 128
+    rotary_dim: Optional[int] = None
+    layout: str = "half"
+    base: float = 1.0e6
+    scaling: str = "none"
+    factor: float = 1.0
+    original_context: int = 0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    attention_factor: float = 0.0
+    freq_factors: Optional[Sequence[float]] = None
+
+    def to_c(self) -> _lib.RopeSpec:
+        """The C struct (it keeps the factors' array alive)."""
+        if self.layout not in _LAYOUTS:
+            raise ValueError(f"rope layout must be one of {sorted(_LAYOUTS)}, got {self.layout!r}")
+        if self.scaling not in _SCALINGS:
+            raise ValueError(f"rope scaling must be one of {sorted(_SCALINGS)}, got {self.scaling!r}")
+        rotary = self.head_dim if self.rotary_dim is None else self.rotary_dim
+        spec = _lib.RopeSpec(_LAYOUTS[self.layout], self.head_dim, rotary, _SCALINGS[self.scaling], self.base,
+                             self.factor, self.original_context, self.beta_fast, self.beta_slow,
+                             self.attention_factor, None)
+        if self.freq_factors is not None:
+            if len(self.freq_factors) != rotary // 2:
+                raise ValueError(f"{rotary // 2} pairs need as many frequency factors, got {len(self.freq_factors)}")
+            spec.freq_factors = (ctypes.c_float * (rotary // 2))(*self.freq_factors)
+        return spec
+
+
+def rope_frequencies(spec: AmdRopeSpec):
+    """Host-only check of a spec; the turns a position adds to each pair's angle, and the gain."""
+    lib = _lib.load()
+    c = spec.to_c()
+    turns = (ctypes.c_double * max(1, c.rotary_dim // 2))()
+    gain = ctypes.c_double()
+    _check(lib.ribn_amd_rope_frequencies(ctypes.byref(c), turns, c.rotary_dim // 2, ctypes.byref(gain)), AmdModelKernelError)
+    return list(turns), gain.value
+
+
+def _length(t) -> int:
+    """Elements from the tensor's first to its storage's end."""
+    return t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
+
+
+class AmdRope:
+    """Rotates rows [tokens][heads][head_dim] (f32, bf16 or f16; any strides over
+    tokens and heads, dims contiguous) by their tokens' positions (device int32)."""
+
+    def __init__(self, ctx, spec: AmdRopeSpec):
+        self.ctx = ctx
+        self.spec = spec
+        self.handle = ctypes.c_void_p()
+        c = spec.to_c()
+        _check(ctx._lib.ribn_amd_rope_create(ctx.handle, ctypes.byref(c), ctypes.byref(self.handle)), AmdModelKernelError)
+        _own(self, RANK_RESOURCE)
+
+    def execute(self, input, positions, output):
+        """output = rope(input); `output` may be `input`."""
+        self.execute_group([input], positions, [output])
+
+    def execute_group(self, inputs, positions, outputs):
+        """Up to four tensors sharing their tokens' positions (queries and keys) in one launch."""
+        import torch
+        if len(inputs) != len(outputs):
+            raise ValueError(f"{len(inputs)} inputs and {len(outputs)} outputs")
+        if positions.dtype != torch.int32 or positions.dim() != 1 or not positions.is_contiguous():
+            raise TypeError("positions must be a contiguous vector of int32")
+        tokens = positions.numel()
+        dtype = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}.get(inputs[0].dtype) if inputs else None
+        rows = (_lib.RopeRows * max(1, len(inputs)))()
+        for r, x, y in zip(rows, inputs, outputs):
+            if dtype is None or x.dtype != inputs[0].dtype or y.dtype != inputs[0].dtype:
+                raise TypeError("rope takes float32, bfloat16 or float16 tensors of one type")
+            if x.dim() != 3 or x.shape != y.shape or x.shape[0] != tokens or x.shape[2] != self.spec.head_dim:
+                raise ValueError(f"rope rows are [{tokens}][heads][{self.spec.head_dim}], got {tuple(x.shape)} and {tuple(y.shape)}")
+            if x.stride(2) != 1 or y.stride(2) != 1:
+                raise ValueError("the dims of a head must be contiguous")
+            r.input, r.input_len = x.data_ptr(), _length(x)
+            r.input_token_stride, r.input_head_stride = x.stride(0), x.stride(1)
+            r.output, r.output_len = y.data_ptr(), _length(y)
+            r.output_token_stride, r.output_head_stride = y.stride(0), y.stride(1)
+            r.heads = x.shape[1]
+        _check(self.ctx._lib.ribn_amd_rope_execute(self.handle, _ptr(positions), tokens, rows, len(inputs), dtype or 0),
+               AmdModelKernelError)
+
+    def close(self):
+        if self.handle and _live():
+            self.ctx._lib.ribn_amd_rope_destroy(self.handle)
+            self.handle = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass

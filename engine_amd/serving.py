@@ -220,6 +220,8 @@ class AmdServingDispatcher(AmdDispatcher):
                                                 ctypes.byref(self.handle)))
         _own(self, RANK_DISPATCHER)
         self._rows = {}
+        if decoder.config.rope is not None:
+            self.with_kv_format(0)
 
     def with_prefill_chunk(self, members: int) -> "AmdServingDispatcher":
         _call(self._lib.ribn_amd_serving_set_prefill_chunk(self.handle, members))
@@ -230,6 +232,14 @@ class AmdServingDispatcher(AmdDispatcher):
         (AmdQwen3Decode.prefill_prompt) in chunks of `chunk_tokens`; 0 turns
         it off. No reference counterpart; reserves the workspace now."""
         _call(self._lib.ribn_amd_serving_set_prompt_prefill(self.handle, chunk_tokens))
+        return self
+
+    def with_kv_format(self, format: int, rope=None) -> "AmdServingDispatcher":
+        """Caches of later states in `format` (KV_F16 or KV_I8) with `rope`, or the
+        decoder config's. No reference counterpart; before the first state."""
+        from .qwen3 import kv_options
+        options = kv_options(self.decoder.config, format, rope)
+        _call(self._lib.ribn_amd_serving_set_kv_options(self.handle, ctypes.byref(options)))
         return self
 
     def with_grouped_decode(self, enabled: bool) -> "AmdServingDispatcher":
@@ -436,6 +446,12 @@ def qwen3_kv_bytes(config, tokens: int) -> int:
     """KvStateSpec::byte_size of a Qwen3 sequence of `tokens` (f16 K and V)."""
     c = config.to_c()
     return int(_lib.load().ribn_amd_qwen3_kv_bytes(ctypes.byref(c), tokens))
+
+
+def kv_bytes(config, tokens: int, format: int) -> int:
+    """Bytes of a sequence's cache of `tokens` in a format (KV_F16 or KV_I8)."""
+    c = config.to_c()
+    return int(_lib.load().ribn_amd_kv_bytes(ctypes.byref(c), tokens, format))
 
 
 def chunked_prefix_len(token_count: int, members: int, requests_sampling: bool) -> int:

@@ -46,9 +46,11 @@ extern "C" {
  * kernels at 8 (quantized.rs:12); this library serves decode batches up to 64. */
 #define RIBN_AMD_MAX_BATCH_MEMBERS 64u
 
-/* Activation element types accepted by ribn_amd_gemm_prefill. */
+/* Activation element types: ribn_amd_gemm_prefill takes the first two,
+ * ribn_amd_rope_execute all three, ribn_amd_kv_cache_write / _read F32 and F16. */
 #define RIBN_AMD_F32 0u
 #define RIBN_AMD_BF16 1u
+#define RIBN_AMD_F16 2u
 
 typedef enum ribn_amd_status {
     RIBN_AMD_OK = 0,
@@ -556,6 +558,136 @@ uint32_t ribn_amd_kv_cache_capacity(const ribn_amd_kv_cache *cache);
 ribn_amd_status ribn_amd_kv_cache_layer(ribn_amd_kv_cache *cache, uint32_t layer, uint16_t **keys,
                                         uint16_t **values);
 
+/* ------------------------------------------------------ rotary positions */
+
+/* Which dims of a head turn together: pairs (i, i + rotary_dim / 2), or
+ * (2i, 2i + 1), of the head's first rotary_dim dims; the others are copied. */
+#define RIBN_AMD_ROPE_HALF 0u
+#define RIBN_AMD_ROPE_INTERLEAVED 1u
+/* How the frequencies base^(-2i / rotary_dim) are stretched for contexts past
+ * the trained length: not at all; all of them divided by `factor` (linear); or
+ * YaRN: those that turn at least beta_fast times within original_context tokens
+ * stay, those that turn beta_slow times or less are divided by `factor`, between
+ * them a linear ramp over the pair index. */
+#define RIBN_AMD_ROPE_UNSCALED 0u
+#define RIBN_AMD_ROPE_LINEAR 1u
+#define RIBN_AMD_ROPE_YARN 2u
+
+typedef struct ribn_amd_rope_spec {
+    uint32_t layout;           /* RIBN_AMD_ROPE_HALF or _INTERLEAVED */
+    uint32_t head_dim;         /* even, 2..1024 */
+    uint32_t rotary_dim;       /* even, 2..head_dim */
+    uint32_t scaling;          /* RIBN_AMD_ROPE_UNSCALED, _LINEAR or _YARN */
+    float base;                /* > 1 */
+    float factor;              /* linear, YaRN: > 0 */
+    uint32_t original_context; /* YaRN: > 0 */
+    float beta_fast;           /* YaRN: > beta_slow */
+    float beta_slow;           /* YaRN: > 0 */
+    float attention_factor;    /* multiplies cosine and sine; 0: 0.1 ln(factor) + 1 for YaRN with factor > 1, else 1 */
+    const float *freq_factors; /* host [rotary_dim / 2] divisors of the frequencies (GGUF's rope_freqs), or NULL */
+} ribn_amd_rope_spec;
+
+/* Host-only: checks a spec (InvalidPlan) and writes what its device table holds,
+ * the turns (2 pi radians each) a position adds to each pair's angle (len ==
+ * rotary_dim / 2, else OutputLength) and the gain of cosine and sine. */
+ribn_amd_status ribn_amd_rope_frequencies(const ribn_amd_rope_spec *spec, double *turns, size_t len, double *gain);
+
+typedef struct ribn_amd_rope ribn_amd_rope;
+
+/* Rotary positions as an operator (CudaQwen35Ops::rope_neox,
+ * model_ops.rs:2012-2070, which has the half layout, unscaled): the spec is
+ * checked (InvalidPlan), its frequencies computed in 64 bits and put on the
+ * context's device. freq_factors is read before the call returns. */
+ribn_amd_status ribn_amd_rope_create(ribn_amd_context *ctx, const ribn_amd_rope_spec *spec, ribn_amd_rope **out);
+void ribn_amd_rope_destroy(ribn_amd_rope *rope);
+
+/* One tensor of rows to rotate: element (t, h, d) lies at t * token_stride +
+ * h * head_stride + d, strides and lengths in elements. `output` may be `input`
+ * with the same strides; it must not overlap it otherwise, nor have rows that
+ * overlap each other (InvalidArgument). */
+typedef struct ribn_amd_rope_rows {
+    const void *input;
+    size_t input_len;
+    size_t input_token_stride;
+    size_t input_head_stride;
+    void *output;
+    size_t output_len;
+    size_t output_token_stride;
+    size_t output_head_stride;
+    size_t heads;
+} ribn_amd_rope_rows;
+
+/* Rotates `count` (1..4) tensors that share their tokens' positions (queries and
+ * keys) in one launch: output = rope(input, positions[t]), `tokens` tokens, all of
+ * element type `dtype` (RIBN_AMD_F32, RIBN_AMD_BF16 or RIBN_AMD_F16). positions is
+ * a device int32 array. Angles are formed in 64 bits, products in f32, rounded
+ * once to the type. The first `rotary_dim` dims turn, the rest is copied. */
+ribn_amd_status ribn_amd_rope_execute(ribn_amd_rope *rope, const int32_t *positions, size_t tokens,
+                                      const ribn_amd_rope_rows *rows, size_t count, uint32_t dtype);
+
+/* ------------------------------------------------ caches of other kinds */
+
+/* What a KV cache holds a value in. RIBN_AMD_KV_F16: f16 (2 bytes a value).
+ * RIBN_AMD_KV_I8: 8-bit whole numbers and, for each block of 32 tokens and KV
+ * head, one power-of-two scale for the keys and one for the values (1.002
+ * bytes a value); the block a sequence stands in stays f16 until its 32nd
+ * token. With x16 = f16(x) (overflow held at +-65504, NaN as 0) and a = max
+ * |x16| over a block: e = max(floor(log2 a) - 6, -24), code =
+ * clamp(rint(x16 * 2^-e), -127, 127), value = code * 2^e. */
+#define RIBN_AMD_KV_F16 0u
+#define RIBN_AMD_KV_I8 1u
+
+typedef struct ribn_amd_kv_options {
+    uint32_t format;                /* RIBN_AMD_KV_F16 or RIBN_AMD_KV_I8 */
+    const ribn_amd_rope_spec *rope; /* how q and k of this cache are rotated; NULL: half layout, unscaled, the config's
+                                       rope_base. Half layout over the whole head (128) only. Copied. */
+} ribn_amd_kv_options;
+
+/* ribn_amd_kv_cache_create with a format and a rope of the cache's own (keys are
+ * cached rotated, so how they are rotated belongs to the cache). Every call that takes
+ * caches takes these: attention, prompt chunks, the decoder's steps. The caches
+ * of one call must be of one kind (InvalidPlan): one format, all with a rope
+ * of their own or none, and the config's rope_base theirs.
+ * NULL options, or F16 without rope, is ribn_amd_kv_cache_create. A cache with a
+ * rope of its own, and every I8 cache, forms angles in 64 bits (the default
+ * one in f32, as the reference does); an I8 cache also normalises and
+ * rotates keys in 64 bits.
+ * I8 caches: tokens are appended at rising positions, or the sequence is taken
+ * back to an earlier one and goes on from there (its block's earlier tokens
+ * are then what their codes stand for, unless the block is the latest). Attention
+ * reads the cache as it stands after the call's own appends: whole blocks from
+ * 8 bits, the last one, while it is not whole, from f16. A call at a position past
+ * the end leaves the skipped tokens, and those of the block the sequence stood in, undefined
+ * (finite). Fresh caches read as zeros; they are set up on ctx's stream, which work
+ * on another stream has to wait for. */
+ribn_amd_status ribn_amd_kv_cache_create_with(ribn_amd_context *ctx, const ribn_amd_qwen3_config *config,
+                                              uint32_t capacity, const ribn_amd_kv_options *options,
+                                              ribn_amd_kv_cache **out);
+uint32_t ribn_amd_kv_cache_format(const ribn_amd_kv_cache *cache);
+/* Bytes of a layer stack's cache of `tokens` capacity in a format (0: bad
+ * arguments); ribn_amd_qwen3_kv_bytes for F16. */
+uint64_t ribn_amd_kv_bytes(const ribn_amd_qwen3_config *config, uint32_t tokens, uint32_t format);
+/* The f16 block an I8 cache's sequence stands in, in place: keys
+ * [kv_heads][32][128], values [kv_heads][128][32], KV heads `head_stride`
+ * elements apart. Unsupported for F16 caches, as ribn_amd_kv_cache_layer is for
+ * I8 ones. */
+ribn_amd_status ribn_amd_kv_cache_tail(ribn_amd_kv_cache *cache, uint32_t layer, uint16_t **keys, uint16_t **values,
+                                       size_t *head_stride);
+/* Puts a context into a cache of either format, on ctx's stream: `tokens` rows of
+ * keys (normalised and rotated already) and values, [tokens][kv_heads][128] of
+ * `dtype` (RIBN_AMD_F16 or RIBN_AMD_F32), at positions position .. position +
+ * tokens - 1 of one layer; len counts each array's elements. An I8 cache
+ * appends them (see above); an F16 one rounds to f16. */
+ribn_amd_status ribn_amd_kv_cache_write(ribn_amd_context *ctx, ribn_amd_kv_cache *cache, uint32_t layer,
+                                        uint32_t position, size_t tokens, const void *keys, const void *values,
+                                        size_t len, uint32_t dtype);
+/* Takes rows out of a cache, in the same layout and types: what attention reads
+ * at those positions (F16 caches and I8 codes are f16 values exactly). Rows of an
+ * I8 cache past its end are zeros. */
+ribn_amd_status ribn_amd_kv_cache_read(ribn_amd_context *ctx, ribn_amd_kv_cache *cache, uint32_t layer,
+                                       uint32_t position, size_t tokens, void *keys, void *values, size_t len,
+                                       uint32_t dtype);
+
 /* One layer's decode attention for `members` sequences, fusing the
  * reference's per-layer sequence (decode.rs:944-1020): per-head q/k RMSNorm
  * (q_gate_norm / strided_rms_norm, model_ops.rs:3784-3839, 2475-2529), NEOX
@@ -750,6 +882,12 @@ ribn_amd_status ribn_amd_serving_set_prompt_prefill(ribn_amd_serving *serving, u
 /* with_grouped_decode (serving.rs:337-341): compatible decode rows of mixed
  * batches are gathered into lanes (opt-in, as in the reference). */
 ribn_amd_status ribn_amd_serving_set_grouped_decode(ribn_amd_serving *serving, int32_t enabled);
+
+/* No reference counterpart: the caches of states materialized from now on are
+ * made with these options (ribn_amd_kv_cache_create_with; budget and state bytes count
+ * the format's), NULL for the default. Caches kept for reuse are freed. Refused
+ * (ExecutionFailed) while any state is materialized: a lane's caches are of one kind. */
+ribn_amd_status ribn_amd_serving_set_kv_options(ribn_amd_serving *serving, const ribn_amd_kv_options *options);
 
 /* NvidiaDispatcher::dispatch_batch (serving.rs:854-882): eager execution of
  * every row in order; returns after the stream drained. outcomes[count]. */
