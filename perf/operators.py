@@ -223,7 +223,8 @@ def _prepare_own(s, case):
         if len(keys):
             cache.write(0, keys, values, 0)
     if kind != "stage":
-        s.tails = [_tails(c, case["kv_heads"]) for c in s.caches]
+        rows = [(n + extra - 1) % BLOCK + 1 for n in s.lengths]
+        s.tails = [(k[:, :n], v[:, :, :n]) for (k, v), n in zip((_tails(c, case["kv_heads"]) for c in s.caches), rows)]
 
 
 def _prepare_plain(s, kv, room):
@@ -395,6 +396,8 @@ def run(s):
             s.caches[0].read(0, 0, *s.back)
         else:
             s.rope.execute_group(s.x, s.positions, s.y)
+        if kind in ("decode", "chunk"):
+            return {"y": s.y, "tail": s.tails}
     else:
         {"decode": _plain_decode, "chunk": _plain_chunk, "stage": _plain_stage, "rope": _plain_rope}[kind](s)
     if kind == "stage":
