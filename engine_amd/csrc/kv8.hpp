@@ -67,14 +67,16 @@ struct KvMoveArgs {
     void* values;
 };
 
-// Keys (RMSNorm and rope in 64 bits, then f32, then f16) and values of the new
-// tokens into 8-bit caches: member m's row at positions[m] of its own cache, or,
-// with `appended`, the members' rows at positions[0] .. + members - 1 of the one they share.
+// Keys (RMSNorm and rope in 64 bits, then f32, then f16) and values of new tokens
+// into 8-bit caches: rows of members that share one, at positions[0] ..
+// positions[0] + members - 1, ahead of an `appended` attention launch; a prompt chunk's.
 hipError_t launch_kv8_append(const AttnArgs& args, int members, hipStream_t stream);
-// The same for a prompt chunk's tokens.
 hipError_t launch_kv8_append_seq(const PrefillAttnArgs& args, hipStream_t stream);
-// Attention over what the caches hold, positions 0 .. positions[m], and the merge of its chunks.
-hipError_t launch_kv8_attention(const AttnArgs& args, int members, hipStream_t stream);
+// Attention of every member over positions 0 .. positions[m], and the merge of
+// its chunks. Without `appended`, the members' new tokens go into their caches
+// (distinct ones) on the way. `host_mem`: the members' descriptors in host memory,
+// instead of args.mem.
+hipError_t launch_kv8_attention(const AttnArgs& args, const AttnMember* host_mem, int members, hipStream_t stream);
 int kv8_grid_chunks(int max_capacity, int members);
 
 // Rows as they are (keys already normalised and rotated) into a cache, and back

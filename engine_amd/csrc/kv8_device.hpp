@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "kquant_device.hpp"
 #include "kv8.hpp"
 
 namespace ribn_amd {
@@ -25,8 +26,30 @@ __device__ __forceinline__ int kv8_exponent(float a) {
     return e < -24 ? -24 : e;
 }
 
-__device__ __forceinline__ uint32_t kv8_code(float v, float inv) {
-    return (uint32_t)(int)(fminf(fmaxf(__builtin_rintf(v * inv), -127.0f), 127.0f) + 128.0f);
+// Largest magnitudes of pairs, and of a pair.
+__device__ __forceinline__ kv8_half2 kv8_top(kv8_half2 top, kv8_half2 x) {
+    return __builtin_elementwise_max(top, __builtin_bit_cast(kv8_half2, __builtin_bit_cast(uint32_t, x) & 0x7fff7fffu));
+}
+
+// A scale's reciprocal 2^-e as two factors f16 holds (e is -24 .. 9).
+struct Kv8Inverse {
+    kv8_half2 a, b;
+    __device__ __forceinline__ explicit Kv8Inverse(int e) {
+        const int h = -e / 2;
+        const _Float16 x = (_Float16)kv8_power(h), y = (_Float16)kv8_power(-e - h);
+        a = kv8_half2{x, x};
+        b = kv8_half2{y, y};
+    }
+};
+
+// Four values to the word of their codes, in packed f16: the products with powers of two
+// are exact (or far below half a code), and 1536 + x is rounded to a whole
+// number, ties to even, whose low byte is that number's.
+__device__ __forceinline__ uint32_t kv8_word(kv8_half2 x, kv8_half2 y, const Kv8Inverse& inv) {
+    const kv8_half2 lim{(_Float16)127.0f, (_Float16)127.0f}, bias{(_Float16)1536.0f, (_Float16)1536.0f};
+    x = __builtin_elementwise_min(__builtin_elementwise_max(x * inv.a * inv.b, -lim), lim) + bias;
+    y = __builtin_elementwise_min(__builtin_elementwise_max(y * inv.a * inv.b, -lim), lim) + bias;
+    return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, y), __builtin_bit_cast(uint32_t, x), 0x06040200u) ^ 0x80808080u;
 }
 
 // Two codes of a word as the whole numbers they are, in f16: the byte under
@@ -48,6 +71,46 @@ __device__ __forceinline__ kv8_half8 kv8_values(uint32_t w0, uint32_t w1, _Float
     const kv8_half2 s{scale, scale};
     const kv8_half2 a = kv8_pair<0>(w0) * s, b = kv8_pair<1>(w0) * s, c = kv8_pair<0>(w1) * s, d = kv8_pair<1>(w1) * s;
     return kv8_half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Reductions over a wave by row rotations and lane reads: no LDS round trips,
+// which follow one another on the way from a launch's first load to its products.
+template <int CTRL>
+__device__ __forceinline__ double dpp_add64(double v) {
+    const uint2 w = __builtin_bit_cast(uint2, v);
+    const uint2 moved = make_uint2((uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.x, CTRL, 0xf, 0xf, false),
+                                   (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.y, CTRL, 0xf, 0xf, false));
+    return v + __builtin_bit_cast(double, moved);
+}
+
+// Sum over a row of 16 lanes, in all of them.
+__device__ __forceinline__ double row_sum64(double v) {
+    v = dpp_add64<0xb1>(v);   // quad_perm [1,0,3,2]
+    v = dpp_add64<0x4e>(v);   // quad_perm [2,3,0,1]
+    v = dpp_add64<0x141>(v);  // row_half_mirror
+    return dpp_add64<0x140>(v);  // row_mirror
+}
+
+__device__ __forceinline__ double wave_sum64(double v) {
+    const uint2 w = __builtin_bit_cast(uint2, row_sum64(v));
+    double r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r[i] = __builtin_bit_cast(double, make_uint2((uint32_t)__builtin_amdgcn_readlane((int)w.x, 16 * i),
+                                                     (uint32_t)__builtin_amdgcn_readlane((int)w.y, 16 * i)));
+    }
+    return (r[0] + r[1]) + (r[2] + r[3]);
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+    v = dpp_max_step<0xb1>(v);
+    v = dpp_max_step<0x4e>(v);
+    v = dpp_max_step<0x141>(v);
+    v = dpp_max_step<0x140>(v);
+    float r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 16 * i));
+    return fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]));
 }
 
 // The parts of a (layer, KV head) region.

@@ -43,12 +43,6 @@ struct Stage {
     float amax[2][4];
 };
 
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
-}
-
 template <int ROWS>
 __device__ __forceinline__ void stage_rows(Stage& st, const Rows& in, int first, int count, int row0, const float* k_norm,
                                            double eps, const double* rope, int position) {
@@ -119,28 +113,19 @@ __device__ __forceinline__ void stage_held(Stage& st, const Kv8Head& h, int b, i
 __device__ __forceinline__ void quantise(Stage& st, const Kv8Head& h, int b) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
     // this thread's 16 keys (one row) and 16 values (8 rows of two dims)
-    float kx[16], vx[16];
-    const kv8_half8* kr = reinterpret_cast<const kv8_half8*>(&st.k[kv8_key_row(wave >> 1, m)][64 * (wave & 1) + 16 * g]);
-    const kv8_half8 k0 = kr[0], k1 = kr[1];
-    float ka = 0.f, va = 0.f;
+    kv8_half2 kx[8], vx[8];
+    const kv8_half2* kr = reinterpret_cast<const kv8_half2*>(&st.k[kv8_key_row(wave >> 1, m)][64 * (wave & 1) + 16 * g]);
+    kv8_half2 kt{}, vt{};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        kx[j] = (float)k0[j];
-        kx[8 + j] = (float)k1[j];
-        const kv8_half2 v = *reinterpret_cast<const kv8_half2*>(&st.v[8 * g + j][32 * wave + 2 * m]);
-        vx[j] = (float)v[0];
-        vx[8 + j] = (float)v[1];
+        kx[j] = kr[j];
+        vx[j] = *reinterpret_cast<const kv8_half2*>(&st.v[8 * g + j][32 * wave + 2 * m]);
+        kt = kv8_top(kt, kx[j]);
+        vt = kv8_top(vt, vx[j]);
     }
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        ka = fmaxf(ka, fabsf(kx[j]));
-        va = fmaxf(va, fabsf(vx[j]));
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        ka = fmaxf(ka, __shfl_xor(ka, off, 64));
-        va = fmaxf(va, __shfl_xor(va, off, 64));
-    }
+    float ka = fmaxf((float)kt[0], (float)kt[1]), va = fmaxf((float)vt[0], (float)vt[1]);
+    ka = wave_max(ka);
+    va = wave_max(va);
     if (lane == 0) {
         st.amax[0][wave] = ka;
         st.amax[1][wave] = va;
@@ -148,16 +133,14 @@ __device__ __forceinline__ void quantise(Stage& st, const Kv8Head& h, int b) {
     __syncthreads();
     const int ek = kv8_exponent(fmaxf(fmaxf(st.amax[0][0], st.amax[0][1]), fmaxf(st.amax[0][2], st.amax[0][3])));
     const int ev = kv8_exponent(fmaxf(fmaxf(st.amax[1][0], st.amax[1][1]), fmaxf(st.amax[1][2], st.amax[1][3])));
-    const float ik = kv8_power(-ek), iv = kv8_power(-ev);
+    const Kv8Inverse ik(ek), iv(ev);
     uint32_t kw[4], vw[4];
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-        kw[w] = vw[w] = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            kw[w] |= kv8_code(kx[4 * w + j], ik) << (8 * j);
-            vw[w] |= kv8_code(vx[4 * w + j], iv) << (8 * j);
-        }
+        kw[w] = kv8_word(kx[2 * w], kx[2 * w + 1], ik);
+        // the pairs hold two dims of a key: words are four keys of a dim
+        const int j = 4 * (w & 1), d = w >> 1;
+        vw[w] = kv8_word(kv8_half2{vx[j][d], vx[j + 1][d]}, kv8_half2{vx[j + 2][d], vx[j + 3][d]}, iv);
     }
     uint8_t* codes = h.codes + (size_t)b * kKv8BlockBytes + tid * 16;
     *reinterpret_cast<uint4*>(codes) = make_uint4(kw[0], kw[1], kw[2], kw[3]);
@@ -208,20 +191,18 @@ __device__ __forceinline__ void append_block(Stage& st, const Kv8Head& h, const 
     if (threadIdx.x == 0) *h.end = end;
 }
 
-// Grid (KV head, member), or (KV head, block) of the one cache the members share.
+// Members that share a cache, at consecutive positions. Grid (KV head, block).
 __global__ __launch_bounds__(256) void kv8_append_kernel(AttnArgs a, int members) {
     __shared__ Stage st;
     const int kvh = blockIdx.x;
-    const int m = members == 0 ? (int)blockIdx.y : 0;
-    const AttnMember mb = a.mem[m];
-    const int pos = a.positions[m];
-    const int tokens = members == 0 ? 1 : members;
-    if (pos < 0 || pos > mb.capacity - tokens) return;
-    const int j = members == 0 ? 0 : (int)blockIdx.y;
-    if (pos / kKv8Block + j > (pos + tokens - 1) / kKv8Block) return;
-    const size_t at = ((size_t)m * a.kv_heads + kvh) * kHeadDim;
+    const AttnMember mb = a.mem[0];
+    const int pos = a.positions[0];
+    if (pos < 0 || pos > mb.capacity - members) return;
+    const int j = blockIdx.y;
+    if (pos / kKv8Block + j > (pos + members - 1) / kKv8Block) return;
+    const size_t at = (size_t)kvh * kHeadDim;
     const Rows in{a.k + at, a.v + at, (size_t)a.kv_heads * kHeadDim};
-    append_block<kRowsRaw>(st, kv8_head(mb, a.layer, kvh), in, pos, tokens, j, a.k_norm, a.eps, mb.rope);
+    append_block<kRowsRaw>(st, kv8_head(mb, a.layer, kvh), in, pos, members, j, a.k_norm, a.eps, mb.rope);
 }
 
 __global__ __launch_bounds__(256) void kv8_append_seq_kernel(PrefillAttnArgs a) {
@@ -304,10 +285,10 @@ __global__ __launch_bounds__(256) void cache_init_kernel(CacheInit a) {
 
 // ---------------------------------------------------------- decode attention
 //
-// kv8_attn_kernel: one layer's attention of decode members over what their
-// caches hold (the append is a launch of its own before it), on the f16 matrix
-// cores: the cache's values are f16 exactly, and 128 query heads' worth of
-// products a byte would leave the VALU behind the memory.
+// kv8_attn_kernel: one layer's attention of decode members over their caches,
+// the new token's key and value appended on the way, on the f16 matrix cores: the
+// cache's values are f16 exactly, and converting and multiplying a byte for eight
+// query heads would leave the VALU behind the memory.
 //
 // Split as attn_decode_kernel's: grid (chunk, KV head, member), a chunk one
 // contiguous run of whole blocks; its waves take the blocks in turn. A block is
@@ -325,13 +306,16 @@ __global__ __launch_bounds__(256) void cache_init_kernel(CacheInit a) {
 // the f32 score; values are scaled as f16 (both exact). The running maximum is
 // the column's and moves only when a score passes it by 2^kLazy (attn_prefill_kernel
 // does the same); denominators are f32 sums of f32 probabilities.
+//
+// The block the sequence stands in is the last wave's: it has the tail's rows in
+// the operands' order, puts the new token's row in from LDS, and, when the block is whole,
+// finds its scales and writes its codes from there, going on with what these stand for.
 constexpr float kLazy = 15.0f;
-constexpr int kRing = 2;
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 
-constexpr int kMinChunk = 128;  // a block a wave
-constexpr int kMinChunkWide = 256;
+constexpr int kMinChunk = 256;  // two blocks a wave
+constexpr int kMinChunkWide = 512;
 constexpr int kBitLaneMembers = 8;
 int kv8_min_chunk(int members) { return members > kBitLaneMembers ? kMinChunkWide : kMinChunk; }
 
@@ -347,9 +331,115 @@ __device__ __forceinline__ float other_half(float v) {
 
 typedef float kv8_float4 __attribute__((ext_vector_type(4)));
 
-template <int QPK>
-__global__ __launch_bounds__(kThreads) void kv8_attn_kernel(AttnArgs a) {
+typedef uint32_t kv8_u4 __attribute__((ext_vector_type(4)));
+
+// The tail's block in the operands' order: keys (tile t, step s) at 4 t + s, values
+// (u, i) at 2 u + i (kv8.hpp's code order, a piece being two of these).
+struct TailBlock {
+    kv8_u4 (&k)[8];
+    kv8_u4 (&v)[8];
+
+    __device__ __forceinline__ static int key_at(int i, int lane) {
+        return kv8_key_row(i >> 2, lane & 15) * kHeadDim + 64 * ((i >> 1) & 1) + 16 * (lane >> 4) + 8 * (i & 1);
+    }
+    __device__ __forceinline__ static int value_at(int i, int lane) {
+        return (32 * (i >> 1) + 2 * (lane & 15) + (i & 1)) * kKv8Block + 8 * (lane >> 4);
+    }
+    __device__ __forceinline__ void load(const Kv8Head& h, int lane) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            k[i] = *reinterpret_cast<const kv8_u4*>(h.tail_k + key_at(i, lane));
+            v[i] = *reinterpret_cast<const kv8_u4*>(h.tail_v + value_at(i, lane));
+        }
+    }
+    __device__ __forceinline__ static void expand(kv8_u4 w, float scale, kv8_u4& x, kv8_u4& y) {
+        x = __builtin_bit_cast(kv8_u4, kv8_values(w.x, w.y, (_Float16)scale));
+        y = __builtin_bit_cast(kv8_u4, kv8_values(w.z, w.w, (_Float16)scale));
+    }
+    // What the codes of block b stand for.
+    __device__ __forceinline__ void load_codes(const Kv8Head& h, int b, int lane) {
+        const kv8_u4* c = reinterpret_cast<const kv8_u4*>(h.codes + (size_t)b * kKv8BlockBytes) + lane;
+        const float2 sc = h.scales[b];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            expand(c[64 * i], sc.x, k[2 * i], k[2 * i + 1]);
+            expand(c[64 * (4 + i)], sc.y, v[2 * i], v[2 * i + 1]);
+        }
+    }
+    __device__ __forceinline__ void store(const Kv8Head& h, int rows, int lane) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (kv8_key_row(i >> 2, lane & 15) < rows) *reinterpret_cast<kv8_u4*>(h.tail_k + key_at(i, lane)) = k[i];
+            *reinterpret_cast<kv8_u4*>(h.tail_v + value_at(i, lane)) = v[i];
+        }
+    }
+    // Row r from `row_k`, `row_v` [128].
+    __device__ __forceinline__ void insert(int r, const _Float16* row_k, const _Float16* row_v, int lane) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (kv8_key_row(i >> 2, lane & 15) == r) k[i] = *reinterpret_cast<const kv8_u4*>(row_k + (key_at(i, lane) & (kHeadDim - 1)));
+            const uint32_t y = 0x10001u * __builtin_bit_cast(uint16_t, row_v[value_at(i, lane) / kKv8Block]);
+            const uint32_t half = (lane >> 4) == (r >> 3) ? ((r & 1) ? 0xffff0000u : 0xffffu) : 0u;
+            uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t mask = j == ((r & 7) >> 1) ? half : 0u;
+                w[j] = (w[j] & ~mask) | (y & mask);
+            }
+            v[i] = kv8_u4{w[0], w[1], w[2], w[3]};
+        }
+    }
+    __device__ __forceinline__ static void quantise_part(kv8_u4 (&x)[8], kv8_u4* codes, float& scale) {
+        auto pair = [](uint32_t w) { return __builtin_bit_cast(kv8_half2, w); };
+        kv8_half2 top{};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = kv8_top(kv8_top(kv8_top(kv8_top(top, pair(x[i].x)), pair(x[i].y)), pair(x[i].z)), pair(x[i].w));
+        const int e = kv8_exponent(wave_max(fmaxf((float)top[0], (float)top[1])));
+        const Kv8Inverse inv(e);
+        scale = kv8_power(e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const kv8_u4 a = x[2 * i], b = x[2 * i + 1];
+            const kv8_u4 w = kv8_u4{kv8_word(pair(a.x), pair(a.y), inv), kv8_word(pair(a.z), pair(a.w), inv),
+                                  kv8_word(pair(b.x), pair(b.y), inv), kv8_word(pair(b.z), pair(b.w), inv)};
+            codes[64 * i] = w;
+            expand(w, scale, x[2 * i], x[2 * i + 1]);
+        }
+    }
+    // Codes and scales of the whole block; its values become what these stand for.
+    __device__ __forceinline__ void quantise(const Kv8Head& h, int b, int lane) {
+        kv8_u4* c = reinterpret_cast<kv8_u4*>(h.codes + (size_t)b * kKv8BlockBytes) + lane;
+        float2 sc;
+        quantise_part(k, c, sc.x);
+        quantise_part(v, c + 256, sc.y);
+        if (lane == 0) h.scales[b] = sc;
+    }
+};
+
+// The members' descriptors: in device memory (a captured step's), or in the
+// launch's own arguments, which saves a call the launch that would put them there and
+// the kernel a load that everything else waits for.
+template <bool INLINE> struct Members {
+    __device__ __forceinline__ AttnMember get(const AttnArgs& a, int m) const { return a.mem[m]; }
+};
+template <> struct Members<true> {
+    AttnMember mem[kAttnMaxMembers];
+    __device__ __forceinline__ AttnMember get(const AttnArgs&, int m) const { return mem[m]; }
+};
+
+// How many tokens a member attends: its position's and those before it, or, where
+// the append was dropped or done for several members at once, what the cache holds.
+__device__ __forceinline__ int kv8_tokens(const AttnArgs& a, const AttnMember& mb, const Kv8Head& head, int pos, int& end) {
+    end = pos + 1;
+    if (a.appended || pos >= mb.capacity) end = *head.end;
+    return min(pos + 1, end);
+}
+
+template <int QPK, bool INLINE>
+__global__ __launch_bounds__(kThreads, 3) void kv8_attn_kernel(AttnArgs a, Members<INLINE> members) {
+    constexpr int kHeadsPerWave = (QPK + kWaves - 1) / kWaves;
     __shared__ __attribute__((aligned(16))) _Float16 qs[2][QPK][kRowHalfs];
+    __shared__ __attribute__((aligned(16))) _Float16 fresh[2][kHeadDim];  // the new token's key and value
     __shared__ float qfac[QPK];
     __shared__ float2 st_ml[kWaves][QPK];
     __shared__ float st_o[kWaves][QPK][kHeadDim];
@@ -362,66 +452,111 @@ __global__ __launch_bounds__(kThreads) void kv8_attn_kernel(AttnArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4;
     const int n = lane & 15;
-    const AttnMember mb = a.mem[m];
+    const AttnMember mb = members.get(a, m);
     const int pos = a.positions[m];
+    // loads that need neither go first: the query heads, the norm weights, the new token's row
+    const float* qm = a.q + ((size_t)m * a.q_heads + (size_t)kvh * QPK) * kHeadDim;
+    float qx[kHeadsPerWave][2];
+#pragma unroll
+    for (int i = 0; i < kHeadsPerWave; ++i) {
+        const int h = min(wave + kWaves * i, QPK - 1);
+        qx[i][0] = qm[h * kHeadDim + lane];
+        qx[i][1] = qm[h * kHeadDim + 64 + lane];
+    }
+    const float qw0 = a.q_norm[lane], qw1 = a.q_norm[lane + 64];
+    float nx0 = 0.f, nx1 = 0.f, kw0 = 0.f, kw1 = 0.f;
+    if (wave < 2) {
+        const float* src = (wave == 0 ? a.k : a.v) + ((size_t)m * a.kv_heads + kvh) * kHeadDim;
+        nx0 = src[lane];
+        nx1 = src[lane + 64];
+        kw0 = a.k_norm[lane];
+        kw1 = a.k_norm[lane + 64];
+    }
+
     const Kv8Head head = kv8_head(mb, a.layer, kvh);
-    const int end = *head.end;
-    // (an append past the capacity was dropped: nothing past `end` is read)
-    const int tokens = min(pos + 1, end);
+    int end;
+    const int tokens = kv8_tokens(a, mb, head, pos, end);
+    const bool append = !a.appended && pos < mb.capacity;
     const int len = kv8_chunk_tokens(tokens, a.chunks, a.min_chunk);
     const int t0 = chunk * len;
-    if (t0 >= tokens) return;
+    if (t0 >= tokens) {
+        if (a.chunks == 1) {  // a member without tokens: zeros
+            for (int i = tid; i < QPK * kHeadDim; i += kThreads) a.out[((size_t)m * a.q_heads + (size_t)kvh * QPK) * kHeadDim + i] = 0.f;
+        }
+        return;
+    }
     const int t1 = min(t0 + len, tokens);
 
-    // ---- blocks of this wave: b0 + wave, + kWaves, ... below `coded`; the block
-    // that is not whole, if the chunk reaches it, is the last wave's first
+    // ---- blocks of this wave: b0 + wave, + kWaves, ... below `coded`, whose codes are
+    // in the cache; the one after them, if the chunk reaches it, is the last wave's first
     const int b0 = t0 / kKv8Block;
-    const int coded = min((t1 + kKv8Block - 1) / kKv8Block, end / kKv8Block);
-    const bool tail = t1 > coded * kKv8Block && wave == kWaves - 1;
+    const int coded = min((t1 + kKv8Block - 1) / kKv8Block, (append ? pos : end) / kKv8Block);
+    const bool has_tail = t1 > coded * kKv8Block;
+    const bool tail = has_tail && wave == kWaves - 1;
     const __amdgpu_buffer_rsrc_t cr = make_rsrc(head.codes, (uint32_t)kv8_tail_offset(mb.capacity));
     const __amdgpu_buffer_rsrc_t sr = make_rsrc(head.scales, (uint32_t)(kv8_blocks(mb.capacity) * sizeof(float2)));
-    uint4 kq[kRing][4], vq[kRing][4];
-    float2 sc[kRing];
-    auto issue = [&](int r, int b) {
-        const uint32_t at = b < coded ? (uint32_t)b * kKv8BlockBytes + 16u * (uint32_t)lane : kOOR;
+    // A block's keys (or values) and their scale, 0 or kKv8PartBytes of it.
+    auto issue = [&](int b, int part, kv8_u4 (&w)[8], float& scale) {
+        const uint32_t at = b < coded ? (uint32_t)b * kKv8BlockBytes + (uint32_t)part + 16u * (uint32_t)lane : kOOR;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) kq[r][i] = load_b128(cr, at + 1024u * i);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vq[r][i] = load_b128(cr, at + kKv8PartBytes + 1024u * i);
-        sc[r] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(sr, (int)(b < coded ? 8u * (uint32_t)b : kOOR), 0, 0));
+        for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(kv8_u4, load_b128(cr, at + 1024u * i));
+        scale = __builtin_bit_cast(float, load_b32(sr, b < coded ? 8u * (uint32_t)b + (part ? 4u : 0u) : kOOR));
     };
-#pragma unroll
-    for (int r = 0; r < kRing; ++r) issue(r, b0 + wave + kWaves * r);
-    kv8_half8 tk[8], tv[8];
+    kv8_u4 kq[8], vq[8];  // a block's codes (the first four), or the tail's block
+    float ks = 0.f, vs = 0.f;
+    TailBlock tb{kq, vq};
+    int old_end = 0;
     if (tail) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {  // keys (t, s), values (u, i)
-            tk[i] = *reinterpret_cast<const kv8_half8*>(head.tail_k + kv8_key_row(i >> 2, n) * kHeadDim + 64 * ((i >> 1) & 1) + 16 * g + 8 * (i & 1));
-            tv[i] = *reinterpret_cast<const kv8_half8*>(head.tail_v + (32 * (i >> 1) + 2 * n + (i & 1)) * kKv8Block + 8 * g);
-        }
+        old_end = *head.end;
+        tb.load(head, lane);
+    } else {
+        issue(b0 + wave, 0, kq, ks);
+        issue(b0 + wave, kKv8PartBytes, vq, vs);
     }
 
     // ---- query heads: norm and rope, scaled by a power of two to just below 2
     // (whatever the norm's weights are, the pieces are in f16's range), in pieces
-    const Rot64 rot = table_rot(mb.rope, 64, lane, pos);
-    const float rc = (float)rot.c, rs = (float)rot.s;
-    const float* qm = a.q + ((size_t)m * a.q_heads + (size_t)kvh * QPK) * kHeadDim;
-    for (int h = wave; h < QPK; h += kWaves) {
-        const float x0 = qm[h * kHeadDim + lane], x1 = qm[h * kHeadDim + 64 + lane];
-        const float ssq = wave_sum(x0 * x0 + x1 * x1);
-        const float inv = 1.0f / sqrtf(ssq / (float)kHeadDim + a.eps);
-        const float y0 = x0 * inv * a.q_norm[lane], y1 = x1 * inv * a.q_norm[lane + 64];
-        const float q0 = y0 * rc - y1 * rs, q1 = y0 * rs + y1 * rc;
-        float top = fmaxf(fabsf(q0), fabsf(q1));
+    const Rot64 rot = turn_sincos((double)pos * mb.rope[lane]);
+    const double gain = mb.rope[kHeadDim / 2];
+    const float rc = (float)(rot.c * gain), rs = (float)(rot.s * gain);
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-        const int e = max(-100, min(100, (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127));
-        const float p0 = q0 * kv8_power(-e), p1 = q1 * kv8_power(-e);
-        qs[0][h][lane] = (_Float16)p0;
-        qs[0][h][lane + 64] = (_Float16)p1;
-        qs[1][h][lane] = (_Float16)(p0 - (float)(_Float16)p0);
-        qs[1][h][lane + 64] = (_Float16)(p1 - (float)(_Float16)p1);
-        if (lane == 0) qfac[h] = a.scale * kv8_power(e);
+    for (int i = 0; i < kHeadsPerWave; ++i) {
+        const int h = wave + kWaves * i;
+        if (h < QPK) {
+            const float ssq = wave_sum_uniform(qx[i][0] * qx[i][0] + qx[i][1] * qx[i][1]);
+            const float inv = 1.0f / sqrtf(ssq / (float)kHeadDim + a.eps);
+            const float y0 = qx[i][0] * inv * qw0, y1 = qx[i][1] * inv * qw1;
+            const float q0 = y0 * rc - y1 * rs, q1 = y0 * rs + y1 * rc;
+            const float top = wave_max(fmaxf(fabsf(q0), fabsf(q1)));
+            const int e = max(-100, min(100, (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127));
+            const float p0 = q0 * kv8_power(-e), p1 = q1 * kv8_power(-e);
+            qs[0][h][lane] = (_Float16)p0;
+            qs[0][h][lane + 64] = (_Float16)p1;
+            qs[1][h][lane] = (_Float16)(p0 - (float)(_Float16)p0);
+            qs[1][h][lane + 64] = (_Float16)(p1 - (float)(_Float16)p1);
+            if (lane == 0) qfac[h] = a.scale * kv8_power(e);
+        }
+    }
+    const int row = pos & (kKv8Block - 1);
+    if (append && has_tail && wave < 2) {  // the new token: wave 0 its key (64 bits), wave 1 its value
+        if (wave == 0) {
+            const double x0 = nx0, x1 = nx1;
+            const double ssq = wave_sum64(__builtin_fma(x0, x0, x1 * x1));
+            const double inv = 1.0 / sqrt(ssq / (double)kHeadDim + (double)a.eps);
+            const double y0 = x0 * inv * (double)kw0 * gain, y1 = x1 * inv * (double)kw1 * gain;
+            nx0 = (float)__builtin_fma(y0, rot.c, -y1 * rot.s);
+            nx1 = (float)__builtin_fma(y0, rot.s, y1 * rot.c);
+        }
+        const _Float16 h0 = kv8_half(nx0), h1 = kv8_half(nx1);
+        fresh[wave][lane] = h0;
+        fresh[wave][lane + 64] = h1;
+        if (wave == 0) {
+            head.tail_k[row * kHeadDim + lane] = h0;
+            head.tail_k[row * kHeadDim + 64 + lane] = h1;
+        } else {
+            head.tail_v[lane * kKv8Block + row] = h0;
+            head.tail_v[(lane + 64) * kKv8Block + row] = h1;
+        }
     }
     __syncthreads();
     const int hn = n & 7;
@@ -476,46 +611,56 @@ __global__ __launch_bounds__(kThreads) void kv8_attn_kernel(AttnArgs a) {
     };
 
     if (tail) {
+        const int b = coded;
+        if (append) {
+            // rows before the new one, if the tail has another block's: what the block's codes stand for
+            const bool held = row == 0 || (old_end > 0 && (old_end - 1) / kKv8Block == b);
+            if (__builtin_expect(!held, 0)) tb.load_codes(head, b, lane);
+            tb.insert(row, fresh[0], fresh[1], lane);
+            if (__builtin_expect(!held, 0)) tb.store(head, row + 1, lane);
+            if (__builtin_expect(row == kKv8Block - 1, 0)) tb.quantise(head, b, lane);
+            if (lane == 0) *head.end = pos + 1;
+        }
         kv8_float4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(tk[4 * t + i], qb[i], s[t], 0, 0, 0);
+            for (int t = 0; t < 2; ++t) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(kv8_half8, kq[4 * t + i]), qb[i], s[t], 0, 0, 0);
         kv8_half8 pb;
-        soften(s, fac, end / kKv8Block, pb);
+        soften(s, fac, b, pb);
 #pragma unroll
-        for (int d = 0; d < 8; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(tv[d], pb, o[d], 0, 0, 0);
+        for (int d = 0; d < 8; ++d) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(kv8_half8, vq[d]), pb, o[d], 0, 0, 0);
+        issue(b0 + wave, 0, kq, ks);
+        issue(b0 + wave, kKv8PartBytes, vq, vs);
     }
-    for (int b = b0 + wave; b < coded; b += kWaves * kRing) {
+    // (the next block's keys are under way as soon as this one's are used, its values likewise)
+    for (int b = b0 + wave; b < coded; b += kWaves) {
+        kv8_float4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-        for (int r = 0; r < kRing; ++r) {
-            const int bb = b + kWaves * r;
-            if (bb < coded) {
-                kv8_float4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const uint4 w = kq[r][2 * t + (i >> 1)];
-                        const kv8_half8 k = (i & 1) ? kv8_whole(w.z, w.w) : kv8_whole(w.x, w.y);
-                        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qb[i], s[t], 0, 0, 0);
-                    }
-                }
-                const _Float16 vs = (_Float16)sc[r].y;
-                kv8_half8 pb;
-                soften(s, fac * sc[r].x, bb, pb);
-#pragma unroll
-                for (int d = 0; d < 8; ++d) {
-                    const uint4 w = vq[r][d >> 1];
-                    const kv8_half8 v = (d & 1) ? kv8_values(w.z, w.w, vs) : kv8_values(w.x, w.y, vs);
-                    o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pb, o[d], 0, 0, 0);
-                }
+            for (int t = 0; t < 2; ++t) {
+                const kv8_u4 w = kq[2 * t + (i >> 1)];
+                const kv8_half8 k = (i & 1) ? kv8_whole(w.z, w.w) : kv8_whole(w.x, w.y);
+                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qb[i], s[t], 0, 0, 0);
             }
-            issue(r, bb + kWaves * kRing);
         }
+        const float scaled = fac * ks;
+        issue(b + kWaves, 0, kq, ks);
+        kv8_half8 pb;
+        soften(s, scaled, b, pb);
+        const _Float16 value_scale = (_Float16)vs;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+            const kv8_u4 w = vq[d >> 1];
+            const kv8_half8 v = (d & 1) ? kv8_values(w.z, w.w, value_scale) : kv8_values(w.x, w.y, value_scale);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pb, o[d], 0, 0, 0);
+        }
+        issue(b + kWaves, kKv8PartBytes, vq, vs);
     }
 
-    // ---- the waves' states meet in LDS: the chunk's partial in attn_decode_kernel's layout
+    // ---- the waves' states meet in LDS: the chunk's partial in attn_decode_kernel's
+    // layout, or the output where a launch has one chunk
     lrun += __shfl_xor(lrun, 16, 64);
     lrun += __shfl_xor(lrun, 32, 64);
 #pragma unroll
@@ -541,6 +686,10 @@ __global__ __launch_bounds__(kThreads) void kv8_attn_kernel(AttnArgs a) {
             l = __builtin_fmaf(st_ml[w][h].y, f, l);
             acc = __builtin_fmaf(st_o[w][h][d], f, acc);
         }
+        if (a.chunks == 1) {
+            a.out[((size_t)m * a.q_heads + (size_t)kvh * QPK) * kHeadDim + i] = acc / l;
+            continue;
+        }
         float* part = own + ((size_t)(kvh * QPK + h) * kAttnChunks + chunk) * kPartStride;
         part[d] = acc;
         if (d == 0) {
@@ -550,28 +699,70 @@ __global__ __launch_bounds__(kThreads) void kv8_attn_kernel(AttnArgs a) {
     }
 }
 
-// The chunks' partials of a (query head, member) merged in chunk order. A
-// member without tokens (a negative position) gets zeros.
-__global__ __launch_bounds__(kHeadDim) void kv8_combine_kernel(AttnArgs a) {
+// The chunks' partials of a (query head, member) merged. 32 lanes hold a row's
+// 128 sums (four each) and take the chunks c, c + 4, ... of the launch's NC or
+// fewer; every slot the launch can hold is loaded before the position says which
+// are live (the others hold stale memory). The four runs meet in LDS in order: a dead
+// slot adds exact zeros, so a member's bits do not depend on NC. A member without
+// tokens (a negative position) gets zeros.
+template <int NC, bool INLINE>
+__global__ __launch_bounds__(128) void kv8_combine_kernel(AttnArgs a, Members<INLINE> members) {
+    constexpr int kRun = NC / 4;
+    __shared__ float4 so[4][32];
+    __shared__ float2 sml[4];
     const int qh = blockIdx.x;
     const int m = blockIdx.y;
-    const int d = threadIdx.x;
-    const AttnMember mb = a.mem[m];
-    const int end = *kv8_head(mb, a.layer, qh / (a.q_heads / a.kv_heads)).end;
-    const int tokens = min(a.positions[m] + 1, end);
+    const int run = (int)threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const AttnMember mb = members.get(a, m);
+    const float* own = a.partials != nullptr ? a.partials + (size_t)m * a.partial_floats : mb.partials;
+    const __amdgpu_buffer_rsrc_t pr =
+        make_rsrc(own + (size_t)qh * kAttnChunks * kPartStride, (uint32_t)(a.chunks * kPartStride * 4));
+    float4 o[kRun];
+    float2 ml[kRun];
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+        const uint32_t row = (uint32_t)((4 * i + run) * kPartStride) * 4u;
+        o[i] = __builtin_bit_cast(float4, load_b128(pr, row + 16u * (uint32_t)lane));
+        ml[i] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(pr, (int)(row + kHeadDim * 4), 0, 0));
+    }
+    int end;
+    const int tokens = kv8_tokens(a, mb, kv8_head(mb, a.layer, qh / (a.q_heads / a.kv_heads)), a.positions[m], end);
     const int len = kv8_chunk_tokens(tokens, a.chunks, a.min_chunk);
     const int chunks = tokens > 0 ? (tokens + len - 1) / len : 0;
-    const float* part = (a.partials != nullptr ? a.partials + (size_t)m * a.partial_floats : mb.partials) +
-                        (size_t)qh * kAttnChunks * kPartStride;
     float mx = -FLT_MAX;
-    for (int c = 0; c < chunks; ++c) mx = fmaxf(mx, part[c * kPartStride + kHeadDim]);
-    float l = 0.f, acc = 0.f;
-    for (int c = 0; c < chunks; ++c) {
-        const float f = __builtin_amdgcn_exp2f(part[c * kPartStride + kHeadDim] - mx);
-        l = __builtin_fmaf(part[c * kPartStride + kHeadDim + 1], f, l);
-        acc = __builtin_fmaf(part[c * kPartStride + d], f, acc);
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+        const bool live = 4 * i + run < chunks;
+        ml[i] = live ? ml[i] : make_float2(-FLT_MAX, 0.f);
+        o[i] = live ? o[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+        mx = fmaxf(mx, ml[i].x);
     }
-    a.out[((size_t)m * a.q_heads + qh) * kHeadDim + d] = chunks > 0 ? acc / l : 0.f;
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+        const float f = __builtin_amdgcn_exp2f(ml[i].x - mx);
+        l = __builtin_fmaf(ml[i].y, f, l);
+        acc.x = __builtin_fmaf(o[i].x, f, acc.x);
+        acc.y = __builtin_fmaf(o[i].y, f, acc.y);
+        acc.z = __builtin_fmaf(o[i].z, f, acc.z);
+        acc.w = __builtin_fmaf(o[i].w, f, acc.w);
+    }
+    so[run][lane] = acc;
+    if (lane == 0) sml[run] = make_float2(mx, l);
+    __syncthreads();
+    const int d = threadIdx.x;
+    mx = fmaxf(fmaxf(sml[0].x, sml[1].x), fmaxf(sml[2].x, sml[3].x));
+    l = 0.f;
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const float f = __builtin_amdgcn_exp2f(sml[r].x - mx);
+        l = __builtin_fmaf(sml[r].y, f, l);
+        sum = __builtin_fmaf(reinterpret_cast<const float*>(so[r])[d], f, sum);
+    }
+    a.out[((size_t)m * a.q_heads + qh) * kHeadDim + d] = chunks > 0 ? sum / l : 0.f;
 }
 
 }  // namespace
@@ -597,8 +788,7 @@ hipError_t launch_kv8_append(const AttnArgs& a, int members, hipStream_t stream)
     if (members < 1 || members > kAttnMaxMembers || a.kv_heads < 1 || a.mem == nullptr) return hipErrorInvalidValue;
     // consecutive positions touch at most one block more than they fill
     const int blocks = (members + kKv8Block - 2) / kKv8Block + 1;
-    hipLaunchKernelGGL(kv8_append_kernel, dim3((unsigned)a.kv_heads, (unsigned)(a.appended ? blocks : members)), dim3(256), 0,
-                       stream, a, a.appended ? members : 0);
+    hipLaunchKernelGGL(kv8_append_kernel, dim3((unsigned)a.kv_heads, (unsigned)blocks), dim3(256), 0, stream, a, members);
     return hipGetLastError();
 }
 
@@ -609,25 +799,38 @@ hipError_t launch_kv8_append_seq(const PrefillAttnArgs& a, hipStream_t stream) {
     return hipGetLastError();
 }
 
-hipError_t launch_kv8_attention(const AttnArgs& args, int members, hipStream_t stream) {
+namespace {
+template <bool INLINE>
+hipError_t launch_members(const AttnArgs& b, const Members<INLINE>& mem, int members, hipStream_t stream) {
+    const dim3 grid((unsigned)b.chunks, (unsigned)b.kv_heads, (unsigned)members);
+    switch (b.q_heads / b.kv_heads) {
+    case 1: hipLaunchKernelGGL((kv8_attn_kernel<1, INLINE>), grid, dim3(kThreads), 0, stream, b, mem); break;
+    case 2: hipLaunchKernelGGL((kv8_attn_kernel<2, INLINE>), grid, dim3(kThreads), 0, stream, b, mem); break;
+    case 4: hipLaunchKernelGGL((kv8_attn_kernel<4, INLINE>), grid, dim3(kThreads), 0, stream, b, mem); break;
+    case 8: hipLaunchKernelGGL((kv8_attn_kernel<8, INLINE>), grid, dim3(kThreads), 0, stream, b, mem); break;
+    default: return hipErrorInvalidValue;
+    }
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || b.chunks == 1) return e;
+    const dim3 rows((unsigned)b.q_heads, (unsigned)members);
+    static_assert(kAttnChunks == 32, "the merge's forms cover the grid's chunks");
+    if (b.chunks <= 8) hipLaunchKernelGGL((kv8_combine_kernel<8, INLINE>), rows, dim3(128), 0, stream, b, mem);
+    else hipLaunchKernelGGL((kv8_combine_kernel<32, INLINE>), rows, dim3(128), 0, stream, b, mem);
+    return hipGetLastError();
+}
+}  // namespace
+
+hipError_t launch_kv8_attention(const AttnArgs& args, const AttnMember* host_mem, int members, hipStream_t stream) {
     if (members < 1 || members > kAttnMaxMembers || args.kv_heads < 1 || args.q_heads % args.kv_heads != 0 ||
-        args.chunks < 1 || args.chunks > kAttnChunks || args.mem == nullptr) {
+        args.chunks < 1 || args.chunks > kAttnChunks || (args.mem == nullptr && (host_mem == nullptr || args.appended))) {
         return hipErrorInvalidValue;
     }
     AttnArgs b = args;
     b.min_chunk = kv8_min_chunk(members);
-    const dim3 grid((unsigned)b.chunks, (unsigned)b.kv_heads, (unsigned)members);
-    switch (b.q_heads / b.kv_heads) {
-    case 1: hipLaunchKernelGGL(kv8_attn_kernel<1>, grid, dim3(kThreads), 0, stream, b); break;
-    case 2: hipLaunchKernelGGL(kv8_attn_kernel<2>, grid, dim3(kThreads), 0, stream, b); break;
-    case 4: hipLaunchKernelGGL(kv8_attn_kernel<4>, grid, dim3(kThreads), 0, stream, b); break;
-    case 8: hipLaunchKernelGGL(kv8_attn_kernel<8>, grid, dim3(kThreads), 0, stream, b); break;
-    default: return hipErrorInvalidValue;
-    }
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kv8_combine_kernel, dim3((unsigned)b.q_heads, (unsigned)members), dim3(kHeadDim), 0, stream, b);
-    return hipGetLastError();
+    if (host_mem == nullptr) return launch_members<false>(b, Members<false>{}, members, stream);
+    Members<true> mem;
+    std::copy(host_mem, host_mem + members, mem.mem);
+    return launch_members<true>(b, mem, members, stream);
 }
 
 namespace {

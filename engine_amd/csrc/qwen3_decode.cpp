@@ -285,17 +285,19 @@ hipError_t wave_shared(const ribn_amd_qwen3_decode* d, const ribn_amd_quantized_
 // kAttnMaxMembers; `appended` first stores the launch's members' K/V.
 // With `partials` set, member m's attention partials live at partials +
 // m * attn_partials_floats (the decoder's own buffer, whose address the merge
-// launch then takes from its arguments); else in the descriptors.
+// launch then takes from its arguments); else in the descriptors. `host_mem`
+// (8-bit caches): descriptors in host memory instead.
 hipError_t attention(const ribn_amd_qwen3_config& cfg, const ribn_amd::AttnMember* mem, int kind, int chunks, bool appended,
                      int members, uint32_t layer, const float* q, const float* k, const float* v, const float* q_norm,
-                     const float* k_norm, const int32_t* positions, float* out, float* partials, hipStream_t stream) {
+                     const float* k_norm, const int32_t* positions, float* out, float* partials, hipStream_t stream,
+                     const ribn_amd::AttnMember* host_mem = nullptr) {
     const size_t part = ribn_amd::attn_partials_floats((int)cfg.q_heads);
     const size_t qdim = (size_t)cfg.q_heads * cfg.head_dim;
     const size_t kvdim = (size_t)cfg.kv_heads * cfg.head_dim;
     for (int m0 = 0; m0 < members; m0 += ribn_amd::kAttnMaxMembers) {
         const int mc = std::min(ribn_amd::kAttnMaxMembers, members - m0);
         ribn_amd::AttnArgs a{};
-        a.mem = mem + m0;
+        a.mem = mem != nullptr ? mem + m0 : nullptr;
         a.layer = (int)layer;
         a.chunks = chunks;
         a.appended = appended ? 1 : 0;
@@ -317,8 +319,8 @@ hipError_t attention(const ribn_amd_qwen3_config& cfg, const ribn_amd::AttnMembe
         const bool table = kind == ribn_amd::kCacheF16Table;
         hipError_t e = hipSuccess;
         if (kind == ribn_amd::kCacheI8) {
-            e = ribn_amd::launch_kv8_append(a, mc, stream);
-            if (e == hipSuccess) e = ribn_amd::launch_kv8_attention(a, mc, stream);
+            if (appended) e = ribn_amd::launch_kv8_append(a, mc, stream);
+            if (e == hipSuccess) e = ribn_amd::launch_kv8_attention(a, host_mem != nullptr ? host_mem + m0 : nullptr, mc, stream);
         } else {
             if (appended) e = ribn_amd::launch_kv_append(a, mc, stream, table);
             if (e == hipSuccess) e = ribn_amd::launch_attention(a, mc, stream, table);
@@ -1033,6 +1035,18 @@ ribn_amd_status ribn_amd_attention_decode(ribn_amd_context* ctx, const ribn_amd_
                     output_len, want);
     }
     DeviceGuard guard(ctx->device);
+    const int kind = caches[0]->kind;
+    if (kind == ribn_amd::kCacheI8) {
+        ribn_amd::AttnMember host_mem[RIBN_AMD_MAX_BATCH_MEMBERS];
+        int max_capacity = 1;
+        for (size_t m = 0; m < members; ++m) {
+            host_mem[m] = descriptor(caches[m], caches[m]->partials);
+            max_capacity = std::max(max_capacity, (int)caches[m]->capacity);
+        }
+        const hipError_t e = attention(*config, nullptr, kind, grid_chunks(kind, max_capacity, (int)members), false, (int)members,
+                                       layer, q, k, v, q_norm, k_norm, positions, output, nullptr, ctx->stream, host_mem);
+        return e == hipSuccess ? ok() : driver(e, "launch attention");
+    }
     // the members' descriptors go to the context's descriptor array, in
     // stream order ahead of the launches that read them
     auto* mem = static_cast<ribn_amd::AttnMember*>(ctx->attn_members);
@@ -1050,7 +1064,6 @@ ribn_amd_status ribn_amd_attention_decode(ribn_amd_context* ctx, const ribn_amd_
     }
     // Positions are device values: the kernel checks them against each cache
     // and drops an append past its capacity.
-    const int kind = caches[0]->kind;
     const int chunks = grid_chunks(kind, max_capacity, (int)members);
     hipError_t e = attention(*config, mem, kind, chunks, false, (int)members, layer, q, k, v, q_norm, k_norm, positions,
                              output, nullptr, ctx->stream);
