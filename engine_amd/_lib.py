@@ -188,7 +188,7 @@ SIGNATURES = {
                                          ctypes.POINTER(ctypes.c_double)]),
     "ribn_amd_rope_create": (_i32, [_vp, ctypes.POINTER(RopeSpec), _pvp]),
     "ribn_amd_rope_destroy": (None, [_vp]),
-    "ribn_amd_rope_execute": (_i32, [_vp, _vp, _sz, ctypes.POINTER(RopeRows), _sz, _u32]),
+    "ribn_amd_rope_execute": (_i32, [_vp, _vp, _sz, _vp, _sz, _u32]),
     "ribn_amd_kv_cache_create_with": (_i32, [_vp, ctypes.POINTER(Qwen3Config), _u32, ctypes.POINTER(KvOptions), _pvp]),
     "ribn_amd_kv_cache_format": (_u32, [_vp]),
     "ribn_amd_kv_bytes": (_u64, [ctypes.POINTER(Qwen3Config), _u32, _u32]),

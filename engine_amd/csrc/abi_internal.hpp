@@ -19,6 +19,7 @@ struct ribn_amd_context {
     size_t workspace_bytes;
     void* act_scratch;  // packed activations of the matrix-core batched GEMV, reserved at creation
     void* attn_members; // cache descriptors of the standalone attention call (same allocation)
+    float* split_partials; // prompt attention's partial rows (kPrefillPartialRows), from the first 8-bit cache on
     // Owner handle plus every decoder and dispatcher built on the context: the
     // device resources are released when the last of them lets go, so handles
     // may be destroyed in any order (e.g. by a garbage collector).

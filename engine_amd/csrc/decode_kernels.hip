@@ -853,7 +853,11 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
             }
         }
     };
-    issue(0);
+    // the key blocks of this workgroup: all of them, or its share (PrefillAttnArgs::splits)
+    const int blocks = last / kPfKeys + 1;
+    const int kb0 = CACHE == kCacheI8 ? blocks * (int)blockIdx.z / a.splits : 0;
+    const int kb1 = CACHE == kCacheI8 ? blocks * ((int)blockIdx.z + 1) / a.splits : blocks;
+    issue(kb0);
 
     // ---- rope angles of the workgroup's tokens, shared by its QPK query
     // heads: entry (row, d) = the rotation of pair (d, d + 64) at position
@@ -933,12 +937,11 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
     pf_float4 o[8];
 #pragma unroll
     for (int d = 0; d < 8; ++d) o[d] = pf_float4{0.f, 0.f, 0.f, 0.f};
-    const int blocks = last / kPfKeys + 1;
-    stage(0, 0);
+    stage(0, kb0);
     __syncthreads();
-    for (int kb = 0; kb < blocks; ++kb) {
-        const int buf = kb & 1;
-        if (kb + 1 < blocks) issue(kb + 1);
+    for (int kb = kb0; kb < kb1; ++kb) {
+        const int buf = (kb - kb0) & 1;
+        if (kb + 1 < kb1) issue(kb + 1);
 
         // S^T for the block's four 16-key tiles, issued tile-interleaved:
         // consecutive MFMAs feed different accumulators
@@ -1036,7 +1039,7 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
         }
         // the next block into the other buffer: every wave finished reading
         // it before the previous barrier
-        if (kb + 1 < blocks) stage(buf ^ 1, kb + 1);
+        if (kb + 1 < kb1) stage(buf ^ 1, kb + 1);
         __syncthreads();
     }
 
@@ -1058,12 +1061,26 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
     float l_tot = l_run + __shfl_xor(l_run, 16, 64);
     l_tot += __shfl_xor(l_tot, 32, 64);
     if (!live) return;
+    if (CACHE == kCacheI8 && a.splits > 1) {
+        float* part = a.partials + (((size_t)t * a.q_heads + hq) * a.splits + blockIdx.z) * kPartStride;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) *reinterpret_cast<float4*>(part + 16 * d + 4 * g) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
+        if (g == 0) *reinterpret_cast<float2*>(part + kHeadDim) = make_float2(m_run, l_tot);
+        return;
+    }
     float* dst = a.out + (size_t)t * qdim + (size_t)hq * kHeadDim + 4 * g;
 #pragma unroll
     for (int d = 0; d < 8; ++d) {
         *reinterpret_cast<float4*>(dst + 16 * d) =
             make_float4(o[d][0] / l_tot, o[d][1] / l_tot, o[d][2] / l_tot, o[d][3] / l_tot);
     }
+}
+
+// The key shares of a (token, query head) merged. A share whose keys the token does
+// not reach has a denominator of 0 and the lowest maximum.
+__global__ __launch_bounds__(128) void prefill_merge_kernel(const float* partials, float* out, int splits) {
+    const size_t row = blockIdx.x;
+    merge_row<32>(partials + row * (size_t)splits * kPartStride, splits, [&] { return splits; }, out + row * kHeadDim);
 }
 
 // attn_prefill_wide_kernel: causal attention of a prompt chunk on the matrix cores
@@ -1636,16 +1653,36 @@ bool wide_prefill(const PrefillAttnArgs& a, int tiles, int cu_count) {
     return 16 * tiles * a.kv_heads >= (qpk == 1 ? 4 : qpk == 8 ? 16 : 11) * cu_count;
 }
 
+// Key shares of a narrow launch over an 8-bit cache: few tokens over a long
+// context leave most CUs without a workgroup and the others with every key block in
+// turn (37 tokens after 2,011, 32 / 8 heads: 24 workgroups, 59 us). Shares of at least
+// kMinShare blocks, as many as two workgroups a CU take, the partials' room and the
+// merge's 32 lanes allow.
+constexpr int kMinShare = 2;
+int prefill_splits(const PrefillAttnArgs& a, int tiles, int cu_count) {
+    if (a.partials == nullptr) return 1;
+    const int blocks = (a.p0 + a.tokens - 1) / kPfKeys + 1;
+    const int fill = 2 * cu_count / (tiles * a.kv_heads);
+    const size_t room = a.partial_rows / ((size_t)a.tokens * a.q_heads);
+    return std::max(1, std::min(std::min(32, fill), std::min(blocks / kMinShare, (int)std::min<size_t>(room, 32))));
+}
+
 template <int QPK, int CACHE>
-hipError_t launch_prefill_heads(const PrefillAttnArgs& a, int cu_count, hipStream_t stream) {
+hipError_t launch_prefill_heads(const PrefillAttnArgs& args, int cu_count, hipStream_t stream) {
     constexpr int TT = QPK < 4 ? 4 / QPK : 1;  // token tiles per workgroup
+    PrefillAttnArgs a = args;
     const int wide = (a.tokens + kPrefillWideTokens * TT - 1) / (kPrefillWideTokens * TT);
     if (wide_prefill(a, wide, cu_count)) {
         hipLaunchKernelGGL((attn_prefill_wide_kernel<QPK, CACHE>), dim3((unsigned)wide * (unsigned)a.kv_heads), dim3(512), 0, stream, a, wide);
-    } else {
-        const int tiles = (a.tokens + kPrefillTileTokens * TT - 1) / (kPrefillTileTokens * TT);
-        hipLaunchKernelGGL((attn_prefill_kernel<QPK, CACHE>), dim3((unsigned)tiles, (unsigned)a.kv_heads), dim3(QPK < 8 ? 256 : 512), 0, stream, a);
+        return hipGetLastError();
     }
+    const int tiles = (a.tokens + kPrefillTileTokens * TT - 1) / (kPrefillTileTokens * TT);
+    a.splits = CACHE == kCacheI8 ? prefill_splits(a, tiles, cu_count) : 1;
+    hipLaunchKernelGGL((attn_prefill_kernel<QPK, CACHE>), dim3((unsigned)tiles, (unsigned)a.kv_heads, (unsigned)a.splits), dim3(QPK < 8 ? 256 : 512), 0, stream, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.splits == 1) return e;
+    const size_t rows = (size_t)a.tokens * a.q_heads;
+    hipLaunchKernelGGL(prefill_merge_kernel, dim3((unsigned)rows), dim3(128), 0, stream, a.partials, a.out, a.splits);
     return hipGetLastError();
 }
 

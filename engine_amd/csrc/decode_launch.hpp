@@ -128,7 +128,12 @@ struct PrefillAttnArgs {
     float eps;
     float rope_base;
     float scale;           // log2(e) / sqrt(head_dim)
+    float* partials;       // room for partial_rows rows of kPartStride floats, or null: 8-bit caches' launches of few
+    size_t partial_rows;   // tokens split the keys over workgroups there and merge the shares
+    int splits;            // launch_prefill_attention sets it
 };
+// Partial rows a context keeps for that (17 MB): two workgroups a CU of 64 rows each.
+constexpr size_t kPrefillPartialRows = 2 * 256 * 64;
 
 // Tokens a prompt-attention wave covers (its wide form: many tokens).
 constexpr int kPrefillTileTokens = 16;

@@ -1,6 +1,7 @@
 // Device-side helpers of the 8-bit KV cache (kv8.hpp has its layout).
 #pragma once
 
+#include <float.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -131,6 +132,65 @@ __device__ __forceinline__ Kv8Head kv8_head(const AttnMember& m, int layer, int 
     h.scales = reinterpret_cast<float2*>(base + kv8_scales_offset(m.capacity));
     h.end = reinterpret_cast<int32_t*>(base + kv8_end_offset(m.capacity));
     return h;
+}
+
+// One row's partials (kPartStride floats each: 128 sums, their maximum in log2
+// units, their denominator) merged by a workgroup of 128 threads:
+//   o = sum_s O_s 2^(m_s - M) / sum_s L_s 2^(m_s - M).
+// 32 lanes hold a partial's sums (four each) and take the slots s, s + 4, ... of NC
+// or fewer (`slots` in memory, the others are not read), all loaded at once; `live()`,
+// called after the loads are out, says how many count. The four runs meet in LDS in
+// order. A slot that does not count adds exact zeros, so the bits do not depend on NC. No slots: zeros.
+template <int NC, class LIVE>
+__device__ __forceinline__ void merge_row(const float* partials, int slots, LIVE live, float* out) {
+    constexpr int kRun = NC / 4;
+    __shared__ float4 so[4][32];
+    __shared__ float2 sml[4];
+    const int run = (int)threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    const __amdgpu_buffer_rsrc_t pr = make_rsrc(partials, (uint32_t)(slots * kPartStride * 4));
+    float4 o[kRun];
+    float2 ml[kRun];
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+        const uint32_t row = (uint32_t)((4 * i + run) * kPartStride) * 4u;
+        o[i] = __builtin_bit_cast(float4, load_b128(pr, row + 16u * (uint32_t)lane));
+        ml[i] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(pr, (int)(row + kHeadDim * 4), 0, 0));
+    }
+    const int count = live();
+    float mx = -FLT_MAX;
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+        const bool counts = 4 * i + run < count;
+        ml[i] = counts ? ml[i] : make_float2(-FLT_MAX, 0.f);
+        o[i] = counts ? o[i] : make_float4(0.f, 0.f, 0.f, 0.f);
+        mx = fmaxf(mx, ml[i].x);
+    }
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+        const float f = __builtin_amdgcn_exp2f(ml[i].x - mx);
+        l = __builtin_fmaf(ml[i].y, f, l);
+        acc.x = __builtin_fmaf(o[i].x, f, acc.x);
+        acc.y = __builtin_fmaf(o[i].y, f, acc.y);
+        acc.z = __builtin_fmaf(o[i].z, f, acc.z);
+        acc.w = __builtin_fmaf(o[i].w, f, acc.w);
+    }
+    so[run][lane] = acc;
+    if (lane == 0) sml[run] = make_float2(mx, l);
+    __syncthreads();
+    const int d = threadIdx.x;
+    mx = fmaxf(fmaxf(sml[0].x, sml[1].x), fmaxf(sml[2].x, sml[3].x));
+    l = 0.f;
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const float f = __builtin_amdgcn_exp2f(sml[r].x - mx);
+        l = __builtin_fmaf(sml[r].y, f, l);
+        sum = __builtin_fmaf(reinterpret_cast<const float*>(so[r])[d], f, sum);
+    }
+    out[d] = count > 0 ? sum / l : 0.f;
 }
 
 }  // namespace ribn_amd

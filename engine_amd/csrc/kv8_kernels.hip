@@ -23,10 +23,14 @@ constexpr int kRowHalfs = kHeadDim + 8;  // LDS row of a staged token (272 B: 16
 // One workgroup a (KV head, block of 32 positions). The block's new rows are
 // staged in LDS as f16; a block that is whole after the append has its earlier
 // rows added (from the tail, or from the codes of a block taken back into), its
-// two scales found and its codes written, 16 of keys and 16 of values a
-// thread. Workgroup 0, which reads the tail as it was, also writes what the
-// tail holds after the call (the last block's rows) and `end`: no other one touches
-// them. Traffic is the rows in (f32) and a byte a value out.
+// two scales found and its codes written, 16 of keys or of values a thread. The
+// last block's workgroup writes what the tail holds after the call (its rows)
+// and `end`, unless workgroup 0 may read the tail as it was (an append into the middle
+// of a block): then that one does both, after its own block. Traffic is the rows in
+// (f32) and a byte a value out.
+
+constexpr int kAppendThreads = 512;  // 16 lanes a row, a block's rows at once
+__device__ __forceinline__ int append_tid() { return threadIdx.x & (kAppendThreads - 1); }
 
 struct Rows {
     const void* k;    // the head's first row
@@ -40,133 +44,182 @@ constexpr int kRowsRaw = 0, kRowsF32 = 1, kRowsF16 = 2;
 struct Stage {
     _Float16 k[kKv8Block][kRowHalfs];
     _Float16 v[kKv8Block][kRowHalfs];
-    float amax[2][4];
+    float amax[8];
 };
 
+// The value of lane ^ 8 within a row of 16 lanes (row_ror 8).
+__device__ __forceinline__ double other_half64(double v) {
+    const uint2 w = __builtin_bit_cast(uint2, v);
+    return __builtin_bit_cast(double, make_uint2((uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.x, 0x128, 0xf, 0xf, false),
+                                                 (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.y, 0x128, 0xf, 0xf, false)));
+}
+
+// Eight values of a row as a cache takes them.
+__device__ __forceinline__ kv8_half8 cache_halfs(const float (&x)[8]) {
+    kv8_half8 h;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h[j] = kv8_half(x[j]);
+    return h;
+}
+__device__ __forceinline__ kv8_half8 cache_halfs(uint4 w) {
+    auto special = [](uint32_t v) { return ((v & 0x7fff7fffu) + 0x04000400u) & 0x80008000u; };  // a half that is not finite
+    kv8_half8 h = __builtin_bit_cast(kv8_half8, w);
+    if (__builtin_expect((special(w.x) | special(w.y) | special(w.z) | special(w.w)) != 0, 0)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[j] = kv8_half((float)h[j]);
+    }
+    return h;
+}
+
+// 1 / sqrt(x) of a normal x in 64 bits: the hardware's estimate (about 2^-23) and
+// two Newton steps, y (3 - x y^2) / 2, where sqrt and a division take some 50 instructions.
+__device__ __forceinline__ double inverse_root(double x) {
+    double y = __builtin_amdgcn_rsq(x);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) y = y * __builtin_fma(-0.5 * x * y, y, 1.5);
+    return y;
+}
+
+// 16 lanes a row: lane c holds dims 8c .. 8c + 7 of row threadIdx / 16.
 template <int ROWS>
 __device__ __forceinline__ void stage_rows(Stage& st, const Rows& in, int first, int count, int row0, const float* k_norm,
                                            double eps, const double* rope, int position) {
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    double w0 = 1.0, w1 = 1.0, turns = 0.0, gain = 1.0;
-    if constexpr (ROWS == kRowsRaw) {
-        w0 = k_norm[lane];
-        w1 = k_norm[lane + 64];
-        turns = rope[lane];
-        gain = rope[64];
+    constexpr int kWords = ROWS == kRowsF16 ? 1 : 2;  // 16-byte pieces of a lane's eight values
+    const int c = append_tid() & 15;
+    const int i = append_tid() >> 4;
+    if (i >= count) return;
+    uint4 kw[kWords], vw[kWords];
+    const size_t at = ((size_t)(first + i) * in.stride + 8 * c) * (ROWS == kRowsF16 ? 2 : 4);
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+        kw[w] = reinterpret_cast<const uint4*>(static_cast<const char*>(in.k) + at)[w];
+        vw[w] = reinterpret_cast<const uint4*>(static_cast<const char*>(in.v) + at)[w];
     }
-    for (int i = wave; i < count; i += 4) {
-        const size_t at = (size_t)(first + i) * in.stride;
-        float k0, k1, v0, v1;
-        if constexpr (ROWS == kRowsF16) {
-            const _Float16* k = static_cast<const _Float16*>(in.k) + at;
-            const _Float16* v = static_cast<const _Float16*>(in.v) + at;
-            k0 = k[lane]; k1 = k[lane + 64];
-            v0 = v[lane]; v1 = v[lane + 64];
-        } else {
-            const float* k = static_cast<const float*>(in.k) + at;
-            const float* v = static_cast<const float*>(in.v) + at;
-            k0 = k[lane]; k1 = k[lane + 64];
-            v0 = v[lane]; v1 = v[lane + 64];
-        }
+    if constexpr (ROWS == kRowsF16) {
+        *reinterpret_cast<kv8_half8*>(&st.k[row0 + i][8 * c]) = cache_halfs(kw[0]);
+        *reinterpret_cast<kv8_half8*>(&st.v[row0 + i][8 * c]) = cache_halfs(vw[0]);
+    } else {
+        float k[8], v[8];
+        __builtin_memcpy(k, kw, 32);
+        __builtin_memcpy(v, vw, 32);
         if constexpr (ROWS == kRowsRaw) {
             // 64 bits up to the one rounding to f32: where a key falls between two
-            // codes then does not depend on the order of a sum
-            const double x0 = k0, x1 = k1;
-            const double ssq = wave_sum64(__builtin_fma(x0, x0, x1 * x1));
-            const double inv = 1.0 / sqrt(ssq / (double)kHeadDim + eps);
-            const Rot64 r = turn_sincos((double)(position + i) * turns);
-            const double y0 = x0 * inv * w0 * gain, y1 = x1 * inv * w1 * gain;
-            k0 = (float)__builtin_fma(y0, r.c, -y1 * r.s);
-            k1 = (float)__builtin_fma(y0, r.s, y1 * r.c);
+            // codes then does not depend on the order of a sum. Lanes c and c ^ 8 hold the
+            // two dims of the same eight pairs and form four of their angles each.
+            const int upper = c >> 3;
+            Rot64 mine[4], theirs[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                mine[j] = turn_sincos((double)(position + i) * rope[8 * (c & 7) + 4 * upper + j]);
+                theirs[j].s = other_half64(mine[j].s);
+                theirs[j].c = other_half64(mine[j].c);
+            }
+            double ssq = 0.0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ssq = __builtin_fma((double)k[j], (double)k[j], ssq);
+            const double inv = inverse_root(row_sum64(ssq) * (1.0 / kHeadDim) + eps) * rope[kHeadDim / 2];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const Rot64 r = (j >> 2) == upper ? mine[j & 3] : theirs[j & 3];
+                const double y = (double)k[j] * inv * (double)k_norm[8 * c + j];
+                const double o = other_half64(y) * r.s;
+                k[j] = (float)__builtin_fma(y, r.c, upper ? o : -o);
+            }
         }
-        st.k[row0 + i][lane] = kv8_half(k0);
-        st.k[row0 + i][lane + 64] = kv8_half(k1);
-        st.v[row0 + i][lane] = kv8_half(v0);
-        st.v[row0 + i][lane + 64] = kv8_half(v1);
+        *reinterpret_cast<kv8_half8*>(&st.k[row0 + i][8 * c]) = cache_halfs(k);
+        *reinterpret_cast<kv8_half8*>(&st.v[row0 + i][8 * c]) = cache_halfs(v);
     }
 }
 
 // Rows 0 .. count - 1 of block b as the cache has them, from its tail or its codes.
 __device__ __forceinline__ void stage_held(Stage& st, const Kv8Head& h, int b, int count, bool tail) {
-    const int tid = threadIdx.x;
+    const int tid = append_tid();
     if (tail) {
-        for (int i = tid; i < count * kHeadDim; i += 256) {
-            st.k[i >> 7][i & 127] = h.tail_k[i];
-            st.v[i >> 7][i & 127] = h.tail_v[(i & 127) * kKv8Block + (i >> 7)];
-        }
+        if (tid < count * 16) *reinterpret_cast<uint4*>(&st.k[tid >> 4][8 * (tid & 15)]) = reinterpret_cast<const uint4*>(h.tail_k)[tid];
+        const int dim = tid >> 2, key = 8 * (tid & 3);  // eight keys of a dim
+        const kv8_half8 x = *reinterpret_cast<const kv8_half8*>(h.tail_v + dim * kKv8Block + key);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (key + j < count) st.v[key + j][dim] = x[j];
         return;
     }
-    const uint8_t* codes = h.codes + (size_t)b * kKv8BlockBytes;
+    // a thread's piece: 256 of keys, then 256 of values, as the codes lie
+    const uint4 w = reinterpret_cast<const uint4*>(h.codes + (size_t)b * kKv8BlockBytes)[tid];
     const float2 sc = h.scales[b];
-    const int lane = tid & 63, g = lane >> 4, m = lane & 15;
-    const int row = kv8_key_row(tid >> 7, m);
-    for (int j = 0; j < 16; ++j) {
-        const int dim = 64 * ((tid >> 6) & 1) + 16 * g + j;
-        if (row < count) st.k[row][dim] = (_Float16)((float)((int)codes[tid * 16 + j] - 128) * sc.x);
-        const int key = 8 * g + (j & 7), vd = 32 * (tid >> 6) + 2 * m + (j >> 3);
-        if (key < count) st.v[key][vd] = (_Float16)((float)((int)codes[kKv8PartBytes + tid * 16 + j] - 128) * sc.y);
+    const bool keys = tid < 256;
+    const int lane = tid & 63, u = (tid >> 6) & 3, g = lane >> 4, m = lane & 15;
+    const _Float16 scale = (_Float16)(keys ? sc.x : sc.y);
+    const kv8_half8 x0 = kv8_values(w.x, w.y, scale), x1 = kv8_values(w.z, w.w, scale);
+    if (keys) {
+        const int row = kv8_key_row(u >> 1, m);
+        if (row < count) {
+            kv8_half8* k = reinterpret_cast<kv8_half8*>(&st.k[row][64 * (u & 1) + 16 * g]);
+            k[0] = x0;
+            k[1] = x1;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (8 * g + j < count) *reinterpret_cast<kv8_half2*>(&st.v[8 * g + j][32 * u + 2 * m]) = kv8_half2{x0[j], x1[j]};
     }
 }
 
-// The staged block's 32 rows into codes and scales.
+// The staged block's 32 rows into codes and scales, a piece a thread.
 __device__ __forceinline__ void quantise(Stage& st, const Kv8Head& h, int b) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = lane >> 4, m = lane & 15;
-    // this thread's 16 keys (one row) and 16 values (8 rows of two dims)
-    kv8_half2 kx[8], vx[8];
-    const kv8_half2* kr = reinterpret_cast<const kv8_half2*>(&st.k[kv8_key_row(wave >> 1, m)][64 * (wave & 1) + 16 * g]);
-    kv8_half2 kt{}, vt{};
+    const int tid = append_tid(), lane = tid & 63, wave = tid >> 6, u = wave & 3, g = lane >> 4, m = lane & 15;
+    const bool keys = tid < 256;
+    kv8_half2 x[8], top{};
+    const kv8_half2* kr = reinterpret_cast<const kv8_half2*>(&st.k[kv8_key_row(u >> 1, m)][64 * (u & 1) + 16 * g]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        kx[j] = kr[j];
-        vx[j] = *reinterpret_cast<const kv8_half2*>(&st.v[8 * g + j][32 * wave + 2 * m]);
-        kt = kv8_top(kt, kx[j]);
-        vt = kv8_top(vt, vx[j]);
+        x[j] = keys ? kr[j] : *reinterpret_cast<const kv8_half2*>(&st.v[8 * g + j][32 * u + 2 * m]);
+        top = kv8_top(top, x[j]);
     }
-    float ka = fmaxf((float)kt[0], (float)kt[1]), va = fmaxf((float)vt[0], (float)vt[1]);
-    ka = wave_max(ka);
-    va = wave_max(va);
-    if (lane == 0) {
-        st.amax[0][wave] = ka;
-        st.amax[1][wave] = va;
-    }
+    const float wave_top = wave_max(fmaxf((float)top[0], (float)top[1]));
+    if (lane == 0) st.amax[wave] = wave_top;
     __syncthreads();
-    const int ek = kv8_exponent(fmaxf(fmaxf(st.amax[0][0], st.amax[0][1]), fmaxf(st.amax[0][2], st.amax[0][3])));
-    const int ev = kv8_exponent(fmaxf(fmaxf(st.amax[1][0], st.amax[1][1]), fmaxf(st.amax[1][2], st.amax[1][3])));
-    const Kv8Inverse ik(ek), iv(ev);
-    uint32_t kw[4], vw[4];
+    const float* parts = st.amax + (wave & 4);
+    const int e = kv8_exponent(fmaxf(fmaxf(parts[0], parts[1]), fmaxf(parts[2], parts[3])));
+    const Kv8Inverse inv(e);
+    if (!keys) {  // pairs of dims to pairs of keys: the first dim's eight, then the second's
+        kv8_half2 y[8];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        kw[w] = kv8_word(kx[2 * w], kx[2 * w + 1], ik);
-        // the pairs hold two dims of a key: words are four keys of a dim
-        const int j = 4 * (w & 1), d = w >> 1;
-        vw[w] = kv8_word(kv8_half2{vx[j][d], vx[j + 1][d]}, kv8_half2{vx[j + 2][d], vx[j + 3][d]}, iv);
+        for (int j = 0; j < 8; ++j) y[j] = kv8_half2{x[2 * (j & 3)][j >> 2], x[2 * (j & 3) + 1][j >> 2]};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = y[j];
     }
-    uint8_t* codes = h.codes + (size_t)b * kKv8BlockBytes + tid * 16;
-    *reinterpret_cast<uint4*>(codes) = make_uint4(kw[0], kw[1], kw[2], kw[3]);
-    *reinterpret_cast<uint4*>(codes + kKv8PartBytes) = make_uint4(vw[0], vw[1], vw[2], vw[3]);
-    if (tid == 0) h.scales[b] = make_float2(kv8_power(ek), kv8_power(ev));
+    reinterpret_cast<uint4*>(h.codes + (size_t)b * kKv8BlockBytes)[tid] =
+        make_uint4(kv8_word(x[0], x[1], inv), kv8_word(x[2], x[3], inv), kv8_word(x[4], x[5], inv), kv8_word(x[6], x[7], inv));
+    if (lane == 0 && u == 0) reinterpret_cast<float*>(h.scales + b)[keys ? 0 : 1] = kv8_power(e);
 }
 
 __device__ __forceinline__ void store_tail(const Stage& st, const Kv8Head& h, int row0, int rows) {
-    for (int i = threadIdx.x; i < (rows - row0) * kHeadDim; i += 256) {
-        const int r = row0 + (i >> 7), d = i & 127;
-        h.tail_k[r * kHeadDim + d] = st.k[r][d];
-        h.tail_v[d * kKv8Block + r] = st.v[r][d];
-    }
+    const int i = row0 * 16 + append_tid();
+    if (i < rows * 16) reinterpret_cast<uint4*>(h.tail_k)[i] = *reinterpret_cast<const uint4*>(&st.k[i >> 4][8 * (i & 15)]);
+    const int d = append_tid() & 127;
+    for (int r = row0 + (append_tid() >> 7); r < rows; r += 4) h.tail_v[d * kKv8Block + r] = st.v[r][d];
 }
 
 // Block p0 / 32 + j of an append of `tokens` rows at p0 (0 <= p0, p0 + tokens <= capacity).
+// Where workgroup 0 keeps the tail besides a block of its own, it has two halves of
+// kAppendThreads: the second one stages the last block meanwhile, and stores it
+// once the first has read the tail.
 template <int ROWS>
-__device__ __forceinline__ void append_block(Stage& st, const Kv8Head& h, const Rows& in, int p0, int tokens, int j,
+__device__ __forceinline__ void append_block(Stage (&stages)[2], const Kv8Head& h, const Rows& in, int p0, int tokens, int j,
                                              const float* k_norm, double eps, const double* rope) {
     const int end = p0 + tokens;
-    const int b = p0 / kKv8Block + j;
+    const int own = p0 / kKv8Block + j;
     const int last = (end - 1) / kKv8Block;
-    const int first = j == 0 ? p0 : b * kKv8Block;             // this block's new positions
-    const int fill = min(end - b * kKv8Block, kKv8Block);      // rows it holds afterwards
+    const bool apart = p0 % kKv8Block == 0;  // nobody reads the old tail: the last block's workgroup may write it
+    const bool keeper = apart ? own == last : j == 0;
+    const bool second = threadIdx.x >= kAppendThreads;
+    if (second && !(keeper && own != last)) return;
+    if (!keeper && end - own * kKv8Block < kKv8Block) return;  // the last block, not whole: workgroup 0's
+    const int b = second ? last : own;
+    Stage& st = stages[second ? 1 : 0];
+    const int first = max(p0, b * kKv8Block);             // this block's new positions
+    const int fill = min(end - b * kKv8Block, kKv8Block);  // rows it holds afterwards
     const bool whole = fill == kKv8Block;
-    if (j != 0 && !whole) return;  // the last block, which workgroup 0 puts into the tail
     const int row0 = first - b * kKv8Block;
     stage_rows<ROWS>(st, in, first - p0, fill - row0, row0, k_norm, eps, rope, first);
     int kept = row0;  // rows of the tail that stay as they are
@@ -177,23 +230,25 @@ __device__ __forceinline__ void append_block(Stage& st, const Kv8Head& h, const 
         if (!held) kept = 0;
     }
     __syncthreads();
-    if (whole) quantise(st, h, b);
-    if (j != 0) return;
-    if (b == last) {
-        store_tail(st, h, kept, fill);
-    } else {
-        __syncthreads();  // the staged rows are read
-        const int f = last * kKv8Block, n = end - f;
-        stage_rows<ROWS>(st, in, f - p0, n, 0, k_norm, eps, rope, f);
-        __syncthreads();
-        store_tail(st, h, 0, n);
+    if (second) {
+        __syncthreads();  // (quantise's)
+    } else if (whole) {
+        quantise(st, h, b);
     }
-    if (threadIdx.x == 0) *h.end = end;
+    if (!keeper || b != last) return;
+    store_tail(st, h, kept, fill);
+    if (append_tid() == 0) *h.end = end;
+}
+
+// Threads of an append's workgroups.
+int append_threads(int p0, int tokens) {
+    const bool twice = p0 % kKv8Block != 0 && (p0 + tokens - 1) / kKv8Block != p0 / kKv8Block;
+    return twice ? 2 * kAppendThreads : kAppendThreads;
 }
 
 // Members that share a cache, at consecutive positions. Grid (KV head, block).
-__global__ __launch_bounds__(256) void kv8_append_kernel(AttnArgs a, int members) {
-    __shared__ Stage st;
+__global__ __launch_bounds__(2 * kAppendThreads) void kv8_append_kernel(AttnArgs a, int members) {
+    __shared__ Stage st[2];
     const int kvh = blockIdx.x;
     const AttnMember mb = a.mem[0];
     const int pos = a.positions[0];
@@ -205,8 +260,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AttnArgs a, int members
     append_block<kRowsRaw>(st, kv8_head(mb, a.layer, kvh), in, pos, members, j, a.k_norm, a.eps, mb.rope);
 }
 
-__global__ __launch_bounds__(256) void kv8_append_seq_kernel(PrefillAttnArgs a) {
-    __shared__ Stage st;
+__global__ __launch_bounds__(2 * kAppendThreads) void kv8_append_seq_kernel(PrefillAttnArgs a) {
+    __shared__ Stage st[2];
     const int kvh = blockIdx.x;
     const size_t at = (size_t)kvh * kHeadDim;
     const Rows in{a.k + at, a.v + at, (size_t)a.kv_heads * kHeadDim};
@@ -214,18 +269,39 @@ __global__ __launch_bounds__(256) void kv8_append_seq_kernel(PrefillAttnArgs a) 
 }
 
 template <int ROWS>
-__global__ __launch_bounds__(256) void kv8_write_kernel(KvMoveArgs a) {
-    __shared__ Stage st;
+__global__ __launch_bounds__(2 * kAppendThreads) void kv8_write_kernel(KvMoveArgs a) {
+    __shared__ Stage st[2];
     const int kvh = blockIdx.x;
     const size_t at = (size_t)kvh * kHeadDim * (ROWS == kRowsF16 ? 2 : 4);
     const Rows in{static_cast<const char*>(a.keys) + at, static_cast<const char*>(a.values) + at, (size_t)a.kv_heads * kHeadDim};
     append_block<ROWS>(st, kv8_head(a.mem, a.layer, kvh), in, a.p0, a.tokens, blockIdx.y, nullptr, 0.0, nullptr);
 }
 
+// Eight values of a row in memory, as f16.
+__device__ __forceinline__ kv8_half8 load_row(const _Float16* p) { return *reinterpret_cast<const kv8_half8*>(p); }
+__device__ __forceinline__ kv8_half8 load_row(const float* p) {
+    kv8_half8 h;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float4 x = reinterpret_cast<const float4*>(p)[i];
+        h[4 * i] = (_Float16)x.x;
+        h[4 * i + 1] = (_Float16)x.y;
+        h[4 * i + 2] = (_Float16)x.z;
+        h[4 * i + 3] = (_Float16)x.w;
+    }
+    return h;
+}
+__device__ __forceinline__ void store_row(_Float16* p, kv8_half8 h) { *reinterpret_cast<kv8_half8*>(p) = h; }
+__device__ __forceinline__ void store_row(float* p, kv8_half8 h) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        reinterpret_cast<float4*>(p)[i] = make_float4((float)h[4 * i], (float)h[4 * i + 1], (float)h[4 * i + 2], (float)h[4 * i + 3]);
+}
+
 // Rows out of an 8-bit cache, grid (KV head, block): the values its codes stand
 // for, the tail's f16 values of the block that is not whole, zeros past `end`.
 template <typename T>
-__global__ __launch_bounds__(256) void kv8_read_kernel(KvMoveArgs a) {
+__global__ __launch_bounds__(kAppendThreads, 4) void kv8_read_kernel(KvMoveArgs a) {
     __shared__ Stage st;
     const int kvh = blockIdx.x;
     const int b = a.p0 / kKv8Block + (int)blockIdx.y;
@@ -234,37 +310,40 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(KvMoveArgs a) {
     const int rows = max(0, min(end - b * kKv8Block, kKv8Block));
     stage_held(st, h, b, rows, rows < kKv8Block);
     __syncthreads();
-    const int lo = max(a.p0, b * kKv8Block), hi = min(a.p0 + a.tokens, (b + 1) * kKv8Block);
-    const int lane = threadIdx.x & 127;
-    for (int p = lo + ((int)threadIdx.x >> 7); p < hi; p += 2) {
-        const int r = p - b * kKv8Block;
-        const size_t at = ((size_t)(p - a.p0) * a.kv_heads + kvh) * kHeadDim + lane;
-        static_cast<T*>(a.keys)[at] = r < rows ? (T)st.k[r][lane] : (T)0.f;
-        static_cast<T*>(a.values)[at] = r < rows ? (T)st.v[r][lane] : (T)0.f;
+    const int lo = max(a.p0, b * kKv8Block) - b * kKv8Block, hi = min(a.p0 + a.tokens, (b + 1) * kKv8Block) - b * kKv8Block;
+    const int c = threadIdx.x & 15;
+    const int r = (int)threadIdx.x >> 4;
+    if (r < lo || r >= hi) return;
+    const size_t at = ((size_t)(b * kKv8Block + r - a.p0) * a.kv_heads + kvh) * kHeadDim + 8 * c;
+    kv8_half8 k{}, v{};
+    if (r < rows) {
+        k = *reinterpret_cast<const kv8_half8*>(&st.k[r][8 * c]);
+        v = *reinterpret_cast<const kv8_half8*>(&st.v[r][8 * c]);
     }
+    store_row(static_cast<T*>(a.keys) + at, k);
+    store_row(static_cast<T*>(a.values) + at, v);
 }
 
-// An f16 cache's rows ([kv_head][token][128]), in and out. Grid (KV head, tokens in turn).
+// An f16 cache's rows ([kv_head][token][128]), in and out: 16 lanes a row, grid
+// (16 tokens, KV head). (f16 overflow gives infinities here, as the appends of f16 caches do.)
 template <typename T>
-__global__ __launch_bounds__(128) void kv16_write_kernel(KvMoveArgs a) {
-    const int kvh = blockIdx.x, d = threadIdx.x;
-    for (int t = blockIdx.y; t < a.tokens; t += gridDim.y) {
-        const size_t to = (size_t)a.layer * a.mem.layer_elems + ((size_t)kvh * a.mem.capacity + (size_t)(a.p0 + t)) * kHeadDim + d;
-        const size_t at = ((size_t)t * a.kv_heads + kvh) * kHeadDim + d;
-        reinterpret_cast<_Float16*>(a.mem.keys)[to] = (_Float16)static_cast<const T*>(a.keys)[at];
-        reinterpret_cast<_Float16*>(a.mem.values)[to] = (_Float16)static_cast<const T*>(a.values)[at];
-    }
+__global__ __launch_bounds__(256) void kv16_write_kernel(KvMoveArgs a) {
+    const int kvh = blockIdx.y, c = threadIdx.x & 15, t = (int)blockIdx.x * 16 + ((int)threadIdx.x >> 4);
+    if (t >= a.tokens) return;
+    const size_t to = (size_t)a.layer * a.mem.layer_elems + ((size_t)kvh * a.mem.capacity + (size_t)(a.p0 + t)) * kHeadDim + 8 * c;
+    const size_t at = ((size_t)t * a.kv_heads + kvh) * kHeadDim + 8 * c;
+    store_row(reinterpret_cast<_Float16*>(a.mem.keys) + to, load_row(static_cast<const T*>(a.keys) + at));
+    store_row(reinterpret_cast<_Float16*>(a.mem.values) + to, load_row(static_cast<const T*>(a.values) + at));
 }
 
 template <typename T>
-__global__ __launch_bounds__(128) void kv16_read_kernel(KvMoveArgs a) {
-    const int kvh = blockIdx.x, d = threadIdx.x;
-    for (int t = blockIdx.y; t < a.tokens; t += gridDim.y) {
-        const size_t from = (size_t)a.layer * a.mem.layer_elems + ((size_t)kvh * a.mem.capacity + (size_t)(a.p0 + t)) * kHeadDim + d;
-        const size_t at = ((size_t)t * a.kv_heads + kvh) * kHeadDim + d;
-        static_cast<T*>(a.keys)[at] = (T)reinterpret_cast<const _Float16*>(a.mem.keys)[from];
-        static_cast<T*>(a.values)[at] = (T)reinterpret_cast<const _Float16*>(a.mem.values)[from];
-    }
+__global__ __launch_bounds__(256) void kv16_read_kernel(KvMoveArgs a) {
+    const int kvh = blockIdx.y, c = threadIdx.x & 15, t = (int)blockIdx.x * 16 + ((int)threadIdx.x >> 4);
+    if (t >= a.tokens) return;
+    const size_t from = (size_t)a.layer * a.mem.layer_elems + ((size_t)kvh * a.mem.capacity + (size_t)(a.p0 + t)) * kHeadDim + 8 * c;
+    const size_t at = ((size_t)t * a.kv_heads + kvh) * kHeadDim + 8 * c;
+    store_row(static_cast<T*>(a.keys) + at, load_row(reinterpret_cast<const _Float16*>(a.mem.keys) + from));
+    store_row(static_cast<T*>(a.values) + at, load_row(reinterpret_cast<const _Float16*>(a.mem.values) + from));
 }
 
 struct CacheInit {
@@ -542,8 +621,8 @@ __global__ __launch_bounds__(kThreads, 3) void kv8_attn_kernel(AttnArgs a, Membe
         if (wave == 0) {
             const double x0 = nx0, x1 = nx1;
             const double ssq = wave_sum64(__builtin_fma(x0, x0, x1 * x1));
-            const double inv = 1.0 / sqrt(ssq / (double)kHeadDim + (double)a.eps);
-            const double y0 = x0 * inv * (double)kw0 * gain, y1 = x1 * inv * (double)kw1 * gain;
+            const double inv = inverse_root(ssq * (1.0 / kHeadDim) + (double)a.eps) * gain;
+            const double y0 = x0 * inv * (double)kw0, y1 = x1 * inv * (double)kw1;
             nx0 = (float)__builtin_fma(y0, rot.c, -y1 * rot.s);
             nx1 = (float)__builtin_fma(y0, rot.s, y1 * rot.c);
         }
@@ -699,70 +778,22 @@ __global__ __launch_bounds__(kThreads, 3) void kv8_attn_kernel(AttnArgs a, Membe
     }
 }
 
-// The chunks' partials of a (query head, member) merged. 32 lanes hold a row's
-// 128 sums (four each) and take the chunks c, c + 4, ... of the launch's NC or
-// fewer; every slot the launch can hold is loaded before the position says which
-// are live (the others hold stale memory). The four runs meet in LDS in order: a dead
-// slot adds exact zeros, so a member's bits do not depend on NC. A member without
-// tokens (a negative position) gets zeros.
+// The chunks' partials of a (query head, member) merged; every slot the launch can
+// hold is loaded before the position says which are live (the others hold stale
+// memory). A member without tokens (a negative position) gets zeros.
 template <int NC, bool INLINE>
 __global__ __launch_bounds__(128) void kv8_combine_kernel(AttnArgs a, Members<INLINE> members) {
-    constexpr int kRun = NC / 4;
-    __shared__ float4 so[4][32];
-    __shared__ float2 sml[4];
     const int qh = blockIdx.x;
     const int m = blockIdx.y;
-    const int run = (int)threadIdx.x >> 5;
-    const int lane = threadIdx.x & 31;
     const AttnMember mb = members.get(a, m);
     const float* own = a.partials != nullptr ? a.partials + (size_t)m * a.partial_floats : mb.partials;
-    const __amdgpu_buffer_rsrc_t pr =
-        make_rsrc(own + (size_t)qh * kAttnChunks * kPartStride, (uint32_t)(a.chunks * kPartStride * 4));
-    float4 o[kRun];
-    float2 ml[kRun];
-#pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-        const uint32_t row = (uint32_t)((4 * i + run) * kPartStride) * 4u;
-        o[i] = __builtin_bit_cast(float4, load_b128(pr, row + 16u * (uint32_t)lane));
-        ml[i] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(pr, (int)(row + kHeadDim * 4), 0, 0));
-    }
-    int end;
-    const int tokens = kv8_tokens(a, mb, kv8_head(mb, a.layer, qh / (a.q_heads / a.kv_heads)), a.positions[m], end);
-    const int len = kv8_chunk_tokens(tokens, a.chunks, a.min_chunk);
-    const int chunks = tokens > 0 ? (tokens + len - 1) / len : 0;
-    float mx = -FLT_MAX;
-#pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-        const bool live = 4 * i + run < chunks;
-        ml[i] = live ? ml[i] : make_float2(-FLT_MAX, 0.f);
-        o[i] = live ? o[i] : make_float4(0.f, 0.f, 0.f, 0.f);
-        mx = fmaxf(mx, ml[i].x);
-    }
-    float l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-        const float f = __builtin_amdgcn_exp2f(ml[i].x - mx);
-        l = __builtin_fmaf(ml[i].y, f, l);
-        acc.x = __builtin_fmaf(o[i].x, f, acc.x);
-        acc.y = __builtin_fmaf(o[i].y, f, acc.y);
-        acc.z = __builtin_fmaf(o[i].z, f, acc.z);
-        acc.w = __builtin_fmaf(o[i].w, f, acc.w);
-    }
-    so[run][lane] = acc;
-    if (lane == 0) sml[run] = make_float2(mx, l);
-    __syncthreads();
-    const int d = threadIdx.x;
-    mx = fmaxf(fmaxf(sml[0].x, sml[1].x), fmaxf(sml[2].x, sml[3].x));
-    l = 0.f;
-    float sum = 0.f;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const float f = __builtin_amdgcn_exp2f(sml[r].x - mx);
-        l = __builtin_fmaf(sml[r].y, f, l);
-        sum = __builtin_fmaf(reinterpret_cast<const float*>(so[r])[d], f, sum);
-    }
-    a.out[((size_t)m * a.q_heads + qh) * kHeadDim + d] = chunks > 0 ? sum / l : 0.f;
+    auto live = [&] {
+        int end;
+        const int tokens = kv8_tokens(a, mb, kv8_head(mb, a.layer, qh / (a.q_heads / a.kv_heads)), a.positions[m], end);
+        const int len = kv8_chunk_tokens(tokens, a.chunks, a.min_chunk);
+        return tokens > 0 ? (tokens + len - 1) / len : 0;
+    };
+    merge_row<NC>(own + (size_t)qh * kAttnChunks * kPartStride, a.chunks, live, a.out + ((size_t)m * a.q_heads + qh) * kHeadDim);
 }
 
 }  // namespace
@@ -788,14 +819,15 @@ hipError_t launch_kv8_append(const AttnArgs& a, int members, hipStream_t stream)
     if (members < 1 || members > kAttnMaxMembers || a.kv_heads < 1 || a.mem == nullptr) return hipErrorInvalidValue;
     // consecutive positions touch at most one block more than they fill
     const int blocks = (members + kKv8Block - 2) / kKv8Block + 1;
-    hipLaunchKernelGGL(kv8_append_kernel, dim3((unsigned)a.kv_heads, (unsigned)blocks), dim3(256), 0, stream, a, members);
+    hipLaunchKernelGGL(kv8_append_kernel, dim3((unsigned)a.kv_heads, (unsigned)blocks), dim3(blocks > 1 ? 2 * kAppendThreads : kAppendThreads), 0,
+                       stream, a, members);
     return hipGetLastError();
 }
 
 hipError_t launch_kv8_append_seq(const PrefillAttnArgs& a, hipStream_t stream) {
     if (a.tokens < 1 || a.kv_heads < 1 || a.p0 < 0 || (long long)a.p0 + a.tokens > a.mem.capacity) return hipErrorInvalidValue;
     const int blocks = (a.p0 + a.tokens - 1) / kKv8Block - a.p0 / kKv8Block + 1;
-    hipLaunchKernelGGL(kv8_append_seq_kernel, dim3((unsigned)a.kv_heads, (unsigned)blocks), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(kv8_append_seq_kernel, dim3((unsigned)a.kv_heads, (unsigned)blocks), dim3(append_threads(a.p0, a.tokens)), 0, stream, a);
     return hipGetLastError();
 }
 
@@ -838,28 +870,28 @@ bool move_fits(const KvMoveArgs& a) {
     return a.tokens >= 1 && a.kv_heads >= 1 && a.p0 >= 0 && (long long)a.p0 + a.tokens <= a.mem.capacity && a.mem.keys != nullptr;
 }
 dim3 move_grid(const KvMoveArgs& a, bool kv8) {
-    const int blocks = (a.p0 + a.tokens - 1) / kKv8Block - a.p0 / kKv8Block + 1;
-    return dim3((unsigned)a.kv_heads, (unsigned)(kv8 ? blocks : std::min(a.tokens, 32768)));
+    if (!kv8) return dim3((unsigned)(a.tokens + 15) / 16, (unsigned)a.kv_heads);
+    return dim3((unsigned)a.kv_heads, (unsigned)((a.p0 + a.tokens - 1) / kKv8Block - a.p0 / kKv8Block + 1));
 }
 }  // namespace
 
 hipError_t launch_kv_write(const KvMoveArgs& a, bool half, bool kv8, hipStream_t stream) {
     if (!move_fits(a)) return hipErrorInvalidValue;
     const dim3 grid = move_grid(a, kv8);
-    if (kv8 && half) hipLaunchKernelGGL(kv8_write_kernel<kRowsF16>, grid, dim3(256), 0, stream, a);
-    else if (kv8) hipLaunchKernelGGL(kv8_write_kernel<kRowsF32>, grid, dim3(256), 0, stream, a);
-    else if (half) hipLaunchKernelGGL(kv16_write_kernel<_Float16>, grid, dim3(128), 0, stream, a);
-    else hipLaunchKernelGGL(kv16_write_kernel<float>, grid, dim3(128), 0, stream, a);
+    if (kv8 && half) hipLaunchKernelGGL(kv8_write_kernel<kRowsF16>, grid, dim3(append_threads(a.p0, a.tokens)), 0, stream, a);
+    else if (kv8) hipLaunchKernelGGL(kv8_write_kernel<kRowsF32>, grid, dim3(append_threads(a.p0, a.tokens)), 0, stream, a);
+    else if (half) hipLaunchKernelGGL(kv16_write_kernel<_Float16>, grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL(kv16_write_kernel<float>, grid, dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
 hipError_t launch_kv_read(const KvMoveArgs& a, bool half, bool kv8, hipStream_t stream) {
     if (!move_fits(a)) return hipErrorInvalidValue;
     const dim3 grid = move_grid(a, kv8);
-    if (kv8 && half) hipLaunchKernelGGL(kv8_read_kernel<_Float16>, grid, dim3(256), 0, stream, a);
-    else if (kv8) hipLaunchKernelGGL(kv8_read_kernel<float>, grid, dim3(256), 0, stream, a);
-    else if (half) hipLaunchKernelGGL(kv16_read_kernel<_Float16>, grid, dim3(128), 0, stream, a);
-    else hipLaunchKernelGGL(kv16_read_kernel<float>, grid, dim3(128), 0, stream, a);
+    if (kv8 && half) hipLaunchKernelGGL(kv8_read_kernel<_Float16>, grid, dim3(kAppendThreads), 0, stream, a);
+    else if (kv8) hipLaunchKernelGGL(kv8_read_kernel<float>, grid, dim3(kAppendThreads), 0, stream, a);
+    else if (half) hipLaunchKernelGGL(kv16_read_kernel<_Float16>, grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL(kv16_read_kernel<float>, grid, dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 

@@ -648,6 +648,8 @@ hipError_t enqueue_prompt_chunk(ribn_amd_qwen3_decode* d, ribn_amd_kv_cache* cac
         a.eps = c.epsilon;
         a.rope_base = c.rope_base;
         a.scale = 1.4426950408889634f / sqrtf((float)c.head_dim);
+        a.partials = d->ctx->split_partials;
+        a.partial_rows = a.partials != nullptr ? ribn_amd::kPrefillPartialRows : 0;
         e = ribn_amd::launch_prefill_attention(a, d->ctx->cu_count, stream, cache->kind);
         if (e != hipSuccess || last) break;
         e = ribn_amd::launch_act_f16(false, d->p_attn, nullptr, 0.f, tokens, qdim, d->p_gemm, stream);
@@ -796,6 +798,12 @@ ribn_amd_status ribn_amd_kv_cache_create_with(ribn_amd_context* ctx, const ribn_
         table_bytes = (size_t)rope_table(*rope, turns) * sizeof(double);
     }
     DeviceGuard guard(ctx->device);
+    if (i8 && ctx->split_partials == nullptr) {
+        void* room = nullptr;
+        const hipError_t e = hipMalloc(&room, ribn_amd::kPrefillPartialRows * ribn_amd::kPartStride * sizeof(float));
+        if (e != hipSuccess) return driver(e, "hipMalloc prompt attention partials");
+        ctx->split_partials = static_cast<float*>(room);
+    }
     void* block = nullptr;
     hipError_t e = hipMalloc(&block, held_bytes + part_bytes + table_bytes);
     if (e != hipSuccess) return driver(e, "hipMalloc KV cache");
@@ -882,9 +890,8 @@ static ribn_amd_status move_rows(ribn_amd_context* ctx, ribn_amd_kv_cache* cache
     if (dtype != RIBN_AMD_F32 && dtype != RIBN_AMD_F16) {
         return fail(RIBN_AMD_INVALID_ARGUMENT, RIBN_AMD_F16, dtype, "cache rows are f32 or f16, not element type %u", dtype);
     }
-    const uintptr_t size = dtype == RIBN_AMD_F16 ? 2 : 4;
-    st = check_device_ptr(ctx, keys, "keys", size);
-    if (st == RIBN_AMD_OK) st = check_device_ptr(ctx, values, "values", size);
+    st = check_device_ptr(ctx, keys, "keys");
+    if (st == RIBN_AMD_OK) st = check_device_ptr(ctx, values, "values");
     if (st != RIBN_AMD_OK) return st;
     if (cache->device != ctx->device) {
         return fail(RIBN_AMD_CONTEXT_MISMATCH, (uint64_t)ctx->device, (uint64_t)cache->device,
@@ -990,6 +997,8 @@ ribn_amd_status ribn_amd_attention_prefill(ribn_amd_context* ctx, const ribn_amd
     a.eps = config->epsilon;
     a.rope_base = config->rope_base;
     a.scale = 1.4426950408889634f / sqrtf((float)config->head_dim);
+    a.partials = ctx->split_partials;
+    a.partial_rows = a.partials != nullptr ? ribn_amd::kPrefillPartialRows : 0;
     hipError_t e = ribn_amd::launch_prefill_attention(a, ctx->cu_count, ctx->stream, cache->kind);
     return e == hipSuccess ? ok() : driver(e, "prompt attention launch");
 }

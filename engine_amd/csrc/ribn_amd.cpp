@@ -484,9 +484,10 @@ void context_retain(ribn_amd_context* ctx) { ctx->refs.fetch_add(1, std::memory_
 void context_release(ribn_amd_context* ctx) {
     if (ctx->refs.fetch_sub(1, std::memory_order_acq_rel) != 1) return;
     DeviceGuard guard(ctx->device);
-    if (ctx->workspace || ctx->act_scratch) hipStreamSynchronize(ctx->stream);
+    if (ctx->workspace || ctx->act_scratch || ctx->split_partials) hipStreamSynchronize(ctx->stream);
     if (ctx->workspace) hipFree(ctx->workspace);
     if (ctx->act_scratch) hipFree(ctx->act_scratch);
+    if (ctx->split_partials) hipFree(ctx->split_partials);
     if (ctx->owns_stream) {
         hipStreamSynchronize(ctx->stream);
         hipStreamDestroy(ctx->stream);

@@ -21,7 +21,7 @@ import numpy as np
 
 from . import _lib
 from .kquant import RANK_CACHE, RANK_DECODER, AmdModelKernelError, _check, _live, _own, _ptr
-from .rope import AmdRopeSpec
+from .rope import AmdRopeSpec, _dtype
 
 # What a KV cache holds a value in: f16, or 8 bits with a power-of-two scale for
 # each block of 32 tokens and KV head.
@@ -97,9 +97,8 @@ class AmdKvCache:
         self._move(self.ctx._lib.ribn_amd_kv_cache_read, layer, position, keys, values)
 
     def _move(self, call, layer, position, keys, values):
-        import torch
-        dtype = {torch.float32: 0, torch.float16: 2}.get(keys.dtype)
-        if dtype is None or values.dtype != keys.dtype:
+        dtype = _dtype(keys)
+        if dtype not in (0, 2) or values.dtype != keys.dtype:
             raise TypeError(f"cache rows are float32 or float16, got {keys.dtype} and {values.dtype}")
         if keys.shape != values.shape or not keys.is_contiguous() or not values.is_contiguous():
             raise ValueError("keys and values must be contiguous and of one shape")

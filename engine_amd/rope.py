@@ -14,7 +14,7 @@ from dataclasses import dataclass
 from typing import Optional, Sequence
 
 from . import _lib
-from .kquant import RANK_RESOURCE, AmdModelKernelError, _check, _live, _own, _ptr
+from .kquant import RANK_RESOURCE, AmdModelKernelError, _check, _live, _own
 
 _LAYOUTS = {"half": 0, "interleaved": 1}
 _SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
@@ -63,6 +63,18 @@ def rope_frequencies(spec: AmdRopeSpec):
     return list(turns), gain.value
 
 
+_POSITIONS = 3
+_DTYPES: dict = {}
+
+
+def _dtype(t):
+    """The C element type of a tensor (_POSITIONS for int32), None for others."""
+    if not _DTYPES:
+        import torch
+        _DTYPES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.int32: _POSITIONS})
+    return _DTYPES.get(t.dtype)
+
+
 def _length(t) -> int:
     """Elements from the tensor's first to its storage's end."""
     return t.untyped_storage().nbytes() // t.element_size() - t.storage_offset()
@@ -86,27 +98,27 @@ class AmdRope:
 
     def execute_group(self, inputs, positions, outputs):
         """Up to four tensors sharing their tokens' positions (queries and keys) in one launch."""
-        import torch
         if len(inputs) != len(outputs):
             raise ValueError(f"{len(inputs)} inputs and {len(outputs)} outputs")
-        if positions.dtype != torch.int32 or positions.dim() != 1 or not positions.is_contiguous():
+        if _dtype(positions) != _POSITIONS or positions.dim() != 1 or not positions.is_contiguous():
             raise TypeError("positions must be a contiguous vector of int32")
         tokens = positions.numel()
-        dtype = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}.get(inputs[0].dtype) if inputs else None
-        rows = (_lib.RopeRows * max(1, len(inputs)))()
-        for r, x, y in zip(rows, inputs, outputs):
-            if dtype is None or x.dtype != inputs[0].dtype or y.dtype != inputs[0].dtype:
+        dim = self.spec.head_dim
+        kind = inputs[0].dtype if inputs else None
+        dtype = _dtype(inputs[0]) if inputs else 0
+        rows = []  # ribn_amd_rope_rows, nine words each
+        for x, y in zip(inputs, outputs):
+            if dtype not in (0, 1, 2) or x.dtype != kind or y.dtype != kind:
                 raise TypeError("rope takes float32, bfloat16 or float16 tensors of one type")
-            if x.dim() != 3 or x.shape != y.shape or x.shape[0] != tokens or x.shape[2] != self.spec.head_dim:
-                raise ValueError(f"rope rows are [{tokens}][heads][{self.spec.head_dim}], got {tuple(x.shape)} and {tuple(y.shape)}")
-            if x.stride(2) != 1 or y.stride(2) != 1:
+            shape = x.shape
+            if len(shape) != 3 or shape != y.shape or shape[0] != tokens or shape[2] != dim:
+                raise ValueError(f"rope rows are [{tokens}][heads][{dim}], got {tuple(shape)} and {tuple(y.shape)}")
+            xs, ys = x.stride(), y.stride()
+            if xs[2] != 1 or ys[2] != 1:
                 raise ValueError("the dims of a head must be contiguous")
-            r.input, r.input_len = x.data_ptr(), _length(x)
-            r.input_token_stride, r.input_head_stride = x.stride(0), x.stride(1)
-            r.output, r.output_len = y.data_ptr(), _length(y)
-            r.output_token_stride, r.output_head_stride = y.stride(0), y.stride(1)
-            r.heads = x.shape[1]
-        _check(self.ctx._lib.ribn_amd_rope_execute(self.handle, _ptr(positions), tokens, rows, len(inputs), dtype or 0),
+            rows += (x.data_ptr(), _length(x), xs[0], xs[1], y.data_ptr(), _length(y), ys[0], ys[1], shape[1])
+        _check(self.ctx._lib.ribn_amd_rope_execute(self.handle, positions.data_ptr(), tokens,
+                                                   (ctypes.c_size_t * max(1, len(rows)))(*rows), len(inputs), dtype),
                AmdModelKernelError)
 
     def close(self):
