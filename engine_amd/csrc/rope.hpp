@@ -30,7 +30,8 @@ struct RopeArgs {
     int count;
     int head_dim;
     int rotary_dim;
-    int slices;  // launch_rope sets it: threads that share a token's heads
+    int slices;     // launch_rope sets it: threads that share a token's heads
+    int per_group;  // and this: tokens of a workgroup
 };
 
 // `dtype` a RIBN_AMD_F32 / BF16 / F16, `layout` a RIBN_AMD_ROPE_*.

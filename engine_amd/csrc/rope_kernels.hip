@@ -3,12 +3,11 @@
 //
 // For the pair (a, b) with angle p = position * turns (64 bits, rope_device.hpp):
 //   a' = a cos p - b sin p,  b' = a sin p + b cos p
-// A thread takes one group of pairs of a token, forms their angles once and
-// turns that group in every slices-th head of every tensor of the call. Bound by
-// memory: each value is read and written once, in 16-byte pieces (a wave
-// covers whole heads), kUnroll heads in flight; the angles, some 50
-// instructions a pair, are spread over the heads a thread takes. Few tokens: the
-// heads are spread over threads instead (slices), down to one each.
+// A workgroup takes a few tokens. Its threads form each of their angles once (some
+// 50 instructions each), into LDS, while their first rows are on the way; then a
+// thread turns one group of pairs in every slices-th head of every tensor of the
+// call. Bound by memory: each value is read and written once, in 16-byte pieces (a
+// wave covers whole heads), kUnroll heads in flight.
 #include "rope.hpp"
 
 #include <algorithm>
@@ -19,8 +18,11 @@ namespace ribn_amd {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kUnroll = 4;
+constexpr int kThreads = 256;     // of a workgroup, or what one head takes: 1,024 dims in single elements, 512
+constexpr int kMaxThreads = 512;
+constexpr int kUnroll = 3;
+constexpr int kHeads = kUnroll;
+constexpr int kThreadsPerCu = 1024;
 
 template <typename T, int E> struct Piece { T v[E]; };
 
@@ -57,63 +59,77 @@ __device__ __forceinline__ void turn(T& a, T& b, float c, float s) {
 // E: elements a thread moves at a time. Half layout: E pairs, two pieces half
 // the rotary part apart. Interleaved: E / 2 pairs, one piece. Dims past the rotary part: one piece, as it is.
 template <typename T, int E, bool HALF>
-__global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
+__global__ __launch_bounds__(kMaxThreads) void rope_kernel(RopeArgs a) {
     constexpr int kPairs = HALF ? E : E / 2;
+    extern __shared__ __attribute__((aligned(16))) float2 angles[];  // [tokens of the workgroup][pairs] cosine, sine
     const int pairs = a.rotary_dim / 2;
-    const uint32_t turning = (uint32_t)(pairs / kPairs);
-    const uint32_t groups = turning + (uint32_t)((a.head_dim - a.rotary_dim) / E);
-    const uint32_t id = blockIdx.x * kThreads + threadIdx.x;
-    const uint32_t group = id % groups;
-    const uint32_t slice = (id / groups) % (uint32_t)a.slices;
-    const size_t t = id / groups / (uint32_t)a.slices;
-    if (t >= a.tokens) return;
+    const int turning = pairs / kPairs;
+    const int groups = turning + (a.head_dim - a.rotary_dim) / E;
+    const int group = (int)threadIdx.x % groups;
+    const int inside = a.slices / (int)gridDim.y;  // slices of this workgroup
+    const int slice = (int)blockIdx.y * inside + (int)threadIdx.x / groups % inside;
+    const int local = (int)threadIdx.x / (groups * inside);
+    const size_t t0 = (size_t)blockIdx.x * a.per_group;
+    const size_t t = t0 + local;
+    const bool mine = local < a.per_group && t < a.tokens;
     const bool turns = group < turning;
-    const int dim = turns ? (int)group * E : a.rotary_dim + (int)(group - turning) * E;
+    const int dim = turns ? group * E : a.rotary_dim + (group - turning) * E;
+
+    Piece<T, E> lo[kUnroll], hi[kUnroll];
+    auto load = [&](const RopeRows& r, int h0) {
+        const T* x = static_cast<const T*>(r.x) + t * r.x_token + dim;
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int h = h0 + u * a.slices;
+            if (h < r.heads) {
+                lo[u] = load_piece<T, E>(x + (size_t)h * r.x_head);
+                if constexpr (HALF) {
+                    if (turns) hi[u] = load_piece<T, E>(x + (size_t)h * r.x_head + pairs);
+                }
+            }
+        }
+    };
+    if (mine) load(a.rows[0], slice);
+    const int here = (int)min((size_t)a.per_group, a.tokens - t0);
+    for (int i = threadIdx.x; i < here * pairs; i += blockDim.x) {
+        const int token = i / pairs, pair = i - token * pairs;
+        const Rot64 r = table_rot(a.table, pairs, pair, a.positions[t0 + token]);
+        angles[i] = make_float2((float)r.c, (float)r.s);
+    }
+    __syncthreads();
+    if (!mine) return;
     float c[kPairs], s[kPairs];
     if (turns) {
-        const int position = a.positions[t];
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
-            const Rot64 r = table_rot(a.table, pairs, (int)group * kPairs + i, position);
-            c[i] = (float)r.c;
-            s[i] = (float)r.s;
+            const float2 r = angles[local * pairs + group * kPairs + i];
+            c[i] = r.x;
+            s[i] = r.y;
         }
     }
     for (int n = 0; n < a.count; ++n) {
         const RopeRows& r = a.rows[n];
-        const T* x = static_cast<const T*>(r.x) + t * r.x_token + dim;
         T* y = static_cast<T*>(r.y) + t * r.y_token + dim;
         // heads are dealt out over the tensors' heads in a row
         const int ahead = r.before % a.slices;
-        const int first = ((int)slice >= ahead ? 0 : a.slices) + (int)slice - ahead;
-        if (turns) {
-            for (int h0 = first; h0 < r.heads; h0 += kUnroll * a.slices) {
-                Piece<T, E> lo[kUnroll], hi[kUnroll];
+        for (int h0 = (slice >= ahead ? 0 : a.slices) + slice - ahead; h0 < r.heads; h0 += kUnroll * a.slices) {
+            if (n > 0 || h0 != slice) load(r, h0);
 #pragma unroll
-                for (int u = 0; u < kUnroll; ++u) {
-                    const int h = h0 + u * a.slices;
-                    if (h < r.heads) {
-                        lo[u] = load_piece<T, E>(x + (size_t)h * r.x_head);
-                        if constexpr (HALF) hi[u] = load_piece<T, E>(x + (size_t)h * r.x_head + pairs);
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < kUnroll; ++u) {
-                    const int h = h0 + u * a.slices;
-                    if (h < r.heads) {
+            for (int u = 0; u < kUnroll; ++u) {
+                const int h = h0 + u * a.slices;
+                if (h < r.heads) {
+                    T* to = y + (size_t)h * r.y_head;
+                    if (turns) {
 #pragma unroll
                         for (int i = 0; i < kPairs; ++i) {
                             if constexpr (HALF) turn(lo[u].v[i], hi[u].v[i], c[i], s[i]);
                             else turn(lo[u].v[2 * i], lo[u].v[2 * i + 1], c[i], s[i]);
                         }
-                        store_piece<T, E>(y + (size_t)h * r.y_head, lo[u]);
-                        if constexpr (HALF) store_piece<T, E>(y + (size_t)h * r.y_head + pairs, hi[u]);
+                        if constexpr (HALF) store_piece<T, E>(to + pairs, hi[u]);
                     }
+                    store_piece<T, E>(to, lo[u]);
                 }
             }
-        } else if (x != y) {
-            for (int h = first; h < r.heads; h += a.slices)
-                store_piece<T, E>(y + (size_t)h * r.y_head, load_piece<T, E>(x + (size_t)h * r.x_head));
         }
     }
 }
@@ -121,14 +137,22 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(RopeArgs a) {
 template <typename T, int E, bool HALF>
 hipError_t launch(RopeArgs a, int cu_count, hipStream_t stream) {
     constexpr int kPairs = HALF ? E : E / 2;
-    const size_t groups = (size_t)(a.rotary_dim / 2 / kPairs + (a.head_dim - a.rotary_dim) / E);
-    int most = 1;
-    for (int i = 0; i < a.count; ++i) most = std::max(most, a.rows[i].before + a.rows[i].heads);
-    // as many threads as keep the CUs full (1,024 each), if the heads allow it
-    const size_t wanted = (size_t)cu_count * 1024;
-    a.slices = (int)std::max<size_t>(1, std::min<size_t>((size_t)most, wanted / std::max<size_t>(1, a.tokens * groups)));
-    // tokens a launch's 32-bit thread ids cover
-    const size_t span = ((size_t)1 << 31) / (groups * (size_t)a.slices);
+    const int groups = a.rotary_dim / 2 / kPairs + (a.head_dim - a.rotary_dim) / E;
+    int heads = 0;
+    for (int i = 0; i < a.count; ++i) heads = std::max(heads, a.rows[i].before + a.rows[i].heads);
+    // Threads that share a token's heads: a head each where the tokens are few (then
+    // over several workgroups, if it takes more than one), else kHeads each.
+    const size_t wanted = (size_t)cu_count * kThreadsPerCu / (a.tokens * (size_t)groups) + 1;
+    const int fit = std::max(1, kThreads / groups);  // slices a workgroup holds
+    const int shared = std::min(fit, (heads + kHeads - 1) / kHeads);
+    const int inside = wanted > (size_t)shared ? (int)std::min<size_t>(std::min<size_t>(wanted, (size_t)heads), (size_t)fit) : shared;
+    const int parts = wanted > (size_t)inside ? (int)std::min<size_t>((wanted + inside - 1) / inside, (size_t)(heads + inside - 1) / inside) : 1;
+    a.slices = inside * parts;
+    a.per_group = std::max(1, kThreads / (groups * inside));
+    const int threads = (a.per_group * groups * inside + 63) / 64 * 64;
+    const size_t lds = (size_t)a.per_group * (a.rotary_dim / 2) * sizeof(float2);
+    // a launch has fewer than 2^32 threads
+    const size_t span = (((size_t)1 << 31) / ((size_t)threads * parts)) * (size_t)a.per_group;
     RopeArgs b = a;
     for (size_t t0 = 0; t0 < a.tokens; t0 += span) {
         b.tokens = std::min(span, a.tokens - t0);
@@ -137,8 +161,8 @@ hipError_t launch(RopeArgs a, int cu_count, hipStream_t stream) {
             b.rows[i].x = static_cast<const T*>(a.rows[i].x) + t0 * a.rows[i].x_token;
             b.rows[i].y = static_cast<T*>(a.rows[i].y) + t0 * a.rows[i].y_token;
         }
-        const size_t threads = b.tokens * groups * (size_t)a.slices;
-        hipLaunchKernelGGL((rope_kernel<T, E, HALF>), dim3((unsigned)((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream, b);
+        const size_t blocks = (b.tokens + a.per_group - 1) / a.per_group;
+        hipLaunchKernelGGL((rope_kernel<T, E, HALF>), dim3((unsigned)blocks, (unsigned)parts), dim3((unsigned)threads), (unsigned)lds, stream, b);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }

@@ -10,6 +10,7 @@ A KV cache takes a spec too (AmdKvCache): its keys are cached rotated.
 from __future__ import annotations
 
 import ctypes
+import struct
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -117,9 +118,10 @@ class AmdRope:
             if xs[2] != 1 or ys[2] != 1:
                 raise ValueError("the dims of a head must be contiguous")
             rows += (x.data_ptr(), _length(x), xs[0], xs[1], y.data_ptr(), _length(y), ys[0], ys[1], shape[1])
-        _check(self.ctx._lib.ribn_amd_rope_execute(self.handle, positions.data_ptr(), tokens,
-                                                   (ctypes.c_size_t * max(1, len(rows)))(*rows), len(inputs), dtype),
-               AmdModelKernelError)
+        status = self.ctx._lib.ribn_amd_rope_execute(self.handle, positions.data_ptr(), tokens,
+                                                     struct.pack(f"{len(rows)}N", *rows), len(inputs), dtype)
+        if status:
+            _check(status, AmdModelKernelError)
 
     def close(self):
         if self.handle and _live():
