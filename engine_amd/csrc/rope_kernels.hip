@@ -18,8 +18,9 @@ namespace ribn_amd {
 
 namespace {
 
-constexpr int kThreads = 256;     // of a workgroup, or what one head takes: 1,024 dims in single elements, 512
-constexpr int kMaxThreads = 512;
+constexpr int kThreads = 256;     // of a workgroup, or what one head takes: up to 1,023 single elements
+constexpr int kMaxThreads = 1024;
+static_assert(kRopeMaxDim <= kMaxThreads, "a head fits a workgroup");
 constexpr int kUnroll = 3;
 constexpr int kHeads = kUnroll;
 constexpr int kThreadsPerCu = 1024;

@@ -73,7 +73,8 @@ def positions(env, tokens, seed, far=131072):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
-@pytest.mark.parametrize("dim,rotary", [(128, 128), (128, 64), (64, 64), (80, 22), (96, 96), (256, 192), (2, 2), (4, 2), (1024, 1024), (130, 128), (128, 126)])
+@pytest.mark.parametrize("dim,rotary", [(128, 128), (128, 64), (64, 64), (80, 22), (96, 96), (256, 192), (2, 2), (4, 2), (1024, 1024), (130, 128), (128, 126),
+                                        (1024, 2), (1022, 510)])
 def test_layouts_and_sizes(env, dtype, layout, dim, rotary):
     case(test="sizes", dtype=dtype, layout=layout, dim=dim, rotary=rotary)
     E = env["E"]
