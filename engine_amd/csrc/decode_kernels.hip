@@ -713,7 +713,8 @@ struct PrefillI8 {
         whole = end / kKv8Block;
         tail_blk = end % kKv8Block != 0 ? whole : -1;
     }
-    __device__ __forceinline__ int block_of(int kb, int idx) const { return 2 * kb + (idx >> 8); }
+    // (256 pieces a block: a wave's are all of one)
+    __device__ __forceinline__ int block_of(int kb, int idx) const { return 2 * kb + __builtin_amdgcn_readfirstlane(idx >> 8); }
     __device__ __forceinline__ uint4 codes(int kb, int idx, int part) const {
         const int b = block_of(kb, idx);
         return load_b128(cr, b < whole ? (uint32_t)b * kKv8BlockBytes + (uint32_t)part + 16u * (uint32_t)(idx & 255) : kOOR);
@@ -1655,29 +1656,49 @@ bool wide_prefill(const PrefillAttnArgs& a, int tiles, int cu_count) {
 
 // Key shares of a narrow launch over an 8-bit cache: few tokens over a long
 // context leave most CUs without a workgroup and the others with every key block in
-// turn (37 tokens after 2,011, 32 / 8 heads: 24 workgroups, 59 us). Shares of at least
-// kMinShare blocks, as many as two workgroups a CU take, the partials' room and the
-// merge's 32 lanes allow.
-constexpr int kMinShare = 2;
-int prefill_splits(const PrefillAttnArgs& a, int tiles, int cu_count) {
-    if (a.partials == nullptr) return 1;
+// turn. The share count of least cost, of those that two workgroups a CU, the partials'
+// room and the merge's 32 slots allow: in microseconds, a key round takes 1.75 with
+// few workgroups on the card, 2.4 with one a CU and 3.2 with two; the merge 4 and
+// the partials' way out and back at 3 TB/s. Whole calls, 32 / 8 heads, unsplit and by this rule:
+// 37 tokens after 2,011 73 and 24 us; 512 after 4,000 about 160 and 117; 512 from
+// position 0 stay unsplit (two shares: 47 for 28).
+int prefill_splits(const PrefillAttnArgs& a, int groups, int cu_count) {
+    const size_t rows = (size_t)a.tokens * a.q_heads;
     const int blocks = (a.p0 + a.tokens - 1) / kPfKeys + 1;
-    const int fill = 2 * cu_count / (tiles * a.kv_heads);
-    const size_t room = a.partial_rows / ((size_t)a.tokens * a.q_heads);
-    return std::max(1, std::min(std::min(32, fill), std::min(blocks / kMinShare, (int)std::min<size_t>(room, 32))));
+    const int most = (int)std::min<size_t>({32, (size_t)blocks, (size_t)(2 * cu_count / groups), a.partial_rows / rows});
+    int best = 1;
+    float least = FLT_MAX;
+    for (int s = 1; s <= most; ++s) {
+        const float load = (float)(groups * s) / (float)cu_count;
+        const float rounds = (float)((blocks + s - 1) / s) * (1.75f + 0.85f * std::max(0.f, load - 0.25f));
+        const float cost = rounds + (s == 1 ? 0.f : 4.f + (float)(rows * s) * (2 * kPartStride * 4) / 3.0e6f);
+        if (cost < least) {
+            least = cost;
+            best = s;
+        }
+    }
+    return best;
 }
+
+// Over an 8-bit cache the narrow form serves up to a workgroup a CU, split by keys
+// (prefill_splits); the wide form takes over past that. Whole calls in us, narrow
+// and wide: 32 / 8 heads, 512 tokens (256 workgroups) after 4,000 117 and 126, after
+// 12,000 261 and 315, 640 tokens 179 and 130, 466 and 317; 16 / 8 heads, 1,024 (256) after
+// 4,000 126 and 138, 1,400 202 and 149; 64 / 8, 512 (256) after 4,000 145 and 218, 640 266 and
+// 222; 32 / 4, 1,024 (256) 157 and 238, 1,400 293 and 254; 8 / 8, 1,400 (176) 126 and 150. From
+// position 0 the two are within 15% of each other around the line.
 
 template <int QPK, int CACHE>
 hipError_t launch_prefill_heads(const PrefillAttnArgs& args, int cu_count, hipStream_t stream) {
     constexpr int TT = QPK < 4 ? 4 / QPK : 1;  // token tiles per workgroup
     PrefillAttnArgs a = args;
     const int wide = (a.tokens + kPrefillWideTokens * TT - 1) / (kPrefillWideTokens * TT);
-    if (wide_prefill(a, wide, cu_count)) {
+    const int tiles = (a.tokens + kPrefillTileTokens * TT - 1) / (kPrefillTileTokens * TT);
+    if (CACHE == kCacheI8 ? tiles * a.kv_heads > cu_count : wide_prefill(a, wide, cu_count)) {
         hipLaunchKernelGGL((attn_prefill_wide_kernel<QPK, CACHE>), dim3((unsigned)wide * (unsigned)a.kv_heads), dim3(512), 0, stream, a, wide);
         return hipGetLastError();
     }
-    const int tiles = (a.tokens + kPrefillTileTokens * TT - 1) / (kPrefillTileTokens * TT);
-    a.splits = CACHE == kCacheI8 ? prefill_splits(a, tiles, cu_count) : 1;
+    a.splits = CACHE == kCacheI8 ? prefill_splits(a, tiles * a.kv_heads, cu_count) : 1;
     hipLaunchKernelGGL((attn_prefill_kernel<QPK, CACHE>), dim3((unsigned)tiles, (unsigned)a.kv_heads, (unsigned)a.splits), dim3(QPK < 8 ? 256 : 512), 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;

@@ -659,7 +659,10 @@ typedef struct ribn_amd_kv_options {
  * 8 bits, the last one, while it is not whole, from f16. A call at a position past
  * the end leaves the skipped tokens, and those of the block the sequence stood in, undefined
  * (finite). Fresh caches read as zeros; they are set up on ctx's stream, which work
- * on another stream has to wait for. */
+ * on another stream has to wait for. A context's first I8 cache reserves 17 MB on it
+ * besides: short prompt chunks on that context keep partial results there in stream order,
+ * as its other scratch is shared (captured calls of one context are replayed one after
+ * another). A context without it does the same work unsplit. */
 ribn_amd_status ribn_amd_kv_cache_create_with(ribn_amd_context *ctx, const ribn_amd_qwen3_config *config,
                                               uint32_t capacity, const ribn_amd_kv_options *options,
                                               ribn_amd_kv_cache **out);
@@ -677,7 +680,7 @@ ribn_amd_status ribn_amd_kv_cache_tail(ribn_amd_kv_cache *cache, uint32_t layer,
  * keys (normalised and rotated already) and values, [tokens][kv_heads][128] of
  * `dtype` (RIBN_AMD_F16 or RIBN_AMD_F32), at positions position .. position +
  * tokens - 1 of one layer; len counts each array's elements. An I8 cache
- * appends them (see above); an F16 one rounds to f16. */
+ * appends them (see above); an F16 one rounds to f16. Pointers are 16-byte aligned. */
 ribn_amd_status ribn_amd_kv_cache_write(ribn_amd_context *ctx, ribn_amd_kv_cache *cache, uint32_t layer,
                                         uint32_t position, size_t tokens, const void *keys, const void *values,
                                         size_t len, uint32_t dtype);

@@ -287,6 +287,32 @@ def test_decode_members(env, members):
     np.testing.assert_array_equal(again, got[order])
 
 
+def test_bits_do_not_depend_on_the_other_members_caches(env):
+    """Capacities of one chunk, a few and many in one launch, each member as on its own."""
+    case(test="capacities")
+    cfg = config(env, 8, 2)
+    rng = np.random.default_rng(77)
+    shape = [(130, 140), (130, 5000), (250, 256), (250, 20000), (700, 701), (700, 12000), (8400, 8500), (8400, 40000)]
+    seqs = []
+    for n, cap in shape:
+        seqs.append(Seq(env, cfg, cap))
+        seqs[-1].fill(np.random.default_rng(n), n)  # the same context for equal lengths
+    step = Step(rng, cfg, len(shape))
+    for i in range(1, len(shape), 2):
+        for a in ("q", "k", "v"):
+            getattr(step, a)[i] = getattr(step, a)[i - 1]
+    lengths = [n for n, _ in shape]
+    got = decode(env, seqs, step, lengths)
+    for i in range(0, len(shape), 2):
+        np.testing.assert_array_equal(got[i], got[i + 1])
+    for i, (n, cap) in enumerate(shape):
+        one = Step(rng, cfg, 1)
+        for a in ("q", "k", "v"):
+            setattr(one, a, getattr(step, a)[i:i + 1])
+        one.qn, one.kn = step.qn, step.kn
+        np.testing.assert_array_equal(decode(env, [seqs[i]], one, [n])[0], got[i])
+
+
 def test_a_sequence_from_its_start(env):
     """Seventy steps from an empty cache, then back into the latest block, into an
     earlier one, onto a block's first position, and on from there."""
