@@ -509,9 +509,10 @@ template <> struct Members<true> {
 // How many tokens a member attends: its position's and those before it, or, where
 // the append was dropped or done for several members at once, what the cache holds.
 __device__ __forceinline__ int kv8_tokens(const AttnArgs& a, const AttnMember& mb, const Kv8Head& head, int pos, int& end) {
-    end = pos + 1;
+    const int reach = min(pos, mb.capacity) + 1;  // (any int32 is a position)
+    end = reach;
     if (a.appended || pos >= mb.capacity) end = *head.end;
-    return min(pos + 1, end);
+    return min(reach, end);
 }
 
 template <int QPK, bool INLINE>

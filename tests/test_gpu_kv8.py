@@ -372,6 +372,25 @@ def test_positions_out_of_range_write_nothing(env):
     assert not read(env, seqs[3].cache, cfg, 0, 0, 64).any()
 
 
+def test_the_largest_and_smallest_positions(env):
+    """Any int32 may be a position: the largest reads what the cache holds, the smallest is no token."""
+    case(test="extreme_positions")
+    cfg = config(env, 4, 2)
+    rng = np.random.default_rng(18)
+    seqs = [Seq(env, cfg, 64) for _ in range(2)]
+    for s in seqs:
+        s.fill(rng, 50)
+    step = Step(rng, cfg, 2)
+    positions = [2 ** 31 - 1, -2 ** 31]
+    got = decode(env, seqs, step, positions)
+    for s in seqs:
+        s.check()
+    # (the query's f32 cosines at 2^31 - 1 are those of 64-bit angles: 2^31 * 2^-53 turns)
+    q, _ = step.turned(positions, table(None))
+    assert max_rel_err(got[0], L.attend(q[0], *seqs[0].model[0].rows())) <= ATTN_TOL
+    assert not got[1].any()
+
+
 @pytest.mark.parametrize("gain", [1e-18, 1e18])
 def test_queries_of_any_size(env, gain):
     """The norm brings q to size; its weight may be anything (here 1e4 times the usual: a softmax of one key)."""
