@@ -12,6 +12,7 @@ bytes unchanged to device memory.
 from __future__ import annotations
 
 import ctypes
+import struct
 from dataclasses import dataclass
 
 from . import _lib
@@ -101,10 +102,12 @@ class GgufFile:
         _check(st, GgufError)
         return _value(v, self.handle, key)
 
-    def metadata_map(self) -> dict:
+    def metadata_keys(self) -> list:
         n = int(self._lib.ribn_amd_gguf_metadata_count(self.handle))
-        keys = [self._lib.ribn_amd_gguf_metadata_key(self.handle, i).decode("utf-8") for i in range(n)]
-        return {k: self.metadata(k) for k in keys}
+        return [self._lib.ribn_amd_gguf_metadata_key(self.handle, i).decode("utf-8") for i in range(n)]
+
+    def metadata_map(self) -> dict:
+        return {k: self.metadata(k) for k in self.metadata_keys()}
 
     def tensors(self) -> list:
         out = []
@@ -195,22 +198,43 @@ def _optional_f32(file: GgufFile, key: str, default: float) -> float:
     return default if v is None else float(v)
 
 
+_ROPE_SCALING_KEYS = {"type", "factor", "original_context_length", "finetuned", "yarn_beta_fast", "yarn_beta_slow"}
+
+
+def _rope_factors(file: GgufFile, pairs: int):
+    """The frequency divisors of a "rope_freqs.weight" tensor, None without one."""
+    info = file.tensor("rope_freqs.weight")
+    if info is None:
+        return None
+    if info.value_type != 0 or info.element_count() != pairs:
+        raise GgufError(36, pairs, info.element_count(), f"UnsupportedRopeScaling: {pairs} f32 rope_freqs")
+    span = file.tensor_data_range("rope_freqs.weight")
+    with open(file.path(), "rb") as f:
+        f.seek(span.start)
+        return struct.unpack(f"<{pairs}f", f.read(4 * pairs))
+
+
 def rope_from_gguf(file: GgufFile, head_dim: int, base: float):
-    """The scaled rope a file's "qwen3.rope.scaling.*" metadata asks for, None if
-    it asks for none. Types other than linear and yarn are refused: run without
-    their scaling such a model answers wrongly."""
+    """The scaled rope that a file's "qwen3.rope.scaling.*" metadata and "rope_freqs.weight"
+    tensor ask for, None if they ask for none. Types other than linear and yarn, and
+    scaling keys not known here, are refused: run without them such a model answers wrongly."""
     from .rope import AmdRopeSpec
 
-    kind = file.metadata("qwen3.rope.scaling.type")
+    prefix = "qwen3.rope.scaling."
+    factors = _rope_factors(file, head_dim // 2)
+    kind = file.metadata(prefix + "type")
     if kind is None or kind == "none":
-        return None
-    if kind not in ("linear", "yarn"):
-        raise GgufError(36, 0, 0, f"UnsupportedRopeScaling: {kind}")
-    factor = file.metadata("qwen3.rope.scaling.factor")
+        return None if factors is None else AmdRopeSpec(head_dim=head_dim, base=base, freq_factors=factors)
+    unknown = [k for k in file.metadata_keys() if k.startswith(prefix) and k[len(prefix):] not in _ROPE_SCALING_KEYS]
+    if kind not in ("linear", "yarn") or unknown:
+        raise GgufError(36, 0, 0, f"UnsupportedRopeScaling: {kind} {unknown}")
+    factor = file.metadata(prefix + "factor")
     if factor is None:
-        raise GgufError(35, 0, 0, "MissingMetadata: qwen3.rope.scaling.factor")
-    original = _required_u32(file, "qwen3.rope.scaling.original_context_length") if kind == "yarn" else 0
-    return AmdRopeSpec(head_dim=head_dim, base=base, scaling=kind, factor=float(factor), original_context=original)
+        raise GgufError(35, 0, 0, f"MissingMetadata: {prefix}factor")
+    original = _required_u32(file, prefix + "original_context_length") if kind == "yarn" else 0
+    return AmdRopeSpec(head_dim=head_dim, base=base, scaling=kind, factor=float(factor), original_context=original,
+                       beta_fast=_optional_f32(file, prefix + "yarn_beta_fast", 32.0),
+                       beta_slow=_optional_f32(file, prefix + "yarn_beta_slow", 1.0), freq_factors=factors)
 
 
 def qwen3_config_from_gguf(file: GgufFile):

@@ -148,13 +148,13 @@ def test_codes_at_the_edges():
     assert list(L.half(np.array([np.nan, np.inf, -1e9, 65519.9]))) == [0, 65504, -65504, 65504]
 
 
-def gguf_file(tmp_path, extra):
+def gguf_file(tmp_path, extra, tensors=()):
     md = [("general.architecture", W.STRING, "qwen3"), ("qwen3.block_count", W.U32, 1),
           ("qwen3.embedding_length", W.U32, 512), ("qwen3.feed_forward_length", W.U32, 768),
           ("qwen3.attention.head_count", W.U32, 4), ("qwen3.attention.head_count_kv", W.U32, 2),
           ("qwen3.attention.key_length", W.U32, 128), *extra]
     path = tmp_path / "m.gguf"
-    path.write_bytes(W.build(md, [("token_embd.weight", [512, 2], 12, bytes(2 * 2 * 144))]))
+    path.write_bytes(W.build(md, [("token_embd.weight", [512, 2], 12, bytes(2 * 2 * 144)), *tensors]))
     return GgufFile.open(str(path))
 
 
@@ -174,3 +174,22 @@ def test_gguf_rope_scaling(tmp_path):
         with pytest.raises(GgufError) as e:
             E.qwen3_config_from_gguf(gguf_file(tmp_path, extra))
         assert e.value.kind == kind
+
+
+def test_gguf_rope_betas_and_factors(tmp_path):
+    key = "qwen3.rope.scaling."
+    yarn = [(key + "type", W.STRING, "yarn"), (key + "factor", W.F32, 4.0), (key + "original_context_length", W.U32, 32768)]
+    cfg = E.qwen3_config_from_gguf(gguf_file(tmp_path, yarn + [(key + "yarn_beta_fast", W.F32, 16.0), (key + "yarn_beta_slow", W.F32, 2.0)]))
+    assert cfg.rope == E.AmdRopeSpec(scaling="yarn", factor=4.0, original_context=32768, beta_fast=16.0, beta_slow=2.0)
+    with pytest.raises(GgufError) as e:  # a key that would change the angles
+        E.qwen3_config_from_gguf(gguf_file(tmp_path, yarn + [(key + "attn_factor", W.F32, 2.0)]))
+    assert e.value.kind == "MetadataTypeMismatch"
+    factors = tuple(float(1 + i % 8) for i in range(64))
+    cfg = E.qwen3_config_from_gguf(gguf_file(tmp_path, [], [("rope_freqs.weight", [64], 0, W.f32_payload(factors))]))
+    assert cfg.rope == E.AmdRopeSpec(freq_factors=factors)
+    turns, gain = E.rope_frequencies(cfg.rope)
+    plain, _ = E.rope_frequencies(E.AmdRopeSpec())
+    np.testing.assert_allclose(turns, np.array(plain) / factors, rtol=1e-15)
+    assert gain == 1.0
+    with pytest.raises(GgufError):
+        E.qwen3_config_from_gguf(gguf_file(tmp_path, [], [("rope_freqs.weight", [32], 0, W.f32_payload(factors[:32]))]))
