@@ -695,7 +695,10 @@ __device__ __forceinline__ float4 nonfinite_values(uint2 w) {
 // (kv8.hpp), dequantised exactly into the f16 the LDS tiles hold. The block
 // that is not whole (keys from the sequence's last multiple of 32 on) comes from the tail, with
 // the same lanes and no prefetch: it is one half pair of a launch. Blocks past it read
-// as zeros.
+// as zeros. The matrix cores bound long chunks as they do over f16 caches, and half the
+// bytes buy little: 2,047 tokens from 0 (32 / 8 heads) take 90 us for 93, 1,999 after 6,203
+// 438 for 439 (each product counted twice, for the two pieces of q and p: 1,080 TFLOP/s);
+// 37 tokens after 2,011, where the keys' split counts, 24 for 55.
 struct PrefillI8 {
     __amdgpu_buffer_rsrc_t cr, sr;
     const _Float16* tail_k;
@@ -1077,8 +1080,8 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
     }
 }
 
-// The key shares of a (token, query head) merged. A share whose keys the token does
-// not reach has a denominator of 0 and the lowest maximum.
+// The key shares of a (token, query head) merged, 11 of 37 x 32 rows in 4 us. A share whose
+// keys the token does not reach has a denominator of 0 and the lowest maximum.
 __global__ __launch_bounds__(128) void prefill_merge_kernel(const float* partials, float* out, int splits) {
     const size_t row = blockIdx.x;
     merge_row<32>(partials + row * (size_t)splits * kPartStride, splits, [&] { return splits; }, out + row * kHeadDim);
@@ -1658,8 +1661,8 @@ bool wide_prefill(const PrefillAttnArgs& a, int tiles, int cu_count) {
 // context leave most CUs without a workgroup and the others with every key block in
 // turn. The share count of least cost, of those that two workgroups a CU, the partials'
 // room and the merge's 32 slots allow: in microseconds, a key round takes 1.75 with
-// few workgroups on the card, 2.4 with one a CU and 3.2 with two; the merge 4 and
-// the partials' way out and back at 3 TB/s. Whole calls, 32 / 8 heads, unsplit and by this rule:
+// few workgroups on the card, 2.4 with one a CU and 3.2 with two; the merge takes 4 and
+// the partials their way out and back at 3 TB/s. Whole calls, 32 / 8 heads, unsplit and by this rule:
 // 37 tokens after 2,011 73 and 24 us; 512 after 4,000 about 160 and 117; 512 from
 // position 0 stay unsplit (two shares: 47 for 28).
 int prefill_splits(const PrefillAttnArgs& a, int groups, int cu_count) {

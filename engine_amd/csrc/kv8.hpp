@@ -14,7 +14,7 @@
 // the f16 matrix cores what the cache stands for, with no second rounding, and
 // a block scaled again from its own values keeps them. It costs half a bit of
 // the 8 on average against a / 127 (an error of 0.29 * 2^e: 0.23% to 0.46% of a).
-// a scale for 32 tokens: the depth of one 16x16x32 product over keys.
+// A scale for 32 tokens: the depth of one 16x16x32 product over keys.
 //
 // Codes are written when a block's last token arrives; until then its tokens are
 // the tail's f16 values, so a token is rounded to 8 bits once and by all 32

@@ -27,7 +27,9 @@ constexpr int kRowHalfs = kHeadDim + 8;  // LDS row of a staged token (272 B: 16
 // last block's workgroup writes what the tail holds after the call (its rows)
 // and `end`, unless workgroup 0 may read the tail as it was (an append into the middle
 // of a block): then that one does both, after its own block. Traffic is the rows in
-// (f32) and a byte a value out.
+// and a byte a value out: 32,768 f16 rows of 8 heads (134 MB in, 67 out) take 48 us, 4.2 TB/s.
+// Short appends are the latency of one row's chain (load, sum of squares, angles, LDS,
+// maximum, codes): 37 prompt tokens 7.0 us, 2,047 (17 MB in, 4 out) 8.8.
 
 constexpr int kAppendThreads = 512;  // 16 lanes a row, a block's rows at once
 __device__ __forceinline__ int append_tid() { return threadIdx.x & (kAppendThreads - 1); }
@@ -299,7 +301,9 @@ __device__ __forceinline__ void store_row(float* p, kv8_half8 h) {
 }
 
 // Rows out of an 8-bit cache, grid (KV head, block): the values its codes stand
-// for, the tail's f16 values of the block that is not whole, zeros past `end`.
+// for, the tail's f16 values of the block that is not whole, zeros past `end`. Through
+// LDS, so that rows leave whole: 32,768 rows of 8 heads (67 MB in, 134 out) in 30.6 us, 6.6 TB/s
+// (the codes had just been written).
 template <typename T>
 __global__ __launch_bounds__(kAppendThreads, 4) void kv8_read_kernel(KvMoveArgs a) {
     __shared__ Stage st;
@@ -367,12 +371,21 @@ __global__ __launch_bounds__(256) void cache_init_kernel(CacheInit a) {
 // kv8_attn_kernel: one layer's attention of decode members over their caches,
 // the new token's key and value appended on the way, on the f16 matrix cores: the
 // cache's values are f16 exactly, and converting and multiplying a byte for eight
-// query heads would leave the VALU behind the memory.
+// query heads would leave the VALU behind the memory. Memory bounds the long cases
+// (131,071 tokens, 269 MB: 49.5 us, 5.4 TB/s), latency the short ones: 5.6 us pass
+// between a launch and its output however little it reads (40 tokens), and 8 members of 3,000
+// (36 MB) take 11, 24 of 1,501 with 64 heads (58 MB) 16, their merge 2 to 3 more.
 //
 // Split as attn_decode_kernel's: grid (chunk, KV head, member), a chunk one
 // contiguous run of whole blocks; its waves take the blocks in turn. A block is
 // 8 KB of codes, eight 16-byte loads a lane, each of them contiguous over
-// the wave (the codes lie in that order), kRing blocks in flight a wave.
+// the wave (the codes lie in that order), one block in flight a wave, up to three
+// workgroups a CU.
+//
+// The chunks are merged by a launch of its own. The last workgroup of a row to arrive could
+// do it, but handing partials over between XCDs costs as much: with write-through
+// stores and loads 8 members of 3,000 took 14.4 us for 13.9, 131,071 tokens 55.0
+// for 52.3, 8 members of 15,000 53 for 40 (with fences, which write back an XCD's whole L2, 70, 74 and 387).
 //
 // S^T = K Q^T (v_mfma_f32_16x16x32_f16: M = 16 keys, N = 16 columns, K = 32
 // dims): the columns are the QPK query heads of the KV head twice, the upper
@@ -393,10 +406,14 @@ constexpr float kLazy = 15.0f;
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 
-constexpr int kMinChunk = 256;  // two blocks a wave
+// Tokens of a chunk: two blocks a wave at least, four where there are many members (more than
+// 8, as for f16 caches: a member's bits do not depend on the others within either range).
+// Whole calls with 128 / 256 / 512 tokens: one member of 2,047 11.0 / 11.4 / 12.2 us, 8
+// of 3,000 15.8 / 14.0 / 13.7; with 256 / 512 / 1,024: 24 of 1,501 20.9 / 19.4 / 21.3.
+constexpr int kMinChunk = 256;
 constexpr int kMinChunkWide = 512;
-constexpr int kBitLaneMembers = 8;
-int kv8_min_chunk(int members) { return members > kBitLaneMembers ? kMinChunkWide : kMinChunk; }
+constexpr int kFewMembers = 8;
+int kv8_min_chunk(int members) { return members > kFewMembers ? kMinChunkWide : kMinChunk; }
 
 __device__ __forceinline__ int kv8_chunk_tokens(int tokens, int chunks, int min_chunk) {
     const int len = max((tokens + chunks - 1) / chunks, min_chunk);
@@ -409,7 +426,6 @@ __device__ __forceinline__ float other_half(float v) {
 }
 
 typedef float kv8_float4 __attribute__((ext_vector_type(4)));
-
 typedef uint32_t kv8_u4 __attribute__((ext_vector_type(4)));
 
 // The tail's block in the operands' order: keys (tile t, step s) at 4 t + s, values

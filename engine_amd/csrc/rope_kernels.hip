@@ -7,7 +7,8 @@
 // 50 instructions each), into LDS, while their first rows are on the way; then a
 // thread turns one group of pairs in every slices-th head of every tensor of the
 // call. Bound by memory: each value is read and written once, in 16-byte pieces (a
-// wave covers whole heads), kUnroll heads in flight.
+// wave covers whole heads), kUnroll heads in flight: 32,768 tokens of 40 f32 heads of 128
+// (1.34 GB) take 230 us, 5.8 TB/s. One token takes 3 us, a launch and one load's way.
 #include "rope.hpp"
 
 #include <algorithm>
@@ -21,8 +22,12 @@ namespace {
 constexpr int kThreads = 256;     // of a workgroup, or what one head takes: up to 1,023 single elements
 constexpr int kMaxThreads = 1024;
 static_assert(kRopeMaxDim <= kMaxThreads, "a head fits a workgroup");
+// Heads a thread has in flight and takes where tokens are many: 32,768 tokens (above) with
+// 1 / 3 / 4 / 8 heads 238 / 232 / 233 / 248 us, with workgroups of 512 239.
 constexpr int kUnroll = 3;
 constexpr int kHeads = kUnroll;
+// Below this many threads a CU a token's heads are spread over more of them: 2,047 tokens of 32
+// bf16 heads, half of each turning, with 512 / 1,024 / 2,048 threads 7.8 / 7.9 / 10.0 us.
 constexpr int kThreadsPerCu = 1024;
 
 template <typename T, int E> struct Piece { T v[E]; };
