@@ -66,6 +66,7 @@ def rope_frequencies(spec: AmdRopeSpec):
 
 _POSITIONS = 3
 _DTYPES: dict = {}
+_ROWS = struct.Struct("18N")  # queries and keys
 
 
 def _dtype(t):
@@ -99,27 +100,29 @@ class AmdRope:
 
     def execute_group(self, inputs, positions, outputs):
         """Up to four tensors sharing their tokens' positions (queries and keys) in one launch."""
-        if len(inputs) != len(outputs):
-            raise ValueError(f"{len(inputs)} inputs and {len(outputs)} outputs")
+        count = len(inputs)
+        if count != len(outputs):
+            raise ValueError(f"{count} inputs and {len(outputs)} outputs")
         if _dtype(positions) != _POSITIONS or positions.dim() != 1 or not positions.is_contiguous():
             raise TypeError("positions must be a contiguous vector of int32")
-        tokens = positions.numel()
+        tokens = positions.shape[0]
         dim = self.spec.head_dim
-        kind = inputs[0].dtype if inputs else None
-        dtype = _dtype(inputs[0]) if inputs else 0
+        kind = inputs[0].dtype if count else None
+        dtype = _DTYPES.get(kind, 0 if kind is None else _POSITIONS)
         rows = []  # ribn_amd_rope_rows, nine words each
         for x, y in zip(inputs, outputs):
-            if dtype not in (0, 1, 2) or x.dtype != kind or y.dtype != kind:
+            if dtype == _POSITIONS or x.dtype is not kind or y.dtype is not kind:
                 raise TypeError("rope takes float32, bfloat16 or float16 tensors of one type")
             shape = x.shape
             if len(shape) != 3 or shape != y.shape or shape[0] != tokens or shape[2] != dim:
                 raise ValueError(f"rope rows are [{tokens}][heads][{dim}], got {tuple(shape)} and {tuple(y.shape)}")
-            xs, ys = x.stride(), y.stride()
-            if xs[2] != 1 or ys[2] != 1:
+            xt, xh, xd = x.stride()
+            yt, yh, yd = y.stride()
+            if xd != 1 or yd != 1:
                 raise ValueError("the dims of a head must be contiguous")
-            rows += (x.data_ptr(), _length(x), xs[0], xs[1], y.data_ptr(), _length(y), ys[0], ys[1], shape[1])
-        status = self.ctx._lib.ribn_amd_rope_execute(self.handle, positions.data_ptr(), tokens,
-                                                     struct.pack(f"{len(rows)}N", *rows), len(inputs), dtype)
+            rows += (x.data_ptr(), _length(x), xt, xh, y.data_ptr(), _length(y), yt, yh, shape[1])
+        status = self.ctx._lib.ribn_amd_rope_execute(self.handle, positions.data_ptr(), tokens, _ROWS.pack(*rows) if count == 2
+                                                     else struct.pack(f"{9 * count}N", *rows), count, dtype)
         if status:
             _check(status, AmdModelKernelError)
 

@@ -603,8 +603,9 @@ void ribn_amd_rope_destroy(ribn_amd_rope *rope);
 
 /* One tensor of rows to rotate: element (t, h, d) lies at t * token_stride +
  * h * head_stride + d, strides and lengths in elements. `output` may be `input`
- * with the same strides; it must not overlap it otherwise, nor have rows that
- * overlap each other (InvalidArgument). */
+ * with the same strides (InvalidArgument with others), and its rows must not overlap
+ * each other (InvalidArgument). No other overlap of an output with an input or with
+ * another output is checked for, and none has a defined result. */
 typedef struct ribn_amd_rope_rows {
     const void *input;
     size_t input_len;
