@@ -484,6 +484,47 @@ def test_chunk_taken_back(env):
 
 # ----------------------------------------------------------------- f16 caches with a rope
 
+@pytest.mark.parametrize("seed", range(6))
+def test_a_walk_of_all_calls(env, seed):
+    """Steps, chunks and rows in, at the end or somewhere before it, in any order over two sequences and two layers:
+    each answer and each cache as the formulas have them."""
+    rng = np.random.default_rng(100 + seed)
+    q_heads, kv_heads = [(4, 2), (2, 2), (8, 1)][seed % 3]
+    cfg = config(env, q_heads, kv_heads, layers=2)
+    seqs = [Seq(env, cfg, 260) for _ in range(2)]
+    tab = table(None)
+    for turn in range(30):
+        layer, s = int(rng.integers(2)), seqs[int(rng.integers(2))]
+        end = s.model[layer].end
+        position = end if end == 0 or rng.random() < 0.6 else int(rng.integers(end))
+        room = s.capacity - position
+        kind = rng.choice(["step", "both", "chunk", "rows"]) if room else "past"
+        n = min(room, int(rng.choice([1, 3, 31, 32, 33, 70])))
+        case(test="walk", seed=seed, turn=turn, kind=str(kind), layer=layer, position=position, n=n)
+        if kind == "step":
+            check_decode(env, [s], Step(rng, cfg, 1), [position], tab, layer)
+        elif kind == "both":
+            positions = [min(x.model[layer].end, x.capacity - 1) for x in seqs]
+            check_decode(env, seqs, Step(rng, cfg, 2), positions, tab, layer)
+        elif kind == "chunk":
+            check_prefill(env, s, Step(rng, cfg, n), n, position, tab, layer)
+        elif kind == "rows":
+            k, v = rows(rng, n, kv_heads)
+            half = rng.random() < 0.5
+            if half:
+                k, v = k.astype(np.float16), v.astype(np.float16)
+            s.cache.write(layer, dev(k), dev(v), position)
+            s.model[layer].append(position, k.astype(np.float32), v.astype(np.float32))
+        else:
+            got = decode(env, [s], step := Step(rng, cfg, 1), [s.capacity + turn], layer)
+            q, _ = step.turned([s.capacity + turn], tab)
+            assert max_rel_err(got[0], L.attend(q[0], *s.model[layer].rows())) <= ATTN_TOL
+        for x in seqs:
+            for i in range(2):
+                if x.model[i].end:
+                    x.check(i)
+
+
 @pytest.mark.parametrize("rope", [dict(), YARN], ids=("plain", "yarn"))
 def test_f16_cache_with_a_rope(env, rope):
     """Decode, many-member and prompt attention over f16 caches whose angles come
