@@ -163,6 +163,30 @@ def test_strides_and_places(env, dtype, layout):
     assert torch.equal(view, y) and bool((flat[0] == 5.0).all()) and bool((flat[1:].view(37, 2, 130)[:, :, 128:] == 5.0).all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dim,rotary", [(96, 42), (128, 14), (80, 68), (256, 2), (64, 62), (192, 190), (128, 6), (1024, 1022), (1024, 520)])
+def test_rotary_parts_that_end_inside_a_piece(env, dtype, layout, dim, rotary):
+    """Whole heads are in 16-byte pieces, the rotary part or its halves are not: three tensors of uneven heads
+    out of a fused row, out of place and in place, the rest of the row as it was."""
+    E, torch = env["E"], env["torch"]
+    spec = E.AmdRopeSpec(head_dim=dim, rotary_dim=rotary, layout=layout, base=1.0e4)
+    rope = E.AmdRope(env["ctx"], spec)
+    for tokens, heads in ((1, (1, 1, 1)), (1, (40, 8, 3)), (7, (33, 1, 2)), (300, (9, 2, 1)), (1500, (3, 1, 1))):
+        case(test="inside", dtype=dtype, layout=layout, dim=dim, rotary=rotary, tokens=tokens, heads=heads)
+        fused, pos = rows(env, tokens, sum(heads) + 2, dim, dtype, tokens + heads[0]), positions(env, tokens, tokens)
+        ends = np.cumsum(heads)
+        parts = [fused[:, e - n:e] for e, n in zip(ends, heads)]
+        outs = [torch.full((tokens, n, dim), 9.0, dtype=fused.dtype, device="cuda:0") for n in heads]
+        rope.execute_group(parts, pos, outs)
+        for x, y in zip(parts, outs):
+            check(env, x, y, pos, spec)
+        rest = fused[:, ends[-1]:].clone()
+        rope.execute_group(parts, pos, parts)
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(parts, outs)) and torch.equal(fused[:, ends[-1]:], rest)
+
+
 def test_four_tensors_of_many_heads(env):
     case(test="four")
     E, torch = env["E"], env["torch"]
