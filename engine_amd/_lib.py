@@ -198,7 +198,7 @@ SIGNATURES = {
     "ribn_amd_kv_cache_destroy": (None, [_vp]),
     "ribn_amd_kv_cache_capacity": (_u32, [_vp]),
     "ribn_amd_kv_cache_layer": (_i32, [_vp, _u32, _pvp, _pvp]),
-    "ribn_amd_attention_decode": (_i32, [_vp, ctypes.POINTER(Qwen3Config), _pvp, _sz, _u32, _vp, _vp, _vp, _vp,
+    "ribn_amd_attention_decode": (_i32, [_vp, ctypes.POINTER(Qwen3Config), _vp, _sz, _u32, _vp, _vp, _vp, _vp,
                                          _vp, _vp, _vp, _sz]),
     "ribn_amd_argmax": (_i32, [_vp, _vp, _sz, _sz, _vp]),
     "ribn_amd_qwen3_decode_create": (_i32, [_vp, ctypes.POINTER(Qwen3Config), _vp, _vp, _vp,
@@ -215,9 +215,9 @@ SIGNATURES = {
     "ribn_amd_qwen3_prefill_prompt": (_i32, [_vp, _vp, ctypes.POINTER(_u32), _sz, _u32, _u32]),
     "ribn_amd_qwen3_reserve_prompt": (_i32, [_vp, _u32]),
     "ribn_amd_qwen3_decode_step": (_i32, [_vp, _vp, _u32, _u32, ctypes.POINTER(_u32)]),
-    "ribn_amd_qwen3_decode_step_batch": (_i32, [_vp, _pvp, ctypes.POINTER(_u32), ctypes.POINTER(_u32), _sz,
+    "ribn_amd_qwen3_decode_step_batch": (_i32, [_vp, _vp, ctypes.POINTER(_u32), ctypes.POINTER(_u32), _sz,
                                                 ctypes.POINTER(_u32)]),
-    "ribn_amd_qwen3_generate": (_i32, [_vp, _pvp, ctypes.POINTER(_u32), ctypes.POINTER(_u32), _sz, _u32,
+    "ribn_amd_qwen3_generate": (_i32, [_vp, _vp, ctypes.POINTER(_u32), ctypes.POINTER(_u32), _sz, _u32,
                                        ctypes.POINTER(_u32)]),
     "ribn_amd_qwen3_copy_hidden": (_i32, [_vp, _sz, _vp, _sz]),
     "ribn_amd_qwen3_copy_logits": (_i32, [_vp, _sz, _vp, _sz]),

@@ -105,7 +105,7 @@ class AmdKvCache:
         row = self.config.kv_heads * self.config.head_dim
         if keys.numel() % row:
             raise ValueError(f"cache rows have {row} values, got {keys.numel()}")
-        _check(call(self.ctx.handle, self.handle, layer, position, keys.numel() // row, _ptr(keys), _ptr(values),
+        _check(call(self.ctx.handle, self.handle, layer, position, keys.numel() // row, keys.data_ptr(), values.data_ptr(),
                     keys.numel(), dtype), AmdModelKernelError)
 
     def capacity(self) -> int:
@@ -132,25 +132,23 @@ class AmdKvCache:
 
 
 def _handles(caches):
-    return (ctypes.c_void_p * len(caches))(*[c.handle.value for c in caches])
+    return b"".join([c.handle for c in caches])  # pointers in a row
 
 
 def attention_decode(ctx, config: AmdQwen3Config, caches, layer: int, q, k, v, q_norm, k_norm, positions, output):
     """One layer's decode attention for len(caches) members (positions: device int32)."""
-    cfg = config.to_c()
-    _check(ctx._lib.ribn_amd_attention_decode(ctx.handle, ctypes.byref(cfg), _handles(caches), len(caches), layer,
-                                              _ptr(q), _ptr(k), _ptr(v), _ptr(q_norm), _ptr(k_norm), _ptr(positions),
-                                              _ptr(output), output.numel()), AmdModelKernelError)
+    _check(ctx._lib.ribn_amd_attention_decode(ctx.handle, ctypes.byref(config.to_c()), _handles(caches), len(caches), layer,
+                                              q.data_ptr(), k.data_ptr(), v.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(),
+                                              positions.data_ptr(), output.data_ptr(), output.numel()), AmdModelKernelError)
 
 
 def attention_prefill(ctx, config: AmdQwen3Config, cache, layer: int, q, k, v, q_norm, k_norm, tokens: int,
                       position: int, output):
     """One layer's causal attention for a prompt chunk of `tokens` tokens at
     `position` (the K/V appended first)."""
-    cfg = config.to_c()
-    _check(ctx._lib.ribn_amd_attention_prefill(ctx.handle, ctypes.byref(cfg), cache.handle, layer, _ptr(q), _ptr(k),
-                                               _ptr(v), _ptr(q_norm), _ptr(k_norm), tokens, position, _ptr(output),
-                                               output.numel()), AmdModelKernelError)
+    _check(ctx._lib.ribn_amd_attention_prefill(ctx.handle, ctypes.byref(config.to_c()), cache.handle, layer, q.data_ptr(),
+                                               k.data_ptr(), v.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(), tokens,
+                                               position, output.data_ptr(), output.numel()), AmdModelKernelError)
 
 
 class AmdQwen3Decode:
