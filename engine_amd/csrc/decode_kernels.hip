@@ -661,7 +661,6 @@ typedef float pf_float4 __attribute__((ext_vector_type(4)));
 
 constexpr int kPfKeys = 64;              // keys per block
 constexpr int kPfVRow = kPfKeys + 4;     // LDS V^T row (halfs): 136 B
-constexpr float kPfLazy = 15.0f;         // log2 headroom of the lazy softmax rescale
 
 // Values that are infinite or NaN. A key past a token's position has probability
 // 0, but 0 * inf is NaN, so in blocks with such keys (those from a workgroup's
@@ -989,41 +988,43 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
         }
         bmax = fmaxf(bmax, __shfl_xor(bmax, 16, 64));
         bmax = fmaxf(bmax, __shfl_xor(bmax, 32, 64));
-        // Lazy rescaling: the reference point m_run moves (to the block's
-        // maximum) only when that maximum passes it by more than kPfLazy.
-        // Until then the probabilities exp2(s - m_run) stay below
-        // 2^kPfLazy, inside f16 range for the hi/lo split, and O and l keep
+        // Lazy rescaling: the reference point m_run moves (to kTopExponent
+        // below the block's maximum) only when that maximum passes it by more
+        // than kMaxExponent. Until then the numerators exp2(s - m_run) stay
+        // inside f16 range for the hi/lo split, and O and l keep
         // their scale; O / l is the same softmax. The first block always
         // moves it (from -FLT_MAX, with a zero correction).
-        const bool move = bmax > m_run + kPfLazy;
+        const bool move = bmax > m_run + kMaxExponent;
         if (__any(move)) {
-            const float m_new = move ? bmax : m_run;
+            const float m_new = move ? bmax - kTopExponent : m_run;
             const float corr = __builtin_amdgcn_exp2f(m_run - m_new);
             m_run = m_new;
             l_run *= corr;
 #pragma unroll
             for (int d = 0; d < 8; ++d) o[d] *= corr;
         }
-        // probabilities in pairs: hi = f16(p) and lo = f16(p - hi), each pair
-        // converted by one packed instruction (round toward zero: hi + lo
-        // still carries 22 bits of p, since p - hi is exact in f32)
+        // numerators in pairs: hi = f16(p) and lo = f16(p - hi), each pair
+        // converted by one packed instruction (kv8_halfs): hi + lo carries 22
+        // bits of p, since p - hi is exact in f32
         pf_half8 pb[2], pl[2];
+        float sum = 0.f;  // (a block's first: many small ones do not each meet a large l)
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
                 const float p0 = __builtin_amdgcn_exp2f(sc[kt][i] - m_run);
                 const float p1 = __builtin_amdgcn_exp2f(sc[kt][i + 1] - m_run);
-                l_run += p0;
-                l_run += p1;
-                const auto h = __builtin_amdgcn_cvt_pkrtz(p0, p1);
-                const auto r = __builtin_amdgcn_cvt_pkrtz(p0 - (float)h[0], p1 - (float)h[1]);
+                sum += p0;
+                sum += p1;
+                const kv8_half2 h = kv8_halfs(p0, p1);
+                const kv8_half2 r = kv8_halfs(p0 - (float)h[0], p1 - (float)h[1]);
                 pb[kt >> 1][4 * (kt & 1) + i] = h[0];
                 pb[kt >> 1][4 * (kt & 1) + i + 1] = h[1];
                 pl[kt >> 1][4 * (kt & 1) + i] = r[0];
                 pl[kt >> 1][4 * (kt & 1) + i + 1] = r[1];
             }
         }
+        l_run += sum;
         // O^T += V^T P^T over the block's two 32-key steps, issued
         // dim-tile-interleaved (eight accumulators between dependent MFMAs)
 #pragma unroll
@@ -1453,15 +1454,15 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
 #pragma unroll
             for (int i = 0; i < 16; ++i) bmax = fmaxf(bmax, sc[kt][i]);
         bmax = pair_combine(bmax, [](float u, float v) { return fmaxf(u, v); }) * a.scale;  // (scale > 0)
-        // Lazy rescaling: the reference point m_run moves (to the block's
-        // maximum) only when that maximum passes it by more than kPfLazy.
-        // Until then the probabilities exp2(s - m_run) stay below
-        // 2^kPfLazy, inside f16 range for the hi/lo split, and O and l keep
+        // Lazy rescaling: the reference point m_run moves (to kTopExponent
+        // below the block's maximum) only when that maximum passes it by more
+        // than kMaxExponent. Until then the numerators exp2(s - m_run) stay
+        // inside f16 range for the hi/lo split, and O and l keep
         // their scale; O / l is the same softmax. The first block always
         // moves it (from -FLT_MAX, with a zero correction).
-        const bool move = bmax > m_run + kPfLazy;
+        const bool move = bmax > m_run + kMaxExponent;
         if (__any(move)) {
-            const float m_new = move ? bmax : m_run;
+            const float m_new = move ? bmax - kTopExponent : m_run;
             const float corr = __builtin_amdgcn_exp2f(m_run - m_new);
             m_run = m_new;
             l_run *= corr;
@@ -1470,10 +1471,11 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= corr;
         }
-        // Per 16-key step: probabilities in pairs, hi = f16(p) and lo =
-        // f16(p - hi), each pair converted by one packed instruction (round
-        // toward zero: hi + lo still carries 22 bits of p, since p - hi is
-        // exact in f32), then O^T += V^T P^T, dim tiles interleaved
+        // Per 16-key step: numerators in pairs, hi = f16(p) and lo =
+        // f16(p - hi), each pair converted by one packed instruction
+        // (kv8_halfs): hi + lo carries 22 bits of p, since p - hi is
+        // exact in f32, then O^T += V^T P^T, dim tiles interleaved
+        float sum = 0.f;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             pf_half8 pb, pl;
@@ -1482,10 +1484,10 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
                 const int i = 8 * (u & 1) + j;
                 const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u >> 1][i], a.scale, -m_run));
                 const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u >> 1][i + 1], a.scale, -m_run));
-                l_run += p0;
-                l_run += p1;
-                const auto hi = __builtin_amdgcn_cvt_pkrtz(p0, p1);
-                const auto lo = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)hi[0], -1.0f, p0), __builtin_fmaf((float)hi[1], -1.0f, p1));
+                sum += p0;
+                sum += p1;
+                const kv8_half2 hi = kv8_halfs(p0, p1);
+                const kv8_half2 lo = kv8_halfs(__builtin_fmaf((float)hi[0], -1.0f, p0), __builtin_fmaf((float)hi[1], -1.0f, p1));
                 pb[j] = hi[0];
                 pb[j + 1] = hi[1];
                 pl[j] = lo[0];
@@ -1499,6 +1501,7 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
 #pragma unroll
             for (int d = 0; d < 4; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d], pl, o[d], 0, 0, 0);
         }
+        l_run += sum;
         // a step's probabilities are formed under the previous step's MFMAs
         __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 4, 0);
         __builtin_amdgcn_sched_group_barrier(kSchedValu, 40, 0);

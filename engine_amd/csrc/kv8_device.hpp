@@ -114,6 +114,23 @@ __device__ __forceinline__ float wave_max(float v) {
     return fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3]));
 }
 
+// Softmax numerators as the matrix-core kernels form them, 2^(x - m) of scores x in log2
+// units, each as two f16 pieces. f16 ends at 2^-24: smaller parts of a numerator are rounded, and one
+// below 2^-25 is lost, while the denominator's f32 sum has it whole. With the largest at 2^0, an early key
+// far above 131,072 others took 3e-3 off the output. So the reference m is set
+// kTopExponent below the largest score (N keys then lose at most N 2^-33 of it), and moves
+// when a score passes it by kMaxExponent, the pieces being still in f16's range. The room between the
+// two keeps moves rare: 1,999 tokens after 6,203 take 435 us with 15 (m at the top), 443 with 7, 448 with 3.
+constexpr float kTopExponent = 8.0f;
+constexpr float kMaxExponent = 15.0f;
+
+// Two values as f16, to nearest even (one instruction here). The pieces of a numerator are
+// rounded so: cut off toward zero they leave lower pieces that are all positive, and what of those
+// a large sum on the matrix cores cannot take (it rounds after every eight products) is lost to
+// one side (1.5e-4 with the 131,072 keys above in one sum).
+typedef float kv8_float2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ kv8_half2 kv8_halfs(float a, float b) { return __builtin_convertvector((kv8_float2{a, b}), kv8_half2); }
+
 // The parts of a (layer, KV head) region.
 struct Kv8Head {
     uint8_t* codes;

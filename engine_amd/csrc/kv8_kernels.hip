@@ -396,14 +396,13 @@ __global__ __launch_bounds__(256) void cache_init_kernel(CacheInit a) {
 // consecutive keys, which is the B operand's share of O^T += V^T P^T (M = 16
 // dims, K = 32 keys), the probabilities again in two pieces by column half.
 // Codes enter the scores as whole numbers, the block's key scale being applied to
-// the f32 score; values are scaled as f16 (both exact). The running maximum is
-// the column's and moves only when a score passes it by 2^kLazy (attn_prefill_kernel
-// does the same); denominators are f32 sums of f32 probabilities.
+// the f32 score; values are scaled as f16 (both exact). The softmax's reference is
+// the column's and moves as kTopExponent says; denominators are f32 sums of f32
+// numerators, a block's first, so that many small ones do not each meet a large sum.
 //
 // The block the sequence stands in is the last wave's: it has the tail's rows in
 // the operands' order, puts the new token's row in from LDS, and, when the block is whole,
 // finds its scales and writes its codes from there, going on with what these stand for.
-constexpr float kLazy = 15.0f;
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 
@@ -683,28 +682,30 @@ __global__ __launch_bounds__(kThreads, 3) void kv8_attn_kernel(AttnArgs a, Membe
         float top = x[0];
 #pragma unroll
         for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
-        if (__any(top > mrun + kLazy)) {
+        if (__any(top > mrun + kMaxExponent)) {
             top = fmaxf(top, __shfl_xor(top, 16, 64));
             top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float mn = top > mrun + kLazy ? top : mrun;
+            const float mn = top > mrun + kMaxExponent ? top - kTopExponent : mrun;
             const float corr = __builtin_amdgcn_exp2f(mrun - mn);
             mrun = mn;
             lrun *= corr;
 #pragma unroll
             for (int d = 0; d < 8; ++d) o[d] *= corr;
         }
+        float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
             const float p0 = __builtin_amdgcn_exp2f(x[j] - mrun), p1 = __builtin_amdgcn_exp2f(x[j + 1] - mrun);
-            lrun += p0;
-            lrun += p1;
-            const auto hi = __builtin_amdgcn_cvt_pkrtz(p0, p1);
-            const auto lo = __builtin_amdgcn_cvt_pkrtz(p0 - (float)hi[0], p1 - (float)hi[1]);
+            sum += p0;
+            sum += p1;
+            const kv8_half2 hi = kv8_halfs(p0, p1);
+            const kv8_half2 lo = kv8_halfs(p0 - (float)hi[0], p1 - (float)hi[1]);
             const uint32_t hw = __builtin_bit_cast(uint32_t, hi), lw = __builtin_bit_cast(uint32_t, lo);
             const kv8_half2 p = __builtin_bit_cast(kv8_half2, n < 8 ? hw : lw);
             pb[j] = p[0];
             pb[j + 1] = p[1];
         }
+        lrun += sum;
     };
 
     if (tail) {

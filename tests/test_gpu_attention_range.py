@@ -1,0 +1,111 @@
+"""GPU tests of attention over 8-bit and f16 caches where its f16 pieces could run out of
+range: probabilities far below the largest, queries of any size. Against the definition
+in 64 bits, over the rows the cache holds (ATTN_TOL and its derivation: test_gpu_kv8).
+"""
+import numpy as np
+import pytest
+
+from .gpu_helpers import max_rel_err
+from .test_gpu_kv8 import ATTN_TOL, BASE, Step, case, config, dev, env, table  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+# turns every pair by next to nothing: a query is the same at every position
+STILL = dict(scaling="linear", factor=1e12)
+FORMATS = ("i8", "f16")
+
+
+def cache_of(env, cfg, capacity, fmt, rope=STILL):
+    E = env["E"]
+    spec = E.AmdRopeSpec(base=BASE, **rope) if rope else None
+    return E.AmdKvCache(env["ctx"], cfg, capacity, format=E.KV_I8 if fmt == "i8" else E.KV_F16, rope=spec)
+
+
+def held(env, cache, cfg, tokens):
+    """Keys and values [tokens][kv_heads][128] as the cache has them, f64 on the GPU."""
+    torch = env["torch"]
+    out = [torch.empty((tokens, cfg.kv_heads, 128), device="cuda:0") for _ in range(2)]
+    cache.read(0, 0, *out)
+    return [o.double() for o in out]
+
+
+def attend(q, keys, values):
+    """q [q_heads][128] (numpy), keys / values as `held`: [q_heads][128] by the definition."""
+    import torch
+    per = q.shape[0] // keys.shape[1]
+    out = []
+    for h in range(q.shape[0]):
+        s = (keys[:, h // per] * dev(np.asarray(q[h], np.float64))).sum(-1) / np.sqrt(128.0)
+        p = torch.exp(s - s.max())
+        out.append(((p[:, None] * values[:, h // per]).sum(0) / p.sum()).cpu().numpy())
+    return np.stack(out)
+
+
+def sink_rows(env, cfg, tokens, nats, seed):
+    """Keys whose scores with a query of +-1 (signs, [128]) are close to 0, but `nats` at token 0, and
+    values of mean 0.5: what the many keys lose against the one is not lost to both sides of the mean."""
+    torch = env["torch"]
+    g = torch.Generator(device="cuda:0")
+    g.manual_seed(seed)
+    signs = torch.where(torch.rand(128, device="cuda:0", generator=g) < 0.5, -1.0, 1.0)
+    k = 0.05 * torch.randn((tokens, cfg.kv_heads, 128), device="cuda:0", generator=g)
+    k[0] = signs * (nats / np.sqrt(128.0))
+    v = 0.5 + 0.05 * torch.randn((tokens, cfg.kv_heads, 128), device="cuda:0", generator=g)
+    return k, v, signs.cpu().numpy()
+
+
+def sink_step(rng, cfg, n, signs):
+    step = Step(rng, cfg, n)
+    step.q[:] = signs
+    step.k *= np.float32(0.05)
+    step.v = (0.5 + 0.05 * step.v).astype(np.float32)
+    step.qn[:] = 1
+    step.kn *= np.float32(0.05)
+    return step
+
+
+@pytest.mark.parametrize("nats", [10, 14])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_decode_after_a_sink(env, fmt, nats):
+    """One early key far above 524,287 others, 4,096 of them in a wave's share: probabilities
+    of 2^-14 to 2^-20 of the largest count with all their bits."""
+    case(test="decode_sink", fmt=fmt, nats=nats)
+    n = 524287
+    cfg = config(env, 2, 1)
+    cache = cache_of(env, cfg, n + 1, fmt)
+    k, v, signs = sink_rows(env, cfg, n, nats, nats)
+    cache.write(0, k, v, 0)
+    step = sink_step(np.random.default_rng(1), cfg, 1, signs)
+    out = dev(np.full(cfg.q_heads * 128, np.nan, np.float32))
+    env["E"].attention_decode(env["ctx"], cfg, [cache], 0, *step.device(), dev(np.array([n], np.int32)), out)
+    q, _ = step.turned([n], table(STILL))
+    want = attend(q[0], *held(env, cache, cfg, n + 1))
+    err = max_rel_err(out.cpu().numpy().reshape(-1, 128), want)
+    print(f"err {err:.2e}", flush=True)
+    assert err <= ATTN_TOL, err
+
+
+# tokens after a context of `position`, narrow and wide forms
+SINK_CHUNKS = [(2, 1, 16, 131072), (8, 1, 20, 131072), (8, 8, 40, 16384), (32, 32, 600, 16384), (64, 8, 1101, 16384)]
+
+
+@pytest.mark.parametrize("nats", [10, 14])
+@pytest.mark.parametrize("chunk", SINK_CHUNKS, ids=lambda c: "x".join(map(str, c)))
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_chunk_after_a_sink(env, fmt, chunk, nats):
+    case(test="chunk_sink", fmt=fmt, chunk=chunk, nats=nats)
+    q_heads, kv_heads, tokens, position = chunk
+    cfg = config(env, q_heads, kv_heads)
+    cache = cache_of(env, cfg, position + tokens, fmt)
+    k, v, signs = sink_rows(env, cfg, position, nats, nats + tokens)
+    cache.write(0, k, v, 0)
+    step = sink_step(np.random.default_rng(tokens), cfg, tokens, signs)
+    out = dev(np.full(tokens * q_heads * 128, np.nan, np.float32))
+    env["E"].attention_prefill(env["ctx"], cfg, cache, 0, *step.device(), tokens, position, out)
+    got = out.cpu().numpy().reshape(tokens, q_heads, 128)
+    assert np.isfinite(got).all()
+    q, _ = step.turned(position + np.arange(tokens), table(STILL))
+    rows = held(env, cache, cfg, position + tokens)
+    worst = max(max_rel_err(got[t], attend(q[t], *(x[:position + t + 1] for x in rows))) for t in (0, tokens // 2, tokens - 1))
+    print(f"err {worst:.2e}", flush=True)
+    assert worst <= ATTN_TOL, worst
