@@ -888,7 +888,7 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
 
     // ---- this lane's query dims 32s + 8g + j (s = 0..3, j = 0..7): RMSNorm
     // over the head's 128 dims (the four lanes of the token add their parts),
-    // NEOX rope of the pairs (d, d + 64) = (s, s + 2), f16
+    // NEOX rope of the pairs (d, d + 64) = (s, s + 2), f16 pieces (query_exponent)
     float x[4][8];
     const float* qrow = a.q + (size_t)t * qdim + (size_t)hq * kHeadDim;
 #pragma unroll
@@ -910,7 +910,7 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
     ssq += __shfl_xor(ssq, 16, 64);
     ssq += __shfl_xor(ssq, 32, 64);
     const float inv = 1.0f / sqrtf(ssq / (float)kHeadDim + a.eps);
-    pf_half8 qb[4], ql[4];
+    float top = 0.f;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
 #pragma unroll
@@ -926,12 +926,24 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
             } else {
                 r = cache_rot<TABLE>(a.mem.rope, d, pos, TABLE ? 0.f : rope_freq(a.rope_base, d));
             }
-            const float q0 = y0 * r.c - y1 * r.s;
-            const float q1 = y0 * r.s + y1 * r.c;
-            qb[s][j] = (_Float16)q0;
-            ql[s][j] = (_Float16)(q0 - (float)qb[s][j]);
-            qb[s + 2][j] = (_Float16)q1;
-            ql[s + 2][j] = (_Float16)(q1 - (float)qb[s + 2][j]);
+            x[s][j] = y0 * r.c - y1 * r.s;
+            x[s + 2][j] = y0 * r.s + y1 * r.c;
+            top = fmaxf(top, fmaxf(fabsf(x[s][j]), fabsf(x[s + 2][j])));
+        }
+    }
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const int qe = query_exponent(top);
+    const float qscale = a.scale * kv8_power(qe);
+    const float qinv = kv8_power(-qe);
+    pf_half8 qb[4], ql[4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float q = x[s][j] * qinv;
+            qb[s][j] = (_Float16)q;
+            ql[s][j] = (_Float16)(q - (float)qb[s][j]);
         }
     }
 
@@ -970,7 +982,7 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
             for (int kt = 0; kt < 4; ++kt) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    sc[kt][i] *= a.scale;
+                    sc[kt][i] *= qscale;
                     bmax = fmaxf(bmax, sc[kt][i]);
                 }
             }
@@ -980,7 +992,7 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int key = kb * kPfKeys + 16 * kt + 4 * g + i;
-                    const float v = key <= pos ? sc[kt][i] * a.scale : -INFINITY;
+                    const float v = key <= pos ? sc[kt][i] * qscale : -INFINITY;
                     sc[kt][i] = v;
                     bmax = fmaxf(bmax, v);
                 }
@@ -1161,7 +1173,8 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
     constexpr int kRows = 128;                        // (token, head) rows of query pieces at a time
     constexpr int kRotRow = 65;                       // float2 per token row (padded)
     constexpr int kQBytes = kRows * kHeadDim * 2 * 2;  // hi and lo
-    constexpr int kPrologue = kQBytes + TT * TOK * kRotRow * 8;
+    constexpr int kRotBytes = TT * TOK * kRotRow * 8;
+    constexpr int kPrologue = kQBytes + kRotBytes + kRows * 4;  // (and the rows' powers of two)
     constexpr int kLoop = 2 * KS * (int)sizeof(Buffer);
     __shared__ __attribute__((aligned(16))) char lds[kLoop > kPrologue ? kLoop : kPrologue];
     Buffer(*const bufs)[KS] = reinterpret_cast<Buffer(*)[KS]>(lds);
@@ -1323,12 +1336,14 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
 
     // ---- query pieces: row (token tile, head, token of the tile), RMSNorm
     // over the head's 128 dims, NEOX rope of the pairs (d, d + 64), f16 hi and
-    // lo. Sixteen lanes a row, eight dims each, in a short loop: a launch
+    // lo (query_exponent). Sixteen lanes a row, eight dims each, in a short loop: a launch
     // fetches its code cold, and unrolled per wave this took 10 us more.
     // 16-byte piece c of row r at slot c ^ (r & 15).
     pf_half8* const q_hi = reinterpret_cast<pf_half8*>(lds);
     pf_half8* const q_lo = q_hi + kRows * 16;
+    float* const q_pow = reinterpret_cast<float*>(lds + kQBytes + kRotBytes);
     pf_half8 qb[8], ql[8];
+    float qscale = 0.f;
     constexpr int kPasses = TT * TOK * QPK / kRows;
 #pragma unroll 1
     for (int pass = 0; pass < kPasses; ++pass) {
@@ -1356,24 +1371,37 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
             ssq = dpp_step<0x140>(ssq);  // row_mirror
             const float inv = 1.0f / sqrtf(ssq / (float)kHeadDim + a.eps);
             const float2* rot = rot_tab + ((unit / QPK) * TOK + (r & (TOK - 1))) * kRotRow + 8 * (c & 7);
-            pf_half8 vh, vl;
+            float q[8], top = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float y = x[j] * inv * w[j];
                 const float other = __builtin_bit_cast(  // dim d +- 64: lane c ^ 8 (row_ror 8)
                     float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, y), 0x128, 0xf, 0xf, false));
                 const float2 cs = rot[j];
-                const float q = y * cs.x + (c < 8 ? -other : other) * cs.y;
-                vh[j] = (_Float16)q;
-                vl[j] = (_Float16)(q - (float)vh[j]);
+                q[j] = y * cs.x + (c < 8 ? -other : other) * cs.y;
+                top = fmaxf(top, fabsf(q[j]));
+            }
+            top = dpp_max_step<0xb1>(top);
+            top = dpp_max_step<0x4e>(top);
+            top = dpp_max_step<0x141>(top);
+            top = dpp_max_step<0x140>(top);
+            const int qe = query_exponent(top);
+            const float qinv = kv8_power(-qe);
+            pf_half8 vh, vl;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                vh[j] = (_Float16)(q[j] * qinv);
+                vl[j] = (_Float16)(q[j] * qinv - (float)vh[j]);
             }
             q_hi[slot] = vh;
             q_lo[slot] = vl;
+            if (c == 0) q_pow[r] = kv8_power(qe);
         }
         __syncthreads();
         if (kPasses == 1 || wave / (kRows / TOK) == pass) {
             // this lane's dims 16s + 8h + j of its token
             const int r = (wave % (kRows / TOK)) * TOK + tl;
+            qscale = a.scale * q_pow[r];
 #pragma unroll
             for (int s = 0; s < 8; ++s) {
                 qb[s] = q_hi[r * 16 + ((2 * s + h) ^ (r & 15))];
@@ -1453,7 +1481,7 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
             for (int i = 0; i < 16; ++i) bmax = fmaxf(bmax, sc[kt][i]);
-        bmax = pair_combine(bmax, [](float u, float v) { return fmaxf(u, v); }) * a.scale;  // (scale > 0)
+        bmax = pair_combine(bmax, [](float u, float v) { return fmaxf(u, v); }) * qscale;  // (above 0)
         // Lazy rescaling: the reference point m_run moves (to kTopExponent
         // below the block's maximum) only when that maximum passes it by more
         // than kMaxExponent. Until then the numerators exp2(s - m_run) stay
@@ -1482,8 +1510,8 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
                 const int i = 8 * (u & 1) + j;
-                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u >> 1][i], a.scale, -m_run));
-                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u >> 1][i + 1], a.scale, -m_run));
+                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u >> 1][i], qscale, -m_run));
+                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[u >> 1][i + 1], qscale, -m_run));
                 sum += p0;
                 sum += p1;
                 const kv8_half2 hi = kv8_halfs(p0, p1);

@@ -124,6 +124,13 @@ __device__ __forceinline__ float wave_max(float v) {
 constexpr float kTopExponent = 8.0f;
 constexpr float kMaxExponent = 15.0f;
 
+// A query head is taken in two f16 pieces too, divided by 2^e, which leaves its largest magnitude `top`
+// just below 2: whatever the norm's weights are, no piece overflows and small heads keep their
+// bits. 2^e goes into the f32 scale of its scores (both products are exact).
+__device__ __forceinline__ int query_exponent(float top) {
+    return max(-100, min(100, (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127));
+}
+
 // Two values as f16, to nearest even (one instruction here). The pieces of a numerator are
 // rounded so: cut off toward zero they leave lower pieces that are all positive, and what of those
 // a large sum on the matrix cores cannot take (it rounds after every eight products) is lost to

@@ -610,8 +610,7 @@ __global__ __launch_bounds__(kThreads, 3) void kv8_attn_kernel(AttnArgs a, Membe
         issue(b0 + wave, kKv8PartBytes, vq, vs);
     }
 
-    // ---- query heads: norm and rope, scaled by a power of two to just below 2
-    // (whatever the norm's weights are, the pieces are in f16's range), in pieces
+    // ---- query heads: norm and rope, scaled by a power of two (query_exponent), in pieces
     const Rot64 rot = turn_sincos((double)pos * mb.rope[lane]);
     const double gain = mb.rope[kHeadDim / 2];
     const float rc = (float)(rot.c * gain), rs = (float)(rot.s * gain);
@@ -624,7 +623,7 @@ __global__ __launch_bounds__(kThreads, 3) void kv8_attn_kernel(AttnArgs a, Membe
             const float y0 = qx[i][0] * inv * qw0, y1 = qx[i][1] * inv * qw1;
             const float q0 = y0 * rc - y1 * rs, q1 = y0 * rs + y1 * rc;
             const float top = wave_max(fmaxf(fabsf(q0), fabsf(q1)));
-            const int e = max(-100, min(100, (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127));
+            const int e = query_exponent(top);
             const float p0 = q0 * kv8_power(-e), p1 = q1 * kv8_power(-e);
             qs[0][h][lane] = (_Float16)p0;
             qs[0][h][lane + 64] = (_Float16)p1;

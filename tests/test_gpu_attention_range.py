@@ -109,3 +109,50 @@ def test_chunk_after_a_sink(env, fmt, chunk, nats):
     worst = max(max_rel_err(got[t], attend(q[t], *(x[:position + t + 1] for x in rows))) for t in (0, tokens // 2, tokens - 1))
     print(f"err {worst:.2e}", flush=True)
     assert worst <= ATTN_TOL, worst
+
+
+# (q_heads, kv_heads, tokens, position): the narrow and the wide form of every group size
+QUERY_CHUNKS = [(2, 2, 40, 150), (4, 2, 37, 150), (8, 2, 37, 150), (16, 2, 20, 150),
+                (8, 8, 2200, 50), (16, 8, 1500, 50), (32, 8, 801, 50), (64, 8, 1101, 50)]
+
+
+@pytest.mark.parametrize("size", ["large", "small"])
+@pytest.mark.parametrize("chunk", QUERY_CHUNKS, ids=lambda c: "x".join(map(str, c)))
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_chunk_queries_of_any_size(env, fmt, chunk, size):
+    """Norm weights far from 1. Large ones (queries past f16's range): a softmax of one key. Small
+    ones, met by keys of thousands: scores as usual, of queries near f16's smallest values."""
+    case(test="chunk_q_size", fmt=fmt, chunk=chunk, size=size)
+    q_heads, kv_heads, tokens, position = chunk
+    cfg = config(env, q_heads, kv_heads)
+    rng = np.random.default_rng(tokens + q_heads)
+    cache = cache_of(env, cfg, position + tokens, fmt, None)
+    step = Step(rng, cfg, tokens)
+    key_size = 2.0 ** 13 if size == "small" else 1.0
+    step.qn *= np.float32(2.0 ** -15 if size == "small" else 1e5)
+    step.kn *= np.float32(key_size)
+    k, v = (rng.standard_normal((position, kv_heads, 128)).astype(np.float32) for _ in range(2))
+    cache.write(0, dev(k * np.float32(key_size)), dev(v), 0)
+    out = dev(np.full(tokens * q_heads * 128, np.nan, np.float32))
+    env["E"].attention_prefill(env["ctx"], cfg, cache, 0, *step.device(), tokens, position, out)
+    got = out.cpu().numpy().reshape(tokens, q_heads, 128)
+    assert np.isfinite(got).all()
+    q, _ = step.turned(position + np.arange(tokens), table(None))
+    keys, values = held(env, cache, cfg, position + tokens)
+    per, checked, seen = q_heads // kv_heads, 0, 0
+    for t in (0, tokens // 2, tokens - 1):
+        n = position + t + 1
+        want = attend(q[t], keys[:n], values[:n])
+        for h in range(q_heads):
+            seen += 1
+            if size == "large":
+                # scores of up to 2.5e6 are off by up to 2 (the derivation of ATTN_TOL, times 1e5): where the
+                # best key leads by 100, the others weigh nothing
+                s = (keys[:n, h // per] * dev(q[t, h])).sum(-1) / np.sqrt(128.0)
+                best = s.topk(2).values
+                if best[0] - best[1] < 100:
+                    continue
+            checked += 1
+            err = max_rel_err(got[t, h], want[h])
+            assert err <= ATTN_TOL, (t, h, err)
+    assert checked >= 0.9 * seen or checked >= seen - 1
