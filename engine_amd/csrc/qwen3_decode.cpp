@@ -739,7 +739,7 @@ ribn_amd_status copy_selected_async(ribn_amd_qwen3_decode* d, size_t member, uin
     return e == hipSuccess ? ok() : driver(e, "copy selected token into pinned memory");
 }
 
-ribn_amd_status check_kv_options(const ribn_amd_kv_options* o) {
+ribn_amd_status check_kv_options(const ribn_amd_kv_options* o, float rope_base) {
     if (o == nullptr) return RIBN_AMD_OK;
     if (o->format > RIBN_AMD_KV_I8) return fail(RIBN_AMD_INVALID_ARGUMENT, RIBN_AMD_KV_I8, o->format, "unknown cache format %u", o->format);
     if (o->rope == nullptr) return RIBN_AMD_OK;
@@ -748,6 +748,10 @@ ribn_amd_status check_kv_options(const ribn_amd_kv_options* o) {
     if (o->rope->layout != RIBN_AMD_ROPE_HALF || o->rope->rotary_dim != o->rope->head_dim || o->rope->head_dim != (uint32_t)ribn_amd::kHeadDim) {
         return fail(RIBN_AMD_INVALID_PLAN, ribn_amd::kHeadDim, o->rope->rotary_dim,
                     "a cache's rope has the half layout over whole heads of %d", ribn_amd::kHeadDim);
+    }
+    // calls go by the config's base: a table of another one would turn q and k by angles nobody asked for
+    if (o->rope->base != rope_base) {
+        return fail(RIBN_AMD_INVALID_PLAN, 0, 0, "the cache's rope has base %g, its config %g", (double)o->rope->base, (double)rope_base);
     }
     return RIBN_AMD_OK;
 }
@@ -770,7 +774,7 @@ ribn_amd_status ribn_amd_kv_cache_create_with(ribn_amd_context* ctx, const ribn_
                                               ribn_amd_kv_cache** out) {
     if (!ctx || !out) return fail(RIBN_AMD_INVALID_ARGUMENT, 0, 0, "null argument");
     ribn_amd_status st = check_config(config);
-    if (st == RIBN_AMD_OK) st = ribn_amd_decode::check_kv_options(options);
+    if (st == RIBN_AMD_OK) st = ribn_amd_decode::check_kv_options(options, config->rope_base);
     if (st != RIBN_AMD_OK) return st;
     if (capacity == 0 || capacity > (1u << 20)) {
         return fail(RIBN_AMD_INVALID_PLAN, 1u << 20, capacity, "KV capacity must be 1..%u tokens", 1u << 20);

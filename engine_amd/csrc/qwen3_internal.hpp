@@ -24,8 +24,8 @@ ribn_amd_status enqueue_prefill_chunk(ribn_amd_qwen3_decode* d, ribn_amd_kv_cach
 // of `member` into pinned host memory, stream-ordered.
 ribn_amd_status copy_selected_async(ribn_amd_qwen3_decode* d, size_t member, uint32_t* pinned);
 
-// The format and rope of a cache's options (null: the default).
-ribn_amd_status check_kv_options(const ribn_amd_kv_options* options);
+// The format and rope of a cache's options (null: the default) for a model with this rope base.
+ribn_amd_status check_kv_options(const ribn_amd_kv_options* options, float rope_base);
 
 ribn_amd_context* context(const ribn_amd_qwen3_decode* d);
 uint32_t max_members(const ribn_amd_qwen3_decode* d);

@@ -648,7 +648,7 @@ ribn_amd_status ribn_amd_serving_set_grouped_decode(ribn_amd_serving* s, int32_t
 ribn_amd_status ribn_amd_serving_set_kv_options(ribn_amd_serving* s, const ribn_amd_kv_options* options) {
     if (!s) return fail(RIBN_AMD_INVALID_ARGUMENT, 0, 0, "null dispatcher");
     ribn_amd_status st = check_health(s);
-    if (st == RIBN_AMD_OK) st = ribn_amd_decode::check_kv_options(options);
+    if (st == RIBN_AMD_OK) st = ribn_amd_decode::check_kv_options(options, s->cfg.rope_base);
     if (st != RIBN_AMD_OK) return st;
     if (!s->states.empty()) {
         return fail(RIBN_AMD_EXECUTION_FAILED, 0, s->states.size(), "%zu states are materialized with the caches' present format",

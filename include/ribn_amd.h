@@ -641,7 +641,8 @@ ribn_amd_status ribn_amd_rope_execute(ribn_amd_rope *rope, const int32_t *positi
 typedef struct ribn_amd_kv_options {
     uint32_t format;                /* RIBN_AMD_KV_F16 or RIBN_AMD_KV_I8 */
     const ribn_amd_rope_spec *rope; /* how q and k of this cache are rotated; NULL: half layout, unscaled, the config's
-                                       rope_base. Half layout over the whole head (128) only. Copied. */
+                                       rope_base. Half layout over the whole head (128) and the config's rope_base
+                                       only (InvalidPlan). Copied. */
 } ribn_amd_kv_options;
 
 /* ribn_amd_kv_cache_create with a format and a rope of the cache's own (keys are

@@ -725,3 +725,23 @@ def test_refusals(env):
     assert name(lib.ribn_amd_kv_cache_write(ctx.handle, i8.handle, 0, 0, 3, ctypes.c_void_p(k.data_ptr() + 2), kp, 768, 0)) == "InvalidArgument"
     host = np.zeros(768, np.float32)
     assert name(lib.ribn_amd_kv_cache_write(ctx.handle, i8.handle, 0, 0, 3, host.ctypes.data_as(ctypes.c_void_p), kp, 768, 0)) == "InvalidArgument"
+
+
+@pytest.mark.parametrize("fmt", ["KV_I8", "KV_F16"])
+def test_a_rope_of_another_base_is_refused(env, fmt):
+    """The base of a cache's rope is its config's: a spec whose base was left at the default, on a
+    model with another one, would turn by angles that no call asks for."""
+    case(test="rope_base", fmt=fmt)
+    E, ctx = env["E"], env["ctx"]
+    cfg = E.AmdQwen3Config(**{**config(env, 4, 2).__dict__, "rope_base": 5.0e5})
+    for given in (cfg, E.AmdQwen3Config(**{**cfg.__dict__, "rope": E.AmdRopeSpec(**YARN)})):
+        with pytest.raises(E.AmdModelKernelError) as e:
+            E.AmdKvCache(ctx, given, 64, format=getattr(E, fmt), rope=None if given.rope else E.AmdRopeSpec(**YARN))
+        assert e.value.kind == "InvalidPlan" and "base 1e+06" in str(e.value) and "500000" in str(e.value), str(e.value)
+    cache = E.AmdKvCache(ctx, cfg, 64, format=getattr(E, fmt), rope=E.AmdRopeSpec(base=5.0e5, **YARN))
+    step = Step(np.random.default_rng(3), cfg, 1)
+    out = dev(np.full(4 * 128, np.nan, np.float32))
+    E.attention_decode(ctx, cfg, [cache], 0, *step.device(), dev(np.zeros(1, np.int32)), out)
+    env["torch"].cuda.synchronize()
+    # one key: its value
+    assert max_rel_err(out.cpu().numpy().reshape(4, 128), L.half(step.v[0]).astype(np.float64).repeat(2, 0)) <= ATTN_TOL

@@ -312,5 +312,20 @@ def test_a_config_with_a_rope_reaches_the_dispatchers_caches(env):
     np.testing.assert_array_equal(dec.copy_logits(0), logits)
 
 
+def test_the_dispatcher_refuses_a_rope_of_another_base(env):
+    case(test="dispatcher_base")
+    E = env["E"]
+    dec = env["decoder"](model(env)[0])
+    disp = S.AmdServingDispatcher(dec, 2)
+    with pytest.raises(S.BackendError) as e:
+        disp.with_kv_format(E.KV_I8, E.AmdRopeSpec(base=5.0e5, **YARN))
+    assert "base 500000" in str(e.value), str(e.value)
+    toks = prompt(40, 3)  # the caches are as they were: f16, unscaled
+    seg = S.ExecutionSegment(request=1, phase=S.Phase.PREFILL, state_position=0, token_count=40, tokens=tuple(toks),
+                             sampling=S.SamplingParams.greedy())
+    disp.dispatch(None, seg, None, _state(1))
+    assert disp.state_bytes() == (S.kv_bytes(dec.config, CAP, E.KV_F16), 0)
+
+
 def _state(i):
     return S.InferenceStateSet(state_id=i, kv_tokens=CAP, token_position=None)
