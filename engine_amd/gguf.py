@@ -216,19 +216,28 @@ def _rope_factors(file: GgufFile, pairs: int):
 
 def rope_from_gguf(file: GgufFile, head_dim: int, base: float):
     """The scaled rope that a file's "qwen3.rope.scaling.*" metadata and "rope_freqs.weight"
-    tensor ask for, None if they ask for none. Types other than linear and yarn, and
-    scaling keys not known here, are refused: run without them such a model answers wrongly."""
+    tensor ask for, None if they ask for none. A factor without a type is a linear one, as
+    "qwen3.rope.scale_linear", its older name, says; beside type none it counts for nothing.
+    Types other than linear and yarn, and scaling keys not known here, are refused: run
+    without them such a model answers wrongly."""
     from .rope import AmdRopeSpec
 
     prefix = "qwen3.rope.scaling."
     factors = _rope_factors(file, head_dim // 2)
+    unscaled = None if factors is None else AmdRopeSpec(head_dim=head_dim, base=base, freq_factors=factors)
     kind = file.metadata(prefix + "type")
-    if kind is None or kind == "none":
-        return None if factors is None else AmdRopeSpec(head_dim=head_dim, base=base, freq_factors=factors)
+    if kind == "none":
+        return unscaled
     unknown = [k for k in file.metadata_keys() if k.startswith(prefix) and k[len(prefix):] not in _ROPE_SCALING_KEYS]
-    if kind not in ("linear", "yarn") or unknown:
+    if kind not in (None, "linear", "yarn") or unknown:
         raise GgufError(36, 0, 0, f"UnsupportedRopeScaling: {kind} {unknown}")
     factor = file.metadata(prefix + "factor")
+    if factor is None:
+        factor = file.metadata("qwen3.rope.scale_linear")
+    if kind is None:
+        if factor is None or float(factor) in (0.0, 1.0):  # (0: not set)
+            return unscaled
+        kind = "linear"
     if factor is None:
         raise GgufError(35, 0, 0, f"MissingMetadata: {prefix}factor")
     original = _required_u32(file, prefix + "original_context_length") if kind == "yarn" else 0

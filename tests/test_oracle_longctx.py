@@ -193,3 +193,30 @@ def test_gguf_rope_betas_and_factors(tmp_path):
     assert gain == 1.0
     with pytest.raises(GgufError):
         E.qwen3_config_from_gguf(gguf_file(tmp_path, [], [("rope_freqs.weight", [32], 0, W.f32_payload(factors[:32]))]))
+
+
+def test_gguf_rope_factor_without_a_type(tmp_path):
+    """A factor without a type is a linear one, under its older name too; keys that are not known are
+    refused whether a type is there or not, and type none leaves the rope unscaled whatever stands beside it."""
+    key = "qwen3.rope.scaling."
+    factor, old = (key + "factor", W.F32, 4.0), ("qwen3.rope.scale_linear", W.F32, 2.0)
+    linear = lambda f, **kw: E.AmdRopeSpec(scaling="linear", factor=f, **kw)  # noqa: E731
+    rope = lambda extra, tensors=(): E.qwen3_config_from_gguf(gguf_file(tmp_path, extra, tensors)).rope  # noqa: E731
+    assert rope([factor]) == linear(4.0)
+    assert rope([old]) == linear(2.0)
+    assert rope([factor, old]) == linear(4.0)
+    assert rope([factor, (key + "original_context_length", W.U32, 32768), (key + "finetuned", W.BOOL, True)]) == linear(4.0)
+    assert rope([(key + "type", W.STRING, "linear"), old]) == linear(2.0)
+    assert rope([(key + "type", W.STRING, "yarn"), old, (key + "original_context_length", W.U32, 32768)]) == \
+        E.AmdRopeSpec(scaling="yarn", factor=2.0, original_context=32768)
+    none = (key + "type", W.STRING, "none")
+    for extra in ([(key + "factor", W.F32, 1.0)], [(key + "factor", W.F32, 0.0)], [(key + "original_context_length", W.U32, 32768)],
+                  [none, factor, old, (key + "attn_factor", W.F32, 2.0)]):
+        assert rope(extra) is None, extra
+    factors = tuple(float(1 + i % 8) for i in range(64))
+    assert rope([factor], [("rope_freqs.weight", [64], 0, W.f32_payload(factors))]) == linear(4.0, freq_factors=factors)
+    for extra in ([(key + "attn_factor", W.F32, 2.0)], [factor, (key + "attn_factor", W.F32, 2.0)],
+                  [factor, (key + "original_context_length", W.U32, 32768), (key + "yarn_ext_factor", W.F32, 1.0)]):
+        with pytest.raises(GgufError) as e:
+            rope(extra)
+        assert e.value.kind == "MetadataTypeMismatch"
