@@ -100,13 +100,13 @@ class AmdKvCache:
         dtype = _dtype(keys)
         if dtype not in (0, 2) or values.dtype != keys.dtype:
             raise TypeError(f"cache rows are float32 or float16, got {keys.dtype} and {values.dtype}")
-        if keys.shape != values.shape or not keys.is_contiguous() or not values.is_contiguous():
+        shape = keys.shape
+        if shape != values.shape or not keys.is_contiguous() or not values.is_contiguous():
             raise ValueError("keys and values must be contiguous and of one shape")
-        row = self.config.kv_heads * self.config.head_dim
-        if keys.numel() % row:
-            raise ValueError(f"cache rows have {row} values, got {keys.numel()}")
-        _check(call(self.ctx.handle, self.handle, layer, position, keys.numel() // row, keys.data_ptr(), values.data_ptr(),
-                    keys.numel(), dtype), AmdModelKernelError)
+        if len(shape) != 3 or shape[1] != self.config.kv_heads or shape[2] != self.config.head_dim:
+            raise ValueError(f"cache rows are [tokens][{self.config.kv_heads}][{self.config.head_dim}], got {tuple(shape)}")
+        _check(call(self.ctx.handle, self.handle, layer, position, shape[0], keys.data_ptr(), values.data_ptr(), keys.numel(),
+                    dtype), AmdModelKernelError)
 
     def capacity(self) -> int:
         return int(self.ctx._lib.ribn_amd_kv_cache_capacity(self.handle))

@@ -745,3 +745,22 @@ def test_a_rope_of_another_base_is_refused(env, fmt):
     env["torch"].cuda.synchronize()
     # one key: its value
     assert max_rel_err(out.cpu().numpy().reshape(4, 128), L.half(step.v[0]).astype(np.float64).repeat(2, 0)) <= ATTN_TOL
+
+
+@pytest.mark.parametrize("fmt", ["KV_I8", "KV_F16"])
+def test_rows_of_another_shape_are_refused(env, fmt):
+    """[kv_heads][tokens][128], an f16 cache's own layout, has as many values: it is no [tokens][kv_heads][128]."""
+    case(test="row_shapes", fmt=fmt)
+    E, torch = env["E"], env["torch"]
+    cfg = config(env, 4, 2)
+    cache = E.AmdKvCache(env["ctx"], cfg, 64, format=getattr(E, fmt))
+    for shape in ((2, 6, 128), (6, 256), (6 * 256,), (1, 6, 2, 128), (12, 1, 128), (6, 4, 64)):
+        x = torch.ones(shape, device="cuda:0")
+        for call in (lambda: cache.write(0, x, x, 0), lambda: cache.read(0, 0, x, x)):
+            with pytest.raises(ValueError, match="cache rows are"):
+                call()
+    x = torch.ones((6, 2, 128), device="cuda:0")
+    cache.write(0, x, x, 0)
+    y = [torch.zeros_like(x) for _ in range(2)]
+    cache.read(0, 0, *y)
+    assert all(torch.equal(v, x) for v in y)
