@@ -15,7 +15,10 @@ namespace ribn_amd {
 
 namespace {
 
-constexpr uint32_t kOOR = 0xffffff00u;  // buffer offset past any region: loads return 0
+// Buffer offset past any head's codes (2^28 bytes with the largest capacity), and still past them with
+// a block's piece added: loads return 0 and fetch nothing.
+constexpr uint32_t kOOR = 0x80000000u;
+static_assert((uint64_t)kOOR >= ((uint64_t)1 << 20) / kKv8Block * kKv8BlockBytes && (uint64_t)kOOR + kKv8BlockBytes <= UINT32_MAX);
 constexpr int kRowHalfs = kHeadDim + 8;  // LDS row of a staged token (272 B: 16-byte reads of 8 rows fall in distinct banks)
 
 // ------------------------------------------------------------------- append
