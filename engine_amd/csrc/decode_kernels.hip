@@ -695,9 +695,9 @@ __device__ __forceinline__ float4 nonfinite_values(uint2 w) {
 // that is not whole (keys from the sequence's last multiple of 32 on) comes from the tail, with
 // the same lanes and no prefetch: it is one half pair of a launch. Blocks past it read
 // as zeros. The matrix cores bound long chunks as they do over f16 caches, and half the
-// bytes buy little: 2,047 tokens from 0 (32 / 8 heads) take 90 us for 93, 1,999 after 6,203
-// 438 for 439 (each product counted twice, for the two pieces of q and p: 1,080 TFLOP/s);
-// 37 tokens after 2,011, where the keys' split counts, 24 for 55.
+// bytes buy little: 2,047 tokens from 0 (32 / 8 heads) take 91 us for 96, 1,999 after 6,203
+// 447 for 446 (each product counted twice, for the two pieces of q and p: 1,060 TFLOP/s);
+// 37 tokens after 2,011, where the keys' split counts, 26 for 55.
 struct PrefillI8 {
     __amdgpu_buffer_rsrc_t cr, sr;
     const _Float16* tail_k;
@@ -1694,7 +1694,7 @@ bool wide_prefill(const PrefillAttnArgs& a, int tiles, int cu_count) {
 // room and the merge's 32 slots allow: in microseconds, a key round takes 1.75 with
 // few workgroups on the card, 2.4 with one a CU and 3.2 with two; the merge takes 4 and
 // the partials their way out and back at 3 TB/s. Whole calls, 32 / 8 heads, unsplit and by this rule:
-// 37 tokens after 2,011 73 and 24 us; 512 after 4,000 about 160 and 117; 512 from
+// 37 tokens after 2,011 73 and 26 us; 512 after 4,000 about 160 and 117; 512 from
 // position 0 stay unsplit (two shares: 47 for 28).
 int prefill_splits(const PrefillAttnArgs& a, int groups, int cu_count) {
     const size_t rows = (size_t)a.tokens * a.q_heads;
