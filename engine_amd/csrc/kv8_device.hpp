@@ -120,7 +120,7 @@ __device__ __forceinline__ float wave_max(float v) {
 // far above 131,072 others took 3e-3 off the output. So the reference m is set
 // kTopExponent below the largest score (N keys then lose at most N 2^-33 of it), and moves
 // when a score passes it by kMaxExponent, the pieces being still in f16's range. The room between the
-// two keeps moves rare: 1,999 tokens after 6,203 take 435 us with 15 (m at the top), 443 with 7, 448 with 3.
+// two keeps moves rare: 1,999 tokens after 6,203 take 437 us with 15 (m at the top), 443 with 7, 448 with 3.
 constexpr float kTopExponent = 8.0f;
 constexpr float kMaxExponent = 15.0f;
 
