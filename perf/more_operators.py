@@ -9,10 +9,10 @@
 
 A cache keeps blocks of 32 tokens. x16 are the values rounded to f16. A group is
 32 tokens of one key channel, or 64 dims of one token's value; with lo and hi its
-smallest and largest x16, s = f16((hi - lo) / 15) (the difference and its product
-with 1/15 in f32), a code is (x16 - lo) * (1 / s) in f32, rounded to the nearest
-whole number (ties to even) and clamped to 0 .. 15 (0 where s is 0), and it stands
-for code * s + lo, rounded to f16. A block that is not whole is kept in f16, keys
+smallest and largest x16, s = (hi - lo) / 15 (the difference and its product with
+1/15 in f32) cut off to f16, so that no value leaves lo .. hi; a code is (x16 - lo)
+* (1 / s) in f32, rounded to the nearest whole number (ties to even) and clamped to
+0 .. 15 (0 where s is 0), and it stands for code * s + lo, rounded to f16. A block that is not whole is kept in f16, keys
 [token][dim] and values [dim][token]. Attention sees the cache as it is after the
 call's own tokens are in it. Keys are normalised and rotated in 64 bits and
 rounded to f32, then to f16.
@@ -302,7 +302,9 @@ def _quantise(x, part):
     """Codes, scales and lows of whole blocks [..., 32, 128] of f16 keys (part 0) or values (1)."""
     grouped, axis = _groups(x, part)
     low, high = grouped.amin(axis, keepdim=True), grouped.amax(axis, keepdim=True)
-    scale = ((high.float() - low.float()) * (1.0 / 15.0)).half()
+    wide = (high.float() - low.float()) * (1.0 / 15.0)
+    scale = wide.half()
+    scale = torch.where(scale.float() > wide, (scale.view(torch.int16) - 1).view(torch.float16), scale)
     inverse = torch.where(scale > 0, 1.0 / scale.float(), 0.0)
     codes = ((grouped.float() - low.float()) * inverse).round().clamp(0, 15).to(torch.uint8)
     return codes.reshape(x.shape), scale, low
@@ -501,7 +503,9 @@ def _stored(x, keys):
         return x
     ordered = rows.sort(-1)[0]
     low, spread = ordered[:, :1], (ordered[:, -1:] - ordered[:, :1]).float().double()
-    scale = (spread * np.float64(np.float32(1 / 15))).float().half().double()
+    scale = (spread * np.float64(np.float32(1 / 15))).float().double()
+    unit = torch.clamp(2.0 ** (torch.frexp(scale)[1].double() - 11.0), min=2.0 ** -24)  # a step of f16 there
+    scale = torch.floor(scale / unit) * unit
     per = torch.where(scale == 0, 0.0, (1 / scale.clamp(min=2.0 ** -24)).float().double())
     codes = torch.round(((rows - low).float().double() * per).float().double())
     held = (torch.clamp(codes, max=15) * scale + low).float().half().double().reshape(x.shape)
