@@ -37,12 +37,14 @@
 // model_ops.rs:201-258) with the same ordering key, tie rule and NaN rule.
 #include "decode_launch.hpp"
 #include "kquant_device.hpp"
+#include "kv4_device.hpp"
 #include "kv8_device.hpp"
 #include "rope_device.hpp"
 
 #include <float.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace ribn_amd {
 
@@ -689,27 +691,25 @@ __device__ __forceinline__ float4 nonfinite_values(uint2 w) {
                        by & 0x8000u ? half_bits_to_float(w.y & 0xffffu) : 0.f, by >> 31 ? half_bits_to_float(w.y >> 16) : 0.f);
 }
 
-// A block pair (64 keys) of an 8-bit cache as the prompt kernels stage it: 512
-// 16-byte pieces of keys and as many of values, in the order of their codes
-// (kv8.hpp), dequantised exactly into the f16 the LDS tiles hold. The block
+// A block pair (64 keys) of an 8-bit or 4-bit cache as the prompt kernels stage it: 512
+// pieces of 16 key dims and as many of eight keys of two value dims, in the order of their codes
+// (kv8.hpp, kv4.hpp), dequantised exactly into the f16 the LDS tiles hold. The block
 // that is not whole (keys from the sequence's last multiple of 32 on) comes from the tail, with
 // the same lanes and no prefetch: it is one half pair of a launch. Blocks past it read
 // as zeros. The matrix cores bound long chunks as they do over f16 caches, and half the
 // bytes buy little: 2,047 tokens from 0 (32 / 8 heads) take 91 us for 96, 1,999 after 6,203
 // 447 for 446 (each product counted twice, for the two pieces of q and p: 1,060 TFLOP/s);
 // 37 tokens after 2,011, where the keys' split counts, 26 for 55.
-struct PrefillI8 {
-    __amdgpu_buffer_rsrc_t cr, sr;
+struct PrefillBlocks {
+    __amdgpu_buffer_rsrc_t cr;
     const _Float16* tail_k;
     const _Float16* tail_v;
     int whole;     // whole blocks
     int tail_blk;  // the block in the tail, or one no launch reaches
 
-    __device__ __forceinline__ PrefillI8(const PrefillAttnArgs& a, int kvh) {
-        const Kv8Head h = kv8_head(a.mem, a.layer, kvh);
+    __device__ __forceinline__ PrefillBlocks(const PrefillAttnArgs& a, const KvHead& h, size_t code_bytes) {
         const int end = a.p0 + a.tokens;
-        cr = make_rsrc(h.codes, (uint32_t)kv8_tail_offset(a.mem.capacity));
-        sr = make_rsrc(h.scales, (uint32_t)(kv8_blocks(a.mem.capacity) * sizeof(float2)));
+        cr = make_rsrc(h.codes, (uint32_t)code_bytes);
         tail_k = h.tail_k;
         tail_v = h.tail_v;
         whole = end / kKv8Block;
@@ -717,38 +717,98 @@ struct PrefillI8 {
     }
     // (256 pieces a block: a wave's are all of one)
     __device__ __forceinline__ int block_of(int kb, int idx) const { return 2 * kb + __builtin_amdgcn_readfirstlane(idx >> 8); }
-    __device__ __forceinline__ uint4 codes(int kb, int idx, int part) const {
-        const int b = block_of(kb, idx);
-        return load_b128(cr, b < whole ? (uint32_t)b * kKv8BlockBytes + (uint32_t)part + 16u * (uint32_t)(idx & 255) : kOOR);
-    }
-    __device__ __forceinline__ float scale(int kb, int idx, int part) const {
-        const int b = block_of(kb, idx);
-        return __builtin_bit_cast(float, load_b32(sr, b < whole ? 8u * (uint32_t)b + (uint32_t)part : kOOR));
-    }
     // keys: the piece's key within the pair, and its first 8-dim slot
     __device__ __forceinline__ int key_of(int idx) const { return 32 * (idx >> 8) + kv8_key_row((idx >> 7) & 1, idx & 15); }
     __device__ __forceinline__ int piece_of(int idx) const { return 8 * ((idx >> 6) & 1) + 2 * ((idx >> 4) & 3); }
     // values: the piece's first dim (of two) and first key (of eight) within the pair
     __device__ __forceinline__ int dim_of(int idx) const { return 32 * ((idx >> 6) & 3) + 2 * (idx & 15); }
     __device__ __forceinline__ int keys_of(int idx) const { return 32 * (idx >> 8) + 8 * ((idx >> 4) & 3); }
-    __device__ __forceinline__ void keys(int kb, int idx, uint4 w, float scale, kv8_half8 (&x)[2]) const {
-        x[0] = kv8_values(w.x, w.y, (_Float16)scale);
-        x[1] = kv8_values(w.z, w.w, (_Float16)scale);
+    // The tail's rows in place of block kb's, if it is the tail's.
+    __device__ __forceinline__ void tail_keys(int kb, int idx, kv8_half8 (&x)[2]) const {
         if (block_of(kb, idx) == tail_blk) {
             const kv8_half8* p = reinterpret_cast<const kv8_half8*>(tail_k + (key_of(idx) & 31) * kHeadDim) + piece_of(idx);
             x[0] = p[0];
             x[1] = p[1];
         }
     }
-    __device__ __forceinline__ void values(int kb, int idx, uint4 w, float scale, kv8_half8 (&x)[2]) const {
-        x[0] = kv8_values(w.x, w.y, (_Float16)scale);
-        x[1] = kv8_values(w.z, w.w, (_Float16)scale);
+    __device__ __forceinline__ void tail_values(int kb, int idx, kv8_half8 (&x)[2]) const {
         if (block_of(kb, idx) == tail_blk) {
             const _Float16* p = tail_v + dim_of(idx) * kKv8Block + (keys_of(idx) & 31);
             x[0] = *reinterpret_cast<const kv8_half8*>(p);
             x[1] = *reinterpret_cast<const kv8_half8*>(p + kKv8Block);
         }
     }
+};
+
+struct PrefillI8 : PrefillBlocks {
+    struct Piece {
+        uint4 w;
+        float scale;
+    };
+    __amdgpu_buffer_rsrc_t sr;
+
+    __device__ __forceinline__ PrefillI8(const PrefillAttnArgs& a, int kvh) : PrefillI8(a, kv8_head(a.mem, a.layer, kvh)) {}
+    __device__ __forceinline__ PrefillI8(const PrefillAttnArgs& a, const KvHead& h) : PrefillBlocks(a, h, kv8_tail_offset(a.mem.capacity)) {
+        sr = make_rsrc(h.scales, (uint32_t)(kv8_blocks(a.mem.capacity) * sizeof(float2)));
+    }
+    __device__ __forceinline__ Piece load(int kb, int idx, int part) const {
+        const int b = block_of(kb, idx);
+        return Piece{load_b128(cr, b < whole ? (uint32_t)b * kKv8BlockBytes + (uint32_t)(part * kKv8PartBytes) + 16u * (uint32_t)(idx & 255) : kOOR),
+                     __builtin_bit_cast(float, load_b32(sr, b < whole ? 8u * (uint32_t)b + 4u * (uint32_t)part : kOOR))};
+    }
+    __device__ __forceinline__ Piece load_keys(int kb, int idx) const { return load(kb, idx, 0); }
+    __device__ __forceinline__ Piece load_values(int kb, int idx) const { return load(kb, idx, 1); }
+    __device__ __forceinline__ void keys(int kb, int idx, const Piece& p, kv8_half8 (&x)[2]) const {
+        x[0] = kv8_values(p.w.x, p.w.y, (_Float16)p.scale);
+        x[1] = kv8_values(p.w.z, p.w.w, (_Float16)p.scale);
+        tail_keys(kb, idx, x);
+    }
+    __device__ __forceinline__ void values(int kb, int idx, const Piece& p, kv8_half8 (&x)[2]) const {
+        x[0] = kv8_values(p.w.x, p.w.y, (_Float16)p.scale);
+        x[1] = kv8_values(p.w.z, p.w.w, (_Float16)p.scale);
+        tail_values(kb, idx, x);
+    }
+};
+
+struct PrefillI4 : PrefillBlocks {
+    typedef uint2 Piece;
+
+    __device__ __forceinline__ PrefillI4(const PrefillAttnArgs& a, int kvh) : PrefillBlocks(a, kv4_head(a.mem, a.layer, kvh), kv4_tail_offset(a.mem.capacity)) {}
+    __device__ __forceinline__ uint32_t base_of(int kb, int idx) const {
+        const int b = block_of(kb, idx);
+        return b < whole ? (uint32_t)b * kKv4BlockBytes : kOOR4;
+    }
+    // offset of a piece's eight bytes in its part
+    __device__ __forceinline__ uint32_t code_of(int idx) const { return 1024u * (uint32_t)((idx >> 7) & 1) + 16u * (uint32_t)(idx & 63) + 8u * (uint32_t)((idx >> 6) & 1); }
+    __device__ __forceinline__ kv4_u4 params(uint32_t at) const { return __builtin_bit_cast(kv4_u4, load_b128(cr, at)); }
+    __device__ __forceinline__ Piece load_keys(int kb, int idx) const {
+        return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(cr, (int)(base_of(kb, idx) + code_of(idx)), 0, 0));
+    }
+    __device__ __forceinline__ Piece load_values(int kb, int idx) const {
+        return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(cr, (int)(base_of(kb, idx) + kKv4Values + code_of(idx)), 0, 0));
+    }
+    __device__ __forceinline__ void keys(int kb, int idx, const Piece& p, kv8_half8 (&x)[2]) const {
+        const uint32_t at = base_of(kb, idx) + kKv4KeyParams + 16u * (uint32_t)piece_of(idx);
+        x[0] = kv4_values(p.x, params(at), params(at + 2u * kHeadDim));
+        x[1] = kv4_values(p.y, params(at + 16u), params(at + 2u * kHeadDim + 16u));
+        tail_keys(kb, idx, x);
+    }
+    __device__ __forceinline__ void values(int kb, int idx, const Piece& p, kv8_half8 (&x)[2]) const {
+        const uint32_t at = base_of(kb, idx) + kKv4ValueParams + (uint32_t)kKv4ValueHalf * (uint32_t)((idx >> 7) & 1) + 2u * (uint32_t)(keys_of(idx) & 31);
+        const kv4_u4 scale = params(at), low = params(at + 2u * kKv8Block);
+        x[0] = kv4_values(p.x, scale, low);
+        x[1] = kv4_values(p.y, scale, low);
+        tail_values(kb, idx, x);
+    }
+    // (offsets within a block are added to it)
+    static constexpr uint32_t kOOR4 = 0x80000000u;
+};
+
+// How a cache's keys and values come to a prompt kernel: a piece of a cache of blocks, or 16 bytes of f16.
+template <int CACHE> struct PrefillCache {
+    static constexpr bool kBlocks = CACHE == kCacheI8 || CACHE == kCacheI4;
+    using Blocks = std::conditional_t<CACHE == kCacheI4, PrefillI4, PrefillI8>;
+    using Piece = std::conditional_t<kBlocks, typename Blocks::Piece, uint4>;
 };
 
 template <int QPK, int CACHE>
@@ -788,78 +848,76 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
     const bool v_unit = tid < 256;
     const int va = tid & 15;        // V unit: keys 4va .. 4va + 3
     const int vc = (tid >> 4) & 15; // dims 8vc .. 8vc + 7
-    uint4 kp[KP], vp[4];
-    const PrefillI8 c8(a, kvh);
-    constexpr int P8 = 512 / NT;  // 16-byte pieces of an 8-bit block pair's keys (values) per thread
-    float kscale[P8], vscale[P8];
+    using Cache = PrefillCache<CACHE>;
+    constexpr int P8 = 512 / NT;  // pieces of a block pair's keys (values) per thread
+    typename Cache::Piece kp[Cache::kBlocks ? P8 : KP], vp[Cache::kBlocks ? P8 : 4];
+    const typename Cache::Blocks blocks_of(a, kvh);
     auto issue = [&](int kb) {
-        if constexpr (CACHE == kCacheI8) {
+        if constexpr (Cache::kBlocks) {
 #pragma unroll
             for (int r = 0; r < P8; ++r) {
-                kp[r] = c8.codes(kb, tid + NT * r, 0);
-                vp[r] = c8.codes(kb, tid + NT * r, kKv8PartBytes);
-                kscale[r] = c8.scale(kb, tid + NT * r, 0);
-                vscale[r] = c8.scale(kb, tid + NT * r, 4);
+                kp[r] = blocks_of.load_keys(kb, tid + NT * r);
+                vp[r] = blocks_of.load_values(kb, tid + NT * r);
             }
-            return;
-        }
+        } else {
 #pragma unroll
-        for (int r = 0; r < KP; ++r) {
-            const int idx = tid + NT * r;
-            kp[r] = load_b128(kr, ((uint32_t)(kb * kPfKeys + (idx >> 4)) * kHeadDim + 8u * (uint32_t)(idx & 15)) * 2u);
-        }
+            for (int r = 0; r < KP; ++r) {
+                const int idx = tid + NT * r;
+                kp[r] = load_b128(kr, ((uint32_t)(kb * kPfKeys + (idx >> 4)) * kHeadDim + 8u * (uint32_t)(idx & 15)) * 2u);
+            }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint32_t off = ((uint32_t)(kb * kPfKeys + 4 * va + r) * kHeadDim + 8u * (uint32_t)vc) * 2u;
-            vp[r] = load_b128(vr, v_unit ? off : kOOR);
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t off = ((uint32_t)(kb * kPfKeys + 4 * va + r) * kHeadDim + 8u * (uint32_t)vc) * 2u;
+                vp[r] = load_b128(vr, v_unit ? off : kOOR);
+            }
         }
     };
     const int wg_first = a.p0 + (int)blockIdx.x * TT * kPrefillTileTokens;  // a token's first position
     if (tid == 0) v_dropped = 0;
     auto stage = [&](int buf, int kb) {
-        if constexpr (CACHE == kCacheI8) {
+        if constexpr (Cache::kBlocks) {
 #pragma unroll
             for (int r = 0; r < P8; ++r) {
                 const int idx = tid + NT * r;
                 kv8_half8 x[2];
-                c8.keys(kb, idx, kp[r], kscale[r], x);
-                const int key = c8.key_of(idx), piece = c8.piece_of(idx);
+                blocks_of.keys(kb, idx, kp[r], x);
+                const int key = blocks_of.key_of(idx), piece = blocks_of.piece_of(idx);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) *reinterpret_cast<kv8_half8*>(&ks[buf][key][8 * ((piece + i) ^ (key & 15))]) = x[i];
-                c8.values(kb, idx, vp[r], vscale[r], x);
+                blocks_of.values(kb, idx, vp[r], x);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const uint4 w = __builtin_bit_cast(uint4, x[i]);
-                    uint2* row = reinterpret_cast<uint2*>(&vt[buf][c8.dim_of(idx) + i][c8.keys_of(idx)]);
+                    uint2* row = reinterpret_cast<uint2*>(&vt[buf][blocks_of.dim_of(idx) + i][blocks_of.keys_of(idx)]);
                     row[0] = make_uint2(w.x, w.y);
                     row[1] = make_uint2(w.z, w.w);
                 }
             }
-            return;
-        }
-        if (kb * kPfKeys + kPfKeys - 1 > wg_first && drop_nonfinite(vp)) v_dropped = 1;
+        } else {
+            if (kb * kPfKeys + kPfKeys - 1 > wg_first && drop_nonfinite(vp)) v_dropped = 1;
 #pragma unroll
-        for (int r = 0; r < KP; ++r) {
-            const int idx = tid + NT * r;
-            *reinterpret_cast<uint4*>(&ks[buf][idx >> 4][8 * ((idx & 15) ^ ((idx >> 4) & 15))]) = kp[r];
-        }
-        if (v_unit) {
-            // row j of the unit: dim 8vc + j of keys 4va .. 4va + 3
-            const uint32_t w[4][4] = {{vp[0].x, vp[0].y, vp[0].z, vp[0].w}, {vp[1].x, vp[1].y, vp[1].z, vp[1].w},
-                                      {vp[2].x, vp[2].y, vp[2].z, vp[2].w}, {vp[3].x, vp[3].y, vp[3].z, vp[3].w}};
+            for (int r = 0; r < KP; ++r) {
+                const int idx = tid + NT * r;
+                *reinterpret_cast<uint4*>(&ks[buf][idx >> 4][8 * ((idx & 15) ^ ((idx >> 4) & 15))]) = kp[r];
+            }
+            if (v_unit) {
+                // row j of the unit: dim 8vc + j of keys 4va .. 4va + 3
+                const uint32_t w[4][4] = {{vp[0].x, vp[0].y, vp[0].z, vp[0].w}, {vp[1].x, vp[1].y, vp[1].z, vp[1].w},
+                                          {vp[2].x, vp[2].y, vp[2].z, vp[2].w}, {vp[3].x, vp[3].y, vp[3].z, vp[3].w}};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int sh = 16 * (j & 1);
-                const uint32_t e0 = (w[0][j >> 1] >> sh) & 0xffffu, e1 = (w[1][j >> 1] >> sh) & 0xffffu;
-                const uint32_t e2 = (w[2][j >> 1] >> sh) & 0xffffu, e3 = (w[3][j >> 1] >> sh) & 0xffffu;
-                *reinterpret_cast<uint2*>(&vt[buf][8 * vc + j][4 * va]) = make_uint2(e0 | (e1 << 16), e2 | (e3 << 16));
+                for (int j = 0; j < 8; ++j) {
+                    const int sh = 16 * (j & 1);
+                    const uint32_t e0 = (w[0][j >> 1] >> sh) & 0xffffu, e1 = (w[1][j >> 1] >> sh) & 0xffffu;
+                    const uint32_t e2 = (w[2][j >> 1] >> sh) & 0xffffu, e3 = (w[3][j >> 1] >> sh) & 0xffffu;
+                    *reinterpret_cast<uint2*>(&vt[buf][8 * vc + j][4 * va]) = make_uint2(e0 | (e1 << 16), e2 | (e3 << 16));
+                }
             }
         }
     };
     // the key blocks of this workgroup: all of them, or its share (PrefillAttnArgs::splits)
     const int blocks = last / kPfKeys + 1;
-    const int kb0 = CACHE == kCacheI8 ? blocks * (int)blockIdx.z / a.splits : 0;
-    const int kb1 = CACHE == kCacheI8 ? blocks * ((int)blockIdx.z + 1) / a.splits : blocks;
+    const int kb0 = Cache::kBlocks ? blocks * (int)blockIdx.z / a.splits : 0;
+    const int kb1 = Cache::kBlocks ? blocks * ((int)blockIdx.z + 1) / a.splits : blocks;
     issue(kb0);
 
     // ---- rope angles of the workgroup's tokens, shared by its QPK query
@@ -1061,7 +1119,7 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
     }
 
     // ---- non-finite values, to the tokens that attend them
-    if (CACHE != kCacheI8 && __builtin_expect(__builtin_amdgcn_readfirstlane(v_dropped) != 0, 0)) {
+    if (!Cache::kBlocks && __builtin_expect(__builtin_amdgcn_readfirstlane(v_dropped) != 0, 0)) {
 #pragma unroll 1
         for (int key = (wg_first + 1) / kPfKeys * kPfKeys; key <= last; ++key) {
             // (the largest offset added to kOOR stays past any cache too)
@@ -1078,7 +1136,7 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
     float l_tot = l_run + __shfl_xor(l_run, 16, 64);
     l_tot += __shfl_xor(l_tot, 32, 64);
     if (!live) return;
-    if (CACHE == kCacheI8 && a.splits > 1) {
+    if (Cache::kBlocks && a.splits > 1) {
         float* part = a.partials + (((size_t)t * a.q_heads + hq) * a.splits + blockIdx.z) * kPartStride;
 #pragma unroll
         for (int d = 0; d < 8; ++d) *reinterpret_cast<float4*>(part + 16 * d + 4 * g) = make_float4(o[d][0], o[d][1], o[d][2], o[d][3]);
@@ -1207,91 +1265,91 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
     const bool v_unit = tid < 256;
     const int va = tid & 15;        // V unit: keys 4va .. 4va + 3
     const int vc = (tid >> 4) & 15; // dims 8vc .. 8vc + 7
-    const PrefillI8 c8(a, kvh);
-    constexpr int P8 = 512 / NT;  // 16-byte pieces of an 8-bit block pair's keys (values) per thread
-    float kscale[P8], vscale[P8];
-    auto issue_k = [&](int kb, uint4 (&kp)[KP]) {
-        if constexpr (CACHE == kCacheI8) {
+    using Cache = PrefillCache<CACHE>;
+    using Piece = typename Cache::Piece;
+    const typename Cache::Blocks blocks_of(a, kvh);
+    constexpr int P8 = 512 / NT;  // pieces of a block pair's keys (values) per thread
+    constexpr int KN = Cache::kBlocks ? P8 : KP, VN = Cache::kBlocks ? P8 : 4;
+    auto issue_k = [&](int kb, Piece (&kp)[KN]) {
+        if constexpr (Cache::kBlocks) {
 #pragma unroll
             for (int r = 0; r < P8; ++r) {
-                kp[r] = c8.codes(kb, tid + NT * r, 0);
-                kscale[r] = c8.scale(kb, tid + NT * r, 0);
+                kp[r] = blocks_of.load_keys(kb, tid + NT * r);
             }
-            return;
-        }
+        } else {
 #pragma unroll
-        for (int r = 0; r < KP; ++r) {
-            const int idx = tid + NT * r;
-            kp[r] = load_b128(kr, ((uint32_t)(kb * kPfKeys + (idx >> 4)) * kHeadDim + 8u * (uint32_t)(idx & 15)) * 2u);
+            for (int r = 0; r < KP; ++r) {
+                const int idx = tid + NT * r;
+                kp[r] = load_b128(kr, ((uint32_t)(kb * kPfKeys + (idx >> 4)) * kHeadDim + 8u * (uint32_t)(idx & 15)) * 2u);
+            }
         }
     };
-    auto stage_k = [&](int buf, int kb, const uint4 (&kp)[KP]) {
-        if constexpr (CACHE == kCacheI8) {
+    auto stage_k = [&](int buf, int kb, const Piece (&kp)[KN]) {
+        if constexpr (Cache::kBlocks) {
 #pragma unroll
             for (int r = 0; r < P8; ++r) {
                 const int idx = tid + NT * r;
                 kv8_half8 x[2];
-                c8.keys(kb, idx, kp[r], kscale[r], x);
-                const int key = c8.key_of(idx), piece = c8.piece_of(idx);
+                blocks_of.keys(kb, idx, kp[r], x);
+                const int key = blocks_of.key_of(idx), piece = blocks_of.piece_of(idx);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) *reinterpret_cast<kv8_half8*>(&bufs[buf][half].k[key][8 * ((piece + i) ^ (key & 15))]) = x[i];
             }
-            return;
-        }
+        } else {
 #pragma unroll
-        for (int r = 0; r < KP; ++r) {
-            const int idx = tid + NT * r;
-            *reinterpret_cast<uint4*>(&bufs[buf][half].k[idx >> 4][8 * ((idx & 15) ^ ((idx >> 4) & 15))]) = kp[r];
+            for (int r = 0; r < KP; ++r) {
+                const int idx = tid + NT * r;
+                *reinterpret_cast<uint4*>(&bufs[buf][half].k[idx >> 4][8 * ((idx & 15) ^ ((idx >> 4) & 15))]) = kp[r];
+            }
         }
     };
-    auto issue_v = [&](int kb, uint4 (&vp)[4]) {
-        if constexpr (CACHE == kCacheI8) {
+    auto issue_v = [&](int kb, Piece (&vp)[VN]) {
+        if constexpr (Cache::kBlocks) {
 #pragma unroll
             for (int r = 0; r < P8; ++r) {
-                vp[r] = c8.codes(kb, tid + NT * r, kKv8PartBytes);
-                vscale[r] = c8.scale(kb, tid + NT * r, 4);
+                vp[r] = blocks_of.load_values(kb, tid + NT * r);
             }
-            return;
-        }
+        } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint32_t off = ((uint32_t)(kb * kPfKeys + 4 * va + r) * kHeadDim + 8u * (uint32_t)vc) * 2u;
-            vp[r] = load_b128(vr, v_unit ? off : kOOR);
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t off = ((uint32_t)(kb * kPfKeys + 4 * va + r) * kHeadDim + 8u * (uint32_t)vc) * 2u;
+                vp[r] = load_b128(vr, v_unit ? off : kOOR);
+            }
         }
     };
     const int wg_first = a.p0 + tile * TT * TOK;  // a token's first position
     if (threadIdx.x == 0) v_dropped = 0;
-    auto stage_v = [&](int buf, int kb, uint4 (&vp)[4]) {
-        if constexpr (CACHE == kCacheI8) {
+    auto stage_v = [&](int buf, int kb, Piece (&vp)[VN]) {
+        if constexpr (Cache::kBlocks) {
 #pragma unroll
             for (int r = 0; r < P8; ++r) {
                 const int idx = tid + NT * r;
                 kv8_half8 x[2];
-                c8.values(kb, idx, vp[r], vscale[r], x);
-                const int k0 = c8.keys_of(idx);
+                blocks_of.values(kb, idx, vp[r], x);
+                const int k0 = blocks_of.keys_of(idx);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const uint4 w = __builtin_bit_cast(uint4, x[i]);
-                    _Float16* row = bufs[buf][half].v[c8.dim_of(idx) + i];
+                    _Float16* row = bufs[buf][half].v[blocks_of.dim_of(idx) + i];
                     *reinterpret_cast<uint2*>(row + vt_pos(k0)) = make_uint2(w.x, w.y);
                     *reinterpret_cast<uint2*>(row + vt_pos(k0 + 4)) = make_uint2(w.z, w.w);
                 }
             }
-            return;
-        }
-        if (v_unit) {
-            if (kb * kPfKeys + kPfKeys - 1 > wg_first && drop_nonfinite(vp)) v_dropped = 1;
-            // row j of the unit: dim 8vc + j of keys 4va .. 4va + 3
-            const uint32_t w[4][4] = {{vp[0].x, vp[0].y, vp[0].z, vp[0].w}, {vp[1].x, vp[1].y, vp[1].z, vp[1].w},
-                                      {vp[2].x, vp[2].y, vp[2].z, vp[2].w}, {vp[3].x, vp[3].y, vp[3].z, vp[3].w}};
-            const int at = vt_pos(4 * va);
+        } else {
+            if (v_unit) {
+                if (kb * kPfKeys + kPfKeys - 1 > wg_first && drop_nonfinite(vp)) v_dropped = 1;
+                // row j of the unit: dim 8vc + j of keys 4va .. 4va + 3
+                const uint32_t w[4][4] = {{vp[0].x, vp[0].y, vp[0].z, vp[0].w}, {vp[1].x, vp[1].y, vp[1].z, vp[1].w},
+                                          {vp[2].x, vp[2].y, vp[2].z, vp[2].w}, {vp[3].x, vp[3].y, vp[3].z, vp[3].w}};
+                const int at = vt_pos(4 * va);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                // halfword j & 1 of words j >> 1 of two keys, packed by one byte permute each
-                const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
-                const uint32_t e01 = __builtin_amdgcn_perm(w[1][j >> 1], w[0][j >> 1], sel);
-                const uint32_t e23 = __builtin_amdgcn_perm(w[3][j >> 1], w[2][j >> 1], sel);
-                *reinterpret_cast<uint2*>(&bufs[buf][half].v[8 * vc + j][at]) = make_uint2(e01, e23);
+                for (int j = 0; j < 8; ++j) {
+                    // halfword j & 1 of words j >> 1 of two keys, packed by one byte permute each
+                    const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
+                    const uint32_t e01 = __builtin_amdgcn_perm(w[1][j >> 1], w[0][j >> 1], sel);
+                    const uint32_t e23 = __builtin_amdgcn_perm(w[3][j >> 1], w[2][j >> 1], sel);
+                    *reinterpret_cast<uint2*>(&bufs[buf][half].v[8 * vc + j][at]) = make_uint2(e01, e23);
+                }
             }
         }
     };
@@ -1299,7 +1357,7 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
     // ---- the prologue's loads, all in flight under the rope angles: the first
     // K/V blocks and the query rows of the first pass (thread: 8 dims of rows
     // tid/16 + 32 i)
-    uint4 kp0[KP], vp0[4];
+    Piece kp0[KN], vp0[VN];
     issue_k(half, kp0);
     issue_v(half, vp0);
     const int c = threadIdx.x & 15;
@@ -1429,7 +1487,7 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
         const int buf = round & 1;
         // the next block: K in flight under the scores, V under the
         // probabilities and the outputs (each held alone: registers)
-        uint4 kp[KP], vp[4];
+        Piece kp[KN], vp[VN];
         if (round + 1 < rounds) issue_k(kb + KS, kp);
 
         // S^T for the block's two 32-key tiles, interleaved: consecutive MFMAs
@@ -1574,7 +1632,7 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
     }
 
     // ---- non-finite values, to the tokens that attend them
-    if (CACHE != kCacheI8 && __builtin_expect(__builtin_amdgcn_readfirstlane(v_dropped) != 0, 0)) {
+    if (!Cache::kBlocks && __builtin_expect(__builtin_amdgcn_readfirstlane(v_dropped) != 0, 0)) {
 #pragma unroll 1
         for (int key = (wg_first + 1) / kPfKeys * kPfKeys; key <= last; ++key) {
             // (the largest offset added to kOOR stays past any cache too)
@@ -1688,7 +1746,7 @@ bool wide_prefill(const PrefillAttnArgs& a, int tiles, int cu_count) {
     return 16 * tiles * a.kv_heads >= (qpk == 1 ? 4 : qpk == 8 ? 16 : 11) * cu_count;
 }
 
-// Key shares of a narrow launch over an 8-bit cache: few tokens over a long
+// Key shares of a narrow launch over an 8-bit or 4-bit cache: few tokens over a long
 // context leave most CUs without a workgroup and the others with every key block in
 // turn. The share count of least cost, of those that two workgroups a CU, the partials'
 // room and the merge's 32 slots allow: in microseconds, a key round takes 1.75 with
@@ -1714,7 +1772,7 @@ int prefill_splits(const PrefillAttnArgs& a, int groups, int cu_count) {
     return best;
 }
 
-// Over an 8-bit cache the narrow form serves up to a workgroup a CU, split by keys
+// Over an 8-bit or 4-bit cache the narrow form serves up to a workgroup a CU, split by keys
 // (prefill_splits); the wide form takes over past that. Whole calls in us, narrow
 // and wide: 32 / 8 heads, 512 tokens (256 workgroups) after 4,000 117 and 126, after
 // 12,000 261 and 315, 640 tokens 179 and 130, 466 and 317; 16 / 8 heads, 1,024 (256) after
@@ -1728,11 +1786,11 @@ hipError_t launch_prefill_heads(const PrefillAttnArgs& args, int cu_count, hipSt
     PrefillAttnArgs a = args;
     const int wide = (a.tokens + kPrefillWideTokens * TT - 1) / (kPrefillWideTokens * TT);
     const int tiles = (a.tokens + kPrefillTileTokens * TT - 1) / (kPrefillTileTokens * TT);
-    if (CACHE == kCacheI8 ? tiles * a.kv_heads > cu_count : wide_prefill(a, wide, cu_count)) {
+    if (PrefillCache<CACHE>::kBlocks ? tiles * a.kv_heads > cu_count : wide_prefill(a, wide, cu_count)) {
         hipLaunchKernelGGL((attn_prefill_wide_kernel<QPK, CACHE>), dim3((unsigned)wide * (unsigned)a.kv_heads), dim3(512), 0, stream, a, wide);
         return hipGetLastError();
     }
-    a.splits = CACHE == kCacheI8 ? prefill_splits(a, tiles * a.kv_heads, cu_count) : 1;
+    a.splits = PrefillCache<CACHE>::kBlocks ? prefill_splits(a, tiles * a.kv_heads, cu_count) : 1;
     hipLaunchKernelGGL((attn_prefill_kernel<QPK, CACHE>), dim3((unsigned)tiles, (unsigned)a.kv_heads, (unsigned)a.splits), dim3(QPK < 8 ? 256 : 512), 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;
@@ -1756,13 +1814,15 @@ hipError_t launch_prefill_cache(const PrefillAttnArgs& a, int cu_count, hipStrea
 hipError_t launch_prefill_attention(const PrefillAttnArgs& a, int cu_count, hipStream_t stream, int cache) {
     if (a.tokens < 1 || a.kv_heads < 1 || a.q_heads % a.kv_heads != 0 || a.p0 < 0 ||
         (long long)a.p0 + a.tokens > a.mem.capacity || a.mem.keys == nullptr ||
-        (cache == kCacheI8 ? a.mem.rope == nullptr : a.mem.values == nullptr)) {
+        (cache == kCacheI8 || cache == kCacheI4 ? a.mem.rope == nullptr : a.mem.values == nullptr)) {
         return hipErrorInvalidValue;
     }
     const dim3 grid((unsigned)a.kv_heads, (unsigned)a.tokens);
     hipError_t e = hipSuccess;
     if (cache == kCacheI8) {
         e = launch_kv8_append_seq(a, stream);
+    } else if (cache == kCacheI4) {
+        e = launch_kv4_append_seq(a, stream);
     } else {
         if (cache == kCacheF16Table) hipLaunchKernelGGL(kv_append_seq_kernel<true>, grid, dim3(128), 0, stream, a);
         else hipLaunchKernelGGL(kv_append_seq_kernel<false>, grid, dim3(128), 0, stream, a);
@@ -1773,6 +1833,7 @@ hipError_t launch_prefill_attention(const PrefillAttnArgs& a, int cu_count, hipS
     case kCacheF16: return launch_prefill_cache<kCacheF16>(a, cu_count, stream);
     case kCacheF16Table: return launch_prefill_cache<kCacheF16Table>(a, cu_count, stream);
     case kCacheI8: return launch_prefill_cache<kCacheI8>(a, cu_count, stream);
+    case kCacheI4: return launch_prefill_cache<kCacheI4>(a, cu_count, stream);
     default: return hipErrorInvalidValue;
     }
 }

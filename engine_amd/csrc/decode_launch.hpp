@@ -26,10 +26,10 @@ constexpr int kPartStride = kHeadDim + 4;
 // One member's cache, as a device-resident descriptor: the attention kernel
 // reads it from memory, so a captured step serves any set of caches.
 struct AttnMember {
-    uint16_t* keys;       // f16 [layers][kv_heads][capacity][128]; an 8-bit cache: its regions [layers][kv_heads] (kv8.hpp)
-    uint16_t* values;     // f16 [layers][kv_heads][capacity][128]; an 8-bit cache: unused
+    uint16_t* keys;       // f16 [layers][kv_heads][capacity][128]; an 8-bit or 4-bit cache: its regions [layers][kv_heads] (kv8.hpp, kv4.hpp)
+    uint16_t* values;     // f16 [layers][kv_heads][capacity][128]; an 8-bit or 4-bit cache: unused
     float* partials;      // [q_heads][kAttnChunks][kPartStride], this member's own
-    uint64_t layer_elems; // kv_heads * capacity * 128: one layer's elements; an 8-bit cache: one layer's bytes
+    uint64_t layer_elems; // kv_heads * capacity * 128: one layer's elements; an 8-bit or 4-bit cache: one layer's bytes
     const double* rope;   // the cache's rotary table (rope_device.hpp), null: f32 angles from the launch's rope base
     int capacity;         // cache tokens per (layer, KV head)
     int pad;
@@ -39,6 +39,7 @@ struct AttnMember {
 constexpr int kCacheF16 = 0;       // f16, f32 angles
 constexpr int kCacheF16Table = 1;  // f16, angles from the caches' rotary tables
 constexpr int kCacheI8 = 2;        // 8 bits (kv8.hpp), angles from the tables
+constexpr int kCacheI4 = 3;        // 4 bits (kv4.hpp), angles from the tables
 
 struct AttnArgs {
     const AttnMember* mem;     // device [members] descriptors
@@ -128,7 +129,7 @@ struct PrefillAttnArgs {
     float eps;
     float rope_base;
     float scale;           // log2(e) / sqrt(head_dim)
-    float* partials;       // room for partial_rows rows of kPartStride floats, or null: 8-bit caches' launches of few
+    float* partials;       // room for partial_rows rows of kPartStride floats, or null: 8-bit and 4-bit caches' launches of few
     size_t partial_rows;   // tokens split the keys over workgroups there and merge the shares
     int splits;            // launch_prefill_attention sets it
 };

@@ -1,0 +1,288 @@
+// Kernels of the 4-bit KV cache for gfx950 (kv4.hpp has the layout and the arithmetic of a
+// code, kvq_device.hpp what other formats share): the append of new tokens, decode attention over the
+// cache, and rows moved in and out of it.
+#include "kv4.hpp"
+
+#include "kv4_device.hpp"
+#include "kvq_device.hpp"
+
+namespace ribn_amd {
+
+namespace {
+
+struct Kv4Format {
+    // Registers of a block's keys: codes 2, scales 4, lows 4 (dims 16 g + 8 h of half i at 2 i + h); of its
+    // values: codes 2, scales 2, lows 2 (half of the head), and room for the tail's.
+    static constexpr int kKeyRegs = 10, kValueRegs = 8;
+    static constexpr int kQuantiseBarriers = 2;
+    struct Scratch {
+        kv8_half2 key_lo[4][64], key_hi[4][64];  // of eight rows each; [0] then of all: low, and
+        float2 key_inv[64];
+        _Float16 value_lo[2][kKv8Block];
+        float value_inv[2][kKv8Block];
+    };
+
+    __device__ __forceinline__ static KvHead head(const AttnMember& m, int layer, int kvh) { return kv4_head(m, layer, kvh); }
+
+    // Rows 0 .. count - 1 of block b: eight bytes a thread, 16 dims of a key or two of eight values.
+    __device__ __forceinline__ static void stage_codes(StageRows& st, const KvHead& h, int b, int count) {
+        const int tid = append_tid(), lane = tid & 63, u = (tid >> 6) & 3, g = lane >> 4, m = lane & 15;
+        const uint8_t* block = h.codes + (size_t)b * kKv4BlockBytes;
+        const int at = 1024 * (u >> 1) + 16 * lane + 8 * (u & 1);
+        if (tid < 256) {
+            const uint2 w = *reinterpret_cast<const uint2*>(block + at);
+            const int row = kv8_key_row(u >> 1, m), dim = 64 * (u & 1) + 16 * g;
+            const kv4_u4* p = reinterpret_cast<const kv4_u4*>(block + kKv4KeyParams + 2 * dim);
+            const kv8_half8 x0 = kv4_values(w.x, p[0], p[16]), x1 = kv4_values(w.y, p[1], p[17]);
+            if (row < count) {
+                kv8_half8* k = reinterpret_cast<kv8_half8*>(&st.k[row][dim]);
+                k[0] = x0;
+                k[1] = x1;
+            }
+        } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(block + kKv4Values + at);
+            const kv4_u4* p = reinterpret_cast<const kv4_u4*>(block + kKv4ValueParams + (u >> 1) * kKv4ValueHalf + 16 * g);
+            const kv8_half8 x0 = kv4_values(w.x, p[0], p[4]), x1 = kv4_values(w.y, p[0], p[4]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (8 * g + j < count) *reinterpret_cast<kv8_half2*>(&st.v[8 * g + j][32 * u + 2 * m]) = kv8_half2{x0[j], x1[j]};
+        }
+    }
+
+    // The staged block's 32 rows into codes, scales and lows.
+    __device__ __forceinline__ static void quantise(Stage<Kv4Format>& st, const KvHead& h, int b) {
+        const int tid = append_tid(), lane = tid & 63, u = (tid >> 6) & 3, g = lane >> 4, m = lane & 15;
+        const bool keys = tid < 256;
+        uint8_t* const block = h.codes + (size_t)b * kKv4BlockBytes;
+        if (keys) {  // a pair of dims over eight rows
+            kv8_half2 lo = *reinterpret_cast<const kv8_half2*>(&st.k[8 * u][2 * lane]), hi = lo;
+#pragma unroll
+            for (int r = 1; r < 8; ++r) {
+                const kv8_half2 x = *reinterpret_cast<const kv8_half2*>(&st.k[8 * u + r][2 * lane]);
+                lo = kv4_min(lo, x);
+                hi = __builtin_elementwise_max(hi, x);
+            }
+            st.x.key_lo[u][lane] = lo;
+            st.x.key_hi[u][lane] = hi;
+        } else {  // 16 dims of a token, four lanes a group
+            const int token = 8 * u + (lane >> 3), half = (lane >> 2) & 1;
+            const kv8_half2* row = reinterpret_cast<const kv8_half2*>(&st.v[token][16 * (lane & 7)]);
+            kv8_half2 lo = row[0], hi = lo;
+#pragma unroll
+            for (int j = 1; j < 8; ++j) {
+                lo = kv4_min(lo, row[j]);
+                hi = __builtin_elementwise_max(hi, row[j]);
+            }
+            // (the largest as the smallest of its negative, in one reduction)
+            const kv8_half2 both = kv4_quad_min(kv8_half2{kv4_min(lo, kv8_half2{lo[1], lo[1]})[0], -__builtin_elementwise_max(hi, kv8_half2{hi[1], hi[1]})[0]});
+            if ((lane & 3) == 0) {
+                const Kv4Scale s(both[0], -both[1]);
+                st.x.value_lo[half][token] = both[0];
+                st.x.value_inv[half][token] = s.inv;
+                _Float16* p = reinterpret_cast<_Float16*>(block + kKv4ValueParams + half * kKv4ValueHalf);
+                p[token] = s.s;
+                p[kKv8Block + token] = both[0];
+            }
+        }
+        __syncthreads();
+        if (tid < 64) {
+            kv8_half2 lo = st.x.key_lo[0][lane], hi = st.x.key_hi[0][lane];
+#pragma unroll
+            for (int r = 1; r < 4; ++r) {
+                lo = kv4_min(lo, st.x.key_lo[r][lane]);
+                hi = __builtin_elementwise_max(hi, st.x.key_hi[r][lane]);
+            }
+            const Kv4Scale a(lo[0], hi[0]), c(lo[1], hi[1]);
+            st.x.key_lo[0][lane] = lo;
+            st.x.key_inv[lane] = make_float2(a.inv, c.inv);
+            kv8_half2* p = reinterpret_cast<kv8_half2*>(block + kKv4KeyParams);
+            p[lane] = kv8_half2{a.s, c.s};
+            p[64 + lane] = lo;
+        }
+        __syncthreads();
+        uint32_t w[2] = {0, 0};
+        if (keys) {
+            const int dim = 64 * (u & 1) + 16 * g;
+            const _Float16* row = &st.k[kv8_key_row(u >> 1, m)][dim];
+            const _Float16* lo = reinterpret_cast<const _Float16*>(st.x.key_lo[0]) + dim;
+            const float* inv = reinterpret_cast<const float*>(st.x.key_inv) + dim;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j >> 3] |= kv4_code(row[j], lo[j], inv[j]) << kv4_shift(j & 7);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int key = 8 * g + j;
+                const kv8_half2 x = *reinterpret_cast<const kv8_half2*>(&st.v[key][32 * u + 2 * m]);
+                const _Float16 lo = st.x.value_lo[u >> 1][key];
+                const float inv = st.x.value_inv[u >> 1][key];
+                w[0] |= kv4_code(x[0], lo, inv) << kv4_shift(j);
+                w[1] |= kv4_code(x[1], lo, inv) << kv4_shift(j);
+            }
+        }
+        *reinterpret_cast<uint2*>(block + (keys ? 0 : kKv4Values) + 1024 * (u >> 1) + 16 * lane + 8 * (u & 1)) = make_uint2(w[0], w[1]);
+    }
+
+    // A block's codes, two 16-byte loads a lane of keys and of values, and their scales and lows.
+    struct Source {
+        __amdgpu_buffer_rsrc_t r;
+        __device__ __forceinline__ Source(const KvHead& h, int capacity) : r(make_rsrc(h.codes, (uint32_t)kv4_tail_offset(capacity))) {}
+        __device__ __forceinline__ kv8_u4 load(uint32_t at) const { return __builtin_bit_cast(kv8_u4, load_b128(r, at)); }
+        __device__ __forceinline__ void keys(int b, int end, int lane, kv8_u4 (&w)[kKeyRegs], float&) const {
+            const uint32_t base = b < end ? (uint32_t)b * kKv4BlockBytes : kCacheOOR;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) w[t] = load(base + 1024u * t + 16u * (uint32_t)lane);
+            const uint32_t p = base + kKv4KeyParams + 32u * (uint32_t)(lane >> 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[2 + i] = load(p + 128u * (i >> 1) + 16u * (i & 1));
+                w[6 + i] = load(p + 2u * kHeadDim + 128u * (i >> 1) + 16u * (i & 1));
+            }
+        }
+        __device__ __forceinline__ void values(int b, int end, int lane, kv8_u4 (&w)[kValueRegs], float&) const {
+            const uint32_t base = b < end ? (uint32_t)b * kKv4BlockBytes : kCacheOOR;
+            const uint32_t p = base + kKv4ValueParams + 16u * (uint32_t)(lane >> 4);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                w[i] = load(base + kKv4Values + 1024u * i + 16u * (uint32_t)lane);
+                w[2 + i] = load(p + (uint32_t)kKv4ValueHalf * i);
+                w[4 + i] = load(p + (uint32_t)kKv4ValueHalf * i + 2u * kKv8Block);
+            }
+        }
+    };
+
+    __device__ __forceinline__ static void scores(const kv8_u4 (&kq)[kKeyRegs], const kv8_half8 (&qb)[4], kv8_float4 (&s)[2]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv4_values(kq[t][i], kq[2 + i], kq[6 + i]), qb[i], s[t], 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ static float scaled(float fac, float) { return fac; }
+    __device__ __forceinline__ static void outputs(const kv8_u4 (&vq)[kValueRegs], float, kv8_half8 pb, kv8_float4 (&o)[8]) {
+#pragma unroll
+        for (int d = 0; d < 8; ++d)
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv4_values(vq[d >> 2][d & 3], vq[2 + (d >> 2)], vq[4 + (d >> 2)]), pb, o[d], 0, 0, 0);
+    }
+
+    // The block in the tail's registers (TailBlock): what the codes of block b stand for.
+    __device__ __forceinline__ static void load_tail(const KvHead& h, int b, int lane, kv8_u4 (&k)[kKeyRegs], kv8_u4 (&v)[kValueRegs]) {
+        const uint8_t* block = h.codes + (size_t)b * kKv4BlockBytes;
+        const kv8_u4* kp = reinterpret_cast<const kv8_u4*>(block + kKv4KeyParams) + 2 * (lane >> 4);
+        const kv8_u4* vp = reinterpret_cast<const kv8_u4*>(block + kKv4ValueParams) + (lane >> 4);
+        const kv8_u4* kc = reinterpret_cast<const kv8_u4*>(block) + lane;
+        const kv8_u4* vc = reinterpret_cast<const kv8_u4*>(block + kKv4Values) + lane;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int s = i & 3;  // key step 4 t + s: dims 64 (s >> 1) + 16 g + 8 (s & 1)
+            k[i] = __builtin_bit_cast(kv8_u4, kv4_values(kc[64 * (i >> 2)][s], kp[8 * (s >> 1) + (s & 1)], kp[16 + 8 * (s >> 1) + (s & 1)]));
+            v[i] = __builtin_bit_cast(kv8_u4, kv4_values(vc[64 * (i >> 2)][s], vp[8 * (i >> 2)], vp[8 * (i >> 2) + 4]));
+        }
+    }
+
+    // Codes, scales and lows of the whole block; its values become what these stand for.
+    __device__ __forceinline__ static void quantise_tail(const KvHead& h, int b, int lane, kv8_u4 (&k)[kKeyRegs], kv8_u4 (&v)[kValueRegs]) {
+        uint8_t* const block = h.codes + (size_t)b * kKv4BlockBytes;
+        auto pair = [](uint32_t w) { return __builtin_bit_cast(kv8_half2, w); };
+        auto word = [](kv8_half2 x) { return __builtin_bit_cast(uint32_t, x); };
+        kv8_u4* const kp = reinterpret_cast<kv8_u4*>(block + kKv4KeyParams) + 2 * (lane >> 4);
+        kv8_u4 kw[2];  // code words, by tile
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            kv8_u4 scale, low;
+            uint32_t w[2] = {0, 0};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {  // a pair of dims, over the two tiles and the row's 16 keys
+                const uint32_t x0 = k[s][j], x1 = k[4 + s][j];
+                const kv8_half2 lo = kv4_row_min(kv4_min(pair(x0), pair(x1))), hi = -kv4_row_min(kv4_min(-pair(x0), -pair(x1)));
+                const Kv4Scale a(lo[0], hi[0]), c(lo[1], hi[1]);
+                scale[j] = word(kv8_half2{a.s, c.s});
+                low[j] = word(lo);
+                w[0] |= kv4_code(pair(x0)[0], lo[0], a.inv) << kv4_shift(2 * j) | kv4_code(pair(x0)[1], lo[1], c.inv) << kv4_shift(2 * j + 1);
+                w[1] |= kv4_code(pair(x1)[0], lo[0], a.inv) << kv4_shift(2 * j) | kv4_code(pair(x1)[1], lo[1], c.inv) << kv4_shift(2 * j + 1);
+            }
+            if ((lane & 15) == 0) {
+                kp[8 * (s >> 1) + (s & 1)] = scale;
+                kp[16 + 8 * (s >> 1) + (s & 1)] = low;
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                kw[t][s] = w[t];
+                k[4 * t + s] = __builtin_bit_cast(kv8_u4, kv4_values(w[t], scale, low));
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) reinterpret_cast<kv8_u4*>(block)[64 * t + lane] = kw[t];
+        kv8_u4* const vp = reinterpret_cast<kv8_u4*>(block + kKv4ValueParams) + (lane >> 4);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            kv8_u4 scale, low;
+            kv8_u4 w = kv8_u4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {  // a pair of keys, over four dims and the row's 16 lanes
+                kv8_half2 lo, hi;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const uint32_t x = v[4 * half + d][j];
+                    lo = d == 0 ? pair(x) : kv4_min(lo, pair(x));
+                    hi = d == 0 ? -pair(x) : kv4_min(hi, -pair(x));
+                }
+                lo = kv4_row_min(lo);
+                hi = -kv4_row_min(hi);
+                const Kv4Scale a(lo[0], hi[0]), c(lo[1], hi[1]);
+                scale[j] = word(kv8_half2{a.s, c.s});
+                low[j] = word(lo);
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const uint32_t x = v[4 * half + d][j];
+                    w[d] |= kv4_code(pair(x)[0], lo[0], a.inv) << kv4_shift(2 * j) | kv4_code(pair(x)[1], lo[1], c.inv) << kv4_shift(2 * j + 1);
+                }
+            }
+            if ((lane & 15) == 0) {
+                vp[8 * half] = scale;
+                vp[8 * half + 4] = low;
+            }
+            reinterpret_cast<kv8_u4*>(block + kKv4Values)[64 * half + lane] = w;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) v[4 * half + d] = __builtin_bit_cast(kv8_u4, kv4_values(w[d], scale, low));
+        }
+    }
+};
+
+__global__ __launch_bounds__(2 * kAppendThreads) void kv4_append_kernel(AttnArgs a, int members) { append_members<Kv4Format>(a, members); }
+__global__ __launch_bounds__(2 * kAppendThreads) void kv4_append_seq_kernel(PrefillAttnArgs a) { append_chunk<Kv4Format>(a); }
+template <int ROWS>
+__global__ __launch_bounds__(2 * kAppendThreads) void kv4_write_kernel(KvMoveArgs a) { write_rows<Kv4Format, ROWS>(a); }
+template <typename T>
+__global__ __launch_bounds__(kAppendThreads, 4) void kv4_read_kernel(KvMoveArgs a) { read_rows<Kv4Format, T>(a); }
+
+template <int QPK, bool INLINE>
+__global__ __launch_bounds__(kAttnThreads, 3) void kv4_attn_kernel(AttnArgs a, Members<INLINE> members) {
+    cache_attention<Kv4Format, QPK, INLINE>(a, members);
+}
+template <int NC, bool INLINE>
+__global__ __launch_bounds__(128) void kv4_combine_kernel(AttnArgs a, Members<INLINE> members) {
+    combine_chunks<Kv4Format, NC, INLINE>(a, members);
+}
+template <bool INLINE>
+constexpr AttnKernels<INLINE> kKernels{{kv4_attn_kernel<1, INLINE>, kv4_attn_kernel<2, INLINE>, kv4_attn_kernel<4, INLINE>, kv4_attn_kernel<8, INLINE>},
+                                       {kv4_combine_kernel<8, INLINE>, kv4_combine_kernel<32, INLINE>}};
+
+}  // namespace
+
+hipError_t launch_kv4_append(const AttnArgs& a, int members, hipStream_t stream) { return launch_append(kv4_append_kernel, a, members, stream); }
+hipError_t launch_kv4_append_seq(const PrefillAttnArgs& a, hipStream_t stream) { return launch_append_chunk(kv4_append_seq_kernel, a, stream); }
+hipError_t launch_kv4_attention(const AttnArgs& a, const AttnMember* host_mem, int members, hipStream_t stream) {
+    return launch_cache_attention(kKernels<true>, kKernels<false>, a, host_mem, members, stream);
+}
+
+hipError_t launch_kv4_write(const KvMoveArgs& a, bool half, hipStream_t stream) {
+    if (!move_fits(a)) return hipErrorInvalidValue;
+    return launch_move(half ? kv4_write_kernel<kRowsF16> : kv4_write_kernel<kRowsF32>, a, append_threads(a.p0, a.tokens), stream);
+}
+hipError_t launch_kv4_read(const KvMoveArgs& a, bool half, hipStream_t stream) {
+    if (!move_fits(a)) return hipErrorInvalidValue;
+    return launch_move(half ? kv4_read_kernel<_Float16> : kv4_read_kernel<float>, a, kAppendThreads, stream);
+}
+
+}  // namespace ribn_amd

@@ -59,9 +59,10 @@ __host__ __device__ inline size_t kv8_head_bytes(int capacity) { return (kv8_end
 // Values: 8 keys 8 g .. + 7 of dims 32 u + 2 m and 32 u + 2 m + 1: 64 u + lane.
 __host__ __device__ inline int kv8_key_row(int t, int m) { return 8 * (m >> 2) + 4 * t + (m & 3); }
 
-// Sets up a cache: its rotary table (128-wide heads) and, of an 8-bit cache (`regions` not
-// null), every region's tail, scales and end to zeros, so that it reads as zeros.
-hipError_t launch_cache_init(void* regions, size_t count, int capacity, const double* table, double* table_dst,
+// Sets up a cache: its rotary table (128-wide heads) and, of a cache of blocks (`regions` not
+// null), each of the regions of `stride` bytes from byte `codes` on to zeros (an 8-bit cache's tail, scales and
+// end: any code is finite; all of a 4-bit cache's), so that it reads as zeros.
+hipError_t launch_cache_init(void* regions, size_t count, size_t stride, size_t codes, const double* table, double* table_dst,
                              hipStream_t stream);
 
 // f16 or f32 rows moved into or out of a cache ([tokens][kv_heads][128]).

@@ -139,17 +139,17 @@ typedef float kv8_float2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ kv8_half2 kv8_halfs(float a, float b) { return __builtin_convertvector((kv8_float2{a, b}), kv8_half2); }
 
 // The parts of a (layer, KV head) region.
-struct Kv8Head {
+struct KvHead {
     uint8_t* codes;
     _Float16* tail_k;
     _Float16* tail_v;
-    float2* scales;
+    float2* scales;  // (8 bits)
     int32_t* end;
 };
 
-__device__ __forceinline__ Kv8Head kv8_head(const AttnMember& m, int layer, int kvh) {
+__device__ __forceinline__ KvHead kv8_head(const AttnMember& m, int layer, int kvh) {
     uint8_t* const base = reinterpret_cast<uint8_t*>(m.keys) + (size_t)layer * m.layer_elems + (size_t)kvh * kv8_head_bytes(m.capacity);
-    Kv8Head h;
+    KvHead h;
     h.codes = base;
     h.tail_k = reinterpret_cast<_Float16*>(base + kv8_tail_offset(m.capacity));
     h.tail_v = h.tail_k + kKv8TailElems;

@@ -40,6 +40,7 @@
 #include "abi_internal.hpp"
 #include "decode_launch.hpp"
 #include "kquant_launch.hpp"
+#include "kv4.hpp"
 #include "kv8.hpp"
 #include "qwen3_internal.hpp"
 #include "rope.hpp"
@@ -53,9 +54,9 @@ struct ribn_amd_kv_cache {
     ribn_amd_qwen3_config cfg;
     uint32_t capacity;
     int kind;            // ribn_amd::kCache*: format, and whether it has a rotary table
-    size_t layer_elems;  // f16: kv_heads * capacity * head_dim; 8 bits: a layer's bytes
+    size_t layer_elems;  // f16: kv_heads * capacity * head_dim; 8 and 4 bits: a layer's bytes
     void* block;         // one allocation: keys, values, partials, rotary table
-    uint16_t* keys;      // f16 [layers][kv_heads][capacity][head_dim]; 8 bits: regions [layers][kv_heads] (kv8.hpp)
+    uint16_t* keys;      // f16 [layers][kv_heads][capacity][head_dim]; 8 and 4 bits: regions [layers][kv_heads] (kv8.hpp, kv4.hpp)
     uint16_t* values;    // f16
     const double* rope;  // rotary table, or null
     float* partials;     // attention partials of the standalone attention call
@@ -149,10 +150,26 @@ ribn_amd_status check_kind(const ribn_amd_kv_cache* cache, const ribn_amd_kv_cac
     return RIBN_AMD_OK;
 }
 
+// Whether a kind keeps blocks of 32 tokens in fewer than 16 bits (kv8.hpp, kv4.hpp).
+bool in_blocks(int kind) { return kind == ribn_amd::kCacheI8 || kind == ribn_amd::kCacheI4; }
+
+// Bytes of a (layer, KV head) region of such a kind, and where its tail lies.
+size_t region_bytes(int kind, int capacity) {
+    return kind == ribn_amd::kCacheI4 ? ribn_amd::kv4_head_bytes(capacity) : ribn_amd::kv8_head_bytes(capacity);
+}
+size_t region_tail(int kind, int capacity) {
+    return kind == ribn_amd::kCacheI4 ? ribn_amd::kv4_tail_offset(capacity) : ribn_amd::kv8_tail_offset(capacity);
+}
+
+uint32_t format_of(int kind) {
+    return kind == ribn_amd::kCacheI8 ? RIBN_AMD_KV_I8 : kind == ribn_amd::kCacheI4 ? RIBN_AMD_KV_I4 : RIBN_AMD_KV_F16;
+}
+
+bool known_format(uint32_t format) { return format == RIBN_AMD_KV_F16 || format == RIBN_AMD_KV_I8 || format == RIBN_AMD_KV_I4; }
+
 // Attention grid of a launch over caches of one kind.
 int grid_chunks(int kind, int max_capacity, int members) {
-    return kind == ribn_amd::kCacheI8 ? ribn_amd::kv8_grid_chunks(max_capacity, members)
-                                      : ribn_amd::attn_grid_chunks(max_capacity, members);
+    return in_blocks(kind) ? ribn_amd::kv8_grid_chunks(max_capacity, members) : ribn_amd::attn_grid_chunks(max_capacity, members);
 }
 
 }  // namespace
@@ -286,7 +303,7 @@ hipError_t wave_shared(const ribn_amd_qwen3_decode* d, const ribn_amd_quantized_
 // With `partials` set, member m's attention partials live at partials +
 // m * attn_partials_floats (the decoder's own buffer, whose address the merge
 // launch then takes from its arguments); else in the descriptors. `host_mem`
-// (8-bit caches): descriptors in host memory instead.
+// (8-bit and 4-bit caches): descriptors in host memory instead.
 hipError_t attention(const ribn_amd_qwen3_config& cfg, const ribn_amd::AttnMember* mem, int kind, int chunks, bool appended,
                      int members, uint32_t layer, const float* q, const float* k, const float* v, const float* q_norm,
                      const float* k_norm, const int32_t* positions, float* out, float* partials, hipStream_t stream,
@@ -318,9 +335,11 @@ hipError_t attention(const ribn_amd_qwen3_config& cfg, const ribn_amd::AttnMembe
         a.scale = 1.4426950408889634f / sqrtf((float)cfg.head_dim);
         const bool table = kind == ribn_amd::kCacheF16Table;
         hipError_t e = hipSuccess;
-        if (kind == ribn_amd::kCacheI8) {
-            if (appended) e = ribn_amd::launch_kv8_append(a, mc, stream);
-            if (e == hipSuccess) e = ribn_amd::launch_kv8_attention(a, host_mem != nullptr ? host_mem + m0 : nullptr, mc, stream);
+        if (in_blocks(kind)) {
+            const bool i4 = kind == ribn_amd::kCacheI4;
+            const ribn_amd::AttnMember* host = host_mem != nullptr ? host_mem + m0 : nullptr;
+            if (appended) e = i4 ? ribn_amd::launch_kv4_append(a, mc, stream) : ribn_amd::launch_kv8_append(a, mc, stream);
+            if (e == hipSuccess) e = i4 ? ribn_amd::launch_kv4_attention(a, host, mc, stream) : ribn_amd::launch_kv8_attention(a, host, mc, stream);
         } else {
             if (appended) e = ribn_amd::launch_kv_append(a, mc, stream, table);
             if (e == hipSuccess) e = ribn_amd::launch_attention(a, mc, stream, table);
@@ -741,7 +760,7 @@ ribn_amd_status copy_selected_async(ribn_amd_qwen3_decode* d, size_t member, uin
 
 ribn_amd_status check_kv_options(const ribn_amd_kv_options* o, float rope_base) {
     if (o == nullptr) return RIBN_AMD_OK;
-    if (o->format > RIBN_AMD_KV_I8) return fail(RIBN_AMD_INVALID_ARGUMENT, RIBN_AMD_KV_I8, o->format, "unknown cache format %u", o->format);
+    if (!known_format(o->format)) return fail(RIBN_AMD_INVALID_ARGUMENT, RIBN_AMD_KV_I8, o->format, "unknown cache format %u", o->format);
     if (o->rope == nullptr) return RIBN_AMD_OK;
     const ribn_amd_status st = check_rope_spec(o->rope);
     if (st != RIBN_AMD_OK) return st;
@@ -779,13 +798,18 @@ ribn_amd_status ribn_amd_kv_cache_create_with(ribn_amd_context* ctx, const ribn_
     if (capacity == 0 || capacity > (1u << 20)) {
         return fail(RIBN_AMD_INVALID_PLAN, 1u << 20, capacity, "KV capacity must be 1..%u tokens", 1u << 20);
     }
-    const bool i8 = options != nullptr && options->format == RIBN_AMD_KV_I8;
+    const uint32_t format = options != nullptr ? options->format : RIBN_AMD_KV_F16;
     const ribn_amd_rope_spec* rope = options != nullptr ? options->rope : nullptr;
-    const bool table = i8 || rope != nullptr;
-    const size_t layer_elems = i8 ? config->kv_heads * ribn_amd::kv8_head_bytes((int)capacity)
-                                  : (size_t)config->kv_heads * capacity * config->head_dim;
-    const size_t cache_bytes = i8 ? layer_elems * config->layers : align_up(layer_elems * config->layers * sizeof(uint16_t));
-    const size_t held_bytes = i8 ? cache_bytes : 2 * cache_bytes;
+    const int kind = format == RIBN_AMD_KV_I8   ? ribn_amd::kCacheI8
+                     : format == RIBN_AMD_KV_I4 ? ribn_amd::kCacheI4
+                     : rope != nullptr          ? ribn_amd::kCacheF16Table
+                                                : ribn_amd::kCacheF16;
+    const bool blocks = in_blocks(kind);
+    const bool table = kind != ribn_amd::kCacheF16;
+    const size_t region = blocks ? region_bytes(kind, (int)capacity) : 0;
+    const size_t layer_elems = blocks ? config->kv_heads * region : (size_t)config->kv_heads * capacity * config->head_dim;
+    const size_t cache_bytes = blocks ? layer_elems * config->layers : align_up(layer_elems * config->layers * sizeof(uint16_t));
+    const size_t held_bytes = blocks ? cache_bytes : 2 * cache_bytes;
     const size_t part_bytes = align_up(ribn_amd::attn_partials_floats((int)config->q_heads) * sizeof(float));
     double turns[ribn_amd::kRopeTableMax];
     size_t table_bytes = 0;
@@ -802,7 +826,7 @@ ribn_amd_status ribn_amd_kv_cache_create_with(ribn_amd_context* ctx, const ribn_
         table_bytes = (size_t)rope_table(*rope, turns) * sizeof(double);
     }
     DeviceGuard guard(ctx->device);
-    if (i8 && ctx->split_partials == nullptr) {
+    if (blocks && ctx->split_partials == nullptr) {
         void* room = nullptr;
         const hipError_t e = hipMalloc(&room, ribn_amd::kPrefillPartialRows * ribn_amd::kPartStride * sizeof(float));
         if (e != hipSuccess) return driver(e, "hipMalloc prompt attention partials");
@@ -814,7 +838,8 @@ ribn_amd_status ribn_amd_kv_cache_create_with(ribn_amd_context* ctx, const ribn_
     char* p = static_cast<char*>(block);
     if (table) {
         // stream-ordered, from kernel arguments: a cache is made while earlier work runs
-        e = ribn_amd::launch_cache_init(i8 ? p : nullptr, (size_t)config->layers * config->kv_heads, (int)capacity, turns,
+        e = ribn_amd::launch_cache_init(blocks ? p : nullptr, (size_t)config->layers * config->kv_heads, region,
+                                        kind == ribn_amd::kCacheI8 ? region_tail(kind, (int)capacity) : 0, turns,
                                         reinterpret_cast<double*>(p + held_bytes + part_bytes), ctx->stream);
     }
     auto* c = e == hipSuccess ? new (std::nothrow) ribn_amd_kv_cache{} : nullptr;
@@ -827,11 +852,11 @@ ribn_amd_status ribn_amd_kv_cache_create_with(ribn_amd_context* ctx, const ribn_
     c->id = g_cache_ids.fetch_add(1);
     c->cfg = *config;
     c->capacity = capacity;
-    c->kind = i8 ? ribn_amd::kCacheI8 : table ? ribn_amd::kCacheF16Table : ribn_amd::kCacheF16;
+    c->kind = kind;
     c->layer_elems = layer_elems;
     c->block = block;
     c->keys = reinterpret_cast<uint16_t*>(p);
-    c->values = i8 ? nullptr : reinterpret_cast<uint16_t*>(p + cache_bytes);
+    c->values = blocks ? nullptr : reinterpret_cast<uint16_t*>(p + cache_bytes);
     c->partials = reinterpret_cast<float*>(p + held_bytes);
     c->rope = table ? reinterpret_cast<const double*>(p + held_bytes + part_bytes) : nullptr;
     // nothing else is cleared: a position is written before it is read, and every
@@ -855,14 +880,14 @@ void ribn_amd_kv_cache_destroy(ribn_amd_kv_cache* cache) {
 uint32_t ribn_amd_kv_cache_capacity(const ribn_amd_kv_cache* cache) { return cache ? cache->capacity : 0; }
 
 uint32_t ribn_amd_kv_cache_format(const ribn_amd_kv_cache* cache) {
-    return cache && cache->kind == ribn_amd::kCacheI8 ? RIBN_AMD_KV_I8 : RIBN_AMD_KV_F16;
+    return cache ? format_of(cache->kind) : RIBN_AMD_KV_F16;
 }
 
 uint64_t ribn_amd_kv_bytes(const ribn_amd_qwen3_config* c, uint32_t tokens, uint32_t format) {
-    if (!c || format > RIBN_AMD_KV_I8) return 0;
+    if (!c || !known_format(format)) return 0;
     if (format == RIBN_AMD_KV_F16) return ribn_amd_qwen3_kv_bytes(c, tokens);
     if (tokens > (1u << 20)) return 0;
-    return (uint64_t)c->layers * c->kv_heads * ribn_amd::kv8_head_bytes((int)tokens);
+    return (uint64_t)c->layers * c->kv_heads * region_bytes(format == RIBN_AMD_KV_I4 ? ribn_amd::kCacheI4 : ribn_amd::kCacheI8, (int)tokens);
 }
 
 static ribn_amd_status check_layer(const ribn_amd_kv_cache* cache, uint32_t layer) {
@@ -878,11 +903,11 @@ ribn_amd_status ribn_amd_kv_cache_tail(ribn_amd_kv_cache* cache, uint32_t layer,
     if (!cache || !keys || !values || !head_stride) return fail(RIBN_AMD_INVALID_ARGUMENT, 0, 0, "null argument");
     const ribn_amd_status st = check_layer(cache, layer);
     if (st != RIBN_AMD_OK) return st;
-    if (cache->kind != ribn_amd::kCacheI8) return fail(RIBN_AMD_UNSUPPORTED, RIBN_AMD_KV_I8, RIBN_AMD_KV_F16, "an f16 cache has no tail block");
+    if (!in_blocks(cache->kind)) return fail(RIBN_AMD_UNSUPPORTED, RIBN_AMD_KV_I8, RIBN_AMD_KV_F16, "an f16 cache has no tail block");
     char* region = reinterpret_cast<char*>(cache->keys) + (size_t)layer * cache->layer_elems;
-    *keys = reinterpret_cast<uint16_t*>(region + ribn_amd::kv8_tail_offset((int)cache->capacity));
+    *keys = reinterpret_cast<uint16_t*>(region + region_tail(cache->kind, (int)cache->capacity));
     *values = *keys + ribn_amd::kKv8TailElems;
-    *head_stride = ribn_amd::kv8_head_bytes((int)cache->capacity) / sizeof(uint16_t);
+    *head_stride = region_bytes(cache->kind, (int)cache->capacity) / sizeof(uint16_t);
     return ok();
 }
 
@@ -922,8 +947,9 @@ static ribn_amd_status move_rows(ribn_amd_context* ctx, ribn_amd_kv_cache* cache
     a.keys = keys;
     a.values = values;
     const bool half = dtype == RIBN_AMD_F16, kv8 = cache->kind == ribn_amd::kCacheI8;
-    const hipError_t e = write ? ribn_amd::launch_kv_write(a, half, kv8, ctx->stream)
-                               : ribn_amd::launch_kv_read(a, half, kv8, ctx->stream);
+    const hipError_t e = cache->kind == ribn_amd::kCacheI4 ? (write ? ribn_amd::launch_kv4_write(a, half, ctx->stream) : ribn_amd::launch_kv4_read(a, half, ctx->stream))
+                         : write                           ? ribn_amd::launch_kv_write(a, half, kv8, ctx->stream)
+                                                           : ribn_amd::launch_kv_read(a, half, kv8, ctx->stream);
     return e == hipSuccess ? ok() : driver(e, write ? "cache write launch" : "cache read launch");
 }
 
@@ -943,8 +969,9 @@ ribn_amd_status ribn_amd_kv_cache_layer(ribn_amd_kv_cache* cache, uint32_t layer
     if (!cache || !keys || !values) return fail(RIBN_AMD_INVALID_ARGUMENT, 0, 0, "null argument");
     const ribn_amd_status st = check_layer(cache, layer);
     if (st != RIBN_AMD_OK) return st;
-    if (cache->kind == ribn_amd::kCacheI8) {
-        return fail(RIBN_AMD_UNSUPPORTED, RIBN_AMD_KV_F16, RIBN_AMD_KV_I8, "an 8-bit cache has no f16 view (ribn_amd_kv_cache_read)");
+    if (in_blocks(cache->kind)) {
+        return fail(RIBN_AMD_UNSUPPORTED, RIBN_AMD_KV_F16, format_of(cache->kind), "an %d-bit cache has no f16 view (ribn_amd_kv_cache_read)",
+                    cache->kind == ribn_amd::kCacheI8 ? 8 : 4);
     }
     *keys = cache->keys + (size_t)layer * cache->layer_elems;
     *values = cache->values + (size_t)layer * cache->layer_elems;
@@ -1049,7 +1076,7 @@ ribn_amd_status ribn_amd_attention_decode(ribn_amd_context* ctx, const ribn_amd_
     }
     DeviceGuard guard(ctx->device);
     const int kind = caches[0]->kind;
-    if (kind == ribn_amd::kCacheI8) {
+    if (in_blocks(kind)) {
         ribn_amd::AttnMember host_mem[RIBN_AMD_MAX_BATCH_MEMBERS];
         int max_capacity = 1;
         for (size_t m = 0; m < members; ++m) {

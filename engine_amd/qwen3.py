@@ -23,9 +23,10 @@ from . import _lib
 from .kquant import RANK_CACHE, RANK_DECODER, AmdModelKernelError, _check, _live, _own, _ptr
 from .rope import AmdRopeSpec, _dtype
 
-# What a KV cache holds a value in: f16, or 8 bits with a power-of-two scale for
-# each block of 32 tokens and KV head.
-KV_F16, KV_I8 = 0, 1
+# What a KV cache holds a value in: f16; 8 bits with a power-of-two scale for
+# each block of 32 tokens and KV head; or 4 bits with a scale and a low for each
+# 32 tokens of a key dim, each 64 dims of a token's value.
+KV_F16, KV_I8, KV_I4 = 0, 1, 4
 
 
 @dataclass(frozen=True)
@@ -61,7 +62,7 @@ def kv_options(config: AmdQwen3Config, format: int = KV_F16, rope: Optional[AmdR
 
 class AmdKvCache:
     """One sequence's KV cache for every layer: f16 ([layer][kv_head][token][head_dim])
-    or, with KV_I8, 8 bits (ribn_amd_kv_cache_create_with). `rope`, or the config's, is how
+    or, with KV_I8 or KV_I4, 8 or 4 bits (ribn_amd_kv_cache_create_with). `rope`, or the config's, is how
     its keys (and the queries that read them) are rotated."""
 
     def __init__(self, ctx, config: AmdQwen3Config, capacity: int, format: int = KV_F16,
@@ -79,7 +80,7 @@ class AmdKvCache:
         return int(self.ctx._lib.ribn_amd_kv_cache_format(self.handle))
 
     def tail(self, layer: int):
-        """Of a KV_I8 cache: device addresses of the f16 block its sequence stands
+        """Of a KV_I8 or KV_I4 cache: device addresses of the f16 block its sequence stands
         in, keys [kv_heads][32][128] and values [kv_heads][128][32], and the
         elements between KV heads."""
         k, v, stride = ctypes.c_void_p(), ctypes.c_void_p(), ctypes.c_size_t()

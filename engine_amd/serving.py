@@ -235,7 +235,7 @@ class AmdServingDispatcher(AmdDispatcher):
         return self
 
     def with_kv_format(self, format: int, rope=None) -> "AmdServingDispatcher":
-        """Caches of later states in `format` (KV_F16 or KV_I8) with `rope`, or the
+        """Caches of later states in `format` (KV_F16, KV_I8 or KV_I4) with `rope`, or the
         decoder config's. No reference counterpart; before the first state."""
         from .qwen3 import kv_options
         options = kv_options(self.decoder.config, format, rope)
@@ -449,7 +449,7 @@ def qwen3_kv_bytes(config, tokens: int) -> int:
 
 
 def kv_bytes(config, tokens: int, format: int) -> int:
-    """Bytes of a sequence's cache of `tokens` in a format (KV_F16 or KV_I8)."""
+    """Bytes of a sequence's cache of `tokens` in a format (KV_F16, KV_I8 or KV_I4)."""
     c = config.to_c()
     return int(_lib.load().ribn_amd_kv_bytes(ctypes.byref(c), tokens, format))
 

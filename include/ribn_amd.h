@@ -643,9 +643,19 @@ ribn_amd_status ribn_amd_rope_execute(ribn_amd_rope *rope, const int32_t *positi
  * (an F16 cache 0.03% to 0.05%). */
 #define RIBN_AMD_KV_F16 0u
 #define RIBN_AMD_KV_I8 1u
+/* RIBN_AMD_KV_I4: 4-bit whole numbers with a scale and a low for each group (0.594
+ * bytes a value), in the same blocks of 32 tokens and with the same f16 block that a sequence
+ * stands in. A group is the 32 tokens of one key dim, or 64 dims (0..63, 64..127) of one
+ * token's value. With x16 as for I8 and lo and hi a group's smallest and largest:
+ * s = (hi - lo) * (1/15) in f32, cut off to f16 (so that no value leaves lo .. hi), code =
+ * clamp(rint((x16 - lo) * (1/s)), 0, 15) in f32 (0 where s is 0), value = code * s + lo, rounded to f16.
+ * What I4 costs: a value is off by 0.29 s rms, 8% to 9% of its group's deviation where the values are
+ * Gaussian, whatever other dims (of keys) or tokens (of values) are like. A block that a sequence is taken
+ * back into is rounded to 4 bits once more when it is whole again. */
+#define RIBN_AMD_KV_I4 4u
 
 typedef struct ribn_amd_kv_options {
-    uint32_t format;                /* RIBN_AMD_KV_F16 or RIBN_AMD_KV_I8 */
+    uint32_t format;                /* RIBN_AMD_KV_F16, RIBN_AMD_KV_I8 or RIBN_AMD_KV_I4 */
     const ribn_amd_rope_spec *rope; /* how q and k of this cache are rotated; NULL: half layout, unscaled, the config's
                                        rope_base. Half layout over the whole head (128) and the config's rope_base
                                        only (InvalidPlan). Copied. */
@@ -659,7 +669,7 @@ typedef struct ribn_amd_kv_options {
  * NULL options, or F16 without rope, is ribn_amd_kv_cache_create. A cache with a
  * rope of its own, and every I8 cache, forms angles in 64 bits (the default
  * one in f32, as the reference does); an I8 cache also normalises and
- * rotates keys in 64 bits.
+ * rotates keys in 64 bits. All that is said of I8 caches here and below holds for I4 ones.
  * I8 caches: tokens are appended at rising positions, or the sequence is taken
  * back to an earlier one and goes on from there (its block's earlier tokens
  * are then what their codes stand for, unless the block is the latest). Attention
@@ -687,7 +697,7 @@ uint64_t ribn_amd_kv_bytes(const ribn_amd_qwen3_config *config, uint32_t tokens,
  * I8 ones. */
 ribn_amd_status ribn_amd_kv_cache_tail(ribn_amd_kv_cache *cache, uint32_t layer, uint16_t **keys, uint16_t **values,
                                        size_t *head_stride);
-/* Puts a context into a cache of either format, on ctx's stream: `tokens` rows of
+/* Puts a context into a cache of any format, on ctx's stream: `tokens` rows of
  * keys (normalised and rotated already) and values, [tokens][kv_heads][128] of
  * `dtype` (RIBN_AMD_F16 or RIBN_AMD_F32), at positions position .. position +
  * tokens - 1 of one layer; len counts each array's elements. An I8 cache

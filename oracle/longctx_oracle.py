@@ -1,7 +1,7 @@
 """Plain 64-bit forms of the long-context operators -- TEST INFRASTRUCTURE ONLY.
 
   rope_turns / rope     rotary positions: layouts, part of the head, scalings
-  Kv8                   one layer's KV cache in 8 bits, appended token by token
+  Kv8, Kv4              one layer's KV cache in 8 (4) bits, appended token by token
   attend                softmax attention over given keys and values
   LongContextQwen3      the oracle decode step (qwen3_oracle) with such a cache,
                         or an f16 one, and any rope
@@ -81,8 +81,41 @@ def quantise(x16):
     return np.clip(np.rint(x / scale), -127, 127), scale
 
 
+GROUP = 64
+
+
+def quantise4(x16, keys):
+    """Codes, scales and lows of blocks [..., 32, 128] of f16 keys (a group: a dim's 32 tokens) or values (64 dims of a
+    token), each of the blocks' shape."""
+    x = np.asarray(x16, np.float16)
+    if keys:
+        lo, hi = x.min(-2, keepdims=True), x.max(-2, keepdims=True)
+    else:
+        g = x.reshape(*x.shape[:-1], HEAD // GROUP, GROUP)
+        lo, hi = (np.repeat(f(-1), GROUP, -1) for f in (g.min, g.max))
+    f32 = lambda v: v.astype(np.float32)  # noqa: E731
+    wide = (f32(hi) - f32(lo)) * np.float32(1.0 / 15.0)
+    s = wide.astype(np.float16)
+    s = np.where(f32(s) > wide, np.nextafter(s, np.float16(0)), s)  # cut off
+    with np.errstate(divide="ignore"):
+        inv = np.where(s > 0, np.float32(1) / f32(s), np.float32(0)).astype(np.float32)
+    codes = np.clip(np.rint((f32(x) - f32(lo)) * inv), 0, 15)
+    return codes.astype(np.float64), *(np.broadcast_to(v, x.shape).astype(np.float64) for v in (s, lo))
+
+
+def values4(codes, s, lo):
+    """What they stand for: f16 values."""
+    return (codes * s + lo).astype(np.float16).astype(np.float64)
+
+
 class Kv8:
     """Keys and values of one layer, [kv_heads] sequences in step."""
+
+    @staticmethod
+    def stored(x16):
+        """What whole blocks [2 (keys, values)][..., 32, 128] are held as."""
+        codes, scale = quantise(x16)
+        return codes * scale
 
     def __init__(self, kv_heads, capacity):
         n = -(-capacity // BLOCK)
@@ -99,8 +132,7 @@ class Kv8:
                 self.tail[:, :, :r] = self.held[:, :, b, :r]
             self.tail[:, :, r] = pair[:, t]
             if r == BLOCK - 1:
-                codes, scale = quantise(self.tail)
-                self.held[:, :, b] = codes * scale
+                self.held[:, :, b] = self.stored(self.tail)
             self.end = position + t + 1
 
     def rows(self, count=None):
@@ -109,6 +141,12 @@ class Kv8:
         x = np.concatenate([self.held[:, :, :whole].reshape(2, self.held.shape[1], -1, HEAD),
                             self.tail[:, :, :self.end % BLOCK].astype(np.float64)], 2)
         return x if count is None else x[:, :, :count]
+
+
+class Kv4(Kv8):
+    @staticmethod
+    def stored(x16):
+        return np.stack([values4(*quantise4(part, i == 0)) for i, part in enumerate(x16)])
 
 
 def attend(q, keys, values):
@@ -123,12 +161,12 @@ def attend(q, keys, values):
 
 
 class LongContextQwen3(OracleQwen3):
-    """The oracle step with attention in 64 bits over an 8-bit (`i8`) or f16 cache and the given rope (turns, gain)."""
+    """The oracle step with attention in 64 bits over a cache in blocks (`i8`: of `kind`) or an f16 one and the given rope (turns, gain)."""
 
-    def __init__(self, cfg, weights, capacity, rope_table, i8=True):
+    def __init__(self, cfg, weights, capacity, rope_table, i8=True, kind=Kv8):
         super().__init__(cfg, weights, capacity)
         self.table, self.i8 = rope_table, i8
-        self.caches = [Kv8(cfg["kv_heads"], capacity) for _ in range(cfg["layers"])]
+        self.caches = [kind(cfg["kv_heads"], capacity) for _ in range(cfg["layers"])]
         self.f16 = [np.zeros((2, cfg["kv_heads"], capacity, HEAD)) for _ in range(cfg["layers"])]
 
     def _attention(self, l, q, k, v, qn, kn, pos):
