@@ -201,6 +201,7 @@ SIGNATURES = {
     "ribn_amd_attention_decode": (_i32, [_vp, ctypes.POINTER(Qwen3Config), _vp, _sz, _u32, _vp, _vp, _vp, _vp,
                                          _vp, _vp, _vp, _sz]),
     "ribn_amd_argmax": (_i32, [_vp, _vp, _sz, _sz, _vp]),
+    "ribn_amd_logprobs": (_i32, [_vp, _vp, _sz, _sz, _sz, _sz, _u32, _vp, _vp, _vp, _vp, _vp, _sz]),
     "ribn_amd_qwen3_decode_create": (_i32, [_vp, ctypes.POINTER(Qwen3Config), _vp, _vp, _vp,
                                             ctypes.POINTER(Qwen3Layer), _u32, _pvp]),
     "ribn_amd_qwen3_decode_destroy": (None, [_vp]),

@@ -42,6 +42,7 @@
 #include "kquant_launch.hpp"
 #include "kv4.hpp"
 #include "kv8.hpp"
+#include "logprob.hpp"
 #include "qwen3_internal.hpp"
 #include "rope.hpp"
 
@@ -1138,6 +1139,59 @@ ribn_amd_status ribn_amd_argmax(ribn_amd_context* ctx, const float* logits, size
         if (e != hipSuccess) return driver(e, "launch argmax");
     }
     return ok();
+}
+
+ribn_amd_status ribn_amd_logprobs(ribn_amd_context* ctx, const void* logits, size_t logits_len, size_t rows, size_t length,
+                                  size_t row_stride, uint32_t dtype, const uint32_t* targets, float* logprobs,
+                                  float* entropy, uint32_t* top_tokens, float* top_logprobs, size_t top) {
+    if (!ctx) return fail(RIBN_AMD_INVALID_ARGUMENT, 0, 0, "null context");
+    if (dtype != RIBN_AMD_F32 && dtype != RIBN_AMD_BF16 && dtype != RIBN_AMD_F16) {
+        return fail(RIBN_AMD_INVALID_ARGUMENT, RIBN_AMD_F16, dtype, "logits are f32, bf16 or f16, not element type %u", dtype);
+    }
+    if (rows == 0 || length == 0) return fail(RIBN_AMD_EMPTY_INPUT, 1, 0, "logits are empty");
+    if (top > RIBN_AMD_MAX_LOGPROB_TOP) {
+        return fail(RIBN_AMD_INVALID_ARGUMENT, RIBN_AMD_MAX_LOGPROB_TOP, top, "at most %u alternatives, not %zu", RIBN_AMD_MAX_LOGPROB_TOP, top);
+    }
+    if ((logprobs != nullptr) != (targets != nullptr)) return fail(RIBN_AMD_INVALID_ARGUMENT, 0, 0, "log probabilities need their tokens, and tokens theirs");
+    if ((top_tokens != nullptr) != (top > 0) || (top_logprobs != nullptr) != (top > 0)) {
+        return fail(RIBN_AMD_INVALID_ARGUMENT, top, 0, "%zu alternatives need arrays of both tokens and log probabilities, none needs none", top);
+    }
+    if (logprobs == nullptr && entropy == nullptr && top == 0) return fail(RIBN_AMD_INVALID_ARGUMENT, 0, 0, "nothing is asked for");
+    const size_t most = (size_t)std::numeric_limits<int>::max();
+    if (length > most || rows > most || row_stride > most) {
+        return fail(RIBN_AMD_SHAPE_OVERFLOW, most, std::max({length, rows, row_stride}), "logits' shape exceeds launch limits");
+    }
+    if (row_stride < length && rows > 1) return fail(RIBN_AMD_INPUT_LENGTH, length, row_stride, "rows of %zu logits lie %zu apart", length, row_stride);
+    const size_t want = (rows - 1) * row_stride + length;
+    if (logits_len < want) return fail(RIBN_AMD_INPUT_LENGTH, want, logits_len, "logits have %zu values, %zu rows need %zu", logits_len, rows, want);
+    if (top > length) return fail(RIBN_AMD_INVALID_ARGUMENT, length, top, "%zu alternatives of %zu tokens", top, length);
+    const struct {
+        const void* ptr;
+        const char* name;
+        uintptr_t align;
+    } ptrs[6] = {{logits, "logits", dtype == RIBN_AMD_F32 ? 4u : 2u}, {targets, "targets", 4}, {logprobs, "logprobs", 4}, {entropy, "entropy", 4},
+                 {top_tokens, "top_tokens", 4}, {top_logprobs, "top_logprobs", 4}};
+    for (int i = 0; i < 6; ++i) {
+        if (i > 0 && ptrs[i].ptr == nullptr) continue;
+        const ribn_amd_status st = check_device_ptr(ctx, ptrs[i].ptr, ptrs[i].name, ptrs[i].align);
+        if (st != RIBN_AMD_OK) return st;
+    }
+    DeviceGuard guard(ctx->device);
+    ribn_amd::LogprobArgs a{};
+    a.logits = logits;
+    a.stride = row_stride;
+    a.length = length;
+    a.rows = rows;
+    a.targets = targets;
+    a.logprobs = logprobs;
+    a.entropy = entropy;
+    a.top_tokens = top_tokens;
+    a.top_logprobs = top_logprobs;
+    a.top = (int)top;
+    static_assert(ribn_amd::kLogprobMaxTop == RIBN_AMD_MAX_LOGPROB_TOP && ribn_amd::kLogitF32 == RIBN_AMD_F32 &&
+                  ribn_amd::kLogitBf16 == RIBN_AMD_BF16 && ribn_amd::kLogitF16 == RIBN_AMD_F16);
+    const hipError_t e = ribn_amd::launch_logprobs(a, (int)dtype, ctx->cu_count, ctx->act_scratch, ribn_amd::gemv_act_scratch_bytes(), ctx->stream);
+    return e == hipSuccess ? ok() : driver(e, "launch logprobs");
 }
 
 ribn_amd_status ribn_amd_qwen3_decode_create(ribn_amd_context* ctx, const ribn_amd_qwen3_config* config,

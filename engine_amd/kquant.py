@@ -480,7 +480,7 @@ class QwenGemvKernel:
 
 
 class AmdQwenOps:
-    """RMSNorm operators of CudaQwen35Ops (model_ops.rs:1714-1824)."""
+    """RMSNorm and selection operators of CudaQwen35Ops (model_ops.rs:1714-1824, 1583-1674), and log probabilities."""
 
     def __init__(self, ctx: AmdContext):
         self.ctx = ctx
@@ -509,6 +509,43 @@ class AmdQwenOps:
         """argmax_into_batch (model_ops.rs:1634-1674): one selection per row of `length`."""
         _check(self._lib.ribn_amd_argmax(self.ctx.handle, _ptr(logits), logits.numel(), length, _ptr(selected)),
                AmdModelKernelError)
+
+    def logprobs_into(self, logits, targets=None, logprobs=None, entropy=None, top_tokens=None, top_logprobs=None):
+        """Log probabilities of given tokens, entropy and likeliest tokens of rows of logits
+        (ribn_amd_logprobs). logits is [rows][tokens] (or one row) of float32, bfloat16 or float16, a row's
+        tokens contiguous; targets [rows] int32, logprobs and entropy [rows] float32, top_tokens int32 and
+        top_logprobs float32 [rows][alternatives], contiguous; what is None is not computed."""
+        from .rope import _dtype, _length
+
+        shape = logits.shape
+        if len(shape) == 1:
+            rows, length, stride = 1, shape[0], shape[0]
+        elif len(shape) == 2:
+            rows, length = shape
+            stride = logits.stride(0) if rows > 1 else length
+        else:
+            raise ValueError(f"logits are [rows][tokens], got {tuple(shape)}")
+        if length > 1 and logits.stride(-1) != 1:
+            raise ValueError("the tokens of a row must be contiguous")
+        dtype = _dtype(logits)
+        if dtype not in (0, 1, 2):
+            raise TypeError(f"logits are float32, bfloat16 or float16, got {logits.dtype}")
+        top = 0 if top_tokens is None else top_tokens.shape[-1]
+        for name, t, kind, want in (("targets", targets, 3, (rows,)), ("logprobs", logprobs, 0, (rows,)), ("entropy", entropy, 0, (rows,)),
+                                    ("top_tokens", top_tokens, 3, (rows, top)), ("top_logprobs", top_logprobs, 0, (rows, top))):
+            if t is None:
+                continue
+            if _dtype(t) != kind:
+                raise TypeError(f"{name} is {'int32' if kind else 'float32'}, got {t.dtype}")
+            if tuple(t.shape) != want and not (len(shape) == 1 and tuple(t.shape) == want[1:]) or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous and {list(want)}, got {tuple(t.shape)}")
+
+        def ptr(t):
+            return None if t is None else t.data_ptr()
+
+        _check(self._lib.ribn_amd_logprobs(self.ctx.handle, logits.data_ptr(), _length(logits), rows, length, stride, dtype, ptr(targets),
+                                           ptr(logprobs), ptr(entropy), ptr(top_tokens) if top else None,
+                                           ptr(top_logprobs) if top else None, top), AmdModelKernelError)
 
 
 def validate_quantized_geometry(kernel_value_type: int, weight_value_type: int, dims, encoded_bytes: int):

@@ -47,7 +47,7 @@ extern "C" {
 #define RIBN_AMD_MAX_BATCH_MEMBERS 64u
 
 /* Activation element types: ribn_amd_gemm_prefill takes the first two,
- * ribn_amd_rope_execute all three, ribn_amd_kv_cache_write / _read F32 and F16. */
+ * ribn_amd_rope_execute and ribn_amd_logprobs all three, ribn_amd_kv_cache_write / _read F32 and F16. */
 #define RIBN_AMD_F32 0u
 #define RIBN_AMD_BF16 1u
 #define RIBN_AMD_F16 2u
@@ -746,6 +746,26 @@ ribn_amd_status ribn_amd_attention_prefill(ribn_amd_context *ctx, const ribn_amd
  * NaN. Its slice results use the context's scratch, in stream order. */
 ribn_amd_status ribn_amd_argmax(ribn_amd_context *ctx, const float *logits, size_t logits_len, size_t length,
                                 uint32_t *selected);
+
+/* Log probabilities, entropy and alternatives from rows of logits; no reference
+ * counterpart (the reference selects greedily and reports none). Row r's logits are the `length` elements of `dtype`
+ * (RIBN_AMD_F32, RIBN_AMD_BF16 or RIBN_AMD_F16) from r * row_stride on; logits_len counts the elements from
+ * the first to the buffer's end. With p = softmax of a row, natural logarithms:
+ *   logprobs[r] = log p(targets[r]) (device u32 array; a token >= length has no probability: -inf),
+ *   entropy[r] = -sum p log p,
+ *   top_tokens[r][i], top_logprobs[r][i], i < top: the i-th likeliest token and its log probability, the lowest
+ *   token first among equals. top is 0..RIBN_AMD_MAX_LOGPROB_TOP and at most length.
+ * Each of logprobs (with targets), entropy and the two top arrays may be NULL, not all of them. A logit of -inf or NaN
+ * has probability 0 (log probability -inf; NaN ranks as -inf); a row of nothing else has log probabilities of
+ * -inf and an entropy of 0. Tokens of +inf share the probability. Logits are aligned to their element.
+ * Sums are formed beside the likeliest token, so that log probabilities near 0 keep their digits as others do (1e-5 of
+ * a result at most, 1e-7 as a rule). A row's last bits may depend on the number of rows. Partial
+ * results use the context's scratch, in stream order. */
+#define RIBN_AMD_MAX_LOGPROB_TOP 32u
+ribn_amd_status ribn_amd_logprobs(ribn_amd_context *ctx, const void *logits, size_t logits_len, size_t rows,
+                                  size_t length, size_t row_stride, uint32_t dtype, const uint32_t *targets,
+                                  float *logprobs, float *entropy, uint32_t *top_tokens, float *top_logprobs,
+                                  size_t top);
 
 /* CudaQwen35Decode::new (decode.rs:412-475) and CudaQwen35BatchDecode::new
  * (1660-1690) in one: validates the plan (geometry of every tensor, non-null
