@@ -756,52 +756,101 @@ struct PrefillI8 : PrefillBlocks {
         return Piece{load_b128(cr, b < whole ? (uint32_t)b * kKv8BlockBytes + (uint32_t)(part * kKv8PartBytes) + 16u * (uint32_t)(idx & 255) : kOOR),
                      __builtin_bit_cast(float, load_b32(sr, b < whole ? 8u * (uint32_t)b + 4u * (uint32_t)part : kOOR))};
     }
-    __device__ __forceinline__ Piece load_keys(int kb, int idx) const { return load(kb, idx, 0); }
-    __device__ __forceinline__ Piece load_values(int kb, int idx) const { return load(kb, idx, 1); }
-    __device__ __forceinline__ void keys(int kb, int idx, const Piece& p, kv8_half8 (&x)[2]) const {
-        x[0] = kv8_values(p.w.x, p.w.y, (_Float16)p.scale);
-        x[1] = kv8_values(p.w.z, p.w.w, (_Float16)p.scale);
-        tail_keys(kb, idx, x);
+    // Pieces tid, tid + 512 / P8, ... of thread tid.
+    template <int P8> __device__ __forceinline__ void load_keys(int kb, int tid, Piece (&p)[P8]) const {
+#pragma unroll
+        for (int r = 0; r < P8; ++r) p[r] = load(kb, tid + 512 / P8 * r, 0);
     }
-    __device__ __forceinline__ void values(int kb, int idx, const Piece& p, kv8_half8 (&x)[2]) const {
-        x[0] = kv8_values(p.w.x, p.w.y, (_Float16)p.scale);
-        x[1] = kv8_values(p.w.z, p.w.w, (_Float16)p.scale);
-        tail_values(kb, idx, x);
+    template <int P8> __device__ __forceinline__ void load_values(int kb, int tid, Piece (&p)[P8]) const {
+#pragma unroll
+        for (int r = 0; r < P8; ++r) p[r] = load(kb, tid + 512 / P8 * r, 1);
+    }
+    // put(piece, its values)
+    template <int P8, class PUT> __device__ __forceinline__ void keys(int kb, int tid, const Piece (&p)[P8], const uint2*, PUT put) const {
+#pragma unroll
+        for (int r = 0; r < P8; ++r) {
+            const int idx = tid + 512 / P8 * r;
+            kv8_half8 x[2] = {kv8_values(p[r].w.x, p[r].w.y, (_Float16)p[r].scale), kv8_values(p[r].w.z, p[r].w.w, (_Float16)p[r].scale)};
+            tail_keys(kb, idx, x);
+            put(idx, x);
+        }
+    }
+    template <int P8, class PUT> __device__ __forceinline__ void values(int kb, int tid, const Piece (&p)[P8], const uint2*, PUT put) const {
+#pragma unroll
+        for (int r = 0; r < P8; ++r) {
+            const int idx = tid + 512 / P8 * r;
+            kv8_half8 x[2] = {kv8_values(p[r].w.x, p[r].w.y, (_Float16)p[r].scale), kv8_values(p[r].w.z, p[r].w.w, (_Float16)p[r].scale)};
+            tail_values(kb, idx, x);
+            put(idx, x);
+        }
     }
 };
 
+// (scales and lows come to LDS a key round ahead: as a piece's operands they are 96 bytes, of which 16 lanes share each)
+constexpr int kPairParams = 2 * kKv4ParamBytes / 8;  // 8-byte pieces of a block pair's
+
 struct PrefillI4 : PrefillBlocks {
     typedef uint2 Piece;
+    Kv4Bias held;  // (the form of two pieces a thread has no registers left for it)
+    template <int P8> __device__ __forceinline__ auto bias() const {
+        if constexpr (P8 == 2) return Kv4Patterns<true>();
+        else return held;
+    }
 
     __device__ __forceinline__ PrefillI4(const PrefillAttnArgs& a, int kvh) : PrefillBlocks(a, kv4_head(a.mem, a.layer, kvh), kv4_tail_offset(a.mem.capacity)) {}
-    __device__ __forceinline__ uint32_t base_of(int kb, int idx) const {
-        const int b = block_of(kb, idx);
-        return b < whole ? (uint32_t)b * kKv4BlockBytes : kOOR4;
-    }
+    // (offsets within a block are added to it)
+    __device__ __forceinline__ uint32_t base_of(int b) const { return b < whole ? (uint32_t)b * kKv4BlockBytes : 0x80000000u; }
     // offset of a piece's eight bytes in its part
     __device__ __forceinline__ uint32_t code_of(int idx) const { return 1024u * (uint32_t)((idx >> 7) & 1) + 16u * (uint32_t)(idx & 63) + 8u * (uint32_t)((idx >> 6) & 1); }
-    __device__ __forceinline__ kv4_u4 params(uint32_t at) const { return __builtin_bit_cast(kv4_u4, load_b128(cr, at)); }
-    __device__ __forceinline__ Piece load_keys(int kb, int idx) const {
-        return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(cr, (int)(base_of(kb, idx) + code_of(idx)), 0, 0));
+    __device__ __forceinline__ Piece load(int kb, int idx, uint32_t part) const {
+        return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(cr, (int)(base_of(block_of(kb, idx)) + part + code_of(idx)), 0, 0));
     }
-    __device__ __forceinline__ Piece load_values(int kb, int idx) const {
-        return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(cr, (int)(base_of(kb, idx) + kKv4Values + code_of(idx)), 0, 0));
+    // Piece i (0 .. kPairParams - 1) of the scales and lows of block pair kb.
+    __device__ __forceinline__ uint2 load_params(int kb, int i) const {
+        const int second = i >= kPairParams / 2;
+        return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(cr, (int)(base_of(2 * kb + second) + kKv4Params + 8u * (uint32_t)(i - second * (kPairParams / 2))), 0, 0));
     }
-    __device__ __forceinline__ void keys(int kb, int idx, const Piece& p, kv8_half8 (&x)[2]) const {
-        const uint32_t at = base_of(kb, idx) + kKv4KeyParams + 16u * (uint32_t)piece_of(idx);
-        x[0] = kv4_values(p.x, params(at), params(at + 2u * kHeadDim));
-        x[1] = kv4_values(p.y, params(at + 16u), params(at + 2u * kHeadDim + 16u));
-        tail_keys(kb, idx, x);
+    // Pieces of thread tid: of two, those that share their scales (the two key tiles, two pairs of value dims).
+    template <int P8> __device__ __forceinline__ static int key_piece(int tid, int r) { return P8 == 1 ? tid : 256 * (tid >> 7) + 128 * r + (tid & 127); }
+    template <int P8> __device__ __forceinline__ static int value_piece(int tid, int r) {
+        return P8 == 1 ? tid : 256 * (tid >> 7) + 128 * ((tid >> 6) & 1) + 64 * r + (tid & 63);
     }
-    __device__ __forceinline__ void values(int kb, int idx, const Piece& p, kv8_half8 (&x)[2]) const {
-        const uint32_t at = base_of(kb, idx) + kKv4ValueParams + (uint32_t)kKv4ValueHalf * (uint32_t)((idx >> 7) & 1) + 2u * (uint32_t)(keys_of(idx) & 31);
-        const kv4_u4 scale = params(at), low = params(at + 2u * kKv8Block);
-        x[0] = kv4_values(p.x, scale, low);
-        x[1] = kv4_values(p.y, scale, low);
-        tail_values(kb, idx, x);
+    template <int P8> __device__ __forceinline__ void load_keys(int kb, int tid, Piece (&p)[P8]) const {
+#pragma unroll
+        for (int r = 0; r < P8; ++r) p[r] = load(kb, key_piece<P8>(tid, r), 0);
     }
-    // (offsets within a block are added to it)
-    static constexpr uint32_t kOOR4 = 0x80000000u;
+    template <int P8> __device__ __forceinline__ void load_values(int kb, int tid, Piece (&p)[P8]) const {
+#pragma unroll
+        for (int r = 0; r < P8; ++r) p[r] = load(kb, value_piece<P8>(tid, r), kKv4Values);
+    }
+    // put(piece, its values)
+    template <int P8, class PUT> __device__ __forceinline__ void keys(int kb, int tid, const Piece (&p)[P8], const uint2* params, PUT put) const {
+        const auto bias = this->template bias<P8>();
+        const int first = key_piece<P8>(tid, 0);
+        const kv4_u4* at = reinterpret_cast<const kv4_u4*>(params) + (first >> 8) * (kKv4ParamBytes / 16) + piece_of(first);
+        const kv4_u4 scale[2] = {at[0], at[1]}, low[2] = {at[kHeadDim / 8], at[kHeadDim / 8 + 1]};
+#pragma unroll
+        for (int r = 0; r < P8; ++r) {
+            const int idx = key_piece<P8>(tid, r);
+            kv8_half8 x[2] = {kv4_values(p[r].x, scale[0], low[0], bias), kv4_values(p[r].y, scale[1], low[1], bias)};
+            tail_keys(kb, idx, x);
+            put(idx, x);
+        }
+    }
+    template <int P8, class PUT> __device__ __forceinline__ void values(int kb, int tid, const Piece (&p)[P8], const uint2* params, PUT put) const {
+        const auto bias = this->template bias<P8>();
+        const int first = value_piece<P8>(tid, 0);
+        const kv4_u4* at = reinterpret_cast<const kv4_u4*>(params) + (first >> 8) * (kKv4ParamBytes / 16) +
+                           (kKv4ValueParams + kKv4ValueHalf * ((first >> 7) & 1)) / 16 + ((first >> 4) & 3);
+        const kv4_u4 scale = at[0], low = at[kKv8Block / 8];
+#pragma unroll
+        for (int r = 0; r < P8; ++r) {
+            const int idx = value_piece<P8>(tid, r);
+            kv8_half8 x[2] = {kv4_values(p[r].x, scale, low, bias), kv4_values(p[r].y, scale, low, bias)};
+            tail_values(kb, idx, x);
+            put(idx, x);
+        }
+    }
 };
 
 // How a cache's keys and values come to a prompt kernel: a piece of a cache of blocks, or 16 bytes of f16.
@@ -852,13 +901,22 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
     constexpr int P8 = 512 / NT;  // pieces of a block pair's keys (values) per thread
     typename Cache::Piece kp[Cache::kBlocks ? P8 : KP], vp[Cache::kBlocks ? P8 : 4];
     const typename Cache::Blocks blocks_of(a, kvh);
+    __shared__ __attribute__((aligned(16))) uint2 params[2][kPairParams];  // (4 bits: of the round staged and the one after)
+    uint2 ahead;  // (a thread's piece of the one after that)
+    auto issue_params = [&](int kb) {
+        if constexpr (CACHE == kCacheI4) {
+            if (tid < kPairParams) ahead = blocks_of.load_params(kb, tid);
+        }
+    };
+    auto stage_params = [&](int slot) {
+        if constexpr (CACHE == kCacheI4) {
+            if (tid < kPairParams) params[slot][tid] = ahead;
+        }
+    };
     auto issue = [&](int kb) {
         if constexpr (Cache::kBlocks) {
-#pragma unroll
-            for (int r = 0; r < P8; ++r) {
-                kp[r] = blocks_of.load_keys(kb, tid + NT * r);
-                vp[r] = blocks_of.load_values(kb, tid + NT * r);
-            }
+            blocks_of.load_keys(kb, tid, kp);
+            blocks_of.load_values(kb, tid, vp);
         } else {
 #pragma unroll
             for (int r = 0; r < KP; ++r) {
@@ -874,17 +932,14 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
     };
     const int wg_first = a.p0 + (int)blockIdx.x * TT * kPrefillTileTokens;  // a token's first position
     if (tid == 0) v_dropped = 0;
-    auto stage = [&](int buf, int kb) {
+    auto stage = [&](int buf, int kb) {  // (buf: the parity of the round, that of its scales too)
         if constexpr (Cache::kBlocks) {
-#pragma unroll
-            for (int r = 0; r < P8; ++r) {
-                const int idx = tid + NT * r;
-                kv8_half8 x[2];
-                blocks_of.keys(kb, idx, kp[r], x);
+            blocks_of.keys(kb, tid, kp, params[buf], [&](int idx, const kv8_half8 (&x)[2]) {
                 const int key = blocks_of.key_of(idx), piece = blocks_of.piece_of(idx);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) *reinterpret_cast<kv8_half8*>(&ks[buf][key][8 * ((piece + i) ^ (key & 15))]) = x[i];
-                blocks_of.values(kb, idx, vp[r], x);
+            });
+            blocks_of.values(kb, tid, vp, params[buf], [&](int idx, const kv8_half8 (&x)[2]) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const uint4 w = __builtin_bit_cast(uint4, x[i]);
@@ -892,7 +947,7 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
                     row[0] = make_uint2(w.x, w.y);
                     row[1] = make_uint2(w.z, w.w);
                 }
-            }
+            });
         } else {
             if (kb * kPfKeys + kPfKeys - 1 > wg_first && drop_nonfinite(vp)) v_dropped = 1;
 #pragma unroll
@@ -918,6 +973,7 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
     const int blocks = last / kPfKeys + 1;
     const int kb0 = Cache::kBlocks ? blocks * (int)blockIdx.z / a.splits : 0;
     const int kb1 = Cache::kBlocks ? blocks * ((int)blockIdx.z + 1) / a.splits : blocks;
+    issue_params(kb0);
     issue(kb0);
 
     // ---- rope angles of the workgroup's tokens, shared by its QPK query
@@ -941,6 +997,8 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
             rot_tab[row * kRotRow + d] = make_float2(rr.c, rr.s);
         }
     }
+    stage_params(0);
+    issue_params(kb0 + 1);
     __syncthreads();
     const int rot_row = (wave / QPK) * kPrefillTileTokens + tl;
 
@@ -1011,10 +1069,12 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
 #pragma unroll
     for (int d = 0; d < 8; ++d) o[d] = pf_float4{0.f, 0.f, 0.f, 0.f};
     stage(0, kb0);
+    stage_params(1);
     __syncthreads();
     for (int kb = kb0; kb < kb1; ++kb) {
         const int buf = (kb - kb0) & 1;
         if (kb + 1 < kb1) issue(kb + 1);
+        if (kb + 2 < kb1) issue_params(kb + 2);
 
         // S^T for the block's four 16-key tiles, issued tile-interleaved:
         // consecutive MFMAs feed different accumulators
@@ -1115,6 +1175,7 @@ __global__ __launch_bounds__(64 * (QPK < 4 ? 4 : QPK)) void attn_prefill_kernel(
         // the next block into the other buffer: every wave finished reading
         // it before the previous barrier
         if (kb + 1 < kb1) stage(buf ^ 1, kb + 1);
+        if (kb + 2 < kb1) stage_params(buf);
         __syncthreads();
     }
 
@@ -1270,12 +1331,21 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
     const typename Cache::Blocks blocks_of(a, kvh);
     constexpr int P8 = 512 / NT;  // pieces of a block pair's keys (values) per thread
     constexpr int KN = Cache::kBlocks ? P8 : KP, VN = Cache::kBlocks ? P8 : 4;
+    __shared__ __attribute__((aligned(16))) uint2 params[2][KS][kPairParams];  // (4 bits: of the round staged and the one after)
+    uint2 ahead;  // (a thread's piece of the one after that)
+    auto issue_params = [&](int kb) {
+        if constexpr (CACHE == kCacheI4) {
+            if (tid < kPairParams) ahead = blocks_of.load_params(kb, tid);
+        }
+    };
+    auto stage_params = [&](int slot) {
+        if constexpr (CACHE == kCacheI4) {
+            if (tid < kPairParams) params[slot][half][tid] = ahead;
+        }
+    };
     auto issue_k = [&](int kb, Piece (&kp)[KN]) {
         if constexpr (Cache::kBlocks) {
-#pragma unroll
-            for (int r = 0; r < P8; ++r) {
-                kp[r] = blocks_of.load_keys(kb, tid + NT * r);
-            }
+            blocks_of.load_keys(kb, tid, kp);
         } else {
 #pragma unroll
             for (int r = 0; r < KP; ++r) {
@@ -1286,15 +1356,11 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
     };
     auto stage_k = [&](int buf, int kb, const Piece (&kp)[KN]) {
         if constexpr (Cache::kBlocks) {
-#pragma unroll
-            for (int r = 0; r < P8; ++r) {
-                const int idx = tid + NT * r;
-                kv8_half8 x[2];
-                blocks_of.keys(kb, idx, kp[r], x);
+            blocks_of.keys(kb, tid, kp, params[buf][half], [&](int idx, const kv8_half8 (&x)[2]) {
                 const int key = blocks_of.key_of(idx), piece = blocks_of.piece_of(idx);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) *reinterpret_cast<kv8_half8*>(&bufs[buf][half].k[key][8 * ((piece + i) ^ (key & 15))]) = x[i];
-            }
+            });
         } else {
 #pragma unroll
             for (int r = 0; r < KP; ++r) {
@@ -1305,10 +1371,7 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
     };
     auto issue_v = [&](int kb, Piece (&vp)[VN]) {
         if constexpr (Cache::kBlocks) {
-#pragma unroll
-            for (int r = 0; r < P8; ++r) {
-                vp[r] = blocks_of.load_values(kb, tid + NT * r);
-            }
+            blocks_of.load_values(kb, tid, vp);
         } else {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -1321,11 +1384,7 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
     if (threadIdx.x == 0) v_dropped = 0;
     auto stage_v = [&](int buf, int kb, Piece (&vp)[VN]) {
         if constexpr (Cache::kBlocks) {
-#pragma unroll
-            for (int r = 0; r < P8; ++r) {
-                const int idx = tid + NT * r;
-                kv8_half8 x[2];
-                blocks_of.values(kb, idx, vp[r], x);
+            blocks_of.values(kb, tid, vp, params[buf][half], [&](int idx, const kv8_half8 (&x)[2]) {
                 const int k0 = blocks_of.keys_of(idx);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
@@ -1334,7 +1393,7 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
                     *reinterpret_cast<uint2*>(row + vt_pos(k0)) = make_uint2(w.x, w.y);
                     *reinterpret_cast<uint2*>(row + vt_pos(k0 + 4)) = make_uint2(w.z, w.w);
                 }
-            }
+            });
         } else {
             if (v_unit) {
                 if (kb * kPfKeys + kPfKeys - 1 > wg_first && drop_nonfinite(vp)) v_dropped = 1;
@@ -1358,6 +1417,7 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
     // K/V blocks and the query rows of the first pass (thread: 8 dims of rows
     // tid/16 + 32 i)
     Piece kp0[KN], vp0[VN];
+    issue_params(half);
     issue_k(half, kp0);
     issue_v(half, vp0);
     const int c = threadIdx.x & 15;
@@ -1390,6 +1450,8 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
         const Rot rr = cache_rot<TABLE>(a.mem.rope, lane, a.p0 + tile * TT * TOK + r, freq);
         rot_tab[r * kRotRow + lane] = make_float2(rr.c, rr.s);
     }
+    stage_params(0);
+    issue_params(half + KS);
     __syncthreads();
 
     // ---- query pieces: row (token tile, head, token of the tile), RMSNorm
@@ -1481,6 +1543,7 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
     const int rounds = (last / kPfKeys + KS) / KS;
     stage_k(0, half, kp0);
     stage_v(0, half, vp0);
+    stage_params(1);
     __syncthreads();
     for (int round = 0; round < rounds; ++round) {
         const int kb = KS * round + half;
@@ -1489,6 +1552,7 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
         // probabilities and the outputs (each held alone: registers)
         Piece kp[KN], vp[VN];
         if (round + 1 < rounds) issue_k(kb + KS, kp);
+        if (round + 2 < rounds) issue_params(kb + 2 * KS);
 
         // S^T for the block's two 32-key tiles, interleaved: consecutive MFMAs
         // feed different accumulators
@@ -1602,6 +1666,7 @@ __global__ __launch_bounds__(512, 2) void attn_prefill_wide_kernel(PrefillAttnAr
         }
         __builtin_amdgcn_sched_group_barrier(kSchedMfma, 8, 0);
         if (round + 1 < rounds) stage_v(buf ^ 1, kb + KS, vp);
+        if (round + 2 < rounds) stage_params(buf);
         __syncthreads();
     }
 

@@ -1,8 +1,8 @@
 // The KV cache in 4 bits: layout, quantisation and launchers (kv4_kernels.hip).
 //
 // A (layer, KV head) region of a cache holds
-//   blocks [ceil(capacity / 32)] of 4864 bytes, one per 32 tokens: 2048 of key codes, the
-//          keys' 128 scales and 128 lows (f16), 2048 of value codes, the values' scales and
+//   blocks [ceil(capacity / 32)] of 4864 bytes, one per 32 tokens: 2048 of key codes, 2048 of
+//          value codes, the keys' 128 scales and 128 lows (f16), the values' scales and
 //          lows [2 halves of the head][scale, low][32 tokens] (f16)
 //   tail   the f16 block the sequence stands in: keys [32][128], values [128][32]
 //   end    int32: one past the last position appended
@@ -31,11 +31,12 @@ namespace ribn_amd {
 
 constexpr int kKv4Group = 64;                                    // dims of a value group
 constexpr int kKv4CodeBytes = kKv8Block * kHeadDim / 2;          // a block's key (value) codes
-constexpr int kKv4KeyParams = kKv4CodeBytes;                     // byte offsets in a block: the keys' scales, then lows
-constexpr int kKv4Values = kKv4KeyParams + 2 * kHeadDim * 2;     // value codes
-constexpr int kKv4ValueParams = kKv4Values + kKv4CodeBytes;      // the values' scales and lows
+constexpr int kKv4Values = kKv4CodeBytes;                        // byte offsets in a block: value codes
+constexpr int kKv4Params = 2 * kKv4CodeBytes;                    // the keys' scales, then lows
+constexpr int kKv4ValueParams = 2 * kHeadDim * 2;                // and from there on the values'
 constexpr int kKv4ValueHalf = 2 * kKv8Block * 2;                 // bytes of one half's
-constexpr int kKv4BlockBytes = kKv4ValueParams + kHeadDim / kKv4Group * kKv4ValueHalf;
+constexpr int kKv4ParamBytes = kKv4ValueParams + kHeadDim / kKv4Group * kKv4ValueHalf;
+constexpr int kKv4BlockBytes = kKv4Params + kKv4ParamBytes;
 static_assert(kKv4BlockBytes == 4864);
 
 __host__ __device__ inline size_t kv4_tail_offset(int capacity) { return kv8_blocks(capacity) * kKv4BlockBytes; }

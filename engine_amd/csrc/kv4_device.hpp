@@ -19,13 +19,28 @@ __device__ __forceinline__ KvHead kv4_head(const AttnMember& m, int layer, int k
     return h;
 }
 
-// Eight codes as the values they stand for, with a scale and a low each: a nibble under 0x64 is 1024 + code
-// (exact), less 1024, then one fused multiply-add in f16.
-__device__ __forceinline__ kv8_half8 kv4_values(uint32_t w, kv4_u4 scale, kv4_u4 low) {
+// Eight codes as the values they stand for, with a scale and a low each: a nibble under 0x64 is 1024 + code, one
+// four bits up under 0x54 is 64 + code (exact), less that, then one fused multiply-add in f16. Thirteen instructions:
+// the two patterns are kept in vector registers (hidden from the compiler, which would take an and and an or for each pair).
+// HERE: formed where it is used, two registers less across a loop that has none left.
+template <bool HERE = false> struct Kv4Patterns {
+    uint32_t low = 0x64006400u, high = 0x54005400u;
+    __device__ __forceinline__ Kv4Patterns() {
+        if constexpr (HERE) asm volatile("" : "+v"(low), "+v"(high));
+        else asm("" : "+v"(low), "+v"(high));
+    }
+};
+using Kv4Bias = Kv4Patterns<>;
+
+template <bool HERE>
+__device__ __forceinline__ kv8_half8 kv4_values(uint32_t w, kv4_u4 scale, kv4_u4 low, const Kv4Patterns<HERE>& bias) {
+    const uint32_t u = w >> 8;
+    const uint32_t biased[4] = {(w & 0x000f000fu) | bias.low, (w & 0x00f000f0u) | bias.high, (u & 0x000f000fu) | bias.low, (u & 0x00f000f0u) | bias.high};
     kv8_half8 x;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const kv8_half2 c = __builtin_bit_cast(kv8_half2, ((w >> (4 * j)) & 0x000f000fu) | 0x64006400u) - kv8_half2{(_Float16)1024.0f, (_Float16)1024.0f};
+        const _Float16 one = (j & 1) ? (_Float16)64.0f : (_Float16)1024.0f;
+        const kv8_half2 c = __builtin_bit_cast(kv8_half2, biased[j]) - kv8_half2{one, one};
         const uint32_t sw = scale[j], lw = low[j];
         const kv8_half2 v = __builtin_elementwise_fma(c, __builtin_bit_cast(kv8_half2, sw), __builtin_bit_cast(kv8_half2, lw));
         x[2 * j] = v[0];
@@ -34,14 +49,14 @@ __device__ __forceinline__ kv8_half8 kv4_values(uint32_t w, kv4_u4 scale, kv4_u4
     return x;
 }
 
-// A group's scale, and its reciprocal in f32.
+// A group's scale, and its reciprocal in f32 (1 for a scale of 0: a group that narrow, under 15 * 2^-24, gets codes of 0 by it).
 struct Kv4Scale {
     _Float16 s;
     float inv;
     __device__ __forceinline__ Kv4Scale(_Float16 lo, _Float16 hi) {
         const float wide = ((float)hi - (float)lo) * (1.0f / 15.0f);
         s = __builtin_bit_cast(kv8_half2, __builtin_amdgcn_cvt_pkrtz(wide, 0.0f))[0];
-        inv = s > (_Float16)0.0f ? 1.0f / (float)s : 0.0f;
+        inv = 1.0f / (s > (_Float16)0.0f ? (float)s : 1.0f);
     }
 };
 

@@ -11,9 +11,10 @@ namespace ribn_amd {
 namespace {
 
 struct Kv4Format {
-    // Registers of a block's keys: codes 2, scales 4, lows 4 (dims 16 g + 8 h of half i at 2 i + h); of its
-    // values: codes 2, scales 2, lows 2 (half of the head), and room for the tail's.
-    static constexpr int kKeyRegs = 10, kValueRegs = 8;
+    // Registers of a block: of its keys two of codes, and the block's scales and lows as they lie, 16 bytes a
+    // lane; of its values two of codes (and the tail all of them).
+    static constexpr int kKeyRegs = 8, kValueRegs = 8;
+    static constexpr bool kFused = true;
     static constexpr int kQuantiseBarriers = 2;
     struct Scratch {
         kv8_half2 key_lo[4][64], key_hi[4][64];  // of eight rows each; [0] then of all: low, and
@@ -29,11 +30,12 @@ struct Kv4Format {
         const int tid = append_tid(), lane = tid & 63, u = (tid >> 6) & 3, g = lane >> 4, m = lane & 15;
         const uint8_t* block = h.codes + (size_t)b * kKv4BlockBytes;
         const int at = 1024 * (u >> 1) + 16 * lane + 8 * (u & 1);
+        const Kv4Bias bias;
         if (tid < 256) {
             const uint2 w = *reinterpret_cast<const uint2*>(block + at);
             const int row = kv8_key_row(u >> 1, m), dim = 64 * (u & 1) + 16 * g;
-            const kv4_u4* p = reinterpret_cast<const kv4_u4*>(block + kKv4KeyParams + 2 * dim);
-            const kv8_half8 x0 = kv4_values(w.x, p[0], p[16]), x1 = kv4_values(w.y, p[1], p[17]);
+            const kv4_u4* p = reinterpret_cast<const kv4_u4*>(block + kKv4Params + 2 * dim);
+            const kv8_half8 x0 = kv4_values(w.x, p[0], p[16], bias), x1 = kv4_values(w.y, p[1], p[17], bias);
             if (row < count) {
                 kv8_half8* k = reinterpret_cast<kv8_half8*>(&st.k[row][dim]);
                 k[0] = x0;
@@ -41,8 +43,8 @@ struct Kv4Format {
             }
         } else {
             const uint2 w = *reinterpret_cast<const uint2*>(block + kKv4Values + at);
-            const kv4_u4* p = reinterpret_cast<const kv4_u4*>(block + kKv4ValueParams + (u >> 1) * kKv4ValueHalf + 16 * g);
-            const kv8_half8 x0 = kv4_values(w.x, p[0], p[4]), x1 = kv4_values(w.y, p[0], p[4]);
+            const kv4_u4* p = reinterpret_cast<const kv4_u4*>(block + kKv4Params + kKv4ValueParams + (u >> 1) * kKv4ValueHalf + 16 * g);
+            const kv8_half8 x0 = kv4_values(w.x, p[0], p[4], bias), x1 = kv4_values(w.y, p[0], p[4], bias);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (8 * g + j < count) *reinterpret_cast<kv8_half2*>(&st.v[8 * g + j][32 * u + 2 * m]) = kv8_half2{x0[j], x1[j]};
@@ -79,7 +81,7 @@ struct Kv4Format {
                 const Kv4Scale s(both[0], -both[1]);
                 st.x.value_lo[half][token] = both[0];
                 st.x.value_inv[half][token] = s.inv;
-                _Float16* p = reinterpret_cast<_Float16*>(block + kKv4ValueParams + half * kKv4ValueHalf);
+                _Float16* p = reinterpret_cast<_Float16*>(block + kKv4Params + kKv4ValueParams + half * kKv4ValueHalf);
                 p[token] = s.s;
                 p[kKv8Block + token] = both[0];
             }
@@ -95,7 +97,7 @@ struct Kv4Format {
             const Kv4Scale a(lo[0], hi[0]), c(lo[1], hi[1]);
             st.x.key_lo[0][lane] = lo;
             st.x.key_inv[lane] = make_float2(a.inv, c.inv);
-            kv8_half2* p = reinterpret_cast<kv8_half2*>(block + kKv4KeyParams);
+            kv8_half2* p = reinterpret_cast<kv8_half2*>(block + kKv4Params);
             p[lane] = kv8_half2{a.s, c.s};
             p[64 + lane] = lo;
         }
@@ -122,84 +124,104 @@ struct Kv4Format {
         *reinterpret_cast<uint2*>(block + (keys ? 0 : kKv4Values) + 1024 * (u >> 1) + 16 * lane + 8 * (u & 1)) = make_uint2(w[0], w[1]);
     }
 
-    // A block's codes, two 16-byte loads a lane of keys and of values, and their scales and lows.
+    // A block's scales and lows, put here by the wave that holds the block: as operands they are 16 bytes each
+    // that 16 lanes share, 48 registers a lane if they were loaded so.
+    using Constants = Kv4Bias;
+    struct WaveScratch {
+        kv8_u4 params[64];
+    };
+
+    // A block's codes, two 16-byte loads a lane of keys and of values, and its scales and lows.
     struct Source {
         __amdgpu_buffer_rsrc_t r;
         __device__ __forceinline__ Source(const KvHead& h, int capacity) : r(make_rsrc(h.codes, (uint32_t)kv4_tail_offset(capacity))) {}
         __device__ __forceinline__ kv8_u4 load(uint32_t at) const { return __builtin_bit_cast(kv8_u4, load_b128(r, at)); }
         __device__ __forceinline__ void keys(int b, int end, int lane, kv8_u4 (&w)[kKeyRegs], float&) const {
             const uint32_t base = b < end ? (uint32_t)b * kKv4BlockBytes : kCacheOOR;
+            w[2] = load(lane < kKv4ParamBytes / 16 ? base + kKv4Params + 16u * (uint32_t)lane : kCacheOOR);
 #pragma unroll
             for (int t = 0; t < 2; ++t) w[t] = load(base + 1024u * t + 16u * (uint32_t)lane);
-            const uint32_t p = base + kKv4KeyParams + 32u * (uint32_t)(lane >> 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w[2 + i] = load(p + 128u * (i >> 1) + 16u * (i & 1));
-                w[6 + i] = load(p + 2u * kHeadDim + 128u * (i >> 1) + 16u * (i & 1));
-            }
         }
         __device__ __forceinline__ void values(int b, int end, int lane, kv8_u4 (&w)[kValueRegs], float&) const {
             const uint32_t base = b < end ? (uint32_t)b * kKv4BlockBytes : kCacheOOR;
-            const uint32_t p = base + kKv4ValueParams + 16u * (uint32_t)(lane >> 4);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                w[i] = load(base + kKv4Values + 1024u * i + 16u * (uint32_t)lane);
-                w[2 + i] = load(p + (uint32_t)kKv4ValueHalf * i);
-                w[4 + i] = load(p + (uint32_t)kKv4ValueHalf * i + 2u * kKv8Block);
-            }
+            for (int h = 0; h < 2; ++h) w[h] = load(base + kKv4Values + 1024u * h + 16u * (uint32_t)lane);
         }
     };
 
-    __device__ __forceinline__ static void scores(const kv8_u4 (&kq)[kKeyRegs], const kv8_half8 (&qb)[4], kv8_float4 (&s)[2]) {
+    // (a wave's LDS accesses come in its order: the block before has read its own)
+    __device__ __forceinline__ static void begin(const kv8_u4 (&kq)[kKeyRegs], WaveScratch& ws, int lane) {
+        lds_order();
+        ws.params[lane] = kq[2];
+        lds_order();
+    }
+    __device__ __forceinline__ static void scores(const kv8_u4 (&kq)[kKeyRegs], const WaveScratch& ws, const Kv4Bias& bias, int g, const kv8_half8 (&qb)[4], kv8_float4 (&s)[2]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4; ++i) {  // step i: dims 64 (i >> 1) + 16 g + 8 (i & 1)
+            const kv8_u4 scale = ws.params[8 * (i >> 1) + 2 * g + (i & 1)], low = ws.params[16 + 8 * (i >> 1) + 2 * g + (i & 1)];
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv4_values(kq[t][i], kq[2 + i], kq[6 + i]), qb[i], s[t], 0, 0, 0);
+            for (int t = 0; t < 2; ++t) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv4_values(kq[t][i], scale, low, bias), qb[i], s[t], 0, 0, 0);
         }
     }
     __device__ __forceinline__ static float scaled(float fac, float) { return fac; }
-    __device__ __forceinline__ static void outputs(const kv8_u4 (&vq)[kValueRegs], float, kv8_half8 pb, kv8_float4 (&o)[8]) {
+    __device__ __forceinline__ static void outputs(const kv8_u4 (&vq)[kValueRegs], float, const WaveScratch& ws, const Kv4Bias& bias, int g, kv8_half8 pb, kv8_float4 (&o)[8]) {
 #pragma unroll
-        for (int d = 0; d < 8; ++d)
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv4_values(vq[d >> 2][d & 3], vq[2 + (d >> 2)], vq[4 + (d >> 2)]), pb, o[d], 0, 0, 0);
+        for (int h = 0; h < 2; ++h) {
+            const kv8_u4 scale = ws.params[32 + 8 * h + g], low = ws.params[36 + 8 * h + g];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) o[4 * h + d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv4_values(vq[h][d], scale, low, bias), pb, o[4 * h + d], 0, 0, 0);
+        }
     }
 
     // The block in the tail's registers (TailBlock): what the codes of block b stand for.
     __device__ __forceinline__ static void load_tail(const KvHead& h, int b, int lane, kv8_u4 (&k)[kKeyRegs], kv8_u4 (&v)[kValueRegs]) {
+        const Kv4Bias bias;
         const uint8_t* block = h.codes + (size_t)b * kKv4BlockBytes;
-        const kv8_u4* kp = reinterpret_cast<const kv8_u4*>(block + kKv4KeyParams) + 2 * (lane >> 4);
-        const kv8_u4* vp = reinterpret_cast<const kv8_u4*>(block + kKv4ValueParams) + (lane >> 4);
+        const kv8_u4* kp = reinterpret_cast<const kv8_u4*>(block + kKv4Params) + 2 * (lane >> 4);
+        const kv8_u4* vp = reinterpret_cast<const kv8_u4*>(block + kKv4Params + kKv4ValueParams) + (lane >> 4);
         const kv8_u4* kc = reinterpret_cast<const kv8_u4*>(block) + lane;
         const kv8_u4* vc = reinterpret_cast<const kv8_u4*>(block + kKv4Values) + lane;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int s = i & 3;  // key step 4 t + s: dims 64 (s >> 1) + 16 g + 8 (s & 1)
-            k[i] = __builtin_bit_cast(kv8_u4, kv4_values(kc[64 * (i >> 2)][s], kp[8 * (s >> 1) + (s & 1)], kp[16 + 8 * (s >> 1) + (s & 1)]));
-            v[i] = __builtin_bit_cast(kv8_u4, kv4_values(vc[64 * (i >> 2)][s], vp[8 * (i >> 2)], vp[8 * (i >> 2) + 4]));
+            k[i] = __builtin_bit_cast(kv8_u4, kv4_values(kc[64 * (i >> 2)][s], kp[8 * (s >> 1) + (s & 1)], kp[16 + 8 * (s >> 1) + (s & 1)], bias));
+            v[i] = __builtin_bit_cast(kv8_u4, kv4_values(vc[64 * (i >> 2)][s], vp[8 * (i >> 2)], vp[8 * (i >> 2) + 4], bias));
         }
     }
 
-    // Codes, scales and lows of the whole block; its values become what these stand for.
-    __device__ __forceinline__ static void quantise_tail(const KvHead& h, int b, int lane, kv8_u4 (&k)[kKeyRegs], kv8_u4 (&v)[kValueRegs]) {
+    // Codes, scales and lows of the whole block; its values become what these stand for. By way of LDS, a piece
+    // at a time: a step in 32 comes here, and unrolled over the registers that hold the block it set the kernel's
+    // count (160, and scratch with a bound of 128).
+    struct Parked {
+        kv8_u4 x[8][64];
+    };
+    __device__ __forceinline__ static void quantise_tail(const KvHead& h, int b, int lane, kv8_u4 (&k)[kKeyRegs], kv8_u4 (&v)[kValueRegs], Parked (&parked)[2]) {
+        const Kv4Bias bias;
         uint8_t* const block = h.codes + (size_t)b * kKv4BlockBytes;
         auto pair = [](uint32_t w) { return __builtin_bit_cast(kv8_half2, w); };
         auto word = [](kv8_half2 x) { return __builtin_bit_cast(uint32_t, x); };
-        kv8_u4* const kp = reinterpret_cast<kv8_u4*>(block + kKv4KeyParams) + 2 * (lane >> 4);
-        kv8_u4 kw[2];  // code words, by tile
+        lds_order();
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
+        for (int i = 0; i < 8; ++i) {
+            parked[0].x[i][lane] = k[i];
+            parked[1].x[i][lane] = v[i];
+        }
+        lds_order();
+        kv8_u4* const kp = reinterpret_cast<kv8_u4*>(block + kKv4Params) + 2 * (lane >> 4);
+#pragma unroll 1
+        for (int s = 0; s < 4; ++s) {  // eight dims, of the two tiles
+            const kv8_u4 x0 = parked[0].x[s][lane], x1 = parked[0].x[4 + s][lane];
             kv8_u4 scale, low;
             uint32_t w[2] = {0, 0};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {  // a pair of dims, over the two tiles and the row's 16 keys
-                const uint32_t x0 = k[s][j], x1 = k[4 + s][j];
-                const kv8_half2 lo = kv4_row_min(kv4_min(pair(x0), pair(x1))), hi = -kv4_row_min(kv4_min(-pair(x0), -pair(x1)));
+                const uint32_t a0 = x0[j], a1 = x1[j];
+                const kv8_half2 lo = kv4_row_min(kv4_min(pair(a0), pair(a1))), hi = -kv4_row_min(kv4_min(-pair(a0), -pair(a1)));
                 const Kv4Scale a(lo[0], hi[0]), c(lo[1], hi[1]);
                 scale[j] = word(kv8_half2{a.s, c.s});
                 low[j] = word(lo);
-                w[0] |= kv4_code(pair(x0)[0], lo[0], a.inv) << kv4_shift(2 * j) | kv4_code(pair(x0)[1], lo[1], c.inv) << kv4_shift(2 * j + 1);
-                w[1] |= kv4_code(pair(x1)[0], lo[0], a.inv) << kv4_shift(2 * j) | kv4_code(pair(x1)[1], lo[1], c.inv) << kv4_shift(2 * j + 1);
+                w[0] |= kv4_code(pair(a0)[0], lo[0], a.inv) << kv4_shift(2 * j) | kv4_code(pair(a0)[1], lo[1], c.inv) << kv4_shift(2 * j + 1);
+                w[1] |= kv4_code(pair(a1)[0], lo[0], a.inv) << kv4_shift(2 * j) | kv4_code(pair(a1)[1], lo[1], c.inv) << kv4_shift(2 * j + 1);
             }
             if ((lane & 15) == 0) {
                 kp[8 * (s >> 1) + (s & 1)] = scale;
@@ -207,25 +229,24 @@ struct Kv4Format {
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                kw[t][s] = w[t];
-                k[4 * t + s] = __builtin_bit_cast(kv8_u4, kv4_values(w[t], scale, low));
+                reinterpret_cast<uint32_t*>(block)[256 * t + 4 * lane + s] = w[t];
+                parked[0].x[4 * t + s][lane] = __builtin_bit_cast(kv8_u4, kv4_values(w[t], scale, low, bias));
             }
         }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) reinterpret_cast<kv8_u4*>(block)[64 * t + lane] = kw[t];
-        kv8_u4* const vp = reinterpret_cast<kv8_u4*>(block + kKv4ValueParams) + (lane >> 4);
-#pragma unroll
+        kv8_u4* const vp = reinterpret_cast<kv8_u4*>(block + kKv4Params + kKv4ValueParams) + (lane >> 4);
+#pragma unroll 1
         for (int half = 0; half < 2; ++half) {
-            kv8_u4 scale, low;
-            kv8_u4 w = kv8_u4{0, 0, 0, 0};
+            kv8_u4 x[4], scale, low, w = kv8_u4{0, 0, 0, 0};
+#pragma unroll
+            for (int d = 0; d < 4; ++d) x[d] = parked[1].x[4 * half + d][lane];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {  // a pair of keys, over four dims and the row's 16 lanes
                 kv8_half2 lo, hi;
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
-                    const uint32_t x = v[4 * half + d][j];
-                    lo = d == 0 ? pair(x) : kv4_min(lo, pair(x));
-                    hi = d == 0 ? -pair(x) : kv4_min(hi, -pair(x));
+                    const uint32_t a = x[d][j];
+                    lo = d == 0 ? pair(a) : kv4_min(lo, pair(a));
+                    hi = d == 0 ? -pair(a) : kv4_min(hi, -pair(a));
                 }
                 lo = kv4_row_min(lo);
                 hi = -kv4_row_min(hi);
@@ -234,8 +255,8 @@ struct Kv4Format {
                 low[j] = word(lo);
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
-                    const uint32_t x = v[4 * half + d][j];
-                    w[d] |= kv4_code(pair(x)[0], lo[0], a.inv) << kv4_shift(2 * j) | kv4_code(pair(x)[1], lo[1], c.inv) << kv4_shift(2 * j + 1);
+                    const uint32_t y = x[d][j];
+                    w[d] |= kv4_code(pair(y)[0], lo[0], a.inv) << kv4_shift(2 * j) | kv4_code(pair(y)[1], lo[1], c.inv) << kv4_shift(2 * j + 1);
                 }
             }
             if ((lane & 15) == 0) {
@@ -244,7 +265,13 @@ struct Kv4Format {
             }
             reinterpret_cast<kv8_u4*>(block + kKv4Values)[64 * half + lane] = w;
 #pragma unroll
-            for (int d = 0; d < 4; ++d) v[4 * half + d] = __builtin_bit_cast(kv8_u4, kv4_values(w[d], scale, low));
+            for (int d = 0; d < 4; ++d) parked[1].x[4 * half + d][lane] = __builtin_bit_cast(kv8_u4, kv4_values(w[d], scale, low, bias));
+        }
+        lds_order();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            k[i] = parked[0].x[i][lane];
+            v[i] = parked[1].x[i][lane];
         }
     }
 };

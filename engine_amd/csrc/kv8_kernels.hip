@@ -12,6 +12,7 @@ namespace ribn_amd {
 namespace {
 
 struct Kv8Format {
+    static constexpr bool kFused = false;
     static constexpr int kKeyRegs = 8, kValueRegs = 8;  // (codes take the first four)
     static constexpr int kQuantiseBarriers = 1;
     struct Scratch {
@@ -79,21 +80,25 @@ struct Kv8Format {
         __device__ __forceinline__ Source(const KvHead& h, int capacity)
             : cr(make_rsrc(h.codes, (uint32_t)kv8_tail_offset(capacity))),
               sr(make_rsrc(h.scales, (uint32_t)(kv8_blocks(capacity) * sizeof(float2)))) {}
-        __device__ __forceinline__ void issue(int b, int end, int part, int lane, kv8_u4 (&w)[8], float& scale) const {
+        __device__ __forceinline__ void part(int b, int end, int part, int lane, kv8_u4 (&w)[8], float& scale) const {
             const uint32_t at = b < end ? (uint32_t)b * kKv8BlockBytes + (uint32_t)part + 16u * (uint32_t)lane : kCacheOOR;
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(kv8_u4, load_b128(cr, at + 1024u * i));
             scale = __builtin_bit_cast(float, load_b32(sr, b < end ? 8u * (uint32_t)b + (part ? 4u : 0u) : kCacheOOR));
         }
-        __device__ __forceinline__ void keys(int b, int end, int lane, kv8_u4 (&w)[8], float& scale) const { issue(b, end, 0, lane, w, scale); }
+        __device__ __forceinline__ void keys(int b, int end, int lane, kv8_u4 (&w)[8], float& scale) const { part(b, end, 0, lane, w, scale); }
         __device__ __forceinline__ void values(int b, int end, int lane, kv8_u4 (&w)[8], float& scale) const {
-            issue(b, end, kKv8PartBytes, lane, w, scale);
+            part(b, end, kKv8PartBytes, lane, w, scale);
         }
     };
 
+    struct Constants {};
+    struct Parked {};
+    struct WaveScratch {};
+    __device__ __forceinline__ static void begin(const kv8_u4 (&)[8], WaveScratch&, int) {}
     // Codes enter the scores as whole numbers, the block's key scale being applied to
     // the f32 score; values are scaled as f16 (both exact).
-    __device__ __forceinline__ static void scores(const kv8_u4 (&kq)[8], const kv8_half8 (&qb)[4], kv8_float4 (&s)[2]) {
+    __device__ __forceinline__ static void scores(const kv8_u4 (&kq)[8], const WaveScratch&, const Constants&, int, const kv8_half8 (&qb)[4], kv8_float4 (&s)[2]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -105,7 +110,7 @@ struct Kv8Format {
         }
     }
     __device__ __forceinline__ static float scaled(float fac, float scale) { return fac * scale; }
-    __device__ __forceinline__ static void outputs(const kv8_u4 (&vq)[8], float scale, kv8_half8 pb, kv8_float4 (&o)[8]) {
+    __device__ __forceinline__ static void outputs(const kv8_u4 (&vq)[8], float scale, const WaveScratch&, const Constants&, int, kv8_half8 pb, kv8_float4 (&o)[8]) {
         const _Float16 value_scale = (_Float16)scale;
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
@@ -150,7 +155,7 @@ struct Kv8Format {
         }
     }
     // Codes and scales of the whole block; its values become what these stand for.
-    __device__ __forceinline__ static void quantise_tail(const KvHead& h, int b, int lane, kv8_u4 (&k)[8], kv8_u4 (&v)[8]) {
+    __device__ __forceinline__ static void quantise_tail(const KvHead& h, int b, int lane, kv8_u4 (&k)[8], kv8_u4 (&v)[8], Parked (&)[2]) {
         kv8_u4* c = reinterpret_cast<kv8_u4*>(h.codes + (size_t)b * kKv8BlockBytes) + lane;
         float2 sc;
         quantise_part(k, c, sc.x);

@@ -6,8 +6,12 @@
 //   head(member, layer, kvh)            a (layer, KV head) region's parts
 //   stage_codes / quantise              a block's codes to f16 rows in LDS, and back
 //   Source                              a head's codes on their way to registers
+//   Constants                           what the kernel keeps in registers
+//   WaveScratch, begin                  LDS of a wave, and what it puts there of a block
 //   scores, scaled, outputs             the matrix products over a block in registers
-//   load_tail / quantise_tail           a block in registers: what its codes stand for, and its codes
+//   kFused                              whether a score's scale and the softmax's reference go into one multiply-add (8-bit
+//                                       caches keep two roundings)
+//   load_tail / quantise_tail           a block in registers: what its codes stand for, and its codes (Parked: LDS for that)
 #pragma once
 
 #include <float.h>
@@ -303,7 +307,7 @@ __device__ __forceinline__ void read_rows(const KvMoveArgs& a) {
 // Split as attn_decode_kernel's: grid (chunk, KV head, member), a chunk one
 // contiguous run of whole blocks; its waves take the blocks in turn. A block's codes lie
 // in the order of the matrix operands, 16 bytes a lane, each load contiguous over
-// the wave, one block in flight a wave, up to three workgroups a CU.
+// the wave, one block in flight a wave.
 //
 // The chunks are merged by a launch of its own. The last workgroup of a row to arrive could
 // do it, but handing partials over between XCDs costs as much (kv8_kernels.hip has the figures).
@@ -321,6 +325,7 @@ __device__ __forceinline__ void read_rows(const KvMoveArgs& a) {
 // The block the sequence stands in is the last wave's: it has the tail's rows in
 // the operands' order, puts the new token's row in from LDS, and, when the block is whole,
 // finds its scales and writes its codes from there, going on with what these stand for.
+
 
 constexpr int kAttnWaves = 4;
 constexpr int kAttnThreads = 64 * kAttnWaves;
@@ -342,6 +347,12 @@ __device__ __forceinline__ int cache_chunk_tokens(int tokens, int chunks, int mi
 // The value of lane ^ 8.
 __device__ __forceinline__ float other_half(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x128, 0xf, 0xf, false));
+}
+
+// LDS written by some lanes of a wave and read by others of it: in order as issued.
+__device__ __forceinline__ void lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 typedef float kv8_float4 __attribute__((ext_vector_type(4)));
@@ -420,6 +431,8 @@ __device__ __forceinline__ void cache_attention(const AttnArgs& a, const Members
     __shared__ float qfac[QPK];
     __shared__ float2 st_ml[kWaves][QPK];
     __shared__ float st_o[kWaves][QPK][kHeadDim];
+    __shared__ __attribute__((aligned(16))) typename F::WaveScratch scratch[kWaves];
+    __shared__ typename F::Parked parked[2];
 
     const int chunk = blockIdx.x;
     const int kvh = blockIdx.y;
@@ -431,7 +444,7 @@ __device__ __forceinline__ void cache_attention(const AttnArgs& a, const Members
     const int n = lane & 15;
     const AttnMember mb = members.get(a, m);
     const int pos = a.positions[m];
-    // loads that need neither go first: the query heads, the norm weights, the new token's row
+    // loads that need neither go first (they come in order): the query heads, the norm weights, the rotary table, the new token's row
     const float* qm = a.q + ((size_t)m * a.q_heads + (size_t)kvh * QPK) * kHeadDim;
     float qx[kHeadsPerWave][2];
 #pragma unroll
@@ -441,6 +454,7 @@ __device__ __forceinline__ void cache_attention(const AttnArgs& a, const Members
         qx[i][1] = qm[h * kHeadDim + 64 + lane];
     }
     const float qw0 = a.q_norm[lane], qw1 = a.q_norm[lane + 64];
+    const double turn = mb.rope[lane], gain = mb.rope[kHeadDim / 2];
     float nx0 = 0.f, nx1 = 0.f, kw0 = 0.f, kw1 = 0.f;
     if (wave < 2) {
         const float* src = (wave == 0 ? a.k : a.v) + ((size_t)m * a.kv_heads + kvh) * kHeadDim;
@@ -484,8 +498,7 @@ __device__ __forceinline__ void cache_attention(const AttnArgs& a, const Members
     }
 
     // ---- query heads: norm and rope, scaled by a power of two (query_exponent), in pieces
-    const Rot64 rot = turn_sincos((double)pos * mb.rope[lane]);
-    const double gain = mb.rope[kHeadDim / 2];
+    const Rot64 rot = turn_sincos((double)pos * turn);
     const float rc = (float)(rot.c * gain), rs = (float)(rot.s * gain);
 #pragma unroll
     for (int i = 0; i < kHeadsPerWave; ++i) {
@@ -541,11 +554,27 @@ __device__ __forceinline__ void cache_attention(const AttnArgs& a, const Members
 #pragma unroll
     for (int d = 0; d < 8; ++d) o[d] = kv8_float4{0.f, 0.f, 0.f, 0.f};
 
+    // The softmax's reference moved where a column's largest score passes it by kMaxExponent.
+    auto move_reference = [&](float top) {
+        if (!__any(top > mrun + kMaxExponent)) return;
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float mn = top > mrun + kMaxExponent ? top - kTopExponent : mrun;
+        const float corr = __builtin_amdgcn_exp2f(mrun - mn);
+        mrun = mn;
+        lrun *= corr;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[d] *= corr;
+    };
     // Scores of a block's two key tiles to probabilities in pieces (s in f32, `scaled` by the key scale).
+    const float piece = n < 8 ? 0.f : -1.f;  // which of a probability's pieces the lane's column takes
     auto soften = [&](kv8_float4 (&s)[2], float scaled, int b, kv8_half8& pb) {
         float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = (s[j >> 2][j & 3] + other_half(s[j >> 2][j & 3])) * scaled;
+        for (int j = 0; j < 8; ++j) {
+            x[j] = s[j >> 2][j & 3] + other_half(s[j >> 2][j & 3]);
+            if constexpr (!F::kFused) x[j] *= scaled;
+        }
         if (b * kKv8Block + kKv8Block > tokens) {  // keys past the member's position
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -554,26 +583,29 @@ __device__ __forceinline__ void cache_attention(const AttnArgs& a, const Members
         float top = x[0];
 #pragma unroll
         for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
-        if (__any(top > mrun + kMaxExponent)) {
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float mn = top > mrun + kMaxExponent ? top - kTopExponent : mrun;
-            const float corr = __builtin_amdgcn_exp2f(mrun - mn);
-            mrun = mn;
-            lrun *= corr;
-#pragma unroll
-            for (int d = 0; d < 8; ++d) o[d] *= corr;
-        }
+        move_reference(F::kFused ? top * scaled : top);
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
-            const float p0 = __builtin_amdgcn_exp2f(x[j] - mrun), p1 = __builtin_amdgcn_exp2f(x[j + 1] - mrun);
+            float p0, p1;
+            if constexpr (F::kFused) {
+                p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j], scaled, -mrun));
+                p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j + 1], scaled, -mrun));
+            } else {
+                p0 = __builtin_amdgcn_exp2f(x[j] - mrun);
+                p1 = __builtin_amdgcn_exp2f(x[j + 1] - mrun);
+            }
             sum += p0;
             sum += p1;
             const kv8_half2 hi = kv8_halfs(p0, p1);
-            const kv8_half2 lo = kv8_halfs(p0 - (float)hi[0], p1 - (float)hi[1]);
-            const uint32_t hw = __builtin_bit_cast(uint32_t, hi), lw = __builtin_bit_cast(uint32_t, lo);
-            const kv8_half2 p = __builtin_bit_cast(kv8_half2, n < 8 ? hw : lw);
+            kv8_half2 p;
+            if constexpr (F::kFused) {  // p, or p less its upper piece, then its f16
+                p = kv8_halfs(__builtin_fmaf((float)hi[0], piece, p0), __builtin_fmaf((float)hi[1], piece, p1));
+            } else {
+                const kv8_half2 lo = kv8_halfs(p0 - (float)hi[0], p1 - (float)hi[1]);
+                const uint32_t hw = __builtin_bit_cast(uint32_t, hi), lw = __builtin_bit_cast(uint32_t, lo);
+                p = __builtin_bit_cast(kv8_half2, n < 8 ? hw : lw);
+            }
             pb[j] = p[0];
             pb[j + 1] = p[1];
         }
@@ -588,7 +620,7 @@ __device__ __forceinline__ void cache_attention(const AttnArgs& a, const Members
             if (__builtin_expect(!held, 0)) F::load_tail(head, b, lane, kq, vq);
             tb.insert(row, fresh[0], fresh[1], lane);
             if (__builtin_expect(!held, 0)) tb.store(head, row + 1, lane);
-            if (__builtin_expect(row == kKv8Block - 1, 0)) F::quantise_tail(head, b, lane, kq, vq);
+            if (__builtin_expect(row == kKv8Block - 1, 0)) F::quantise_tail(head, b, lane, kq, vq, parked);
             if (lane == 0) *head.end = pos + 1;
         }
         kv8_float4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -603,15 +635,17 @@ __device__ __forceinline__ void cache_attention(const AttnArgs& a, const Members
         source.keys(b0 + wave, coded, lane, kq, ks);
         source.values(b0 + wave, coded, lane, vq, vs);
     }
+    const typename F::Constants constants;
     // (the next block's keys are under way as soon as this one's are used, its values likewise)
     for (int b = b0 + wave; b < coded; b += kWaves) {
         kv8_float4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-        F::scores(kq, qb, s);
+        F::begin(kq, scratch[wave], lane);
+        F::scores(kq, scratch[wave], constants, g, qb, s);
         const float scaled = F::scaled(fac, ks);
         source.keys(b + kWaves, coded, lane, kq, ks);
         kv8_half8 pb;
         soften(s, scaled, b, pb);
-        F::outputs(vq, vs, pb, o);
+        F::outputs(vq, vs, scratch[wave], constants, g, pb, o);
         source.values(b + kWaves, coded, lane, vq, vs);
     }
 
