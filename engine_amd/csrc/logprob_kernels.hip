@@ -1,22 +1,24 @@
 // Log probabilities of given tokens, the entropy of their distributions and the likeliest
 // alternatives, from rows of logits, in one pass over them (gfx950).
 //
-// With M a row's largest logit, t = (x - M) log2 e, R = sum of 2^t over all tokens but one
-// at M, and E = sum t 2^t:
-//   log p(x) = (x - M) - log1p(R),   entropy = log1p(R) - ln 2 E / (1 + R).
+// With c = log2 e (as f32), M a row's largest logit and M2 = f32(M c), t = x c - M2 by one multiply-add, and over all
+// tokens but one at M: R = sum 2^t, E = sum t 2^t. With w = 2^(M c - M2) (nearly 1: what M2 was rounded by), R and E
+// are brought to M itself at the end, R' = R / w and E' likewise, and
+//   log p(x) = (x - M) - log1p(R'),   entropy = log1p(R') - ln 2 E' / (1 + R').
 // The token at M is left out of R, and log1p taken of the rest, since a certain model's log
-// probability is R itself, which a sum with the 1 in it rounds away. A lane's sums are f32 (some hundred
-// terms of at most 1), those over lanes, waves and workgroups f64.
+// probability is R itself, which a sum with the 1 in it rounds away. A lane's sums are f32, 16 terms
+// first; those over lanes, waves and workgroups f64.
 //
-// NaN and -inf have probability 0: t is raised to -160, where 2^t is 0 and so is t 2^t, and a maximum takes
-// the operand that is a number. A row of nothing else has no M (-inf): its log probabilities are -inf and
-// its entropy 0. Of +inf the limit is taken: the tokens at it share the probability.
+// NaN and -inf have probability 0: where an iteration's E is no number it is formed again with t raised to -160, where
+// 2^t is 0 and so is t 2^t (and a maximum takes the operand that is a number). A row of nothing else has no M (-inf):
+// its log probabilities are -inf and its entropy 0. Of +inf the limit is taken: the tokens at it share the probability.
+// An M past 65,536 either way, whose M2 would be off by much of a power of two, takes t = (x - M) c, two roundings (Wave::wide).
 //
 // A workgroup takes a row, or one of `splits` parts of it; its four waves take 1,024 logits in turn, 16 a
 // lane in 16-byte loads (those before the row's first and after its last such piece are the first
 // workgroup's, one a lane), the next ones under way meanwhile. Each wave has its own M and its own alternatives, so
-// the loop has no barrier. An iteration whose logits all lie below both M and the wave's last alternative
-// (most of them, after the first ones) costs about ten VALU slots a logit. Others move M, or
+// the loop has no barrier. An iteration whose logits all lie below both M and what the row's alternatives are known to
+// reach (most of them, after the first ones) costs eight VALU slots a logit, four of which are the exponential. Others move M, or
 // hand their candidates to the wave's Best.
 #include "logprob.hpp"
 
@@ -32,11 +34,13 @@ constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 constexpr int kValues = 16;                    // logits a lane and iteration
 constexpr int kIteration = kThreads * kValues;
+typedef float Logits __attribute__((ext_vector_type(kValues)));  // (a vector: of an array, a choice by lane is a load from scratch)
 constexpr int kBest = 128;                     // candidates a wave holds
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLeast = -160.0f;              // 2^kLeast is 0 in f32
+constexpr float kWide = 65536.0f;
 
-// Orders as (logit, lower token first): larger keys are better, 0 is none. x is a number, and no negative zero.
+// A number's place among all, a negative zero not among them.
 __device__ __forceinline__ uint32_t order_of(float x) {
     const uint32_t b = __builtin_bit_cast(uint32_t, x);
     return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
@@ -45,8 +49,14 @@ __device__ __forceinline__ float logit_of(uint64_t key) {
     const uint32_t o = (uint32_t)(key >> 32);
     return __builtin_bit_cast(float, o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
 }
+// Orders as (logit, lower token first): larger keys are better, 0 is none.
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t token) {
-    return ((uint64_t)order_of(x == x ? x : -INFINITY) << 32) | (uint32_t)~token;
+    return ((uint64_t)order_of(x == x ? x + 0.0f : -INFINITY) << 32) | (uint32_t)~token;
+}
+// The number after x (any but NaN; -inf: the lowest one).
+__device__ __forceinline__ float above_next(float x) {
+    const uint32_t o = order_of(x + 0.0f) + (x < INFINITY ? 1u : 0u);
+    return __builtin_bit_cast(float, o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
 }
 __device__ __forceinline__ uint32_t token_of(uint64_t key) { return ~(uint32_t)key; }
 
@@ -56,16 +66,39 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// The best `top` of n <= kBest distinct keys, in order, by counting: a key's place is the number of larger ones.
+__device__ __forceinline__ uint64_t key_of_lane(uint64_t key, int lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(key >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)key, lane);
+}
+
+// The best `top` of n <= kBest distinct keys, in order, by counting: a key's place is the number of larger ones. (The others
+// come by lane reads: from LDS each took its latency, 4 us for 80 keys. Eight at a time: one by one 1.2 us for 24, now 0.4.)
 __device__ __forceinline__ void sort_best(uint64_t* keys, int n, int top) {
     const int lane = threadIdx.x & 63;
     wave_sync();
     const uint64_t a = lane < n ? keys[lane] : 0, b = lane + 64 < n ? keys[lane + 64] : 0;
     int ra = 0, rb = 0;
-    for (int i = 0; i < n; ++i) {
-        const uint64_t k = keys[i];
-        ra += k > a;
-        rb += k > b;
+    if (n <= 64) {
+#pragma unroll 1
+        for (int i = 0; i < n; i += 8)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ra += key_of_lane(a, i + j) > a;
+    } else {
+#pragma unroll 1
+        for (int i = 0; i < 64; i += 8)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint64_t k = key_of_lane(a, i + j);
+                ra += k > a;
+                rb += k > b;
+            }
+#pragma unroll 1
+        for (int i = 0; i < n - 64; i += 8)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint64_t k = key_of_lane(b, i + j);
+                ra += k > a;
+                rb += k > b;
+            }
     }
     wave_sync();
     if (lane < n && ra < top) keys[ra] = a;
@@ -73,16 +106,20 @@ __device__ __forceinline__ void sort_best(uint64_t* keys, int n, int top) {
     wave_sync();
 }
 
-// A wave's best `top` keys so far: candidates are appended, and sorted out when more than 64 are there.
+// A wave's best `top` keys so far: candidates are appended, and sorted out when kRoom more are there.
 struct Best {
+    static constexpr int kRoom = 24;
     uint64_t* keys;      // LDS [kBest]
     int top;
     int count = 0;
+    bool sorted = true;
     uint64_t least = 0;  // keys up to this one are none of the best
 
     __device__ __forceinline__ Best(uint64_t* room, int n) : keys(room), top(n) {}
     __device__ __forceinline__ float least_logit() const { return top == 0 ? INFINITY : least == 0 ? -INFINITY : logit_of(least); }
     __device__ __forceinline__ void sort() {
+        if (sorted) return;
+        sorted = true;
         sort_best(keys, count, top);
         count = min(count, top);
         if (count == top && top > 0) least = keys[top - 1];
@@ -94,12 +131,13 @@ struct Best {
         if (who == 0) return;
         if (has) keys[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key;
         count += __popcll(who);
+        sorted = false;
         if (count > kBest - 64) sort();
     }
-    // From each lane's best key: what the top-th of them bounds from below.
+    // From each lane's best logit: what the top-th of them bounds from below, by its upper 18 bits.
     __device__ __forceinline__ void bound(uint32_t order) {
         uint32_t v = 0;
-        for (int bit = 31; bit >= 0; --bit) {
+        for (int bit = 31; bit >= 14; --bit) {
             const uint32_t up = v | (1u << bit);
             if (__popcll(__ballot(order >= up)) >= top) v = up;
         }
@@ -108,27 +146,36 @@ struct Best {
     }
 };
 
-// A part's sums: M, R without the token at M, E in log2 units.
+// A part's sums: its M, R and E over the tokens but one at M, relative to the reference `ref` (log2 units).
 struct Sums {
+    float m;
+    double ref, r, e;
+};
+
+// A row's: R' and E' relative to M.
+struct Row {
     float m;
     double r, e;
 };
 
-// Parts i of `count` lanes (the others hold m = -inf, 0, 0), merged over a wave: every part's own token
-// at its m counts but one at the largest.
-__device__ __forceinline__ Sums merge_sums(Sums s) {
+// Parts, one a lane (the others hold m = -inf), merged over a wave. Every part's own token at its m counts
+// but one at the largest.
+__device__ __forceinline__ Row merge_sums(const Sums& s) {
+    constexpr double c = kLog2e;
     const float m = wave_max(s.m);
-    if (m == -INFINITY) return Sums{m, 0.0, 0.0};
+    if (m == -INFINITY) return Row{m, 0.0, 0.0};
     const uint64_t at = __ballot(s.m == m);
     const bool left_out = (threadIdx.x & 63) == (unsigned)(__ffsll((long long)at) - 1);
     double r = 0.0, e = 0.0;
     if (s.m != -INFINITY) {
-        const double d = s.m == m ? 0.0 : fmax(((double)s.m - (double)m) * 1.4426950408889634074, -1100.0);
-        const double f = exp2(d);
-        r = f * (s.r + (left_out ? 0.0 : 1.0));
-        e = f * (s.e + d * (s.r + 1.0));
+        // the part's reference and its M above the row's M (both 0 where all are infinite)
+        const double d = s.m == m && !(fabsf(m) < INFINITY) ? 0.0 : fmax(s.ref - (double)m * c, -1100.0);
+        const double own = s.m == m ? 0.0 : fmax(((double)s.m - (double)m) * c, -1100.0);
+        const double f = __builtin_amdgcn_exp2f((float)d), w = left_out ? 0.0 : (double)__builtin_amdgcn_exp2f((float)own);
+        r = f * s.r + w;
+        e = f * (s.e + d * s.r) + w * own;
     }
-    return Sums{m, wave_sum64(r), wave_sum64(e)};
+    return Row{m, wave_sum64(r), wave_sum64(e)};
 }
 
 template <int DT> __device__ __forceinline__ float load_logit(const void* p, size_t i) {
@@ -137,20 +184,23 @@ template <int DT> __device__ __forceinline__ float load_logit(const void* p, siz
     else return __builtin_bit_cast(float, (uint32_t)static_cast<const uint16_t*>(p)[i] << 16);
 }
 
+// The given token's logit, -inf for one outside the row (loaded ahead of what it is used after).
+template <int DT> __device__ __forceinline__ float given_logit(const LogprobArgs& a, size_t row) {
+    if (a.logprobs == nullptr) return 0.f;
+    const size_t t = a.targets[row];
+    return t < a.length ? load_logit<DT>(a.logits, row * a.stride + t) : -INFINITY;
+}
+
 // A row's results by a wave, from its sums and its best keys in order.
-template <int DT>
-__device__ __forceinline__ void finish(const LogprobArgs& a, size_t row, const Sums& s, const uint64_t* best) {
+__device__ __forceinline__ void finish(const LogprobArgs& a, size_t row, const Row& s, float given, const uint64_t* best) {
     const int lane = threadIdx.x & 63;
-    const double rest = log1p(s.r);
+    const double rest = log1pf((float)s.r);  // (all of a result's parts have its sign: f32 is as good as its own rounding)
     auto logprob = [&](float x) {
         if (!(x > -INFINITY)) return -INFINITY;  // (or no number)
         return (float)((x == s.m ? 0.0 : (double)x - (double)s.m) - rest);
     };
     if (lane == 0) {
-        if (a.logprobs != nullptr) {
-            const size_t t = a.targets[row];
-            a.logprobs[row] = t < a.length ? logprob(load_logit<DT>(a.logits, row * a.stride + t)) : -INFINITY;
-        }
+        if (a.logprobs != nullptr) a.logprobs[row] = logprob(given);
         if (a.entropy != nullptr) a.entropy[row] = s.m == -INFINITY ? 0.f : (float)fmax(rest - 0.69314718055994530942 * s.e / (1.0 + s.r), 0.0);
     }
     if (lane < a.top) {
@@ -160,73 +210,108 @@ __device__ __forceinline__ void finish(const LogprobArgs& a, size_t row, const S
     }
 }
 
-// What a wave has seen: a lane's sums relative to the wave's m.
+// What a wave has seen: a lane's sums relative to the wave's reference.
 struct Wave {
-    float m = -INFINITY, l = 0.f, e = 0.f;
+    float m = -INFINITY, ref = 0.f;
+    float l = 0.f, e = 0.f;
+    bool wide = false;  // |m| past kWide: the reference is m c exactly, t = (x - m) c
 
-    // 16 logits a lane (-inf: none); key(i): the i-th's key, 0: none.
-    template <class KEY>
-    __device__ __forceinline__ void take(float (&x)[kValues], Best& best, KEY key) {
-#pragma unroll
-        for (int i = 0; i < kValues; ++i) x[i] += 0.0f;  // one zero, and no signaling NaN
-        float top = x[0];
-#pragma unroll
-        for (int i = 1; i < kValues; ++i) top = fmaxf(top, x[i]);
-        top = fmaxf(top, -INFINITY);  // (a number, if all are none)
-        if (__any(top > m || top >= best.least_logit())) {
-            if (best.top > 0) {
-                if (best.count < best.top) best.bound(order_of(top));
-                const float least = best.least_logit();
-                uint32_t slots = 0;  // with a candidate in some lane
-#pragma unroll
-                for (int i = 0; i < kValues; ++i) slots |= __ballot(!(x[i] < least)) != 0 ? 1u << i : 0u;
-                while (slots != 0) {
-                    const int i = __ffs(slots) - 1;
-                    slots &= slots - 1;
-                    float v = x[0];
-#pragma unroll
-                    for (int j = 1; j < kValues; ++j) v = i == j ? x[j] : v;
-                    best.add(key(v, i));
-                }
-            }
-            const float most = wave_max(top);
-            if (most > m) {
-                if (m > -INFINITY) {
-                    if ((threadIdx.x & 63) == 0) l += 1.0f;
-                    const float d = fmaxf((m - most) * kLog2e, kLeast), f = __builtin_amdgcn_exp2f(d);
-                    e = f * __builtin_fmaf(d, l, e);
-                    l *= f;
-                }
-                m = most;
-                bool found = false;  // one of those at m is left out
-#pragma unroll
-                for (int i = 0; i < kValues; ++i) {
-                    const uint64_t at = __ballot(x[i] == m);
-                    if (!found && at != 0) {
-                        if ((threadIdx.x & 63) == (unsigned)(__ffsll((long long)at) - 1)) x[i] = -INFINITY;
-                        found = true;
-                    }
-                }
-            }
+    __device__ __forceinline__ float above(float x) const { return wide ? (x - m) * kLog2e : __builtin_fmaf(x, kLog2e, -ref); }
+
+    // m moves to the largest of the lanes' `most`, and one of the logits at it (x is set to -inf) is left out; the one left
+    // out so far counts.
+    __device__ __forceinline__ void move(float to, float most, Logits& x) {
+        const int lane = threadIdx.x & 63;
+        const bool was_wide = wide;
+        const float old = m, old_ref = ref;
+        if (m > -INFINITY && lane == 0) {
+            const float t = wide ? 0.f : __builtin_fmaf(m, kLog2e, -ref), w = __builtin_amdgcn_exp2f(t);
+            l += w;
+            e = __builtin_fmaf(t, w, e);
         }
-        if (m == -INFINITY) return;
-        if (__builtin_expect(m == INFINITY, 0)) {
-#pragma unroll
-            for (int i = 0; i < kValues; ++i) l += x[i] == m ? 1.0f : 0.0f;
-            return;
+        m = to;
+        wide = !(fabsf(m) < kWide);
+        ref = wide ? 0.f : m * kLog2e;
+        if (old > -INFINITY) {
+            const float d = fmaxf(wide || was_wide ? (old - m) * kLog2e : old_ref - ref, kLeast), f = __builtin_amdgcn_exp2f(d);
+            e = f * __builtin_fmaf(d, l, e);
+            l *= f;
         }
-        float l16 = 0.f, e16 = 0.f;  // (an iteration's first: a lane's rounding errors are those of 16 + 40 terms, not of 600)
+        bool here = lane == __ffsll((long long)__ballot(most == m)) - 1;
 #pragma unroll
         for (int i = 0; i < kValues; ++i) {
-            const float t = fmaxf((x[i] - m) * kLog2e, kLeast);
-            const float p = __builtin_amdgcn_exp2f(t);
+            const bool at = here && x[i] == m;
+            x[i] = at ? -INFINITY : x[i];
+            here = here && !at;
+        }
+    }
+
+    // The t from which a logit is past m (without an m any: the lowest numbers' t is -inf too).
+    __device__ __forceinline__ float past() const { return m == -INFINITY ? m : above_next(__builtin_fmaf(m, kLog2e, -ref)); }
+
+    // 16 logits a lane (-inf: none), none of them past m.
+    __device__ __forceinline__ void add(const Logits& t) {
+        float l16 = 0.f, e16 = 0.f;
+#pragma unroll
+        for (int i = 0; i < kValues; ++i) {
+            const float p = __builtin_amdgcn_exp2f(t[i]);
             l16 += p;
-            e16 = __builtin_fmaf(t, p, e16);
+            e16 = __builtin_fmaf(t[i], p, e16);
+        }
+        if (__builtin_expect(__any(!(e16 == e16)), 0)) {  // -inf, NaN
+            l16 = e16 = 0.f;
+#pragma unroll
+            for (int i = 0; i < kValues; ++i) {
+                const float raised = fmaxf(t[i], kLeast), p = __builtin_amdgcn_exp2f(raised);
+                l16 += p;
+                e16 = __builtin_fmaf(raised, p, e16);
+            }
         }
         l += l16;
         e += e16;
     }
+
+    // 16 logits a lane, some of which may be past m.
+    __device__ __forceinline__ void take(Logits x, float most) {
+        const float to = wave_max(most);
+        if (to > m) move(to, most, x);
+        if (m == -INFINITY) return;
+        if (m == INFINITY) {
+#pragma unroll
+            for (int i = 0; i < kValues; ++i) l += x[i] == m ? 1.0f : 0.0f;
+            return;
+        }
+        Logits t;
+#pragma unroll
+        for (int i = 0; i < kValues; ++i) t[i] = above(x[i]);
+        add(t);
+    }
 };
+
+__device__ __forceinline__ float most_of(const Logits& x) {
+    float most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kValues; ++i) most = fmaxf(most, x[i] + 0.0f);  // (of a signaling NaN, a quiet one)
+    return most;
+}
+
+// The candidates among 16 logits a lane, those of `least` or more: each lane's first ones, its second ones and so on.
+// key(x, i): the i-th's key, 0: none.
+template <class KEY>
+__device__ __forceinline__ void collect(Best& best, const Logits& x, float least, KEY key) {
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < kValues; ++i) mine |= x[i] >= least ? 1u << i : 0u;
+    if (least == -INFINITY) mine = (1u << kValues) - 1;  // (any, NaN too)
+    while (__any(mine != 0)) {
+        const int i = __ffs(mine) - 1;
+        float v = x[0];
+#pragma unroll
+        for (int j = 1; j < kValues; ++j) v = i == j ? x[j] : v;
+        best.add(mine != 0 ? key(v, i) : 0);
+        mine &= mine - 1;
+    }
+}
 
 // Grid (row, split).
 template <int DT>
@@ -235,8 +320,11 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
     constexpr int kPer = 16 / kSize;            // logits a piece
     constexpr int kPieces = kValues / kPer;     // pieces a lane and iteration
     __shared__ uint64_t keys[kWaves][kBest];
+    __shared__ uint64_t merged[kLogprobMaxTop];
+    __shared__ int counts[kWaves];
+    __shared__ float reached[kWaves];  // each wave's (top / 4)-th best logit: all four reach the least of them
     __shared__ float part_m[kWaves];
-    __shared__ double part_r[kWaves], part_e[kWaves];
+    __shared__ double part_ref[kWaves], part_r[kWaves], part_e[kWaves];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -244,109 +332,188 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
     const int split = blockIdx.y;
     const char* const base = static_cast<const char*>(a.logits) + row * a.stride * kSize;
     // the row's pieces: 16-byte aligned and whole; the first `head` logits and those after the last piece are single
-    const size_t head = std::min<size_t>(a.length, ((16 - ((uintptr_t)base & 15)) & 15) / kSize);
-    const size_t pieces = (a.length - head) / kPer;
+    const uint32_t length = (uint32_t)a.length;
+    const uint32_t head = std::min<uint32_t>(length, (uint32_t)((16 - ((uintptr_t)base & 15)) & 15) / kSize);
+    const uint32_t pieces = (length - head) / kPer;
     const uint4* const body = reinterpret_cast<const uint4*>(base + head * kSize);
-    const size_t first = pieces * (size_t)split / (size_t)a.splits, last = pieces * ((size_t)split + 1) / (size_t)a.splits;
+    const uint32_t first = (uint32_t)((uint64_t)pieces * (unsigned)split / (unsigned)a.splits);
+    const uint32_t last = (uint32_t)((uint64_t)pieces * ((unsigned)split + 1) / (unsigned)a.splits);
 
     Best best(keys[wave], a.top);
     Wave w;
     uint4 raw[kPieces];
-    auto load = [&](size_t at) {
+    uint32_t at = first + (uint32_t)wave * 64 * kPieces;
+    // (without a branch: past the part's end its last piece once more, a single line)
+    auto load = [&] {
 #pragma unroll
-        for (int u = 0; u < kPieces; ++u)
-            if (at + 64u * u + lane < last) raw[u] = body[at + 64u * u + lane];
+        for (int u = 0; u < kPieces; ++u) raw[u] = body[min(at + 64 * u + lane, last - 1)];
     };
-    size_t at = first + (size_t)wave * 64 * kPieces;
-    load(at);
-    if (split == 0 && wave == 0) {  // the single ones
-        const size_t end = head + pieces * kPer, singles = head + (a.length - end);
-        float x[kValues];
+    if (at < last) load();
+    const float given = wave == 0 && a.splits == 1 ? given_logit<DT>(a, row) : 0.f;
+    if (threadIdx.x < kWaves) reached[threadIdx.x] = -INFINITY;
+    __syncthreads();
+    const int share = (a.top + kWaves - 1) / kWaves;
+    auto sort = [&] {
+        best.sort();
+        if (share > 0 && best.count >= share && lane == 0) __hip_atomic_store(&reached[wave], logit_of(keys[wave][share - 1]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    };
+    // What a candidate is at least: past the wave's own (its tokens rise, so that of equals the earlier is in), and
+    // what the four waves reach together. `past` and `from`: the t past m, and that of such a candidate too.
+    float least = a.top > 0 ? -INFINITY : INFINITY, past = -INFINITY, from = -INFINITY;
+    auto thresholds = [&] {
+        if (a.top > 0) {
+            least = INFINITY;
 #pragma unroll
-        for (int i = 0; i < kValues; ++i) x[i] = -INFINITY;
-        const size_t token = (size_t)lane < head ? (size_t)lane : end + ((size_t)lane - head);
-        if ((size_t)lane < singles) x[0] = load_logit<DT>(base, token);
-        if (singles > 0) w.take(x, best, [&](float v, int i) { return i == 0 && (size_t)lane < singles ? key_of(v, (uint32_t)token) : 0; });
-    }
-    for (; at < last; at += (size_t)kThreads * kPieces) {
-        float x[kValues];
+            for (int i = 0; i < kWaves; ++i) least = fminf(least, __hip_atomic_load(&reached[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+            if (best.least != 0) least = fmaxf(least, above_next(logit_of(best.least)));
+        }
+        from = least <= w.m ? fminf(past, __builtin_fmaf(least, kLog2e, -w.ref)) : past;
+    };
+    // the single ones: a last iteration of the first wave, one a lane (of equals, a token before the others' wins)
+    const uint32_t end = head + pieces * kPer, singles = split == 0 && wave == 0 ? head + (length - end) : 0;
+    const uint32_t token = (uint32_t)lane < head ? (uint32_t)lane : end + ((uint32_t)lane - head);
+    const float one = (uint32_t)lane < singles ? load_logit<DT>(base, token) : -INFINITY;
+    bool single = false;
+    for (uint32_t round = 0;; ++round) {
+        Logits x;
+        const uint32_t now = at;
+        if (at < last) {
 #pragma unroll
-        for (int u = 0; u < kPieces; ++u) {
-            const bool live = at + 64u * u + lane < last;
-            const uint32_t words[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+            for (int u = 0; u < kPieces; ++u) {
+                const uint32_t words[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                float v;
-                if constexpr (DT == kLogitF32) v = __builtin_bit_cast(float, words[j]);
-                else if constexpr (DT == kLogitF16) v = half_bits_to_float((words[j >> 1] >> (16 * (j & 1))) & 0xffffu);
-                else v = __builtin_bit_cast(float, (j & 1) ? words[j >> 1] & 0xffff0000u : words[j >> 1] << 16);
-                x[kPer * u + j] = live ? v : -INFINITY;
+                for (int j = 0; j < kPer; ++j) {
+                    if constexpr (DT == kLogitF32) x[kPer * u + j] = __builtin_bit_cast(float, words[j]);
+                    else if constexpr (DT == kLogitF16) x[kPer * u + j] = half_bits_to_float((words[j >> 1] >> (16 * (j & 1))) & 0xffffu);
+                    else x[kPer * u + j] = __builtin_bit_cast(float, (j & 1) ? words[j >> 1] & 0xffff0000u : words[j >> 1] << 16);
+                }
+            }
+            at += kThreads * kPieces;
+            load();
+            if (now + 64 * kPieces > last) {
+#pragma unroll
+                for (int i = 0; i < kValues; ++i) x[i] = now + 64 * (unsigned)(i / kPer) + lane < last ? x[i] : -INFINITY;
+            }
+        } else {
+            if (single || singles == 0) break;
+            single = true;
+            x = -INFINITY;
+            x[0] = one;
+        }
+        Logits t;
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kValues; ++i) {
+            t[i] = __builtin_fmaf(x[i], kLog2e, -w.ref);
+            top = fmaxf(top, t[i]);
+        }
+        bool changed = (round & 3) == 3, taken = false;
+        if (w.wide || single || __any(top >= from)) {
+            if (a.top > 0) {
+                if (best.count < a.top) best.bound(order_of(most_of(x)));
+                collect(best, x, single ? best.least_logit() : fmaxf(least, best.least_logit()), [&](float v, int i) {
+                    if (single) return i == 0 && (uint32_t)lane < singles ? key_of(v, token) : 0;
+                    const uint32_t piece = now + 64 * (unsigned)(i / kPer) + lane;
+                    return piece < last ? key_of(v, head + piece * kPer + (unsigned)(i % kPer)) : 0;
+                });
+                if (best.count > a.top + (round == 0 ? 0 : Best::kRoom)) {
+                    sort();
+                    changed = true;
+                }
+            }
+            if (w.wide || __any(top >= past)) {
+                w.take(x, most_of(x));
+                past = w.past();
+                changed = taken = true;
             }
         }
-        const size_t now = at;
-        load(at + (size_t)kThreads * kPieces);
-        w.take(x, best, [&](float v, int i) {
-            const size_t piece = now + 64u * (unsigned)(i / kPer) + lane;
-            return piece < last ? key_of(v, (uint32_t)(head + piece * kPer + (unsigned)(i % kPer))) : 0;
-        });
+        if (!taken) w.add(t);
+        if (changed) thresholds();
     }
     best.sort();
-    if (lane == 0) part_m[wave] = w.m;
     const double r = wave_sum64((double)w.l), e = wave_sum64((double)w.e);
     if (lane == 0) {
+        part_m[wave] = w.m;
+        part_ref[wave] = w.wide ? (double)w.m * (double)kLog2e : (double)w.ref;
         part_r[wave] = r;
         part_e[wave] = e;
+        counts[wave] = best.count;
     }
-    // the waves' lists one after another
-    __shared__ int counts[kWaves];
-    if (lane == 0) counts[wave] = best.count;
+    __syncthreads();
+    // the waves' lists in one: a key's place is its own and the larger ones of the three others
+    {
+        const uint64_t key = lane < best.count ? keys[wave][lane] : 0;
+        int larger[kWaves - 1] = {};
+#pragma unroll
+        for (int step = 32; step > 0; step >>= 1) {
+            uint64_t k[kWaves - 1];
+#pragma unroll
+            for (int i = 0; i < kWaves - 1; ++i) k[i] = keys[(wave + 1 + i) % kWaves][larger[i] + step - 1];  // (at most 62)
+#pragma unroll
+            for (int i = 0; i < kWaves - 1; ++i)
+                if (larger[i] + step <= counts[(wave + 1 + i) % kWaves] && k[i] > key) larger[i] += step;
+        }
+        const int place = lane + larger[0] + larger[1] + larger[2];
+        if (lane < best.count && place < a.top) merged[place] = key;
+    }
     __syncthreads();
     if (wave != 0) return;
-    Sums s{-INFINITY, 0.0, 0.0};
-    if (lane < kWaves) s = Sums{part_m[lane], part_r[lane], part_e[lane]};
-    s = merge_sums(s);
-    int n = best.count;
-    for (int i = 1; i < kWaves; ++i) {
-        if (lane < counts[i]) keys[0][n + lane] = keys[i][lane];
-        n += counts[i];
-    }
-    sort_best(keys[0], n, a.top);
+    Sums s{-INFINITY, 0.0, 0.0, 0.0};
+    if (lane < kWaves) s = Sums{part_m[lane], part_ref[lane], part_r[lane], part_e[lane]};
+    const Row all = merge_sums(s);
     if (a.splits == 1) {
-        finish<DT>(a, row, s, keys[0]);
+        finish(a, row, all, given, merged);
         return;
     }
+    const int n = counts[0] + counts[1] + counts[2] + counts[3];
     uint64_t* part = a.partials + (row * (size_t)a.splits + (size_t)split) * (size_t)(3 + a.top);
     if (lane == 0) {
-        part[0] = __builtin_bit_cast(uint32_t, s.m);
-        part[1] = __builtin_bit_cast(uint64_t, s.r);
-        part[2] = __builtin_bit_cast(uint64_t, s.e);
+        part[0] = __builtin_bit_cast(uint32_t, all.m);
+        part[1] = __builtin_bit_cast(uint64_t, all.r);
+        part[2] = __builtin_bit_cast(uint64_t, all.e);
     }
-    if (lane < a.top) part[3 + lane] = lane < n ? keys[0][lane] : 0;
+    if (lane < a.top) part[3 + lane] = lane < n ? merged[lane] : 0;
 }
 
-// A row's parts, one a lane.
+// A row's parts: sums one a lane, keys one after another.
 template <int DT>
 __global__ __launch_bounds__(64) void logprob_merge_kernel(LogprobArgs a) {
     __shared__ uint64_t keys[kBest];
+    constexpr int kAhead = 12;  // keys a lane under way
     const int lane = threadIdx.x;
     const size_t row = blockIdx.x;
-    const bool live = lane < a.splits;
-    const uint64_t* part = a.partials + (row * (size_t)a.splits + (size_t)lane) * (size_t)(3 + a.top);
-    Sums s{-INFINITY, 0.0, 0.0};
-    if (live) s = Sums{__builtin_bit_cast(float, (uint32_t)part[0]), __builtin_bit_cast(double, part[1]), __builtin_bit_cast(double, part[2])};
-    Best best(keys, a.top);
-    constexpr int kAhead = 4;
-    for (int j = 0; j < a.top; j += kAhead) {
-        uint64_t k[kAhead];
+    const uint64_t* parts = a.partials + row * (size_t)a.splits * (size_t)(3 + a.top);
+    const int total = a.splits * a.top;
+    uint64_t k[kAhead];
+    auto load = [&](int e0) {  // key e: the (e / splits)-th best of part e % splits
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) k[i] = live && j + i < a.top ? part[3 + j + i] : 0;
-        if (j == 0) best.bound((uint32_t)(k[0] >> 32));
-        if (!__any(k[0] > best.least)) break;  // (lists are in order)
+        for (int i = 0; i < kAhead; ++i) {
+            const int e = e0 + 64 * i + lane;
+            k[i] = e < total ? parts[(unsigned)e % (unsigned)a.splits * (unsigned)(3 + a.top) + 3u + (unsigned)e / (unsigned)a.splits] : 0;
+        }
+    };
+    load(0);
+    Sums s{-INFINITY, 0.0, 0.0, 0.0};
+    if (lane < a.splits) {
+        const uint64_t* part = parts + (size_t)lane * (size_t)(3 + a.top);
+        const float m = __builtin_bit_cast(float, (uint32_t)part[0]);
+        s = Sums{m, (double)m * (double)kLog2e, __builtin_bit_cast(double, part[1]), __builtin_bit_cast(double, part[2])};
+    }
+    const float given = given_logit<DT>(a, row);
+    Best best(keys, a.top);
+    for (int e = 0; e < total; e += 64 * kAhead) {
+        if (e > 0) load(e);
+        if (e == 0) {
+            uint64_t most = k[0];
+#pragma unroll
+            for (int i = 1; i < kAhead; ++i) most = max(most, k[i]);
+            best.bound((uint32_t)(most >> 32));
+        }
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) best.add(k[i]);
     }
     best.sort();
-    finish<DT>(a, row, merge_sums(s), keys);
+    finish(a, row, merge_sums(s), given, keys);
 }
 
 template <int DT>
