@@ -15,7 +15,7 @@ from .kquant import (  # noqa: F401
     validate_quantized_geometry,
 )
 from .gguf import GgufError, GgufFile, TensorInfo, load_qwen3_decode, qwen3_config_from_gguf, rope_from_gguf  # noqa: F401
-from .qwen3 import KV_F16, KV_I4, KV_I8, AmdKvCache, AmdQwen3Config, AmdQwen3Decode, QWEN3_8B, attention_decode, attention_prefill  # noqa: F401
+from .qwen3 import KV_F16, KV_I4, KV_I8, AmdKvCache, AmdQwen3Config, AmdQwen3Decode, QWEN3_8B, TokenLogprobs, attention_decode, attention_prefill  # noqa: F401
 from .rope import AmdRope, AmdRopeSpec, rope_frequencies  # noqa: F401
 from .serving import AmdBackend, AmdDispatcher, AmdServingDispatcher, BackendError, plan_memory  # noqa: F401
 
@@ -24,7 +24,7 @@ __all__ = [
     "AmdQ4KGemv", "AmdQ5KGemv", "AmdQ6KGemv", "QwenGemvKernel", "AmdQwenOps", "AmdQ4KEmbedding",
     "AmdKQuantEmbedding", "AmdKernelError",
     "AmdQuantizedKernelError", "AmdModelKernelError", "AmdWeightError", "validate_quantized_geometry",
-    "AmdKvCache", "AmdQwen3Config", "AmdQwen3Decode", "QWEN3_8B", "attention_decode", "attention_prefill",
+    "AmdKvCache", "AmdQwen3Config", "AmdQwen3Decode", "QWEN3_8B", "TokenLogprobs", "attention_decode", "attention_prefill",
     "KV_F16", "KV_I8", "KV_I4", "AmdRope", "AmdRopeSpec", "rope_frequencies",
     "AmdQ8_1Quantizer", "AmdQ4KQ8_1Gemv", "AmdQ5KQ8_1Gemv", "AmdQ6KQ8_1Gemv",
     "GgufError", "GgufFile", "TensorInfo", "load_qwen3_decode", "qwen3_config_from_gguf", "rope_from_gguf",

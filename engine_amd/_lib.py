@@ -214,6 +214,8 @@ SIGNATURES = {
                                        _u32, _vp, _sz]),
     "ribn_amd_probe_mfma_peak": (_i32, [_vp, _u32, _u32, ctypes.POINTER(ctypes.c_double)]),
     "ribn_amd_qwen3_prefill_prompt": (_i32, [_vp, _vp, ctypes.POINTER(_u32), _sz, _u32, _u32]),
+    "ribn_amd_qwen3_score_prompt": (_i32, [_vp, _vp, _vp, _sz, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _sz]),
+    "ribn_amd_qwen3_logprobs": (_i32, [_vp, _sz, _vp, _vp, _vp, _vp, _vp, _sz]),
     "ribn_amd_qwen3_reserve_prompt": (_i32, [_vp, _u32]),
     "ribn_amd_qwen3_decode_step": (_i32, [_vp, _vp, _u32, _u32, ctypes.POINTER(_u32)]),
     "ribn_amd_qwen3_decode_step_batch": (_i32, [_vp, _vp, ctypes.POINTER(_u32), ctypes.POINTER(_u32), _sz,

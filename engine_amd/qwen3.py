@@ -4,7 +4,8 @@
   AmdKvCache       <- CudaKvState, the KV part of CudaHybridState (state.rs:99-254, 529-660)
   AmdQwen3Decode   <- CudaQwen35Decode (decode.rs:236-800) and CudaQwen35BatchDecode
                       (decode.rs:1626-1960): new, prefill_step, decode_step,
-                      decode_step_batch, copy_hidden, copy_logits
+                      decode_step_batch, copy_hidden, copy_logits; score_prompt and
+                      logprobs (TokenLogprobs) have no counterpart
   attention_decode <- the per-layer sequence q/k norm + rope + kv_append_f16 +
                       attn_score_gqa (decode.rs:929-1034)
 
@@ -152,6 +153,25 @@ def attention_prefill(ctx, config: AmdQwen3Config, cache, layer: int, q, k, v, q
                                                position, output.data_ptr(), output.numel()), AmdModelKernelError)
 
 
+@dataclass
+class TokenLogprobs:
+    """Log probabilities of rows (tokens of a prompt, members of a step); what was not asked for is None."""
+
+    logprobs: Optional[np.ndarray]      # [rows] of the targets
+    entropy: Optional[np.ndarray]       # [rows]
+    top_tokens: Optional[np.ndarray]    # [rows][top], the likeliest first
+    top_logprobs: Optional[np.ndarray]  # [rows][top]
+
+    @staticmethod
+    def _room(rows: int, logprobs: bool, entropy: bool, top: int) -> "TokenLogprobs":
+        def new(want, *shape, dtype=np.float32):
+            return np.zeros(shape, dtype) if want else None
+        return TokenLogprobs(new(logprobs, rows), new(entropy, rows), new(top > 0, rows, top, dtype=np.uint32), new(top > 0, rows, top))
+
+    def _pointers(self):
+        return [None if a is None else a.ctypes.data for a in (self.logprobs, self.entropy, self.top_tokens, self.top_logprobs)]
+
+
 class AmdQwen3Decode:
     """Decode-step executor (CudaQwen35Decode + CudaQwen35BatchDecode).
 
@@ -214,6 +234,36 @@ class AmdQwen3Decode:
         ptr = tok.ctypes.data_as(ctypes.POINTER(ctypes.c_uint32))
         _check(self.ctx._lib.ribn_amd_qwen3_prefill_prompt(self.handle, cache.handle, ptr, tok.size, position,
                                                            chunk_tokens), AmdModelKernelError)
+
+    def score_prompt(self, cache: AmdKvCache, tokens, position: int, targets=None, entropy: bool = False, top: int = 0,
+                     chunk_tokens: int = 0) -> TokenLogprobs:
+        """prefill_prompt, and of each token's successor: the log probability of targets[i] (host tokens, one per prompt
+        token; one outside the vocabulary has -inf), the distribution's entropy, and the `top` likeliest tokens with
+        their log probabilities (ribn_amd_qwen3_score_prompt). Blocking."""
+        tok = np.ascontiguousarray(np.asarray(tokens, dtype=np.uint32).reshape(-1))
+        goal = None if targets is None else np.ascontiguousarray(np.asarray(targets, dtype=np.uint32).reshape(-1))
+        if goal is not None and goal.size != tok.size:
+            raise ValueError(f"{tok.size} tokens need as many targets, got {goal.size}")
+        if not 0 <= top <= self.config.vocab:
+            raise ValueError(f"{top} alternatives of {self.config.vocab} tokens")
+        out = TokenLogprobs._room(tok.size, goal is not None, entropy, top)
+        _check(self.ctx._lib.ribn_amd_qwen3_score_prompt(self.handle, cache.handle, tok.ctypes.data, tok.size, position, chunk_tokens,
+                                                         None if goal is None else goal.ctypes.data, *out._pointers(), top),
+               AmdModelKernelError)
+        return out
+
+    def logprobs(self, members: int = 1, targets=None, logprobs: bool = True, entropy: bool = False, top: int = 0) -> TokenLogprobs:
+        """Log probabilities of the last step's first `members` members: of `targets` (host tokens, by default the ones
+        the step selected), the entropy, and the `top` likeliest tokens (ribn_amd_qwen3_logprobs). Blocking."""
+        goal = None if targets is None else np.ascontiguousarray(np.asarray(targets, dtype=np.uint32).reshape(-1))
+        if goal is not None and goal.size != members:
+            raise ValueError(f"{members} members need as many targets, got {goal.size}")
+        if not 0 <= top <= self.config.vocab:
+            raise ValueError(f"{top} alternatives of {self.config.vocab} tokens")
+        out = TokenLogprobs._room(members, logprobs, entropy, top)
+        _check(self.ctx._lib.ribn_amd_qwen3_logprobs(self.handle, members, None if goal is None else goal.ctypes.data, *out._pointers(), top),
+               AmdModelKernelError)
+        return out
 
     def reserve_prompt(self, chunk_tokens: int = 0):
         """Allocates the prompt workspace for chunks of `chunk_tokens` tokens ahead of prefill_prompt."""

@@ -823,6 +823,17 @@ ribn_amd_status ribn_amd_qwen3_prefill_chunk(ribn_amd_qwen3_decode *decode, ribn
 ribn_amd_status ribn_amd_qwen3_prefill_prompt(ribn_amd_qwen3_decode *decode, ribn_amd_kv_cache *cache,
                                               const uint32_t *tokens, size_t count, uint32_t position,
                                               uint32_t chunk_tokens);
+/* ribn_amd_qwen3_prefill_prompt, and the log probabilities of what follows each of its tokens (no reference
+ * counterpart): row i is of the distribution of the token after tokens[i], with ribn_amd_logprobs' definitions, and
+ * targets[i] the token whose log probability is asked (tokens[i + 1] of a text; one >= vocab: -inf). targets and the results
+ * are host arrays of `count` rows (top_*: [count][top]); each of logprobs (with targets), entropy and the two top arrays
+ * may be NULL, not all of them. The cache is left as ribn_amd_qwen3_prefill_prompt leaves it, and the call can go on
+ * where an earlier one ended. The logits come from the prefill matmul: within its tolerance of the decode steps'.
+ * Blocking; its workspace (up to 1,024 rows of logits) is allocated and grown as the prompt's is. */
+ribn_amd_status ribn_amd_qwen3_score_prompt(ribn_amd_qwen3_decode *decode, ribn_amd_kv_cache *cache,
+                                            const uint32_t *tokens, size_t count, uint32_t position,
+                                            uint32_t chunk_tokens, const uint32_t *targets, float *logprobs,
+                                            float *entropy, uint32_t *top_tokens, float *top_logprobs, size_t top);
 /* Allocates (grows) the prompt workspace for chunks of `chunk_tokens` tokens
  * (0 means 2048) ahead of ribn_amd_qwen3_prefill_prompt. No reference
  * counterpart (the reference sizes its batch scratch at construction,
@@ -850,6 +861,13 @@ ribn_amd_status ribn_amd_qwen3_generate(ribn_amd_qwen3_decode *decode, ribn_amd_
  * residual stream [hidden] or logits [vocab] after the last step, to host. */
 ribn_amd_status ribn_amd_qwen3_copy_hidden(ribn_amd_qwen3_decode *decode, size_t member, float *host, size_t len);
 ribn_amd_status ribn_amd_qwen3_copy_logits(ribn_amd_qwen3_decode *decode, size_t member, float *host, size_t len);
+/* Log probabilities, entropy and alternatives (ribn_amd_logprobs' definitions; no reference counterpart) of the first
+ * `members` members of the last step with an output head, from the logits that ribn_amd_qwen3_copy_logits copies. targets:
+ * host array [members], NULL: the tokens the step selected (of ribn_amd_qwen3_generate, its last ones). Results are host arrays, [members] and
+ * [members][top]; each of logprobs, entropy and the two top arrays may be NULL, not all of them. Blocking. */
+ribn_amd_status ribn_amd_qwen3_logprobs(ribn_amd_qwen3_decode *decode, size_t members, const uint32_t *targets,
+                                        float *logprobs, float *entropy, uint32_t *top_tokens, float *top_logprobs,
+                                        size_t top);
 
 /* ------------------------------------------------------ serving dispatcher */
 

@@ -200,7 +200,7 @@ class LongContextQwen3(OracleQwen3):
                 normed = O.rms_norm_raw(h, self.w[p + "ffn_norm"], c["epsilon"])
                 act = O.swiglu(self._gemv(p + "ffn_gate", normed), self._gemv(p + "ffn_up", normed))
                 hs[i] = (h + self._gemv(p + "ffn_down", act)).astype(np.float32)
-        self.hidden = hs[-1]
+        self.hiddens, self.hidden = hs, hs[-1]
         return self.hidden
 
     def step(self, token, pos, head=True):

@@ -210,6 +210,20 @@ def test_the_top_moves_far(env):
     check(run(env, view, t, 32), values, t, 32)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_the_lowest_after_nothing(env, dtype):
+    """A row of nothing but -inf for long, then of its type's lowest value only, one token or many."""
+    case(test="lowest_after_nothing", dtype=dtype)
+    torch = env["torch"]
+    low = float(torch.finfo(getattr(torch, dtype)).min)
+    x = np.full((4, 60000), -np.inf)
+    x[0, 55001], x[1, 59999] = low, low
+    x[2, 40000:], x[3, 40000::3] = low, low / 2
+    view, values = typed(env, x, dtype)
+    for top in (0, 1, 20):
+        check(run(env, view, [55001, 59999, 50000, 1], top), values, [55001, 59999, 50000, 1], top)
+
+
 def test_certain_models(env):
     """Log probabilities and entropies near 0 keep their digits."""
     case(test="certain")
