@@ -189,28 +189,41 @@ struct Kv4Format {
         }
     }
 
-    // Codes, scales and lows of the whole block; its values become what these stand for. By way of LDS, a piece
-    // at a time: a step in 32 comes here, and unrolled over the registers that hold the block it set the kernel's
-    // count (160, and scratch with a bound of 128).
+    // Codes, scales and lows of the whole block; its values become what these stand for. By way of LDS, where each
+    // wave takes a share: a step in 32 comes here, one of a batch's nearly always. One wave did it in 6.7 us, while the
+    // others waited (and unrolled over the registers that hold the block it set the kernel's count).
+    static constexpr bool kSharedQuantise = true;
     struct Parked {
         kv8_u4 x[8][64];
     };
-    __device__ __forceinline__ static void quantise_tail(const KvHead& h, int b, int lane, kv8_u4 (&k)[kKeyRegs], kv8_u4 (&v)[kValueRegs], Parked (&parked)[2]) {
-        const Kv4Bias bias;
-        uint8_t* const block = h.codes + (size_t)b * kKv4BlockBytes;
-        auto pair = [](uint32_t w) { return __builtin_bit_cast(kv8_half2, w); };
-        auto word = [](kv8_half2 x) { return __builtin_bit_cast(uint32_t, x); };
-        lds_order();
+    __device__ __forceinline__ static void park(Parked (&parked)[2], int lane, const kv8_u4 (&k)[kKeyRegs], const kv8_u4 (&v)[kValueRegs]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             parked[0].x[i][lane] = k[i];
             parked[1].x[i][lane] = v[i];
         }
-        lds_order();
+    }
+    __device__ __forceinline__ static void unpark(const Parked (&parked)[2], int lane, kv8_u4 (&k)[kKeyRegs], kv8_u4 (&v)[kValueRegs]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            k[i] = parked[0].x[i][lane];
+            v[i] = parked[1].x[i][lane];
+        }
+    }
+    __device__ __forceinline__ static void quantise_share(const KvHead& h, int b, int wave, int lane, Parked (&parked)[2]) {
+        const Kv4Bias bias;
+        uint8_t* const block = h.codes + (size_t)b * kKv4BlockBytes;
+        if (wave < 2) quantise_keys(block, 2 * wave, lane, parked[0], bias);
+        else quantise_values(block, wave - 2, lane, parked[1], bias);
+    }
+    __device__ __forceinline__ static kv8_half2 pair(uint32_t w) { return __builtin_bit_cast(kv8_half2, w); }
+    __device__ __forceinline__ static uint32_t word(kv8_half2 x) { return __builtin_bit_cast(uint32_t, x); }
+    // Steps `step` and the next one of the keys.
+    __device__ __forceinline__ static void quantise_keys(uint8_t* block, int step, int lane, Parked& parked, const Kv4Bias& bias) {
         kv8_u4* const kp = reinterpret_cast<kv8_u4*>(block + kKv4Params) + 2 * (lane >> 4);
 #pragma unroll 1
-        for (int s = 0; s < 4; ++s) {  // eight dims, of the two tiles
-            const kv8_u4 x0 = parked[0].x[s][lane], x1 = parked[0].x[4 + s][lane];
+        for (int s = step; s < step + 2; ++s) {  // eight dims, of the two tiles
+            const kv8_u4 x0 = parked.x[s][lane], x1 = parked.x[4 + s][lane];
             kv8_u4 scale, low;
             uint32_t w[2] = {0, 0};
 #pragma unroll
@@ -230,49 +243,43 @@ struct Kv4Format {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 reinterpret_cast<uint32_t*>(block)[256 * t + 4 * lane + s] = w[t];
-                parked[0].x[4 * t + s][lane] = __builtin_bit_cast(kv8_u4, kv4_values(w[t], scale, low, bias));
+                parked.x[4 * t + s][lane] = __builtin_bit_cast(kv8_u4, kv4_values(w[t], scale, low, bias));
             }
         }
-        kv8_u4* const vp = reinterpret_cast<kv8_u4*>(block + kKv4Params + kKv4ValueParams) + (lane >> 4);
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-            kv8_u4 x[4], scale, low, w = kv8_u4{0, 0, 0, 0};
+    }
+    // Half `half` of the values.
+    __device__ __forceinline__ static void quantise_values(uint8_t* block, int half, int lane, Parked& parked, const Kv4Bias& bias) {
+        kv8_u4 x[4], scale, low, w = kv8_u4{0, 0, 0, 0};
 #pragma unroll
-            for (int d = 0; d < 4; ++d) x[d] = parked[1].x[4 * half + d][lane];
+        for (int d = 0; d < 4; ++d) x[d] = parked.x[4 * half + d][lane];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {  // a pair of keys, over four dims and the row's 16 lanes
-                kv8_half2 lo, hi;
+        for (int j = 0; j < 4; ++j) {  // a pair of keys, over four dims and the row's 16 lanes
+            kv8_half2 lo, hi;
 #pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const uint32_t a = x[d][j];
-                    lo = d == 0 ? pair(a) : kv4_min(lo, pair(a));
-                    hi = d == 0 ? -pair(a) : kv4_min(hi, -pair(a));
-                }
-                lo = kv4_row_min(lo);
-                hi = -kv4_row_min(hi);
-                const Kv4Scale a(lo[0], hi[0]), c(lo[1], hi[1]);
-                scale[j] = word(kv8_half2{a.s, c.s});
-                low[j] = word(lo);
-#pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const uint32_t y = x[d][j];
-                    w[d] |= kv4_code(pair(y)[0], lo[0], a.inv) << kv4_shift(2 * j) | kv4_code(pair(y)[1], lo[1], c.inv) << kv4_shift(2 * j + 1);
-                }
+            for (int d = 0; d < 4; ++d) {
+                const uint32_t a = x[d][j];
+                lo = d == 0 ? pair(a) : kv4_min(lo, pair(a));
+                hi = d == 0 ? -pair(a) : kv4_min(hi, -pair(a));
             }
-            if ((lane & 15) == 0) {
-                vp[8 * half] = scale;
-                vp[8 * half + 4] = low;
+            lo = kv4_row_min(lo);
+            hi = -kv4_row_min(hi);
+            const Kv4Scale a(lo[0], hi[0]), c(lo[1], hi[1]);
+            scale[j] = word(kv8_half2{a.s, c.s});
+            low[j] = word(lo);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const uint32_t y = x[d][j];
+                w[d] |= kv4_code(pair(y)[0], lo[0], a.inv) << kv4_shift(2 * j) | kv4_code(pair(y)[1], lo[1], c.inv) << kv4_shift(2 * j + 1);
             }
-            reinterpret_cast<kv8_u4*>(block + kKv4Values)[64 * half + lane] = w;
-#pragma unroll
-            for (int d = 0; d < 4; ++d) parked[1].x[4 * half + d][lane] = __builtin_bit_cast(kv8_u4, kv4_values(w[d], scale, low, bias));
         }
-        lds_order();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            k[i] = parked[0].x[i][lane];
-            v[i] = parked[1].x[i][lane];
+        if ((lane & 15) == 0) {
+            kv8_u4* const p = reinterpret_cast<kv8_u4*>(block + kKv4Params + kKv4ValueParams) + (lane >> 4) + 8 * half;
+            p[0] = scale;
+            p[4] = low;
         }
+        reinterpret_cast<kv8_u4*>(block + kKv4Values)[64 * half + lane] = w;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) parked.x[4 * half + d][lane] = __builtin_bit_cast(kv8_u4, kv4_values(w[d], scale, low, bias));
     }
 };
 

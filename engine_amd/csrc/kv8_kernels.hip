@@ -93,6 +93,7 @@ struct Kv8Format {
     };
 
     struct Constants {};
+    static constexpr bool kSharedQuantise = false;
     struct Parked {};
     struct WaveScratch {};
     __device__ __forceinline__ static void begin(const kv8_u4 (&)[8], WaveScratch&, int) {}
@@ -155,7 +156,7 @@ struct Kv8Format {
         }
     }
     // Codes and scales of the whole block; its values become what these stand for.
-    __device__ __forceinline__ static void quantise_tail(const KvHead& h, int b, int lane, kv8_u4 (&k)[8], kv8_u4 (&v)[8], Parked (&)[2]) {
+    __device__ __forceinline__ static void quantise_tail(const KvHead& h, int b, int lane, kv8_u4 (&k)[8], kv8_u4 (&v)[8]) {
         kv8_u4* c = reinterpret_cast<kv8_u4*>(h.codes + (size_t)b * kKv8BlockBytes) + lane;
         float2 sc;
         quantise_part(k, c, sc.x);

@@ -11,7 +11,8 @@
 //   scores, scaled, outputs             the matrix products over a block in registers
 //   kFused                              whether a score's scale and the softmax's reference go into one multiply-add (8-bit
 //                                       caches keep two roundings)
-//   load_tail / quantise_tail           a block in registers: what its codes stand for, and its codes (Parked: LDS for that)
+//   load_tail                           a block in registers: what its codes stand for
+//   quantise_tail                       its codes, by the wave that holds it; or (kSharedQuantise) quantise_share by all four of a workgroup, from LDS (Parked, park, unpark)
 #pragma once
 
 #include <float.h>
@@ -430,7 +431,7 @@ __device__ __forceinline__ void cache_attention(const AttnArgs& a, const Members
     __shared__ __attribute__((aligned(16))) _Float16 fresh[2][kHeadDim];  // the new token's key and value
     __shared__ float qfac[QPK];
     __shared__ float2 st_ml[kWaves][QPK];
-    __shared__ float st_o[kWaves][QPK][kHeadDim];
+    __shared__ float st_o[kWaves][QPK][kHeadDim + 1];  // (a column's heads in banks of their own: 1 us of a call)
     __shared__ __attribute__((aligned(16))) typename F::WaveScratch scratch[kWaves];
     __shared__ typename F::Parked parked[2];
 
@@ -612,15 +613,30 @@ __device__ __forceinline__ void cache_attention(const AttnArgs& a, const Members
         lrun += sum;
     };
 
+    auto insert_row = [&] {
+        // rows before the new one, if the tail has another block's: what the block's codes stand for
+        const bool held = row == 0 || (old_end > 0 && (old_end - 1) / kKv8Block == coded);
+        if (__builtin_expect(!held, 0)) F::load_tail(head, coded, lane, kq, vq);
+        tb.insert(row, fresh[0], fresh[1], lane);
+        if (__builtin_expect(!held, 0)) tb.store(head, row + 1, lane);
+    };
+    if constexpr (F::kSharedQuantise) {
+        if (tail && append) insert_row();
+        if (__builtin_expect(append && has_tail && row == kKv8Block - 1, 0)) {  // by way of LDS, a share a wave
+            if (tail) F::park(parked, lane, kq, vq);
+            __syncthreads();
+            F::quantise_share(head, coded, wave, lane, parked);
+            __syncthreads();
+            if (tail) F::unpark(parked, lane, kq, vq);
+        }
+    }
     if (tail) {
         const int b = coded;
         if (append) {
-            // rows before the new one, if the tail has another block's: what the block's codes stand for
-            const bool held = row == 0 || (old_end > 0 && (old_end - 1) / kKv8Block == b);
-            if (__builtin_expect(!held, 0)) F::load_tail(head, b, lane, kq, vq);
-            tb.insert(row, fresh[0], fresh[1], lane);
-            if (__builtin_expect(!held, 0)) tb.store(head, row + 1, lane);
-            if (__builtin_expect(row == kKv8Block - 1, 0)) F::quantise_tail(head, b, lane, kq, vq, parked);
+            if constexpr (!F::kSharedQuantise) {
+                insert_row();
+                if (__builtin_expect(row == kKv8Block - 1, 0)) F::quantise_tail(head, b, lane, kq, vq);
+            }
             if (lane == 0) *head.end = pos + 1;
         }
         kv8_float4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -664,6 +680,7 @@ __device__ __forceinline__ void cache_attention(const AttnArgs& a, const Members
     if (g == 0 && n < QPK) st_ml[wave][n] = make_float2(mrun, lrun);
     __syncthreads();
     float* const own = a.partials != nullptr ? a.partials + (size_t)m * a.partial_floats : mb.partials;
+#pragma unroll
     for (int i = tid; i < QPK * kHeadDim; i += kThreads) {
         const int h = i >> 7, d = i & 127;
         float mx = -FLT_MAX;
