@@ -699,7 +699,8 @@ __device__ __forceinline__ float4 nonfinite_values(uint2 w) {
 // as zeros. The matrix cores bound long chunks as they do over f16 caches, and half the
 // bytes buy little: 2,047 tokens from 0 (32 / 8 heads) take 91 us for 96, 1,999 after 6,203
 // 447 for 446 (each product counted twice, for the two pieces of q and p: 1,060 TFLOP/s);
-// 37 tokens after 2,011, where the keys' split counts, 26 for 55.
+// 37 tokens after 2,011, where the keys' split counts, 26 for 55. In 4 bits 2,047 tokens from 0 take 94 us, 1,801
+// after 8,192 540 (990 TFLOP/s), 29 after 3,040 22.3.
 struct PrefillBlocks {
     __amdgpu_buffer_rsrc_t cr;
     const _Float16* tail_k;
@@ -786,7 +787,8 @@ struct PrefillI8 : PrefillBlocks {
     }
 };
 
-// (scales and lows come to LDS a key round ahead: as a piece's operands they are 96 bytes, of which 16 lanes share each)
+// (scales and lows come to LDS a key round ahead: as a piece's operands they are 96 bytes, of which 16 lanes share each,
+// and loaded so 1,801 tokens after 8,192 took 597 us of the 540)
 constexpr int kPairParams = 2 * kKv4ParamBytes / 8;  // 8-byte pieces of a block pair's
 
 struct PrefillI4 : PrefillBlocks {

@@ -190,8 +190,8 @@ struct Kv4Format {
     }
 
     // Codes, scales and lows of the whole block; its values become what these stand for. By way of LDS, where each
-    // wave takes a share: a step in 32 comes here, one of a batch's nearly always. One wave did it in 6.7 us, while the
-    // others waited (and unrolled over the registers that hold the block it set the kernel's count).
+    // wave takes a share: a step in 32 comes here, one of a batch's nearly always. One wave took 6.7 us for it, four take
+    // 2.1 (a whole call of one member 12.4 and 7.6 us; unrolled over the registers that hold the block it set the kernel's count).
     static constexpr bool kSharedQuantise = true;
     struct Parked {
         kv8_u4 x[8][64];
@@ -283,17 +283,32 @@ struct Kv4Format {
     }
 };
 
+// Appends and writes: 8 KB of rows in LDS a block and part, three passes with a barrier between (smallest and largest,
+// scales, codes). 32,768 f16 rows of 8 heads (134 MB in, 39 out) take 42 us, 4.1 TB/s: round trips of the passes at four workgroups a CU (a
+// fifth less instructions changed nothing). A prompt's keys are formed in 64 bits first: 29 tokens 5.5 us, 2,047 (17 MB in, 2.4
+// out) 8.9, latency both.
 __global__ __launch_bounds__(2 * kAppendThreads) void kv4_append_kernel(AttnArgs a, int members) { append_members<Kv4Format>(a, members); }
 __global__ __launch_bounds__(2 * kAppendThreads) void kv4_append_seq_kernel(PrefillAttnArgs a) { append_chunk<Kv4Format>(a); }
 template <int ROWS>
 __global__ __launch_bounds__(2 * kAppendThreads) void kv4_write_kernel(KvMoveArgs a) { write_rows<Kv4Format, ROWS>(a); }
+// 32,768 rows (39 MB in, 134 out) in 27 us, 6.4 TB/s (the codes had just been written).
 template <typename T>
 __global__ __launch_bounds__(kAppendThreads, 4) void kv4_read_kernel(KvMoveArgs a) { read_rows<Kv4Format, T>(a); }
 
+// Decode attention (kvq_device.hpp). Memory bounds the long contexts (131,071 tokens, 159 MB: 35 us, 4.6 TB/s, at one wave a
+// SIMD, whose VALU is busy half of that; 30 would be a copy's), round trips and ramp the short ones: 5.4 us pass with
+// one block. With 8 members of 4,001 tokens (27 MB) the codes come in about 3 of 12 us; norms, angles and the first loads take 2,
+// the waves' meeting 1, the launch and its ramp the rest.
+// A block costs some 200 instructions a wave: its codes by the two patterns of kv4_values 13 for eight, the softmax as for 8 bits. What
+// has been tried: a lane's own scales and lows as 16-byte loads (12 a block, 48 registers) took 52 us of the 39 of one member
+// of 131,071; two blocks in flight a wave 43.0 of 42.9 then; eight waves a workgroup 40.7, but 28 of 17.9 with 8
+// members of 4,001; a bound of four workgroups a CU spills (131,071 tokens 57.7 us). LDS shared between the last block's values and the waves' outputs
+// would let a fourth workgroup of eight query heads on the CU, but took 13 registers more: 8 members 17.0 of 15.4.
 template <int QPK, bool INLINE>
 __global__ __launch_bounds__(kAttnThreads, 3) void kv4_attn_kernel(AttnArgs a, Members<INLINE> members) {
     cache_attention<Kv4Format, QPK, INLINE>(a, members);
 }
+// The chunks' merge: 2 to 4 us, a launch's ramp and one round trip.
 template <int NC, bool INLINE>
 __global__ __launch_bounds__(128) void kv4_combine_kernel(AttnArgs a, Members<INLINE> members) {
     combine_chunks<Kv4Format, NC, INLINE>(a, members);

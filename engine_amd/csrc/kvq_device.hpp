@@ -431,7 +431,7 @@ __device__ __forceinline__ void cache_attention(const AttnArgs& a, const Members
     __shared__ __attribute__((aligned(16))) _Float16 fresh[2][kHeadDim];  // the new token's key and value
     __shared__ float qfac[QPK];
     __shared__ float2 st_ml[kWaves][QPK];
-    __shared__ float st_o[kWaves][QPK][kHeadDim + 1];  // (a column's heads in banks of their own: 1 us of a call)
+    __shared__ float st_o[kWaves][QPK][kHeadDim + 1];  // (heads in banks of their own: 31 members of 4,000 tokens in 4 bits 42.2 us without, 40.4)
     __shared__ __attribute__((aligned(16))) typename F::WaveScratch scratch[kWaves];
     __shared__ typename F::Parked parked[2];
 

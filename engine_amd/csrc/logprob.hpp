@@ -25,7 +25,7 @@ struct LogprobArgs {
     float* top_logprobs;      // [rows][top], or null
     int top;
     int splits;               // workgroups a row (launch_logprobs sets it)
-    uint64_t* partials;       // [rows][splits][2 + top], splits > 1
+    uint64_t* partials;       // [rows][splits][3 + top], splits > 1
 };
 
 // `scratch`: room of `scratch_bytes` for the partials of split rows.
