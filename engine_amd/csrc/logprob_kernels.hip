@@ -536,7 +536,7 @@ hipError_t launch(const LogprobArgs& a, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_logprobs(const LogprobArgs& args, int dtype, int cu_count, void* scratch, size_t scratch_bytes, hipStream_t stream) {
-    if (args.rows == 0 || args.rows > 0x7fffffffu || args.length == 0 || args.top < 0 || args.top > kLogprobMaxTop || args.top > (long long)args.length) return hipErrorInvalidValue;
+    if (args.rows == 0 || args.rows > 0xffffffffu / kThreads || args.length == 0 || args.top < 0 || args.top > kLogprobMaxTop || args.top > (long long)args.length) return hipErrorInvalidValue;
     LogprobArgs a = args;
     // Parts: until four workgroups a CU are there, of an iteration at least. With one, two, three, four, six a CU: 500 rows of
     // 151,936 bf16 with 20 alternatives 64.2, 64.3, 64.4, 63.5, 67.5 us; 64 of f32 31.1, 26.0, 26.4, 26.3, 30.0, without

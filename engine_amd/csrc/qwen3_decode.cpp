@@ -1258,20 +1258,26 @@ ribn_amd_status ribn_amd_logprobs(ribn_amd_context* ctx, const void* logits, siz
         if (st != RIBN_AMD_OK) return st;
     }
     DeviceGuard guard(ctx->device);
-    ribn_amd::LogprobArgs a{};
-    a.logits = logits;
-    a.stride = row_stride;
-    a.length = length;
-    a.rows = rows;
-    a.targets = targets;
-    a.logprobs = logprobs;
-    a.entropy = entropy;
-    a.top_tokens = top_tokens;
-    a.top_logprobs = top_logprobs;
-    a.top = (int)top;
+    // (a grid's threads are counted in 32 bits)
+    constexpr size_t kGroup = (size_t)1 << 22;
+    auto from = [](auto* p, size_t at) { return p != nullptr ? p + at : nullptr; };
+    hipError_t e = hipSuccess;
+    for (size_t r0 = 0; r0 < rows && e == hipSuccess; r0 += kGroup) {
+        ribn_amd::LogprobArgs a{};
+        a.logits = static_cast<const char*>(logits) + r0 * row_stride * (dtype == RIBN_AMD_F32 ? 4 : 2);
+        a.stride = row_stride;
+        a.length = length;
+        a.rows = std::min(rows - r0, kGroup);
+        a.targets = from(targets, r0);
+        a.logprobs = from(logprobs, r0);
+        a.entropy = from(entropy, r0);
+        a.top_tokens = from(top_tokens, r0 * top);
+        a.top_logprobs = from(top_logprobs, r0 * top);
+        a.top = (int)top;
+        e = ribn_amd::launch_logprobs(a, (int)dtype, ctx->cu_count, ctx->act_scratch, ribn_amd::gemv_act_scratch_bytes(), ctx->stream);
+    }
     static_assert(ribn_amd::kLogprobMaxTop == RIBN_AMD_MAX_LOGPROB_TOP && ribn_amd::kLogitF32 == RIBN_AMD_F32 &&
                   ribn_amd::kLogitBf16 == RIBN_AMD_BF16 && ribn_amd::kLogitF16 == RIBN_AMD_F16);
-    const hipError_t e = ribn_amd::launch_logprobs(a, (int)dtype, ctx->cu_count, ctx->act_scratch, ribn_amd::gemv_act_scratch_bytes(), ctx->stream);
     return e == hipSuccess ? ok() : driver(e, "launch logprobs");
 }
 

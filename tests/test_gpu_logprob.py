@@ -224,6 +224,32 @@ def test_the_lowest_after_nothing(env, dtype):
         check(run(env, view, [55001, 59999, 50000, 1], top), values, [55001, 59999, 50000, 1], top)
 
 
+def test_very_many_rows(env):
+    """More rows than a grid's 32-bit count of threads has room for, two tokens each: log p by the logits' difference."""
+    case(test="very_many_rows")
+    torch = env["torch"]
+    rows = 2 ** 24 + 5
+    g = torch.Generator(device="cuda:0").manual_seed(3)
+    x = (4 * torch.randn((rows, 2), device="cuda:0", generator=g)).half()
+    t = torch.randint(0, 3, (rows,), device="cuda:0", generator=g, dtype=torch.int32)  # 2: outside
+    lp, h = (torch.full((rows,), 7.0, device="cuda:0") for _ in range(2))
+    ids, alt = torch.full((rows, 1), -7, dtype=torch.int32, device="cuda:0"), torch.full((rows, 1), 7.0, device="cuda:0")
+    env["ops"].logprobs_into(x, t, lp, h, ids, alt)
+    torch.cuda.synchronize()
+    d = x[:, 0].double() - x[:, 1].double()
+    both = torch.stack((-torch.log1p(torch.exp(-d)), -torch.log1p(torch.exp(d))), 1)
+    want = torch.where(t == 0, both[:, 0], torch.where(t == 1, both[:, 1], torch.full_like(d, -float("inf"))))
+    inside = t < 2
+    assert torch.isinf(lp[~inside]).all()
+    rest = torch.expm1(-both.max(1)[0])
+    off = EPS * torch.clamp(rest, max=1.0) + HALF_STEP * want.abs()
+    assert ((lp.double() - want)[inside].abs() <= off[inside]).all()
+    assert torch.equal(ids[:, 0], (d < 0).int())
+    assert ((alt[:, 0].double() - both.max(1)[0]).abs() <= EPS * torch.clamp(rest, max=1.0) + HALF_STEP * both.max(1)[0].abs()).all()
+    entropy = -(both * torch.exp(both)).sum(1)
+    assert ((h.double() - entropy).abs() <= (2 * EPS + HALF_STEP) * entropy).all()
+
+
 def test_certain_models(env):
     """Log probabilities and entropies near 0 keep their digits."""
     case(test="certain")

@@ -265,6 +265,39 @@ def test_prompts_are_scored(env, fmt, chunk, gain):
     agree(dec.logprobs(targets=[5], entropy=True, top=32), logits[None], [5], 32)
 
 
+@pytest.mark.parametrize("vocab", [1237, 300, 33])
+def test_odd_vocabularies(env, vocab):
+    """Output matrices whose rows end inside a tile of the prefill matmul, and alternatives of nearly all tokens."""
+    case(test="vocab", vocab=vocab)
+    E = env["E"]
+    geometry = dict(TINY, vocab=vocab, layers=1)
+    w = small_weights(geometry, 12, centered=True)
+    store, handles = E.AmdWeightStore(env["ctx"]), {}
+    for name, val in w.items():
+        if isinstance(val, tuple):
+            t, k, n, enc = val
+            store.materialize_quantized(name, [k, n], t, enc)
+            handles[name] = store.quantized_tensor(name)
+        else:
+            handles[name] = to_dev(val)
+    layers = [{f: handles[f"blk.0.{f}"] for f in ("attn_q", "attn_k", "attn_v", "attn_output", "ffn_gate", "ffn_up", "ffn_down", "attn_norm",
+                                                  "attn_q_norm", "attn_k_norm", "ffn_norm")}]
+    cfg = E.AmdQwen3Config(**geometry)
+    dec = E.AmdQwen3Decode(env["ctx"], cfg, handles["token_embd"], handles["output"], handles["output_norm"], layers, 2)
+    cache = E.AmdKvCache(env["ctx"], cfg, 64)
+    toks = [int(t) for t in np.random.default_rng(3).integers(0, vocab, 38)]
+    got = dec.score_prompt(cache, toks[:37], 0, toks[1:], entropy=True, top=32)
+    orc = L.LongContextQwen3(geometry, w, 64, L.rope_turns(128, TINY["rope_base"]), i8=False)
+    orc.chunk(toks[:37], 0)
+    logits = np.stack([orc._gemv("output", O.rms_norm_raw(h, orc.w["output_norm"], TINY["epsilon"])) for h in orc.hiddens]).astype(np.float64)
+    off = 2 * MATMUL_TOL * np.abs(logits).max(1)
+    given, _, _, alternatives = P.logprobs(logits, toks[1:], 32)
+    assert (np.abs(got.logprobs - given) <= off).all() and (np.abs(got.top_logprobs - alternatives) <= off[:, None]).all()
+    assert (got.top_tokens < vocab).all() and all(len(set(r)) == 32 for r in got.top_tokens.tolist())
+    dec.decode_step(cache, toks[37], 37)
+    agree(dec.logprobs(targets=[vocab - 1], entropy=True, top=32), dec.copy_logits(0)[None], [vocab - 1], 32)
+
+
 @pytest.mark.parametrize("fmt", ["KV_F16", "KV_I4"])
 def test_scores_in_pieces(env, fmt):
     """Calls that go on from one another are the chunks of one call; what is not asked for changes nothing."""
