@@ -181,6 +181,39 @@ def test_decode_members(env, members):
     np.testing.assert_array_equal(again, got[order])
 
 
+@pytest.mark.parametrize("heads", [(2, 2), (4, 2), (8, 2), (16, 2)])
+def test_steps_that_fill_blocks(env, heads):
+    """Members whose new token is a block's last, among others, in caches with room for just that and for more; the codes
+    they leave, and the next steps over these."""
+    case(test="fill", heads=heads)
+    cfg = config(env, *heads)
+    rng = np.random.default_rng(heads[0])
+    lengths = [31, 63, 30, 511, 255, 1023, 31]
+    seqs = [Seq(env, cfg, n + room) for n, room in zip(lengths, (4, 200, 3, 4, 900, 4, 2000))]
+    for s, n in zip(seqs, lengths):
+        s.fill(rng, n)
+    for step in range(3):
+        check_decode(env, seqs, Step(rng, cfg, len(seqs)), [n + step for n in lengths], table(None))
+        for s in seqs:
+            s.check()
+    full = Seq(env, cfg, 32)
+    full.fill(rng, 31)
+    check_decode(env, [full], Step(rng, cfg, 1), [31], table(None))
+    full.check()
+
+
+def test_a_cache_of_one_token(env):
+    case(test="one")
+    cfg = config(env, 4, 2)
+    rng = np.random.default_rng(8)
+    s = Seq(env, cfg, 1)
+    check_decode(env, [s], Step(rng, cfg, 1), [0], table(None))
+    s.check()
+    t = Seq(env, cfg, 1)
+    check_prefill(env, t, Step(rng, cfg, 1), 1, 0, table(None))
+    t.check()
+
+
 def test_a_sequence_from_its_start(env):
     """Seventy steps from an empty cache, then back into the latest block, into an
     earlier one, onto a block's first position, and on from there."""
