@@ -21,13 +21,17 @@
 // reach (most of them, after the first ones) costs eight and a half VALU slots a logit, four of which are the exponential. Others move M, or
 // hand their candidates to the wave's Best.
 //
-// Memory bounds many rows: 2,047 of 151,936 f32 logits (1.24 GB) with one alternative 218 us, 5.7 TB/s; bf16 without
-// alternatives 120 (5.2 TB/s), with 1, 5, 20 of them 140, 150, 169: at 37 iterations a wave, nearly half hold one
+// What a row's alternatives reach: each wave publishes a logit that a fourth of `top` of its own are no less than, of
+// its first iteration from the lanes' largest ones, later from its sorted list. All four are no less than the least of these.
+//
+// Memory bounds many rows: 2,047 of 151,936 f32 logits (1.24 GB) with one alternative 217 us, 5.7 TB/s; bf16 without
+// alternatives 119 (5.2 TB/s), with 1, 5, 20 of them 138, 146, 164: at 37 iterations a wave, nearly half hold one
 // of the row's best so far. Of few rows, launches and round trips: one row of 151,936 with 5 10.5 us (7 and 3.5
-// on the card), 33 of 32,001 bf16 with 20 12.7 (9 and 4). A wave of one iteration takes 14,000 cycles for 20
-// alternatives: 2,200 until its logits are there, 1,100 their bound, 2,300 the candidates, 1,900 their sort, 2,500 M and the sums,
-// 1,000 until the others are there, 1,200 the waves' lists into one, 1,200 the sums' merge. (18,600, and 15.7 us of the 12.7, with candidates
-// taken register by register, keys compared one by one and twice, and the token at M found by branches.)
+// on the card), 33 of 32,001 bf16 with 20 12.3 (9 and 4). A wave of one iteration takes 12,200 cycles for 20
+// alternatives: 1,100 until its logits are there, 1,200 what they reach, 1,100 for the others' and again the logits, 2,000 its
+// candidates, 2,400 M and the sums, 900 sorting eight candidates, 900 for the others', 1,200 the waves' lists into one, 1,200 the sums' merge.
+// (18,600, and 15.7 us of the 12.3, with each wave bounding its own 20, candidates taken register by register, keys compared one by
+// one and twice, and the token at M found by branches.)
 #include "logprob.hpp"
 
 #include <algorithm>
@@ -47,6 +51,9 @@ constexpr int kBest = 128;                     // candidates a wave holds
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLeast = -160.0f;              // 2^kLeast is 0 in f32
 constexpr float kWide = 65536.0f;
+// Candidates a wave takes between two sorts. 8 / 12 / 24: 2,047 rows of 151,936 bf16 with 1 alternative 136.6 / 139.5 / 144.0 us, with 5
+// 144.7 / 146.8 / 152.7, with 20 165.4 / 165.0 / 166.7; 64 f32 rows with 20 25.0 / 24.8 / 24.0; 33 of 32,001 12.6 / 12.3 / 12.1.
+constexpr int kRoom = 12;
 
 // A number's place among all, a negative zero not among them.
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -114,22 +121,30 @@ __device__ __forceinline__ void sort_best(uint64_t* keys, int n, int top) {
     wave_sync();
 }
 
-// A wave's best `top` keys so far: candidates are appended, and sorted out when kRoom more are there.
+// What the n-th largest of a wave's `order`s is at least, by its upper 18 bits; 0 if that is no number.
+__device__ __forceinline__ uint32_t bound_of(uint32_t order, int n) {
+    uint32_t v = 0;
+    for (int bit = 31; bit >= 14; --bit) {
+        const uint32_t up = v | (1u << bit);
+        if (__popcll(__ballot(order >= up)) >= n) v = up;
+    }
+    return v > order_of(-INFINITY) ? v : 0;
+}
+
+// A wave's best `top` keys so far: candidates are appended, and sorted out when kRoom new ones are there.
 struct Best {
-    static constexpr int kRoom = 24;
     uint64_t* keys;      // LDS [kBest]
     int top;
     int count = 0;
-    bool sorted = true;
+    int sorted = 0;      // keys in order
     uint64_t least = 0;  // keys up to this one are none of the best
 
     __device__ __forceinline__ Best(uint64_t* room, int n) : keys(room), top(n) {}
     __device__ __forceinline__ float least_logit() const { return top == 0 ? INFINITY : least == 0 ? -INFINITY : logit_of(least); }
     __device__ __forceinline__ void sort() {
-        if (sorted) return;
-        sorted = true;
+        if (sorted == count) return;
         sort_best(keys, count, top);
-        count = min(count, top);
+        sorted = count = min(count, top);
         if (count == top && top > 0) least = keys[top - 1];
     }
     // One candidate a lane (0: none).
@@ -139,18 +154,12 @@ struct Best {
         if (who == 0) return;
         if (has) keys[count + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key;
         count += __popcll(who);
-        sorted = false;
         if (count > kBest - 64) sort();
     }
-    // From each lane's best logit: what the top-th of them bounds from below, by its upper 18 bits.
+    // From each lane's best logit: what the top-th of them bounds from below.
     __device__ __forceinline__ void bound(uint32_t order) {
-        uint32_t v = 0;
-        for (int bit = 31; bit >= 14; --bit) {
-            const uint32_t up = v | (1u << bit);
-            if (__popcll(__ballot(order >= up)) >= top) v = up;
-        }
-        // (the order before v's is a logit's while v is not that of -inf, below which nothing is)
-        if (v > order_of(-INFINITY)) least = ((uint64_t)v << 32) - 1;
+        const uint32_t v = bound_of(order, top);
+        if (v != 0) least = ((uint64_t)v << 32) - 1;  // (the order before v's is a logit's)
     }
 };
 
@@ -224,8 +233,6 @@ struct Wave {
     float l = 0.f, e = 0.f;
     bool wide = false;  // |m| past kWide: the reference is m c exactly, t = (x - m) c
 
-    __device__ __forceinline__ float above(float x) const { return wide ? (x - m) * kLog2e : __builtin_fmaf(x, kLog2e, -ref); }
-
     // m moves to the largest of the lanes' `most`, and one of the logits at it (x is set to -inf) is left out; the one left
     // out so far counts.
     __device__ __forceinline__ void move(float to, float most, Logits& x) {
@@ -290,8 +297,13 @@ struct Wave {
             return;
         }
         Logits t;
+        if (wide) {
 #pragma unroll
-        for (int i = 0; i < kValues; ++i) t[i] = above(x[i]);
+            for (int i = 0; i < kValues; ++i) t[i] = (x[i] - m) * kLog2e;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kValues; ++i) t[i] = __builtin_fmaf(x[i], kLog2e, -ref);
+        }
         add(t);
     }
 };
@@ -357,23 +369,44 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
         for (int u = 0; u < kPieces; ++u) raw[u] = body[min(at + 64 * u + lane, last - 1)];
     };
     if (at < last) load();
+    auto unpack = [&](uint32_t now) {
+        Logits x;
+#pragma unroll
+        for (int u = 0; u < kPieces; ++u) {
+            const uint32_t words[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                if constexpr (DT == kLogitF32) x[kPer * u + j] = __builtin_bit_cast(float, words[j]);
+                else if constexpr (DT == kLogitF16) x[kPer * u + j] = half_bits_to_float((words[j >> 1] >> (16 * (j & 1))) & 0xffffu);
+                else x[kPer * u + j] = __builtin_bit_cast(float, (j & 1) ? words[j >> 1] & 0xffff0000u : words[j >> 1] << 16);
+            }
+        }
+        if (now + 64 * kPieces > last) {
+#pragma unroll
+            for (int i = 0; i < kValues; ++i) x[i] = now + 64 * (unsigned)(i / kPer) + lane < last ? x[i] : -INFINITY;
+        }
+        return x;
+    };
     const float given = wave == 0 && a.splits == 1 ? given_logit<DT>(a, row) : 0.f;
-    if (threadIdx.x < kWaves) reached[threadIdx.x] = -INFINITY;
-    __syncthreads();
     const int share = (a.top + kWaves - 1) / kWaves;
+    if (a.top > 0) {
+        const uint32_t v = at < last ? bound_of(order_of(most_of(unpack(at))), share) : 0;
+        if (lane == 0) reached[wave] = v != 0 ? logit_of((uint64_t)v << 32) : -INFINITY;
+    }
+    __syncthreads();
     auto sort = [&] {
         best.sort();
-        if (share > 0 && best.count >= share && lane == 0) __hip_atomic_store(&reached[wave], logit_of(keys[wave][share - 1]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        if (best.count >= share && lane == 0) __hip_atomic_store(&reached[wave], logit_of(keys[wave][share - 1]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     };
     // What a candidate is at least: past the wave's own (its tokens rise, so that of equals the earlier is in), and
     // what the four waves reach together. `past` and `from`: the t past m, and that of such a candidate too.
-    float least = a.top > 0 ? -INFINITY : INFINITY, past = -INFINITY, from = -INFINITY;
+    float shared = INFINITY, least = INFINITY, past = -INFINITY, from = -INFINITY;
     auto thresholds = [&] {
         if (a.top > 0) {
-            least = INFINITY;
+            shared = INFINITY;
 #pragma unroll
-            for (int i = 0; i < kWaves; ++i) least = fminf(least, __hip_atomic_load(&reached[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
-            if (best.least != 0) least = fmaxf(least, above_next(logit_of(best.least)));
+            for (int i = 0; i < kWaves; ++i) shared = fminf(shared, __hip_atomic_load(&reached[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+            least = best.least != 0 ? fmaxf(shared, above_next(logit_of(best.least))) : shared;
         }
         from = least <= w.m ? fminf(past, __builtin_fmaf(least, kLog2e, -w.ref)) : past;
     };
@@ -382,26 +415,14 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
     const uint32_t token = (uint32_t)lane < head ? (uint32_t)lane : end + ((uint32_t)lane - head);
     const float one = (uint32_t)lane < singles ? load_logit<DT>(base, token) : -INFINITY;
     bool single = false;
+    thresholds();
     for (uint32_t round = 0;; ++round) {
         Logits x;
         const uint32_t now = at;
         if (at < last) {
-#pragma unroll
-            for (int u = 0; u < kPieces; ++u) {
-                const uint32_t words[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-#pragma unroll
-                for (int j = 0; j < kPer; ++j) {
-                    if constexpr (DT == kLogitF32) x[kPer * u + j] = __builtin_bit_cast(float, words[j]);
-                    else if constexpr (DT == kLogitF16) x[kPer * u + j] = half_bits_to_float((words[j >> 1] >> (16 * (j & 1))) & 0xffffu);
-                    else x[kPer * u + j] = __builtin_bit_cast(float, (j & 1) ? words[j >> 1] & 0xffff0000u : words[j >> 1] << 16);
-                }
-            }
+            x = unpack(now);
             at += kThreads * kPieces;
             load();
-            if (now + 64 * kPieces > last) {
-#pragma unroll
-                for (int i = 0; i < kValues; ++i) x[i] = now + 64 * (unsigned)(i / kPer) + lane < last ? x[i] : -INFINITY;
-            }
         } else {
             if (single || singles == 0) break;
             single = true;
@@ -418,13 +439,13 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
         bool changed = (round & 3) == 3, taken = false;
         if (w.wide || single || __any(top >= from)) {
             if (a.top > 0) {
-                if (best.count < a.top) best.bound(order_of(most_of(x)));
-                collect(best, x, single ? best.least_logit() : fmaxf(least, best.least_logit()), [&](float v, int i) {
+                if (best.count < a.top && least == -INFINITY) best.bound(order_of(most_of(x)));
+                collect(best, x, fmaxf(single ? shared : least, best.least_logit()), [&](float v, int i) {
                     if (single) return i == 0 && (uint32_t)lane < singles ? key_of(v, token) : 0;
                     const uint32_t piece = now + 64 * (unsigned)(i / kPer) + lane;
                     return piece < last ? key_of(v, head + piece * kPer + (unsigned)(i % kPer)) : 0;
                 });
-                if (best.count > a.top + (round == 0 ? 0 : Best::kRoom)) {
+                if (best.count >= best.sorted + kRoom) {
                     sort();
                     changed = true;
                 }
