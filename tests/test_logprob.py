@@ -84,3 +84,26 @@ def test_python_checks():
 def test_no_context_is_refused():
     lib = _lib.load()
     assert _lib.STATUS_NAMES[lib.ribn_amd_logprobs(None, None, 0, 0, 0, 0, 0, None, None, None, None, None, 0)] == "InvalidArgument"
+
+
+def test_no_decoder_is_refused():
+    lib = _lib.load()
+    one, out = (ctypes.c_uint32 * 1)(0), (ctypes.c_float * 1)()
+    for status in (lib.ribn_amd_qwen3_logprobs(None, 1, None, out, None, None, None, 0),
+                   lib.ribn_amd_qwen3_score_prompt(None, None, one, 1, 0, 0, one, out, None, None, None, 0)):
+        assert _lib.STATUS_NAMES[status] == "InvalidArgument"
+    assert out[0] == 0.0
+
+
+class FakeDecoder(E.AmdQwen3Decode):
+    def __init__(self):
+        self.ctx, self.config, self.handle = FakeCtx(), E.AmdQwen3Config(vocab=40), ctypes.c_void_p(0)
+
+
+def test_python_checks_of_a_decoder():
+    dec, cache = FakeDecoder(), FakeCtx()
+    for bad in (lambda: dec.logprobs(2, targets=[1]), lambda: dec.logprobs(1, top=41), lambda: dec.logprobs(1, top=-1),
+                lambda: dec.score_prompt(cache, [1, 2, 3], 0, [2, 3]), lambda: dec.score_prompt(cache, [1], 0, [1], top=41),
+                lambda: dec.score_prompt(cache, [1], 0, top=-1)):
+        with pytest.raises(ValueError):
+            bad()
