@@ -226,6 +226,8 @@ struct ribn_amd_qwen3_decode {
     // Log probabilities (ribn_amd_qwen3_logprobs, ribn_amd_qwen3_score_prompt): one allocation, grown on demand.
     void* score_block;
     size_t score_bytes;
+    char* score_host;     // pinned, for its results on their way to the caller
+    size_t score_host_bytes;
 };
 
 namespace {
@@ -689,7 +691,7 @@ hipError_t enqueue_prompt_chunk(ribn_amd_qwen3_decode* d, ribn_amd_kv_cache* cac
     return e;
 }
 
-// Device arrays of the log probabilities of `rows` rows, and `logit_rows` rows of logits, in the score block.
+// Device arrays of the log probabilities of `rows` rows, the four results one behind another, and rows of logits, in the score block.
 struct ScoreBuffers {
     uint32_t* targets;
     float* logprobs;
@@ -697,33 +699,41 @@ struct ScoreBuffers {
     uint32_t* top_tokens;
     float* top_logprobs;
     float* logits;
+    size_t rows;
 };
 
-// Grows the score block, synchronising the context stream then.
+// Grows the score block and its host side, synchronising the context stream then.
 ribn_amd_status reserve_score(ribn_amd_qwen3_decode* d, size_t rows, size_t top, size_t logit_rows, ScoreBuffers* out) {
-    const size_t sizes[6] = {rows, rows, rows, rows * top, rows * top, logit_rows * d->cfg.vocab};
-    size_t offsets[6], bytes = 0;
-    for (int i = 0; i < 6; ++i) {
-        offsets[i] = bytes;
-        bytes += align_up(sizes[i] * sizeof(float));
-    }
-    if (bytes > d->score_bytes) {
+    const size_t results = rows * (2 + 2 * top) * sizeof(float);
+    const size_t targets_bytes = align_up(rows * sizeof(uint32_t)), bytes = targets_bytes + align_up(results) + logit_rows * d->cfg.vocab * sizeof(float);
+    if (bytes > d->score_bytes || results > d->score_host_bytes) {
         hipError_t e = hipStreamSynchronize(d->ctx->stream);
         if (e != hipSuccess) return driver(e, "synchronize before replacing the score workspace");
-        if (d->score_block != nullptr) hipFree(d->score_block);
-        d->score_block = nullptr;
-        d->score_bytes = 0;
-        e = hipMalloc(&d->score_block, bytes);
-        if (e != hipSuccess) {
+        if (bytes > d->score_bytes) {
+            if (d->score_block != nullptr) hipFree(d->score_block);
             d->score_block = nullptr;
-            return driver(e, "hipMalloc score workspace");
+            d->score_bytes = 0;
+            void* block = nullptr;
+            e = hipMalloc(&block, bytes);
+            if (e != hipSuccess) return driver(e, "hipMalloc score workspace");
+            d->score_block = block;
+            d->score_bytes = bytes;
         }
-        d->score_bytes = bytes;
+        if (results > d->score_host_bytes) {
+            if (d->score_host != nullptr) hipHostFree(d->score_host);
+            d->score_host = nullptr;
+            d->score_host_bytes = 0;
+            void* host = nullptr;
+            e = hipHostMalloc(&host, results, hipHostMallocDefault);
+            if (e != hipSuccess) return driver(e, "hipHostMalloc score results");
+            d->score_host = static_cast<char*>(host);
+            d->score_host_bytes = results;
+        }
     }
     char* p = static_cast<char*>(d->score_block);
-    *out = ScoreBuffers{reinterpret_cast<uint32_t*>(p + offsets[0]), reinterpret_cast<float*>(p + offsets[1]),
-                        reinterpret_cast<float*>(p + offsets[2]),    reinterpret_cast<uint32_t*>(p + offsets[3]),
-                        reinterpret_cast<float*>(p + offsets[4]),    reinterpret_cast<float*>(p + offsets[5])};
+    float* f = reinterpret_cast<float*>(p + targets_bytes);
+    *out = ScoreBuffers{reinterpret_cast<uint32_t*>(p), f, f + rows, reinterpret_cast<uint32_t*>(f + 2 * rows), f + (2 + top) * rows,
+                        reinterpret_cast<float*>(p + targets_bytes + align_up(results)), rows};
     return RIBN_AMD_OK;
 }
 
@@ -756,17 +766,26 @@ hipError_t enqueue_logprobs(ribn_amd_qwen3_decode* d, const float* logits, const
     return ribn_amd::launch_logprobs(a, ribn_amd::kLogitF32, d->ctx->cu_count, d->ctx->act_scratch, ribn_amd::gemv_act_scratch_bytes(), d->ctx->stream);
 }
 
-// Copies the score buffers' first `rows` rows to host arrays (null: not asked for).
+// Copies the score buffers' first `rows` rows to host arrays (null: not asked for): those from the first array asked for to
+// the last at once, by way of pinned memory (with a copy of its own into each of the caller's, ribn_amd_qwen3_logprobs of 8 members and
+// 20 alternatives took 73.9 us, so 30.0).
 hipError_t read_scores(ribn_amd_qwen3_decode* d, const ScoreBuffers& b, size_t rows, float* logprobs, float* entropy, uint32_t* top_tokens,
                        float* top_logprobs, size_t top) {
     void* const host[4] = {logprobs, entropy, top_tokens, top_logprobs};
-    const void* const device[4] = {b.logprobs, b.entropy, b.top_tokens, b.top_logprobs};
+    const size_t begin[5] = {0, b.rows, 2 * b.rows, (2 + top) * b.rows, (2 + 2 * top) * b.rows};
+    int first = 4, last = 0;
     for (int i = 0; i < 4; ++i) {
         if (host[i] == nullptr) continue;
-        const hipError_t e = hipMemcpyAsync(host[i], device[i], rows * (i < 2 ? 1 : top) * sizeof(float), hipMemcpyDeviceToHost, d->ctx->stream);
-        if (e != hipSuccess) return e;
+        first = std::min(first, i);
+        last = i;
     }
-    return hipStreamSynchronize(d->ctx->stream);
+    const size_t from = begin[first] * sizeof(float), bytes = begin[last + 1] * sizeof(float) - from;
+    hipError_t e = hipMemcpyAsync(d->score_host + from, reinterpret_cast<const char*>(b.logprobs) + from, bytes, hipMemcpyDeviceToHost, d->ctx->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(d->ctx->stream);
+    for (int i = first; i <= last && e == hipSuccess; ++i) {
+        if (host[i] != nullptr) std::memcpy(host[i], d->score_host + begin[i] * sizeof(float), rows * (i < 2 ? 1 : top) * sizeof(float));
+    }
+    return e;
 }
 
 // Rows of logits at once: 2,048 tokens of a vocabulary of 151,936 (2 layers of 4,096) take 6.5 ms by 256, 6.1 by 512, 5.7 by
@@ -1399,6 +1418,7 @@ void ribn_amd_qwen3_decode_destroy(ribn_amd_qwen3_decode* d) {
     hipFree(d->block);
     if (d->prompt_block) hipFree(d->prompt_block);
     if (d->score_block) hipFree(d->score_block);
+    if (d->score_host) hipHostFree(d->score_host);
     ribn_amd_context* ctx = d->ctx;
     delete d;
     context_release(ctx);
