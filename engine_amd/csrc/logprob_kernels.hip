@@ -23,6 +23,8 @@
 //
 // What a row's alternatives reach: each wave publishes a logit that a fourth of `top` of its own are no less than, of
 // its first iteration from the lanes' largest ones, later from its sorted list. All four are no less than the least of these.
+// (When a wave sees what the others publish is a matter of time, and decides which logits it looks at as candidates, never a result: the
+// sums take either way by the wave's own M.)
 //
 // Memory bounds many rows: 2,047 of 151,936 f32 logits (1.24 GB) with one alternative 217 us, 5.7 TB/s; bf16 without
 // alternatives 119 (5.2 TB/s), with 1, 5, 20 of them 138, 146, 164: at 37 iterations a wave, nearly half hold one
