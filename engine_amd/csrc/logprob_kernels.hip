@@ -250,7 +250,9 @@ struct Wave {
         wide = !(fabsf(m) < kWide);
         ref = wide ? 0.f : m * kLog2e;
         if (old > -INFINITY) {
-            const float d = fmaxf(wide || was_wide ? (old - m) * kLog2e : old_ref - ref, kLeast), f = __builtin_amdgcn_exp2f(d);
+            // between what the sums are relative to: with |m| past kWide m c itself, else its f32
+            const double from = was_wide ? (double)old * (double)kLog2e : (double)old_ref, at = wide ? (double)m * (double)kLog2e : (double)ref;
+            const float d = fmaxf((float)(from - at), kLeast), f = __builtin_amdgcn_exp2f(d);
             e = f * __builtin_fmaf(d, l, e);
             l *= f;
         }

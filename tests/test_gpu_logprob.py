@@ -408,3 +408,32 @@ def test_refusals(env):
     assert call(out=p(lp, 2)) == "InvalidArgument"
     assert call(logits=p(x, 2), dtype=1, n=239) == "Ok"
     env["torch"].cuda.synchronize()
+
+
+@pytest.mark.parametrize("rows,n", [(6, 12300), (64, 100003), (520, 12300)])
+def test_the_top_crosses_two_to_the_sixteen(env, rows, n):
+    """Rows whose largest logit so far passes 65,536 or -65,536 by little, while many tokens lie at what it was before:
+    one workgroup a row and several, one iteration of a wave and more. Each of at most six moves scales the sums by a factor
+    off by 2^-23 and two roundings, 1.8e-6 in all, and |x - M| is 3 at most (4e-7): within EPS."""
+    case(test="crosses", rows=rows, n=n)
+    rng = np.random.default_rng(n)
+    at = np.arange(n)
+    x = np.zeros((rows, n))
+    for r in range(rows):
+        low, high = [(65535.5, 65536.0), (-65536.5, -65535.5), (65535.0, 65537.0), (-65537.0, -65534.5)][r % 4]
+        kind = (r // 4) % 5
+        if kind == 0:    # the last token alone
+            x[r] = np.where(at == n - 1, high, low)
+        elif kind == 1:  # halves
+            x[r] = np.where(at < n // 2, low, high)
+        elif kind == 2:  # 4,096 tokens in turn, as a workgroup takes them
+            x[r] = np.where(at // 4096 % 2, high, low)
+        elif kind == 3:  # in four steps
+            x[r] = low + (high - low) / 4 * (5 * at // n)
+        else:            # among others, over the border and back
+            x[r] = np.where(at // 4096 % 2, high, low) - rng.integers(0, 64, n) / 64
+    view, values = typed(env, x, "float32")
+    np.testing.assert_array_equal(values, x)
+    t = rng.integers(0, n, rows)
+    for top in (0, 5):
+        check(run(env, view, t, top), values, t, top)
