@@ -7,7 +7,8 @@
 //   log p(x) = (x - M) - log1p(R'),   entropy = log1p(R') - ln 2 E' / (1 + R').
 // The token at M is left out of R, and log1p taken of the rest, since a certain model's log
 // probability is R itself, which a sum with the 1 in it rounds away. A lane's sums are f32, 16 terms
-// first; those over lanes, waves and workgroups f64.
+// first; those over lanes, waves and workgroups f64. A term is off by t's rounding, up to 6e-8 |x - M| of it, either way; what c is
+// short of log2 e would add 1.3e-8 |x - M| to each, always up, and is taken back at the end (finish).
 //
 // NaN and -inf have probability 0: where an iteration's E is no number it is formed again with t raised to -160, where
 // 2^t is 0 and so is t 2^t (and a maximum takes the operand that is a number). A row of nothing else has no M (-inf):
@@ -51,6 +52,8 @@ constexpr int kIteration = kThreads * kValues;
 typedef float Logits __attribute__((ext_vector_type(kValues)));  // (a vector: of an array, a choice by lane is a load from scratch)
 constexpr int kBest = 128;                     // candidates a wave holds
 constexpr float kLog2e = 1.44269504088896341f;
+constexpr double kLn2 = 0.69314718055994530942;
+constexpr double kShort = 1.0 - (double)kLog2e * kLn2;  // 1.335e-8: what c is short of log2 e, of itself
 constexpr float kLeast = -160.0f;              // 2^kLeast is 0 in f32
 constexpr float kWide = 65536.0f;
 // Candidates a wave takes between two sorts. 8 / 12 / 24: 2,047 rows of 151,936 bf16 with 1 alternative 136.6 / 139.5 / 144.0 us, with 5
@@ -213,14 +216,21 @@ template <int DT> __device__ __forceinline__ float given_logit(const LogprobArgs
 // A row's results by a wave, from its sums and its best keys in order.
 __device__ __forceinline__ void finish(const LogprobArgs& a, size_t row, const Row& s, float given, const uint64_t* best) {
     const int lane = threadIdx.x & 63;
-    const double rest = log1pf((float)s.r);  // (all of a result's parts have its sign: f32 is as good as its own rounding)
+    // e^(x - M) = 2^t (1 + kShort ln2 t) to first order, so that E times kShort ln 2 is what R' lacks; what E' lacks is the
+    // second moment's, which is E'^2 / R' of tokens that lie equally far below M, and more of others by their variance.
+    double r = s.r, e = s.e;
+    if (r > 0.0) {
+        r += kShort * kLn2 * e;
+        e += kShort * (e + kLn2 * e * e / s.r);
+    }
+    const double rest = log1pf((float)r);  // (all of a result's parts have its sign: f32 is as good as its own rounding)
     auto logprob = [&](float x) {
         if (!(x > -INFINITY)) return -INFINITY;  // (or no number)
         return (float)((x == s.m ? 0.0 : (double)x - (double)s.m) - rest);
     };
     if (lane == 0) {
         if (a.logprobs != nullptr) a.logprobs[row] = logprob(given);
-        if (a.entropy != nullptr) a.entropy[row] = s.m == -INFINITY ? 0.f : (float)fmax(rest - 0.69314718055994530942 * s.e / (1.0 + s.r), 0.0);
+        if (a.entropy != nullptr) a.entropy[row] = s.m == -INFINITY ? 0.f : (float)fmax(rest - kLn2 * e / (1.0 + r), 0.0);
     }
     if (lane < a.top) {
         const uint64_t key = best[lane];

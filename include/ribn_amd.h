@@ -759,8 +759,9 @@ ribn_amd_status ribn_amd_argmax(ribn_amd_context *ctx, const float *logits, size
  * has probability 0 (log probability -inf; NaN ranks as -inf); a row of nothing else has log probabilities of
  * -inf and an entropy of 0. Tokens of +inf share the probability. Logits are aligned to their element.
  * Sums are formed beside the likeliest token, so that log probabilities near 0 keep their digits as others do (1e-5 of
- * a result at most, 1e-7 as a rule). A row's last bits may depend on the number of rows. Partial
- * results use the context's scratch, in stream order. */
+ * a result at most, 1e-7 as a rule; where a single token g below the likeliest is nearly all the rest, up to 6e-8 g;
+ * what is below 1e-37 may come out as 0).
+ * A row's last bits may depend on the number of rows. Partial results use the context's scratch, in stream order. */
 #define RIBN_AMD_MAX_LOGPROB_TOP 32u
 ribn_amd_status ribn_amd_logprobs(ribn_amd_context *ctx, const void *logits, size_t logits_len, size_t rows,
                                   size_t length, size_t row_stride, uint32_t dtype, const uint32_t *targets,

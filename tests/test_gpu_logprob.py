@@ -437,3 +437,31 @@ def test_the_top_crosses_two_to_the_sixteen(env, rows, n):
     t = rng.integers(0, n, rows)
     for top in (0, 5):
         check(run(env, view, t, top), values, t, top)
+
+
+@pytest.mark.parametrize("n", [3000, 20000])
+@pytest.mark.parametrize("gap", [50, 65, 80, 86])
+def test_far_runners_up_keep_their_digits(env, n, gap):
+    """One token `gap` nats below the likeliest and no other: log p of the likeliest is -R = -2^t, t = (x - M) log2 e, with
+    M = 0 and t all but free of rounding (x is chosen so), which leaves the exponential's last place (2^-23), log1p's two
+    and R's rounding to f32: 3 * 2^-23 + 2^-24 = 4.2e-7 of it at any gap. The entropy (1 + gap) R: the same and
+    its own rounding."""
+    case(test="runner_up", n=n, gap=gap)
+    rng = np.random.default_rng(gap)
+    log2e = np.float64(np.float32(1.44269504088896341))
+    x = -(gap + rng.random(40000)).astype(np.float32)
+    exact = x.astype(np.float64) * log2e  # (48 bits)
+    best = np.argsort(np.abs(exact.astype(np.float32).astype(np.float64) - exact), kind="stable")[:12]
+    x = x[best].astype(np.float64)
+    assert (np.abs((x * log2e).astype(np.float32) - x * log2e) < 2.0 ** -27).all()
+    rows = np.full((12, n), -1000.0)
+    rows[:, n // 3] = 0.0
+    rows[np.arange(12), rng.permutation(n // 3)[:12]] = x
+    view, values = typed(env, rows, "float32")
+    lp, h, _, _ = run(env, view, [n // 3] * 12, 2)
+    want = np.log1p(np.exp(x))
+    print("CASE off", float(np.abs(-lp / want - 1).max()), float(np.abs(h / (want - x * np.exp(x) / (1 + np.exp(x))) - 1).max()))
+    bound = 3 * 2.0 ** -23 + 2.0 ** -24 + 2.0 ** -27
+    assert (np.abs(-lp.astype(np.float64) - want) <= bound * want).all()
+    entropy = want - x * np.exp(x) / (1 + np.exp(x))
+    assert (np.abs(h - entropy) <= (bound + 2.0 ** -24) * entropy).all()
