@@ -192,6 +192,7 @@ struct ribn_amd_qwen3_decode {
     float* gate;      // [members][ffn]
     float* up;
     float* logits;    // [members][vocab]
+    int logit_members;    // rows of logits that the last step with an output head left (0: none yet)
     uint32_t* tokens;     // [members] input token of the next step
     uint32_t* selected;   // [members] greedy selection of the last step
     int32_t* positions;   // [members]
@@ -433,9 +434,12 @@ void destroy_graphs(ribn_amd_qwen3_decode* d) {
 ribn_amd_status run_step(ribn_amd_qwen3_decode* d, int members, bool head, bool advance, bool appended = false) {
     hipStream_t stream = d->ctx->stream;
     const GraphKey key{members, head, advance, appended, d->chunks, d->cache};
+    if (head) d->logit_members = 0;  // (while its launches may fail)
     if (!d->graphs) {
         hipError_t e = enqueue_step(d, key, stream);
-        return e == hipSuccess ? ok() : driver(e, "launch decode step");
+        if (e != hipSuccess) return driver(e, "launch decode step");
+        if (head) d->logit_members = members;
+        return ok();
     }
     GraphEntry* hit = nullptr;
     for (GraphEntry& g : d->graph_cache) {
@@ -471,7 +475,9 @@ ribn_amd_status run_step(ribn_amd_qwen3_decode* d, int members, bool head, bool 
         hit = &d->graph_cache.back();
     }
     hipError_t e = hipGraphLaunch(hit->exec, stream);
-    return e == hipSuccess ? ok() : driver(e, "hipGraphLaunch");
+    if (e != hipSuccess) return driver(e, "hipGraphLaunch");
+    if (head) d->logit_members = members;
+    return ok();
 }
 
 ribn_amd_status check_weight(const ribn_amd_context* ctx, const ribn_amd_quantized_weight* w, uint64_t K, uint64_t N,
@@ -1636,6 +1642,10 @@ ribn_amd_status ribn_amd_qwen3_logprobs(ribn_amd_qwen3_decode* d, size_t members
     if (members == 0) return fail(RIBN_AMD_INPUT_LENGTH, 1, 0, "log probabilities need at least one member");
     if (members > d->max_members) {
         return fail(RIBN_AMD_INVALID_PLAN, d->max_members, members, "the decoder was built for %u members", d->max_members);
+    }
+    if (members > (size_t)d->logit_members) {
+        return fail(RIBN_AMD_INVALID_PLAN, (uint64_t)d->logit_members, members, "the last step with an output head had %d members, not %zu",
+                    d->logit_members, members);
     }
     // (no targets: the tokens selected)
     ribn_amd_status st = check_logprob_request(targets != nullptr || logprobs != nullptr, logprobs != nullptr, entropy != nullptr, top_tokens != nullptr,

@@ -253,8 +253,9 @@ class AmdQwen3Decode:
         return out
 
     def logprobs(self, members: int = 1, targets=None, logprobs: bool = True, entropy: bool = False, top: int = 0) -> TokenLogprobs:
-        """Log probabilities of the last step's first `members` members: of `targets` (host tokens, by default the ones
-        the step selected), the entropy, and the `top` likeliest tokens (ribn_amd_qwen3_logprobs). Blocking."""
+        """Log probabilities of the first `members` members of the last step with an output head (no more than it had): of
+        `targets` (host tokens, by default the ones the step selected), the entropy, and the `top` likeliest tokens
+        (ribn_amd_qwen3_logprobs). Blocking."""
         goal = None if targets is None else np.ascontiguousarray(np.asarray(targets, dtype=np.uint32).reshape(-1))
         if goal is not None and goal.size != members:
             raise ValueError(f"{members} members need as many targets, got {goal.size}")

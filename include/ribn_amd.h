@@ -865,7 +865,8 @@ ribn_amd_status ribn_amd_qwen3_copy_logits(ribn_amd_qwen3_decode *decode, size_t
 /* Log probabilities, entropy and alternatives (ribn_amd_logprobs' definitions; no reference counterpart) of the first
  * `members` members of the last step with an output head, from the logits that ribn_amd_qwen3_copy_logits copies. targets:
  * host array [members], NULL: the tokens the step selected (of ribn_amd_qwen3_generate, its last ones). Results are host arrays, [members] and
- * [members][top]; each of logprobs, entropy and the two top arrays may be NULL, not all of them. Blocking. */
+ * [members][top]; each of logprobs, entropy and the two top arrays may be NULL, not all of them. More members than that step
+ * had are refused, and any before the first one (InvalidPlan). Blocking. */
 ribn_amd_status ribn_amd_qwen3_logprobs(ribn_amd_qwen3_decode *decode, size_t members, const uint32_t *targets,
                                         float *logprobs, float *entropy, uint32_t *top_tokens, float *top_logprobs,
                                         size_t top);

@@ -460,3 +460,45 @@ def test_refusals(env):
     assert lib.ribn_amd_qwen3_score_prompt(n, cache.handle, n, 1, 0, 0, n, n, n, n, n, 0) != 0
     np.testing.assert_array_equal(dec.copy_logits(0), logits)  # nothing ran
     agree(step(1, targets=[TINY["vocab"]], top=1), logits[None], [TINY["vocab"]], 1)
+
+
+def test_rows_that_no_step_computed_are_refused(env):
+    """Log probabilities are of the last step with an output head: of no more members than it had, of none before it."""
+    case(test="no_step")
+    E = env["E"]
+    cfg, _ = model(env)
+    dec = env["decoder"](cfg, 4)
+    caches = [E.AmdKvCache(env["ctx"], cfg, CAP, format=E.KV_I4) for _ in range(4)]
+    toks = prompt(40)
+
+    def have(n):
+        got = dec.logprobs(n, entropy=True, top=3) if n else None
+        for m in range(n + 1, 5):
+            with pytest.raises(E.AmdKernelError) as e:
+                dec.logprobs(m, entropy=True, top=3)
+            assert e.value.kind == "InvalidPlan", str(e.value)
+        if n:
+            agree(got, np.stack([dec.copy_logits(i) for i in range(n)]), got.top_tokens[:, 0], 3)
+
+    have(0)
+    dec.prefill_step(caches[0], toks[0], 0)
+    dec.prefill_chunk(caches[0], toks[1:4], 1)
+    dec.prefill_prompt(caches[0], toks[4:20], 4)
+    dec.score_prompt(caches[0], toks[20:39], 20, toks[21:40])
+    have(0)
+    dec.decode_step(caches[0], toks[39], 39)
+    have(1)
+    dec.decode_step_batch(caches[1:], [1, 2, 3], [0, 0, 0])
+    have(3)
+    dec.prefill_chunk(caches[0], [4, 5, 6, 7], 40)  # (no output head)
+    have(3)
+    dec.set_graphs(False)
+    dec.decode_step_batch(caches[1:3], [1, 2], [1, 1])
+    have(2)
+    with pytest.raises(E.AmdKernelError):
+        dec.decode_step_batch(caches, [1, 2, 3, 4], [44, 2, 2, CAP])  # refused before anything runs
+    have(2)
+    dec.generate(caches, [1, 2, 3, 4], [44, 2, 2, 1], 3)
+    have(4)
+    dec.decode_step(caches[0], 1, 47)
+    have(1)
