@@ -172,6 +172,16 @@ class TokenLogprobs:
         return [None if a is None else a.ctypes.data for a in (self.logprobs, self.entropy, self.top_tokens, self.top_logprobs)]
 
 
+def _host_tokens(tokens, vocab: int) -> np.ndarray:
+    """Whole numbers as the library takes tokens, those outside the vocabulary as one that 32 bits hold."""
+    t = np.asarray(tokens).reshape(-1)
+    if t.size and t.dtype.kind not in "iu":
+        raise TypeError(f"tokens are whole numbers, got {t.dtype}")
+    out = t.astype(np.uint32)
+    out[(t < 0) | (t >= vocab)] = 0xffffffff
+    return out
+
+
 class AmdQwen3Decode:
     """Decode-step executor (CudaQwen35Decode + CudaQwen35BatchDecode).
 
@@ -240,8 +250,8 @@ class AmdQwen3Decode:
         """prefill_prompt, and of each token's successor: the log probability of targets[i] (host tokens, one per prompt
         token; one outside the vocabulary has -inf), the distribution's entropy, and the `top` likeliest tokens with
         their log probabilities (ribn_amd_qwen3_score_prompt). Blocking."""
-        tok = np.ascontiguousarray(np.asarray(tokens, dtype=np.uint32).reshape(-1))
-        goal = None if targets is None else np.ascontiguousarray(np.asarray(targets, dtype=np.uint32).reshape(-1))
+        tok = _host_tokens(tokens, self.config.vocab)
+        goal = None if targets is None else _host_tokens(targets, self.config.vocab)
         if goal is not None and goal.size != tok.size:
             raise ValueError(f"{tok.size} tokens need as many targets, got {goal.size}")
         if not 0 <= top <= self.config.vocab:
@@ -256,7 +266,7 @@ class AmdQwen3Decode:
         """Log probabilities of the first `members` members of the last step with an output head (no more than it had): of
         `targets` (host tokens, by default the ones the step selected), the entropy, and the `top` likeliest tokens
         (ribn_amd_qwen3_logprobs). Blocking."""
-        goal = None if targets is None else np.ascontiguousarray(np.asarray(targets, dtype=np.uint32).reshape(-1))
+        goal = None if targets is None else _host_tokens(targets, self.config.vocab)
         if goal is not None and goal.size != members:
             raise ValueError(f"{members} members need as many targets, got {goal.size}")
         if not 0 <= top <= self.config.vocab:

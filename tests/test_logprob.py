@@ -107,3 +107,56 @@ def test_python_checks_of_a_decoder():
                 lambda: dec.score_prompt(cache, [1], 0, top=-1)):
         with pytest.raises(ValueError):
             bad()
+
+
+class Recorder(FakeDecoder):
+    """Host tokens as the library is given them."""
+
+    def __init__(self):
+        super().__init__()
+        self.seen = []
+
+        def words(at, n):
+            return None if at is None else list((ctypes.c_uint32 * n).from_address(at))
+
+        def score(handle, cache, tokens, count, position, chunk, targets, *rest):
+            self.seen.append((words(tokens, count), words(targets, count)))
+            return 0
+
+        def step(handle, members, targets, *rest):
+            self.seen.append(words(targets, members))
+            return 0
+
+        self.ctx._lib.ribn_amd_qwen3_score_prompt, self.ctx._lib.ribn_amd_qwen3_logprobs = score, step
+
+
+OUTSIDE = [-1, -100, 2 ** 32 + 5, 2 ** 32, 40, -2 ** 32 + 3, 2 ** 32 - 1]
+
+
+@pytest.mark.parametrize("as_", [list, tuple, lambda x: np.array(x, np.int64)], ids=("list", "tuple", "int64"))
+def test_tokens_outside_32_bits(as_):
+    """A target outside the vocabulary, -1 among them, has no probability: it must not become a token by its lower 32
+    bits. A prompt's own token outside it reaches the library as one that it refuses."""
+    dec, cache = Recorder(), FakeCtx()
+    goal = as_([3, 39] + OUTSIDE)
+    dec.score_prompt(cache, [1] * 9, 0, goal)
+    (tokens, targets), = dec.seen
+    assert tokens == [1] * 9 and targets[:2] == [3, 39] and min(targets[2:]) >= 40
+    dec.logprobs(9, goal)
+    assert dec.seen[1][:2] == [3, 39] and min(dec.seen[1][2:]) >= 40
+    for bad in OUTSIDE:
+        dec.score_prompt(cache, as_([1, bad, 2]), 0, [1, 2, 3])
+        assert dec.seen[-1][0][::2] == [1, 2] and dec.seen[-1][0][1] >= 40
+
+
+def test_tokens_are_whole_numbers():
+    dec, cache = Recorder(), FakeCtx()
+    for bad in (lambda: dec.score_prompt(cache, [1, 2], 0, [1.5, 2.0]), lambda: dec.logprobs(1, [0.5]), lambda: dec.score_prompt(cache, [1.5], 0, [1])):
+        with pytest.raises(TypeError):
+            bad()
+    assert not dec.seen
+    for kind in (np.int8, np.uint8, np.int32, np.uint32, np.int64, np.uint64):
+        dec.score_prompt(cache, np.array([1, 2], kind), 0, np.array([3, 4], kind))
+        assert dec.seen[-1] == ([1, 2], [3, 4])
+    dec.score_prompt(cache, [], 0, [])
+    assert dec.seen[-1] == ([], [])
