@@ -502,3 +502,96 @@ def test_rows_that_no_step_computed_are_refused(env):
     have(4)
     dec.decode_step(caches[0], 1, 47)
     have(1)
+
+
+# ------------------------------------------- scored prompts by their whole distributions
+
+WHOLE = dict(TINY, vocab=32)  # as many tokens as there are alternatives: every token's log probability of every row
+FLAT = np.float32(1 / 64)     # of the output norm: logits up to 9, entropies of 0.1 to 2.7
+
+
+@pytest.fixture(scope="module")
+def whole(env):
+    E = env["E"]
+    w = small_weights(WHOLE, 12, centered=True)
+    w["output_norm"] = w["output_norm"] * FLAT
+    store, handles = E.AmdWeightStore(env["ctx"]), {}
+    for name, val in w.items():
+        if isinstance(val, tuple):
+            t, k, n, enc = val
+            store.materialize_quantized(name, [k, n], t, enc)
+            handles[name] = store.quantized_tensor(name)
+        else:
+            handles[name] = to_dev(val)
+    layers = [{f: handles[f"blk.{l}.{f}"] for f in ("attn_q", "attn_k", "attn_v", "attn_output", "ffn_gate", "ffn_up", "ffn_down", "attn_norm",
+                                                    "attn_q_norm", "attn_k_norm", "ffn_norm")} for l in range(WHOLE["layers"])]
+    cfg = E.AmdQwen3Config(**WHOLE)
+    return cfg, w, E.AmdQwen3Decode(env["ctx"], cfg, handles["token_embd"], handles["output"], handles["output_norm"], layers, 2)
+
+
+def distributions(got, targets):
+    """[rows][tokens] log probabilities, all of which the alternatives are. What was given of targets is among them bit for bit;
+    they add up to 1; and the entropy is theirs: each is off by eps = EPS and a rounding, p log p by p |log p + 1| eps at
+    most, the entropy itself by 2 EPS and a rounding."""
+    lp = np.full(got.top_tokens.shape, np.nan)
+    np.put_along_axis(lp, got.top_tokens.astype(np.int64), got.top_logprobs.astype(np.float64), 1)
+    assert np.isfinite(lp).all()
+    np.testing.assert_array_equal(got.logprobs, lp[np.arange(len(lp)), targets].astype(np.float32))
+    eps = EPS + HALF_STEP * np.abs(lp).max(1)
+    p = np.exp(lp)
+    assert (np.abs(p.sum(1) - 1) <= eps * (1 + eps)).all()
+    h = -(p * lp).sum(1)
+    assert (np.abs(got.entropy - h) <= (h + 1) * eps * (1 + eps) + (2 * EPS + HALF_STEP) * h).all()
+    return lp
+
+
+@pytest.mark.parametrize("fmt", ["KV_F16", "KV_I8", "KV_I4"])
+@pytest.mark.parametrize("chunk", [16, 48, 2048])
+def test_scores_are_whole_distributions(env, whole, fmt, chunk):
+    """Every row against the oracle's, whose neighbouring rows are further apart than the bars: with logits off by d, a log
+    probability is off by 2 d, and the entropy log Z - sum p x by 2 d + (e^2d - 1) sum p |x - sum p x|, since no p changes by
+    more than e^2d."""
+    case(test="whole", fmt=fmt, chunk=chunk)
+    E = env["E"]
+    cfg, w, dec = whole
+    toks = [int(t) for t in np.random.default_rng(6).integers(0, 32, 91)]
+    cache = E.AmdKvCache(env["ctx"], cfg, CAP, format=getattr(E, fmt))
+    got = dec.score_prompt(cache, toks[:90], 0, toks[1:], entropy=True, top=32, chunk_tokens=chunk)
+    lp = distributions(got, toks[1:])
+    orc = L.LongContextQwen3(WHOLE, w, CAP, L.rope_turns(128, WHOLE["rope_base"]), i8=fmt != "KV_F16", kind=L.Kv4 if fmt == "KV_I4" else L.Kv8)
+    x = []
+    for c0 in range(0, 90, chunk):
+        orc.chunk(toks[c0:min(c0 + chunk, 90)], c0)
+        x += [orc._gemv("output", O.rms_norm_raw(h, orc.w["output_norm"], WHOLE["epsilon"])) for h in orc.hiddens]
+    x = np.stack(x).astype(np.float64)
+    _, entropy, order, alternatives = P.logprobs(x, None, 32)
+    want = np.empty_like(x)
+    np.put_along_axis(want, order, alternatives, 1)
+    d = {"KV_F16": MATMUL_TOL, "KV_I8": MATMUL_TOL + 6e-3, "KV_I4": PROMPT_TOL}[fmt] * np.abs(x).max(1)
+    assert (np.abs(lp - want) <= 2 * d[:, None]).all()
+    assert (np.abs(want[1:] - want[:-1]).max(1) > 4 * d[1:]).mean() > 0.9
+    p = np.exp(want)
+    bound = 2 * d + np.expm1(2 * d) * (p * np.abs(x - (p * x).sum(1, keepdims=True))).sum(1)
+    assert (np.abs(got.entropy - entropy) <= bound).all()
+    if fmt == "KV_F16":
+        assert (np.abs(entropy[1:] - entropy[:-1]) > 2 * bound[1:]).mean() > 0.7
+
+
+@pytest.mark.parametrize("fmt", ["KV_F16", "KV_I4"])
+def test_rows_past_the_first_logits(env, whole, fmt):
+    """1,100 rows, of which logits are held of 1,024 at once, against the same text by 256 (one group a chunk). A row's
+    largest |logit| is no more than its log probabilities' span, logits of both signs being there; two calls' are
+    off by 2 tol of it each. Neighbouring rows are further apart."""
+    case(test="past_1024", fmt=fmt)
+    E = env["E"]
+    cfg, _, dec = whole
+    toks = [int(t) for t in np.random.default_rng(16).integers(0, 32, 1101)]
+    caches = [E.AmdKvCache(env["ctx"], cfg, 1200, format=getattr(E, fmt)) for _ in range(3)]
+    one = dec.score_prompt(caches[0], toks[:1100], 0, toks[1:], entropy=True, top=32)
+    several = dec.score_prompt(caches[1], toks[:1100], 0, toks[1:], entropy=True, top=32, chunk_tokens=256)
+    a, b = distributions(one, toks[1:]), distributions(several, toks[1:])
+    far = 4 * (MATMUL_TOL if fmt == "KV_F16" else PROMPT_TOL) * (b.max(1) - b.min(1))
+    assert (np.abs(a - b).max(1) <= far).all()
+    assert (np.abs(b[1:] - b[:-1]).max(1) > far[1:]).mean() > (0.9 if fmt == "KV_F16" else 0.5)
+    only = dec.score_prompt(caches[2], toks[:1100], 0, entropy=True)
+    np.testing.assert_array_equal(only.entropy, one.entropy)
