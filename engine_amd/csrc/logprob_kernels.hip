@@ -218,11 +218,9 @@ __device__ __forceinline__ void finish(const LogprobArgs& a, size_t row, const R
     const int lane = threadIdx.x & 63;
     // e^(x - M) = 2^t (1 + kShort ln2 t) to first order, so that E times kShort ln 2 is what R' lacks; what E' lacks is the
     // second moment's, which is E'^2 / R' of tokens that lie equally far below M, and more of others by their variance.
-    double r = s.r, e = s.e;
-    if (r > 0.0) {
-        r += kShort * kLn2 * e;
-        e += kShort * (e + kLn2 * e * e / s.r);
-    }
+    const double r = __builtin_fma(kShort * kLn2, s.e, s.r);
+    double e = s.e;
+    if (e != 0.0) e = __builtin_fma(kShort * e, __builtin_fma(kLn2 * e, __builtin_amdgcn_rcp(s.r), 1.0), e);  // (an estimate is enough)
     const double rest = log1pf((float)r);  // (all of a result's parts have its sign: f32 is as good as its own rounding)
     auto logprob = [&](float x) {
         if (!(x > -INFINITY)) return -INFINITY;  // (or no number)
@@ -261,8 +259,12 @@ struct Wave {
         ref = wide ? 0.f : m * kLog2e;
         if (old > -INFINITY) {
             // between what the sums are relative to: with |m| past kWide m c itself, else its f32
-            const double from = was_wide ? (double)old * (double)kLog2e : (double)old_ref, at = wide ? (double)m * (double)kLog2e : (double)ref;
-            const float d = fmaxf((float)(from - at), kLeast), f = __builtin_amdgcn_exp2f(d);
+            float d = old_ref - ref;
+            if (__builtin_expect(wide || was_wide, 0)) {
+                d = (float)((was_wide ? (double)old * (double)kLog2e : (double)old_ref) - (wide ? (double)m * (double)kLog2e : (double)ref));
+            }
+            d = fmaxf(d, kLeast);
+            const float f = __builtin_amdgcn_exp2f(d);
             e = f * __builtin_fmaf(d, l, e);
             l *= f;
         }
