@@ -15,6 +15,7 @@ struct Kv4Format {
     // lane; of its values two of codes (and the tail all of them).
     static constexpr int kKeyRegs = 8, kValueRegs = 8;
     static constexpr bool kFused = true;
+    static constexpr bool kTableFirst = true;
     static constexpr int kQuantiseBarriers = 2;
     struct Scratch {
         kv8_half2 key_lo[4][64], key_hi[4][64];  // of eight rows each; [0] then of all: low, and

@@ -13,6 +13,7 @@ namespace {
 
 struct Kv8Format {
     static constexpr bool kFused = false;
+    static constexpr bool kTableFirst = false;
     static constexpr int kKeyRegs = 8, kValueRegs = 8;  // (codes take the first four)
     static constexpr int kQuantiseBarriers = 1;
     struct Scratch {
