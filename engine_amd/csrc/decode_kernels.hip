@@ -1853,7 +1853,8 @@ bool wide_prefill(const PrefillAttnArgs& a, int tiles, int cu_count) {
 // few workgroups on the card, 2.4 with one a CU and 3.2 with two; the merge takes 4 and
 // the partials their way out and back at 3 TB/s. Whole calls, 32 / 8 heads, unsplit and by this rule:
 // 37 tokens after 2,011 73 and 26 us; 512 after 4,000 about 160 and 117; 512 from
-// position 0 stay unsplit (two shares: 47 for 28).
+// position 0 stay unsplit (two shares: 47 for 28). (These are 8-bit caches'. In 4 bits 29 tokens after 3,040 take 22.3 us by
+// the rule and 22.7 to 26.4 with other shares.)
 int prefill_splits(const PrefillAttnArgs& a, int groups, int cu_count) {
     const size_t rows = (size_t)a.tokens * a.q_heads;
     const int blocks = (a.p0 + a.tokens - 1) / kPfKeys + 1;

@@ -758,8 +758,8 @@ ribn_amd_status ribn_amd_argmax(ribn_amd_context *ctx, const float *logits, size
  * Each of logprobs (with targets), entropy and the two top arrays may be NULL, not all of them. A logit of -inf or NaN
  * has probability 0 (log probability -inf; NaN ranks as -inf); a row of nothing else has log probabilities of
  * -inf and an entropy of 0. Tokens of +inf share the probability. Logits are aligned to their element.
- * Sums are formed beside the likeliest token, so that log probabilities near 0 keep their digits as others do (1e-5 of
- * a result at most, 1e-7 as a rule; where a single token g below the likeliest is nearly all the rest, up to 6e-8 g;
+ * Sums are formed beside the likeliest token, so that log probabilities near 0 keep their digits as others do (in rows of up to
+ * 262,144 tokens 1e-5 of a result at most, 1e-7 as a rule; where a single token g below the likeliest is nearly all the rest, up to 6e-8 g;
  * what is below 1e-37 may come out as 0).
  * A row's last bits may depend on the number of rows. Partial results use the context's scratch, in stream order. */
 #define RIBN_AMD_MAX_LOGPROB_TOP 32u
