@@ -218,9 +218,11 @@ __device__ __forceinline__ void finish(const LogprobArgs& a, size_t row, const R
     const int lane = threadIdx.x & 63;
     // e^(x - M) = 2^t (1 + kShort ln2 t) to first order, so that E times kShort ln 2 is what R' lacks; what E' lacks is the
     // second moment's, which is E'^2 / R' of tokens that lie equally far below M, and more of others by their variance.
-    const double r = __builtin_fma(kShort * kLn2, s.e, s.r);
-    double e = s.e;
-    if (e != 0.0) e = __builtin_fma(kShort * e, __builtin_fma(kLn2 * e, __builtin_amdgcn_rcp(s.r), 1.0), e);  // (an estimate is enough)
+    double r = s.r, e = s.e;
+    if (r > 0.0) {  // (R may be 0 in f32 where E is not)
+        r = __builtin_fma(kShort * kLn2, s.e, s.r);
+        e = __builtin_fma(kShort * s.e, __builtin_fma(kLn2 * s.e, __builtin_amdgcn_rcp(s.r), 1.0), s.e);  // (an estimate is enough)
+    }
     const double rest = log1pf((float)r);  // (all of a result's parts have its sign: f32 is as good as its own rounding)
     auto logprob = [&](float x) {
         if (!(x > -INFINITY)) return -INFINITY;  // (or no number)
